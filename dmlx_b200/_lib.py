@@ -291,6 +291,21 @@ class DeltaShape(C.Structure):
 
 
 _sig("b200_decoder_delta", i32, vp, i32, P(DeltaShape), vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, vp, i32, vp)
+
+
+class NormRope(C.Structure):
+    _fields_ = [(n, i32) for n in ("n_q_heads", "n_kv_heads", "head_dim", "rot_dim", "interleaved")] + [("eps", f32), ("theta", C.c_double)]
+
+
+_sig("b200_qk_norm_rope", i32, P(NormRope), vp, vp, i32, i32, vp, vp, vp, i32, vp, vp, i32, i32, vp)
+_sig("b200_kv_norm_rope_append", i32, vp, i32, P(NormRope), vp, vp, vp, i32, i32, i32, vp, vp, vp, vp, i32, vp, i32, vp)
+_sig("b200_lora_create", i32, i32, i32, i32, i32, P(vp))
+_sig("b200_lora_destroy", None, vp)
+_sig("b200_lora_set", i32, vp, i32, i32, f32, vp, vp)
+_sig("b200_lora_batch_create", i32, i32, i32, i32, P(vp))
+_sig("b200_lora_batch_destroy", None, vp)
+_sig("b200_lora_plan", i32, vp, vp, i32, vp)
+_sig("b200_lora_apply", i32, vp, vp, vp, i32, vp, i32, vp, i32, vp)
 _sig("b200_kv_create_layers", i32, P(KvConfig), P(KvLayer), P(vp))
 _sig("b200_argmax_f32", i32, vp, i32, i32, vp, vp)
 _sig("b200_qmm_f32", i32, vp, vp, i32, vp, i32, i32, i32, vp)

@@ -160,6 +160,20 @@ class PagedKVCache:
         _lib.check(lib.b200_kv_rope_append_partials(self._h, layer, C.byref(parts), _ptr(q_buf), q_stride, _ptr(positions), _ptr(row_seq),
                                                     positions.shape[0], n_q_heads, theta, _stream()))
 
+    def norm_rope_append(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, row_seq: torch.Tensor,
+                         q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-5, theta: float = 10000.0,
+                         rot_dim: Optional[int] = None, interleaved: bool = False, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """b200_kv_norm_rope_append: qk_norm_rope with k and v going into the pages reserved for this step.  Returns q; on FP8 pools k is overwritten
+        with the rotated keys."""
+        t, hq, d = q.shape
+        strides = _rows(q, t, hq, d), _rows(k, t, k.shape[1], d), _rows(v, t, k.shape[1], d)
+        q_out = q_out if q_out is not None else torch.empty((t, hq, d), dtype=q.dtype, device=q.device)
+        shape = _norm_rope_shape(q, k, q_weight, k_weight, eps, theta, rot_dim, interleaved)
+        _lib.check(lib.b200_kv_norm_rope_append(self._h, layer, C.byref(shape), q.data_ptr(), k.data_ptr(), v.data_ptr(), *strides, _ptr(q_weight),
+                                                _ptr(k_weight), _ptr(_ints(positions, t)), _ptr(_ints(row_seq, t)), t, q_out.data_ptr(),
+                                                _rows(q_out, t, hq, d), _stream()))
+        return q_out
+
     def append(self, layer: int, k_rows: torch.Tensor, v_rows: torch.Tensor):
         assert k_rows.dtype == torch.bfloat16 and v_rows.dtype == torch.bfloat16
         _lib.check(lib.b200_kv_append(self._h, layer, _ptr(k_rows), _ptr(v_rows), k_rows.shape[0], _stream()))
@@ -315,6 +329,114 @@ class LayeredKVCache(PagedKVCache):
         if word:
             raise _lib.B200Error(word)
         return out
+
+
+def _here(t: torch.Tensor) -> bool:
+    return t.is_cuda and t.device.index == torch.cuda.current_device()
+
+
+def _rows(t: torch.Tensor, *shape) -> int:
+    """Checks bf16 rows on the device whose numbers lie one behind the other within a row (shape: None = any length); returns the elements between
+    rows."""
+    if not (_here(t) and t.dtype == torch.bfloat16 and t.dim() == len(shape) and all(want is None or have == want for have, want in zip(t.shape, shape))):
+        raise ValueError(f"expected bf16 rows of shape {shape} on the current device, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    inner = 1
+    for n, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        if n > 1 and stride != inner:
+            raise ValueError(f"the numbers of a row are not contiguous: strides {t.stride()}")
+        inner *= n
+    return t.stride(0) if t.shape[0] > 1 else inner
+
+
+def _ints(t: torch.Tensor, n: int) -> torch.Tensor:
+    if not (_here(t) and t.dtype == torch.int32 and tuple(t.shape) == (n,) and t.is_contiguous()):
+        raise ValueError(f"expected {n} contiguous int32 on the current device, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t
+
+
+def _norm_rope_shape(q: torch.Tensor, k: torch.Tensor, q_weight, k_weight, eps: float, theta: float, rot_dim: Optional[int], interleaved: bool):
+    d = q.shape[-1]
+    for w in (q_weight, k_weight):
+        if w is not None:
+            _rows(w, d)
+    return _lib.NormRope(q.shape[1], k.shape[1], d, d if rot_dim is None else rot_dim, int(interleaved), eps, theta)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
+                 k_weight: Optional[torch.Tensor] = None, eps: float = 1e-5, theta: float = 10000.0, rot_dim: Optional[int] = None,
+                 interleaved: bool = False, q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None):
+    """b200_qk_norm_rope: RMSNorm of every head of q [T, Hq, D] and k [T, Hkv, D] (rows may be strided) and the rotation of its first rot_dim numbers
+    (default: all) in one pass.  Returns (q, k) as new tensors, or q_out and k_out, which may be q and k themselves."""
+    t, hq, d = q.shape
+    q_stride, k_stride = _rows(q, t, hq, d), _rows(k, t, k.shape[1], d)
+    q_out = q_out if q_out is not None else torch.empty((t, hq, d), dtype=q.dtype, device=q.device)
+    k_out = k_out if k_out is not None else torch.empty((t, k.shape[1], d), dtype=k.dtype, device=k.device)
+    qo_stride, ko_stride = _rows(q_out, t, hq, d), _rows(k_out, t, k.shape[1], d)
+    shape = _norm_rope_shape(q, k, q_weight, k_weight, eps, theta, rot_dim, interleaved)
+    _lib.check(lib.b200_qk_norm_rope(C.byref(shape), q.data_ptr(), k.data_ptr(), q_stride, k_stride, _ptr(q_weight), _ptr(k_weight), _ptr(_ints(positions, t)),
+                                     t, q_out.data_ptr(), k_out.data_ptr(), qo_stride, ko_stride, _stream()))
+    return q_out, k_out
+
+
+class LoraAdapters:
+    """Low-rank adapters of one projection [n, k] (b200_lora): slot i holds A [rank, k], B [n, rank] and a scale once set() has put them there."""
+
+    def __init__(self, n_adapters: int, n: int, k: int, max_rank: int):
+        h = C.c_void_p()
+        _lib.check(lib.b200_lora_create(n_adapters, n, k, max_rank, C.byref(h)))
+        self._h, self.n_adapters, self.n, self.k, self.max_rank = h.value, n_adapters, n, k, max_rank
+
+    def close(self):
+        if getattr(self, "_h", None) and lib is not None:
+            lib.b200_lora_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        self.close()
+
+    def set(self, slot: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0):
+        """a [rank, k] and b [n, rank] bf16, wherever they lie."""
+        rank = a.shape[0]
+        if a.dtype != torch.bfloat16 or b.dtype != torch.bfloat16 or tuple(a.shape) != (rank, self.k) or tuple(b.shape) != (self.n, rank):
+            raise ValueError(f"adapter of {tuple(a.shape)} and {tuple(b.shape)} for a projection of {self.n} x {self.k}")
+        a, b = a.detach().cpu().contiguous(), b.detach().cpu().contiguous()
+        _lib.check(lib.b200_lora_set(self._h, slot, rank, scale, a.data_ptr(), b.data_ptr()))
+
+    def clear(self, slot: int):
+        _lib.check(lib.b200_lora_set(self._h, slot, 0, 0.0, None, None))
+
+    def apply(self, batch: "LoraBatch", x: torch.Tensor, y: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """b200_lora_apply: y + scale * B (A x) row by row, x [T, k], y [T, n] (rows may be strided), T the rows of the batch's plan.  out may be y."""
+        t = x.shape[0]
+        if t != batch.rows:
+            raise ValueError(f"{t} rows, the batch's plan has {batch.rows}")
+        out = out if out is not None else torch.empty((t, self.n), dtype=y.dtype, device=y.device)
+        strides = _rows(x, t, self.k), _rows(y, t, self.n), _rows(out, t, self.n)
+        _lib.check(lib.b200_lora_apply(self._h, batch._h, x.data_ptr(), strides[0], y.data_ptr(), strides[1], out.data_ptr(), strides[2], _stream()))
+        return out
+
+
+class LoraBatch:
+    """The rows of a step in the order of their adapters (b200_lora_batch), planned once per step and used by every projection."""
+
+    def __init__(self, max_rows: int, max_adapters: int, max_rank: int):
+        h = C.c_void_p()
+        _lib.check(lib.b200_lora_batch_create(max_rows, max_adapters, max_rank, C.byref(h)))
+        self._h, self.rows = h.value, None
+
+    def close(self):
+        if getattr(self, "_h", None) and lib is not None:
+            lib.b200_lora_batch_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        self.close()
+
+    def plan(self, row_adapter: torch.Tensor):
+        """b200_lora_plan: the adapter of every row, -1 for none."""
+        rows = row_adapter.shape[0]
+        _lib.check(lib.b200_lora_plan(self._h, _ptr(_ints(row_adapter, rows)), rows, _stream()))
+        self.rows = rows
 
 
 def set_attn_pages_per_chunk(n: int):

@@ -363,6 +363,28 @@ b200_status b200_rmsnorm(const void* d_x, const void* d_weight, void* d_out, int
 b200_status b200_rope(void* d_q, void* d_k, const int32_t* d_positions, int32_t rows,
                       int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t q_stride,
                       int32_t k_stride, float theta, void* stream);
+/* Norm of every q and k head with the rotation in the same pass (no reference counterpart): n = x / sqrt(mean(x^2) + eps) * w over a head's
+ * numbers, then the first rot_dim of them rotate in pairs by position * theta^(-2i / rot_dim).  f32 in between, angles exact for every 32-bit
+ * position, one rounding.  Rows [heads][head_dim] bf16 with strides in elements (multiples of 8, 16-byte aligned); weights bf16 [head_dim], null =
+ * ones.  d_q_out / d_k_out may be d_q / d_k (with their strides), and do not overlap them otherwise. */
+typedef struct b200_norm_rope {
+  int32_t n_q_heads, n_kv_heads; /* either may be 0: its pointers are then not looked at */
+  int32_t head_dim;              /* 64, 128 or 256 */
+  int32_t rot_dim;               /* multiple of 16 up to head_dim; 0 = no rotation */
+  int32_t interleaved;           /* pairs (2i, 2i+1) instead of (i, i + rot_dim / 2) */
+  float eps;
+  double theta;
+} b200_norm_rope;
+b200_status b200_qk_norm_rope(const b200_norm_rope* shape, const void* d_q, const void* d_k, int32_t q_stride, int32_t k_stride,
+                              const void* d_q_weight, const void* d_k_weight, const int32_t* d_positions, int32_t rows, void* d_q_out,
+                              void* d_k_out, int32_t q_out_stride, int32_t k_out_stride, void* stream);
+/* The same with k and v going straight into the pages reserved for the step (b200_kv_reserve), as b200_kv_rope_append does; same bits as
+ * b200_qk_norm_rope followed by b200_kv_append.  On FP8 pools, where a page's scale depends on all its new rows, that is what runs, and d_k is
+ * overwritten with the rotated keys. */
+b200_status b200_kv_norm_rope_append(b200_kv* kv, int32_t layer, const b200_norm_rope* shape, const void* d_q, void* d_k, const void* d_v,
+                                     int32_t q_stride, int32_t k_stride, int32_t v_stride, const void* d_q_weight, const void* d_k_weight,
+                                     const int32_t* d_positions, const int32_t* d_row_seq, int32_t rows, void* d_q_out, int32_t q_out_stride,
+                                     void* stream);
 b200_status b200_embed_gather(const void* d_table, const uint32_t* d_ids, void* d_out, int32_t rows,
                               int32_t hidden, void* stream);                      /* :566 */
 /* Greedy: first strict maximum per row of bf16 logits [rows, vocab] (src/sampling.zig:22-39). */
@@ -508,6 +530,28 @@ b200_status b200_qmm_debug_wait_runs_out(int32_t polls, void* stream);
 b200_status b200_qmm_static_scratch(const b200_qweight* w, const void* d_x, int32_t rows, void* d_y,
                                     int32_t epilogue, const void* d_residual, float swiglu_limit,
                                     void* stream);
+
+/* ---- low-rank adapters of many requests beside a shared projection ------------------------------ */
+/* No counterpart in the reference.  out[r] = y[r] + scale_a * B_a (A_a x[r]), a = the row's adapter: y is the result of the projection that all
+ * requests share (b200_qmm on the same x), A_a [rank, k] and B_a [n, rank] are bf16, sums are f32, the result is rounded once.
+ * A b200_lora holds the adapters of one projection, a b200_lora_batch the rows of a step in the order of their adapters: it is planned once per
+ * step (device, asynchronous) and used by every projection of every layer whose handle has as many adapters.  A batch handle is the workspace of
+ * its plan: steps that may run at the same time (two captured graphs on two streams) have a batch handle each. */
+typedef struct b200_lora b200_lora;
+typedef struct b200_lora_batch b200_lora_batch;
+/* Up to 4096 adapters of rank up to 128; n and k multiples of 8.  All start without matrices (rank 0). */
+b200_status b200_lora_create(int32_t n_adapters, int32_t n, int32_t k, int32_t max_rank, b200_lora** out);
+void b200_lora_destroy(b200_lora* l);
+/* Host pointers, bf16: A [rank, k], B [n, rank]; rank 0 takes the adapter out.  Synchronous; no step that uses this adapter may be in flight. */
+b200_status b200_lora_set(b200_lora* l, int32_t adapter, int32_t rank, float scale, const void* h_a, const void* h_b);
+b200_status b200_lora_batch_create(int32_t max_rows, int32_t max_adapters, int32_t max_rank, b200_lora_batch** out);
+void b200_lora_batch_destroy(b200_lora_batch* b);
+/* d_row_adapter [rows]: the adapter of every row; a number that is none (-1) leaves the row as it is, and so does an adapter of rank 0. */
+b200_status b200_lora_plan(b200_lora_batch* b, const int32_t* d_row_adapter, int32_t rows, void* stream);
+/* Over the rows of the batch's plan, bf16, strides in elements (multiples of 8, rows start on 16 bytes).  d_out may be d_y (rows without an adapter
+ * are then not touched); otherwise the two do not overlap and rows without an adapter are copied.  Same bits for a row whatever shares its batch. */
+b200_status b200_lora_apply(const b200_lora* l, const b200_lora_batch* b, const void* d_x, int32_t x_stride, const void* d_y, int32_t y_stride,
+                            void* d_out, int32_t out_stride, void* stream);
 
 /* ---- LLaMA-architecture decode step over a packed ragged batch --------------------------------- */
 /* Stands in for ModelVTable.forward + the greedy branch of generateBatchStep
