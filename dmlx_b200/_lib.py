@@ -299,6 +299,10 @@ class NormRope(C.Structure):
 
 _sig("b200_qk_norm_rope", i32, P(NormRope), vp, vp, i32, i32, vp, vp, vp, i32, vp, vp, i32, i32, vp)
 _sig("b200_kv_norm_rope_append", i32, vp, i32, P(NormRope), vp, vp, vp, i32, i32, i32, vp, vp, vp, vp, i32, vp, i32, vp)
+_sig("b200_prefix_attn_create", i32, vp, i32, P(vp))
+_sig("b200_prefix_attn_destroy", None, vp)
+_sig("b200_prefix_attn_plan", i32, vp, vp, vp, i32, vp)
+_sig("b200_prefix_attn_run", i32, vp, i32, vp, i32, vp, i32, vp)
 _sig("b200_lora_create", i32, i32, i32, i32, i32, P(vp))
 _sig("b200_lora_destroy", None, vp)
 _sig("b200_lora_set", i32, vp, i32, i32, f32, vp, vp)

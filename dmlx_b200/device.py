@@ -378,6 +378,40 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, q_we
     return q_out, k_out
 
 
+class SharedPrefixAttention:
+    """Attention of a batch whose sequences share pages (b200_prefix_attn): plan() once per step, run() per layer.  What PagedKVCache.attention gives,
+    with every page that several rows see read once for all of them."""
+
+    def __init__(self, cache: PagedKVCache, max_rows: int):
+        h = C.c_void_p()
+        _lib.check(lib.b200_prefix_attn_create(cache._h, max_rows, C.byref(h)))
+        self._h, self.cache, self.rows = h.value, cache, None
+
+    def close(self):
+        if getattr(self, "_h", None) and lib is not None:
+            lib.b200_prefix_attn_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        self.close()
+
+    def plan(self, row_seq: torch.Tensor, row_ctx: torch.Tensor):
+        """b200_prefix_attn_plan: row r is to see the first row_ctx[r] tokens of slot row_seq[r]."""
+        rows = row_seq.shape[0]
+        _lib.check(lib.b200_prefix_attn_plan(self._h, _ptr(_ints(row_seq, rows)), _ptr(_ints(row_ctx, rows)), rows, _stream()))
+        self.rows = rows
+
+    def run(self, layer: int, q: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """b200_prefix_attn_run: q [T, Hq, D] (rows may be strided), T the rows of the plan."""
+        c = self.cache.cfg
+        if q.shape[0] != self.rows:
+            raise ValueError(f"{q.shape[0]} rows, the plan has {self.rows}")
+        out = out if out is not None else torch.empty((self.rows, c.n_q_heads, c.head_dim), dtype=q.dtype, device=q.device)
+        strides = _rows(q, self.rows, c.n_q_heads, c.head_dim), _rows(out, self.rows, c.n_q_heads, c.head_dim)
+        _lib.check(lib.b200_prefix_attn_run(self._h, layer, q.data_ptr(), strides[0], out.data_ptr(), strides[1], _stream()))
+        return out
+
+
 class LoraAdapters:
     """Low-rank adapters of one projection [n, k] (b200_lora): slot i holds A [rank, k], B [n, rank] and a scale once set() has put them there."""
 

@@ -346,6 +346,19 @@ b200_status b200_paged_attn_prefill(b200_kv* kv, int32_t layer, const void* d_q,
                                     const int32_t* d_row_seq, const int32_t* d_row_ctx,
                                     int32_t total_rows, void* d_out, void* stream);
 
+/* Attention of a batch whose sequences share pages (b200_kv_fork, prefix sharing): the contract of b200_paged_attn_decode, with every page that
+ * several rows see read and multiplied once for all of them (no reference counterpart).  The plan, once per step, finds on the device what the rows'
+ * page tables have in common and copies the row arrays; the layers of the step then take q, [q heads][head_dim] rows of bf16 with strides in
+ * elements (multiples of 8, rows on 16 bytes), and out likewise.  A row of context 0, or of a slot that is none, gets zeros.  Rows of any order; a
+ * slot may have several.  A plan is valid until pages are reserved, released or forked.  A handle belongs to one pool, which outlives it, and is the
+ * workspace of its plan: steps that may run at the same time have a handle each.  Up to 4096 rows, 16 query heads per kv head; bf16 pools, and
+ * FP8 pools of head_dim 128. */
+typedef struct b200_prefix_attn b200_prefix_attn;
+b200_status b200_prefix_attn_create(b200_kv* kv, int32_t max_rows, b200_prefix_attn** out);
+void b200_prefix_attn_destroy(b200_prefix_attn* h);
+b200_status b200_prefix_attn_plan(b200_prefix_attn* h, const int32_t* d_row_seq, const int32_t* d_row_ctx, int32_t rows, void* stream);
+b200_status b200_prefix_attn_run(b200_prefix_attn* h, int32_t layer, const void* d_q, int32_t q_stride, void* d_out, int32_t out_stride, void* stream);
+
 /* Tuning hook with no reference counterpart: pages per split-K chunk, 4..32; 0 (default) = 8, 16 or 32 chosen on
  * the device from the batch's mean context. */
 void b200_set_attn_pages_per_chunk(int32_t n);

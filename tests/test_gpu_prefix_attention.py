@@ -1,0 +1,424 @@
+"""Attention of a batch whose sequences share pages, against softmax(q k / sqrt(d)) v in 64 bits over the tokens that the cache gives back.
+
+Tolerance, per number: half a step of bf16 of the result, 2^-8 of it; the weights are rounded to bf16 before their product, 2^-8 of each, so 2^-8 of
+E = sum p |v| / sum p; and a score is off by its f32 sum, (d / 16 + 2) 2^-22 of S = |q| |k| / sqrt(d), and by its exponent's argument and the
+exponential, 2^-20 together for |scores| up to 16 or S: a weight and the sum by twice that, relative."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+
+def _random(*shape, seed, scale=1.0):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * scale).bfloat16().cuda()
+
+
+def _ints(*values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def _append(cache, counts, seed, layers=1):
+    """counts: {slot: tokens} behind what the slots hold."""
+    c = cache.cfg
+    desc = [[slot, n, cache.seq_len(slot), 0] for slot, n in counts.items()]
+    rows = sum(counts.values())
+    cache.reserve(torch.tensor(desc, dtype=torch.int32, device="cuda"))
+    for layer in range(layers):
+        cache.append(layer, _random(rows, c.n_kv_heads, c.head_dim, seed=seed + layer), _random(rows, c.n_kv_heads, c.head_dim, seed=seed + 50 + layer))
+    assert cache.error_word() == 0
+
+
+def _held(cache, layer, slots):
+    """Keys and values of the slots' tokens in 64 bits.  (gather() rounds what 8-bit pages hold to bf16; a page's codes times its scale are exact.)"""
+    if cache.cfg.kv_dtype == 0:
+        return {s: tuple(x.double() for x in cache.gather(layer, s)) for s in slots}
+    pages, held = {}, {}
+    for s in slots:
+        table = cache.block_table(s)
+        for p in table:
+            if p not in pages:
+                k, v, ks, vs = (torch.from_numpy(x) for x in cache.page_raw(layer, p))
+                pages[p] = [(x.view(torch.float8_e4m3fn).double() * sc.double()[:, None, None]).permute(1, 0, 2) for x, sc in ((k, ks), (v, vs))]
+        held[s] = tuple(torch.cat([pages[p][i] for p in table] or [torch.zeros((0, cache.cfg.n_kv_heads, cache.cfg.head_dim))]).cuda() for i in range(2))
+    return held
+
+
+def _want(cache, layer, q, row_seq, row_ctx):
+    held = _held(cache, layer, {s for s in row_seq if 0 <= s < cache.cfg.max_seqs})
+    t, hq, d = q.shape
+    group = hq // cache.cfg.n_kv_heads
+    want, tol = torch.zeros(q.shape, dtype=torch.float64, device="cuda"), torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    for r, (s, n) in enumerate(zip(row_seq, row_ctx)):
+        if s not in held or n <= 0:
+            continue
+        k, v = (x[:n].repeat_interleave(group, 1) for x in held[s])
+        scores = torch.einsum("hd,thd->ht", q[r].double(), k) / math.sqrt(d)
+        top = torch.einsum("hd,thd->ht", q[r].double().abs(), k.abs()).amax(1) / math.sqrt(d)
+        p = torch.softmax(scores, 1)
+        want[r] = torch.einsum("ht,thd->hd", p, v)
+        e = torch.einsum("ht,thd->hd", p, v.abs())
+        tol[r] = 2.0 ** -8 * want[r].abs() + (2.0 ** -8 + 2 * ((d / 16 + 2) * 2.0 ** -22 * top[:, None] + 2.0 ** -20 * (top[:, None] / 16).clamp(min=1))) * e
+    return want, tol
+
+
+def _check(got, want, tol):
+    off = (got.double() - want).abs()
+    assert bool((off <= tol).all()), float((off - tol).max())
+
+
+def _run(cache, q, row_seq, row_ctx, layer=0, handle=None, **how):
+    from dmlx_b200 import device as dev
+
+    handle = handle or dev.SharedPrefixAttention(cache, max(len(row_seq), 1))
+    handle.plan(_ints(*row_seq), _ints(*row_ctx))
+    got = handle.run(layer, q, **how)
+    assert cache.error_word() == 0
+    return got
+
+
+def _tree(dev, rows, system, docs, doc, own, hq, hkv, d, fp8=False, layers=1, seed=0):
+    """`rows` sequences behind a common text and one of `docs` texts behind that, each with tokens of its own; (cache, slots, contexts)."""
+    parents = 1 + docs
+    longest = system + doc + max(own) + 64
+    pages = -(-longest // 32)
+    cache = dev.PagedKVCache(layers, hkv, d, pages * (parents + 1) + rows * (max(own) // 32 + 4), parents + rows, pages, hq, max_rows=max(longest, rows * max(own), 64),
+                             kv_dtype=dev.KV_FP8_E4M3 if fp8 else dev.KV_BF16)
+    if system:
+        _append(cache, {0: system}, seed, layers)
+    for i in range(docs):
+        cache.fork(0, 1 + i, system)
+        _append(cache, {1 + i: doc}, seed + 100 + i, layers)
+    slots = [parents + i for i in range(rows)]
+    for i, s in enumerate(slots):
+        parent = 1 + i % docs if docs else 0
+        if system + doc:
+            cache.fork(parent, s, system + doc)
+    mine = {s: own[i % len(own)] for i, s in enumerate(slots) if own[i % len(own)]}
+    if mine:
+        _append(cache, mine, seed + 200, layers)
+    return cache, slots, [cache.seq_len(s) for s in slots]
+
+
+CASES = [  # rows, system, docs, doc, own tokens, hq, hkv, d, fp8
+    (1, 0, 0, 0, [1], 4, 1, 64, False),
+    (1, 0, 0, 0, [1000], 8, 2, 128, False),
+    (2, 64, 0, 0, [1, 33], 8, 8, 128, False),
+    (4, 500, 0, 0, [1, 20, 40], 32, 8, 128, False),
+    (5, 96, 0, 0, [0, 1], 16, 1, 64, False),           # a context that is the shared pages alone; 16 query heads per kv head
+    (7, 1100, 0, 0, [5, 64, 100], 12, 4, 128, False),  # 3 query heads per kv head
+    (33, 300, 3, 1001, [1, 31, 32, 200], 16, 4, 64, False),
+    (70, 2048, 0, 0, [3, 40], 32, 4, 128, False),      # more rows than two tiles hold
+    (140, 129, 2, 64, [1, 70], 4, 2, 64, False),
+    (40, 31, 4, 40, [1], 8, 2, 128, False),            # a prefix of less than a page, small nodes
+    (3, 260, 0, 0, [9, 1], 8, 2, 128, True),
+    (6, 1300, 0, 0, [33, 2], 16, 4, 128, True),
+    (50, 700, 2, 333, [1, 64, 90], 32, 4, 128, True),
+    (9, 40, 0, 0, [1], 6, 1, 128, True),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,system,docs,doc,own,hq,hkv,d,fp8", CASES)
+def test_rows_of_a_tree(rows, system, docs, doc, own, hq, hkv, d, fp8):
+    from dmlx_b200 import device as dev
+
+    cache, slots, ctx = _tree(dev, rows, system, docs, doc, own, hq, hkv, d, fp8)
+    order = torch.randperm(rows, generator=torch.Generator().manual_seed(rows)).tolist()
+    slots, ctx = [slots[i] for i in order], [ctx[i] for i in order]
+    q = _random(rows, hq, d, seed=9, scale=2.0)
+    want, tol = _want(cache, 0, q, slots, ctx)
+    _check(_run(cache, q, slots, ctx), want, tol)
+    shorter = [max(1, n - 1 - 37 * i % n) for i, n in enumerate(ctx)]  # rows that see less than their slots hold
+    _check(_run(cache, q, slots, shorter), *_want(cache, 0, q, slots, shorter))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+def test_rows_of_any_kind_together(fp8):
+    """A portion of a prompt (rows of one slot), the same row twice, rows without a context, slots that are none, and sequences that share nothing."""
+    from dmlx_b200 import device as dev
+
+    cache, slots, ctx = _tree(dev, 12, 200, 0, 0, [5, 70, 1], 16, 4, 128, fp8)
+    row_seq = [slots[0]] * 40 + [slots[3], -1, slots[3], 0, 13, slots[5], slots[6], slots[7], slots[8]]
+    row_ctx = list(range(ctx[0] - 39, ctx[0] + 1)) + [ctx[3], 50, ctx[3], 32, 7, 0, 31, -4, 1]
+    q = _random(len(row_seq), 16, 128, seed=3, scale=2.0)
+    q[42] = q[40]
+    got = _run(cache, q, row_seq, row_ctx)
+    _check(got, *_want(cache, 0, q, row_seq, row_ctx))
+    assert torch.equal(got[40], got[42])
+    assert not bool(got[41].any()) and not bool(got[45].any()) and not bool(got[47].any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_as_the_decode_step_s_attention_has_it(d):
+    from dmlx_b200 import device as dev
+
+    cache, slots, ctx = _tree(dev, 24, 515, 2, 190, [1, 45], 8, 2, d, layers=3)
+    handle = dev.SharedPrefixAttention(cache, 64)
+    handle.plan(_ints(*slots), _ints(*ctx))
+    for layer in range(3):
+        q = _random(24, 8, d, seed=layer, scale=2.0)
+        got = handle.run(layer, q)
+        want, tol = _want(cache, layer, q, slots, ctx)
+        _check(got, want, tol)
+        _check(cache.attention(layer, q, _ints(*slots), _ints(*ctx)), want, tol)
+        assert torch.equal(got, handle.run(layer, q))
+    assert cache.error_word() == 0
+
+
+@pytest.mark.gpu
+def test_a_prefix_of_many_pages_and_rows_of_several_tiles():
+    from dmlx_b200 import device as dev
+
+    cache, slots, ctx = _tree(dev, 100, 9000, 0, 0, [1, 40, 300], 16, 2, 128)
+    q = _random(100, 16, 128, seed=1, scale=3.0)
+    _check(_run(cache, q, slots, ctx), *_want(cache, 0, q, slots, ctx))
+
+
+@pytest.mark.gpu
+def test_scores_that_grow_and_scores_that_are_large():
+    """Rows whose largest score comes late, again and again, and far above the others."""
+    from dmlx_b200 import device as dev
+
+    cache = dev.PagedKVCache(1, 1, 128, 128, 40, 60, 8, max_rows=2048)
+    cache.reserve(torch.tensor([[0, 1600, 0, 0]], dtype=torch.int32, device="cuda"))
+    k, v = _random(1600, 1, 128, seed=1), _random(1600, 1, 128, seed=2)
+    k *= torch.linspace(0.01, 4.0, 1600, device="cuda").bfloat16()[:, None, None]
+    cache.append(0, k, v)
+    slots = list(range(1, 21))
+    for s in slots:
+        cache.fork(0, s, 1600)
+    q = _random(20, 8, 128, seed=3, scale=2.0)
+    ctx = [1600 - 3 * i for i in range(20)]
+    _check(_run(cache, q, slots, ctx), *_want(cache, 0, q, slots, ctx))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+def test_what_lies_behind_a_context_has_no_part_in_it(fp8):
+    """Keys and values that are no numbers behind the tokens of a row's last page, from a sequence that had the page before."""
+    from dmlx_b200 import device as dev
+
+    cache = dev.PagedKVCache(1, 2, 128, 8, 6, 4, 8, max_rows=64, kv_dtype=dev.KV_FP8_E4M3 if fp8 else dev.KV_BF16)
+    for page in range(8):
+        k, v, ks, vs = cache.page_raw(0, page)
+        k[:], v[:] = (0x7F, 0x7F) if fp8 else (0x7FC0, 0x7F80)  # NaN, infinity
+        cache.page_load(0, page, k, v, ks + 1, vs + 1)
+    _append(cache, {0: 32}, 1)
+    for s in (1, 2, 3):
+        cache.fork(0, s, 32)
+    _append(cache, {1: 1, 2: 5, 3: 31}, 2)
+    q = _random(4, 8, 128, seed=3)
+    row_seq, row_ctx = [1, 2, 3, 0], [33, 37, 63, 7]
+    got = _run(cache, q, row_seq, row_ctx)
+    want, tol = _want(cache, 0, q, row_seq, row_ctx)
+    assert bool(want.isfinite().all())
+    _check(got, want, tol)
+
+
+@pytest.mark.gpu
+def test_numbers_that_are_not_finite_stay_in_their_row():
+    from dmlx_b200 import device as dev
+
+    cache, slots, ctx = _tree(dev, 20, 400, 0, 0, [3, 40], 8, 2, 128)
+    q = _random(20, 8, 128, seed=5, scale=2.0)
+    want, tol = _want(cache, 0, q, slots, ctx)
+    q[4, 3, 7] = float("nan")
+    q[11, 6, 0] = float("inf")
+    got = _run(cache, q, slots, ctx)
+    fine = torch.ones(20, 8, dtype=torch.bool, device="cuda")
+    fine[4, 3] = fine[11, 6] = False
+    assert bool(((got.double() - want).abs() <= tol)[fine].all())
+    assert not bool(got[4, 3].any())  # scores that are no numbers weigh nothing
+
+
+@pytest.mark.gpu
+def test_strided_rows_and_what_lies_around_them():
+    from dmlx_b200 import device as dev
+
+    cache, slots, ctx = _tree(dev, 18, 130, 0, 0, [2, 50], 8, 2, 64)
+    qkv = _random(18, 8 * 64 + 256, seed=6, scale=2.0)
+    q = qkv[:, :512].unflatten(1, (8, 64))
+    out = torch.full((20, 512 + 24), 5.0, dtype=torch.bfloat16, device="cuda")
+    _run(cache, q, slots, ctx, out=out[:18, 8:520].unflatten(1, (8, 64)))
+    _check(out[:18, 8:520].unflatten(1, (8, 64)), *_want(cache, 0, q, slots, ctx))
+    assert bool((out[18:] == 5).all()) and bool((out[:, :8] == 5).all()) and bool((out[:, 520:] == 5).all())
+
+
+@pytest.mark.gpu
+def test_graphs_with_handles_of_their_own_on_two_streams():
+    from dmlx_b200 import device as dev
+
+    cache, slots, ctx = _tree(dev, 30, 333, 0, 0, [1, 64], 8, 2, 128)
+    sides = []
+    for rows in (30, 11):
+        row_seq, row_ctx, q = _ints(*slots[:rows]), _ints(*ctx[:rows]), torch.zeros((rows, 8, 128), dtype=torch.bfloat16, device="cuda")
+        handle, out = dev.SharedPrefixAttention(cache, 32), torch.zeros_like(q)
+        handle.plan(row_seq, row_ctx)
+        handle.run(0, q, out=out)
+        torch.cuda.synchronize()
+        graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(graph, stream=stream):
+            handle.plan(row_seq, row_ctx)
+            handle.run(0, q, out=out)
+        sides.append((row_seq, row_ctx, q, out, handle, graph, stream))
+    for turn in range(3):
+        for i, (row_seq, row_ctx, q, *_) in enumerate(sides):
+            rows = q.shape[0]
+            pick = torch.randperm(30, generator=torch.Generator().manual_seed(10 * turn + i))[:rows].tolist()
+            row_seq.copy_(_ints(*[slots[p] for p in pick]))
+            row_ctx.copy_(_ints(*[max(0, ctx[p] - turn * 50 * (p % 3)) for p in pick]))
+            q.copy_(_random(rows, 8, 128, seed=turn + i, scale=2.0))
+        torch.cuda.synchronize()
+        for *_, graph, stream in sides:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for row_seq, row_ctx, q, out, *_ in sides:
+            _check(out, *_want(cache, 0, q, row_seq.tolist(), row_ctx.tolist()))
+    assert cache.error_word() == 0
+
+
+@pytest.mark.gpu
+def test_plans_follow_the_pages():
+    """A handle through a life: rows join, write into shared pages (copied first), leave, and their pages go to others."""
+    from dmlx_b200 import device as dev
+
+    cache = dev.PagedKVCache(1, 2, 128, 64, 8, 16, 8, max_rows=256)
+    handle = dev.SharedPrefixAttention(cache, 8)
+    _append(cache, {0: 150}, 1)
+    for s in (1, 2, 3):
+        cache.fork(0, s, 150)  # (a page is shared that is not full)
+    steps = [lambda: None, lambda: _append(cache, {1: 1, 2: 1, 0: 1}, 2), lambda: _append(cache, {1: 60, 3: 40}, 3), lambda: cache.rollback(1, 70),
+             lambda: _append(cache, {1: 90}, 4), lambda: cache.release([0, 2]), lambda: _append(cache, {0: 100, 4: 20}, 5), lambda: cache.fork(1, 5, 96),
+             lambda: _append(cache, {5: 3, 1: 2}, 6)]
+    for n, step in enumerate(steps):
+        step()
+        slots = [s for s in range(6) if cache.seq_len(s)]
+        ctx = [cache.seq_len(s) for s in slots]
+        q = _random(len(slots), 8, 128, seed=20 + n, scale=2.0)
+        _check(_run(cache, q, slots, ctx, handle=handle), *_want(cache, 0, q, slots, ctx))
+
+
+@pytest.mark.gpu
+def test_as_many_rows_as_a_handle_holds():
+    from dmlx_b200 import device as dev
+
+    cache = dev.PagedKVCache(1, 1, 64, 4100, 4096, 3, 2, max_rows=4096)
+    _append(cache, {0: 64}, 1)
+    for s in range(1, 4096):
+        cache.fork(0, s, 64)
+    for lo in (1, 2049):
+        _append(cache, {s: 1 for s in range(lo, min(lo + 2048, 4096))}, lo)
+    slots = list(range(4096))
+    ctx = [64] + [65] * 4095
+    q = _random(4096, 2, 64, seed=2, scale=2.0)
+    handle = dev.SharedPrefixAttention(cache, 4096)
+    got = _run(cache, q, slots, ctx, handle=handle)
+    some = list(range(0, 4096, 97))
+    _check(got[some], *_want(cache, 0, q[some], [slots[i] for i in some], [ctx[i] for i in some]))
+    alone = [0] * 4096  # no two rows share a page
+    _check(_run(cache, q, slots, alone, handle=handle), torch.zeros_like(q).double(), torch.zeros_like(q).double())
+
+
+@pytest.mark.gpu
+def test_a_step_s_attention_half():
+    """Projection, adapters, norms and rotation into pages, attention over the shared prefix, output projection with adapters: as a step calls them."""
+    from dmlx_b200 import device as dev
+
+    rows, hidden, hq, hkv, d = 21, 512, 8, 2, 64
+    cache, slots, ctx = _tree(dev, rows, 333, 0, 0, [4, 40], hq, hkv, d)
+    n = (hq + 2 * hkv) * d
+    x = _random(rows, hidden, seed=1)
+    w_qkv, w_o = _random(n, hidden, seed=2, scale=hidden ** -0.5), _random(hidden, hq * d, seed=3, scale=(hq * d) ** -0.5)
+    adapters = [dev.LoraAdapters(3, n, hidden, 16), dev.LoraAdapters(3, hidden, hq * d, 16)]
+    pairs = []
+    for which, (w, (rows_out, cols)) in enumerate(zip(adapters, ((n, hidden), (hidden, hq * d)))):
+        pairs.append({})
+        for slot, rank in ((0, 16), (2, 5)):
+            a, b = _random(rank, cols, seed=10 + slot + which, scale=cols ** -0.5), _random(rows_out, rank, seed=20 + slot + which, scale=rank ** -0.5)
+            w.set(slot, a, b, 0.5)
+            pairs[-1][slot] = (a.double(), b.double())
+    row_adapter = [i % 4 - 1 for i in range(rows)]
+    batch = dev.LoraBatch(32, 3, 16)
+    batch.plan(_ints(*row_adapter))
+    handle = dev.SharedPrefixAttention(cache, 32)
+    cache.reserve(torch.tensor([[s, 1, c, 0] for s, c in zip(slots, ctx)], dtype=torch.int32, device="cuda"))
+    after = [c + 1 for c in ctx]
+    handle.plan(_ints(*slots), _ints(*after))
+    wq, wk = _random(d, seed=30), _random(d, seed=31)
+    # here the projections are plain products; in a step they are b200_qmm
+    qkv = (x.float() @ w_qkv.float().T).bfloat16()
+    adapters[0].apply(batch, x, qkv, out=qkv)
+    q, k, v = (t.unflatten(1, (-1, d)) for t in qkv.split((hq * d, hkv * d, hkv * d), 1))
+    turned = cache.norm_rope_append(0, q, k, v, _ints(*ctx), _ints(*slots), wq, wk)
+    got = handle.run(0, turned)
+    want, tol = _want(cache, 0, turned, slots, after)
+    _check(got, want, tol)
+    flat = got.flatten(1)
+    y = (flat.float() @ w_o.float().T).bfloat16()
+    out = adapters[1].apply(batch, flat, y)
+    for r, slot in enumerate(row_adapter):
+        if slot in pairs[1]:
+            a, b = pairs[1][slot]
+            delta = 0.5 * b @ (a @ flat[r].double())
+            assert bool(((out[r].double() - y[r].double() - delta).abs() <= 2.0 ** -8 * (y[r].double() + delta).abs() + 1e-5).all())
+            a, b = pairs[0][slot]
+        else:
+            assert torch.equal(out[r], y[r])
+    # the new key of a row is what the cache holds at its last place
+    rows_q, rows_k = dev.qk_norm_rope(q, k, _ints(*ctx), wq, wk)
+    assert torch.equal(rows_q, turned)
+    for r, s in enumerate(slots):
+        held_k, held_v = cache.gather(0, s)
+        assert torch.equal(held_k[-1], rows_k[r]) and torch.equal(held_v[-1], v[r])
+
+
+def test_what_is_refused():
+    from dmlx_b200 import _lib
+
+    lib, h = _lib.lib, C.c_void_p()
+    bad = _lib.ERR_INVALID_ARGUMENT
+    assert lib.b200_prefix_attn_create(None, 8, C.byref(h)) == bad and h.value is None
+    assert lib.b200_prefix_attn_create(None, 8, None) == bad
+    assert lib.b200_prefix_attn_plan(None, None, None, 0, None) == bad
+    assert lib.b200_prefix_attn_run(None, 0, None, 8, None, 8, None) == bad
+    lib.b200_prefix_attn_destroy(None)
+
+
+@pytest.mark.gpu
+def test_what_is_refused_of_a_handle():
+    from dmlx_b200 import _lib
+    from dmlx_b200 import device as dev
+
+    lib, bad, h = _lib.lib, _lib.ERR_INVALID_ARGUMENT, C.c_void_p()
+    cache = dev.PagedKVCache(2, 2, 64, 8, 4, 4, 8, max_rows=16)
+    for rows in (0, -1, 4097):
+        assert lib.b200_prefix_attn_create(cache._h, rows, C.byref(h)) == bad and h.value is None
+    for other in (dev.PagedKVCache(1, 1, 64, 8, 4, 4, 32, max_rows=16), dev.PagedKVCache(1, 2, 64, 8, 4, 4, 8, max_rows=16, kv_dtype=dev.KV_FP8_E4M3),
+                  dev.LayeredKVCache([(2, 64, 64)], 8, 4, 4, 8, max_rows=16)):
+        assert lib.b200_prefix_attn_create(other._h, 4, C.byref(h)) == _lib.ERR_UNSUPPORTED and h.value is None
+    handle = dev.SharedPrefixAttention(cache, 8)
+    x = torch.zeros((9, 1024), dtype=torch.bfloat16, device="cuda")
+    p, ints = x.data_ptr(), torch.zeros(9, dtype=torch.int32, device="cuda")
+    assert lib.b200_prefix_attn_run(handle._h, 0, p, 512, p, 512, None) == bad  # no plan yet
+    assert lib.b200_prefix_attn_plan(handle._h, ints.data_ptr(), ints.data_ptr(), 9, None) == _lib.ERR_CAPACITY
+    assert lib.b200_prefix_attn_plan(handle._h, None, ints.data_ptr(), 2, None) == bad
+    assert lib.b200_prefix_attn_plan(handle._h, ints.data_ptr(), None, 2, None) == bad
+    assert lib.b200_prefix_attn_plan(handle._h, ints.data_ptr(), ints.data_ptr(), -1, None) == bad
+    handle.plan(ints[:2], ints[:2])
+    for args in ((2, p, 512, p, 512), (-1, p, 512, p, 512), (0, None, 512, p, 512), (0, p, 512, None, 512), (0, p + 2, 512, p, 512), (0, p, 504, p, 512), (0, p, 516, p, 512),
+                 (0, p, 512, p + 8, 512), (0, p, 512, p, 448)):
+        assert lib.b200_prefix_attn_run(handle._h, *args, None) == bad, args
+    q = x[:2, :512].unflatten(1, (8, 64))
+    assert not bool(handle.run(0, q).any())
+    with pytest.raises(ValueError):
+        handle.run(0, x[:3, :512].unflatten(1, (8, 64)))
+    with pytest.raises(ValueError):
+        handle.run(0, q.float())
+    with pytest.raises(ValueError):
+        handle.plan(ints[:2].long(), ints[:2])
+    handle.plan(ints[:0], ints[:0])
+    assert handle.run(0, q[:0]).shape == (0, 8, 64)
