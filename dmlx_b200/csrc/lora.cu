@@ -1,19 +1,19 @@
 // Low-rank adapters of many requests beside a projection that they share: out[r] = y[r] + s_a B_a (A_a x[r]) with a = the row's adapter.
 //
-// The plan sorts a batch's rows by adapter and cuts each adapter's rows into tiles.  A cluster of eight CTAs takes a tile through both products
-// in one launch: its 64 warps share K between them for u = A x (f32), the parts are summed through distributed shared memory, and each CTA then
-// has all of u for its share of the N columns of y.  So u never goes to memory, a tile's x, y, A and B cross the chip once, and there is no second
-// launch to wait for.  A tile of a step that has few of them is given to several clusters, which all form u and share the columns.
+// The plan sorts a batch's rows by adapter and cuts each adapter's rows into tiles.  Then two kernels per projection:
+//   * down: an item is a tile and a quarter of K, u = A x in f32, a warp for 16 rows; the block that is the last of its tile adds the quarters up;
+//   * up: out = y + u B^T by steps of 32 rows of an adapter and 256 columns, of which every block has an equal share.
+// Both are bound by what they read and write once (x and A; y, B and out), so what they multiply comes through rings in shared memory, loads of later
+// items under way while the present one is multiplied (cp.async; the rows of a tile may lie anywhere).  The second kernel's blocks are on their SMs,
+// with y and B on the way, when the first one ends.
 //
-// The products run on mma.sync m16n8k16 with fragments straight from global memory: a lane loads 16 (or 8) neighbouring bytes of a row, which are
-// its places of the MMA's K in one or two steps (both operands agree on the order), and in the second product its places of N as well, so that it
-// holds eight neighbouring columns of y.  At ranks up to 64 a byte of x or y has fewer than 64 multiplications, an order below what would ask for
-// more than mma.sync.
+// The products run on mma.sync m16n8k16.  A lane takes 16 neighbouring bytes of a row of x as its places of K in two MMAs, four neighbouring ranks
+// as its places in one of the second product, and eight neighbouring columns of y as its places of N.  A, B and u lie in memory as the lanes take
+// them, so that a warp's share of an MMA is 512 contiguous bytes.  At ranks up to 64 a byte of x or y has fewer than 64 multiplications, an order
+// below what would ask for more than mma.sync.
 //
-// A row's u is summed in the same order whatever shares its tile: within a warp's 1/64 of K by the MMAs, then over the eight warps, then over the
-// eight CTAs.  It goes into the second product as two bf16 numbers (u - hi, exactly, and that rounded), which leaves 2^-17 of it, and the sum with
-// y is rounded once.
-#include <cooperative_groups.h>
+// A row's u is summed in the same order whatever shares its tile: 1/64 of K by the MMAs, sixteen of those, then the quarters.  It goes into the
+// second product as two bf16 numbers (u - hi, exactly, and that rounded), which leaves 2^-17 of it, and the sum with y is rounded once.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -23,47 +23,66 @@
 #include "launch.cuh"
 #include "ptx.cuh"
 
-namespace cg = cooperative_groups;
-
-// Adapters of one projection.  Rank rows are padded to rs (16, 32, 64 or 128).
+// Adapters of one projection.  Rank rows are padded to rs (16, 32, 64 or 128), k and n to 32, with zeros.
+//   a: [adapter][step of 32 of K][8 ranks][lane (g, t)] 16 bytes: rank g of the eight, K 8 t .. 8 t + 7 of the step
+//   b: [adapter][32 columns][16 ranks][2][lane (g, t)] 16 bytes, two halves of 8: half h of the i-th: column 8 (g / 2) + 2 (2 i + h) + g % 2, ranks 4 t .. 4 t + 3
 struct b200_lora {
   int n_adapters = 0, n = 0, k = 0, max_rank = 0, rs = 0;
-  __nv_bfloat16 *a = nullptr, *b = nullptr;  // [adapter][rs][k], [adapter][n][rs]
-  int* rank = nullptr;                       // [adapter], 0: none
+  uint4 *a = nullptr, *b = nullptr;
+  int* rank = nullptr;  // [adapter], 0: none
   float* scale = nullptr;
+  size_t a_units() const { return (size_t)(k + 31) / 32 * rs * 4; }  // of 16 bytes, of an adapter
+  size_t b_units() const { return (size_t)(n + 31) / 32 * rs * 4; }
 };
 
-// The rows of a step by adapter: order[max_rows], tiles of {adapter or -1, first place in order, rows, -}, header {tiles}.
+// The rows of a step by adapter: order[max_rows]; tiles of {adapter or -1, first place in order, rows, first slot} (those of many rows from the front
+// on, those of few from the back); groups of 32 rows of an adapter {adapter, first place, rows, -}, each two slots of 16; header {tiles of many rows,
+// groups, tiles of few, error word}.  And what goes from the first product to the second.
 struct b200_lora_batch {
   int max_rows = 0, max_adapters = 0, max_rank = 0, max_tiles = 0, rows = -1;
   int* order = nullptr;
   int4* tiles = nullptr;
   int* hdr = nullptr;
+  int4* groups = nullptr;   // [max_tiles]
+  int* done = nullptr;      // [max_tiles] quarters of a tile that are there
+  float* parts = nullptr;   // [quarter][max_rows][rank rows]
+  uint32_t* u = nullptr;    // [slot][16 ranks][hi, lo][lane (g, t)] rows g and g + 8, ranks 4 t and 4 t + 1, then the same of 4 t + 2 and 4 t + 3
 };
 
 namespace {
 
-constexpr int kCluster = 8, kWarps = 8, kThreads = kWarps * 32;
-constexpr int kMaxAdapters = 4096, kMaxRank = 128;
-constexpr int kEnoughTiles = 72;  // about twice the clusters that run at a time: beyond that, larger tiles rather than more of them
+constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr int kSlices = 4;        // of K
+constexpr int kFewRows = 16;      // of a tile whose slice of K the warps of a block share
+constexpr int kMaxAdapters = 4096, kMaxRank = 128, kTileRows = 128, kGroupRows = 32;
+constexpr int kEnoughTiles = 74;  // half the SMs (a tile is four items of the first product): beyond that, larger tiles rather than more of them
 
-__host__ __device__ constexpr int most_tile_rows(int rs) { return rs > 64 ? 64 : 128; }
+int rank_rows(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
 
 // ---- the plan ------------------------------------------------------------------------------------------------------
-__global__ void __launch_bounds__(1024) lora_plan_kernel(const int* row_adapter, int rows, int n_adapters, int most_rows, int* __restrict__ order,
-                                                         int4* __restrict__ tiles, int* __restrict__ hdr) {
+// Places, tiles and groups are handed out as the atomics come: no row's result depends on its place, its tile or its block.
+__global__ void __launch_bounds__(1024) lora_plan_kernel(const int* row_adapter, int rows, int n_adapters, int max_tiles, int* __restrict__ order,
+                                                         int4* __restrict__ tiles, int4* __restrict__ groups, int* __restrict__ hdr) {
   after_previous();
-  __shared__ int count[kMaxAdapters + 1], warp_sums[32], total[4], carry[2];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bins = n_adapters + 1;
+  __shared__ int count[kMaxAdapters + 1], total[4], next[4];  // next: place, group, tile of many rows, tile of few
+  const int tid = threadIdx.x, lane = tid & 31, bins = n_adapters + 1;
   for (int i = tid; i < bins; i += blockDim.x) count[i] = 0;
-  if (tid < 4) total[tid] = 0;
-  if (tid < 2) carry[tid] = 0;
+  if (tid < 4) total[tid] = next[tid] = 0;
   __syncthreads();
-  auto bin = [&](int r) {
-    const int a = row_adapter[r];
-    return a >= 0 && a < n_adapters ? a : n_adapters;
+  // Adds one to the count of each lane's adapter (prompts are runs of one, so lanes with the same one add together); the count before, for this lane.
+  auto count_rows = [&](int r) {
+    int b = -1;
+    if (r < rows) {
+      const int a = row_adapter[r];
+      b = a >= 0 && a < n_adapters ? a : n_adapters;
+    }
+    const unsigned same = __match_any_sync(0xffffffffu, b);
+    const int first = __ffs(same) - 1;
+    int before = 0;
+    if (lane == first && b >= 0) before = atomicAdd(&count[b], __popc(same));
+    return __shfl_sync(0xffffffffu, before, first) + __popc(same & ((1u << lane) - 1));
   };
-  for (int r = tid; r < rows; r += blockDim.x) atomicAdd(&count[bin(r)], 1);
+  for (int base = 0; base < rows; base += blockDim.x) count_rows(base + tid);
   __syncthreads();
   int mine[4] = {0, 0, 0, 0};  // tiles of 16, 32, 64, 128 rows
   for (int i = tid; i < bins; i += blockDim.x) {
@@ -77,50 +96,42 @@ __global__ void __launch_bounds__(1024) lora_plan_kernel(const int* row_adapter,
   }
   __syncthreads();
   int shift = 4;
-  while ((1 << shift) < most_rows && total[shift - 4] > kEnoughTiles) ++shift;
-  // places of each adapter's rows and tiles: a scan over the bins
-  for (int base = 0; base < bins; base += blockDim.x) {
-    const int i = base + tid, c = i < bins ? count[i] : 0, t = (c + (1 << shift) - 1) >> shift;
-    int ic = c, it = t;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int uc = __shfl_up_sync(0xffffffffu, ic, o), ut = __shfl_up_sync(0xffffffffu, it, o);
-      if (lane >= o) { ic += uc; it += ut; }
+  while ((1 << shift) < kTileRows && total[shift - 4] > kEnoughTiles) ++shift;
+  for (int i = tid; i < bins; i += blockDim.x) {
+    const int c = count[i];
+    if (c == 0) continue;
+    const int adapter = i < n_adapters ? i : -1, first = atomicAdd(&next[0], c), group = atomicAdd(&next[1], (c + kGroupRows - 1) / kGroupRows);
+    for (int j = 0; j < c; j += kGroupRows) groups[group + j / kGroupRows] = make_int4(adapter, first + j, min(kGroupRows, c - j), 0);
+    for (int j = 0; j < c; j += 1 << shift) {
+      const int n = min(1 << shift, c - j);
+      const int at = n > kFewRows ? atomicAdd(&next[2], 1) : max_tiles - 1 - atomicAdd(&next[3], 1);
+      tiles[at] = make_int4(adapter, first + j, n, group * (kGroupRows / 16) + j / 16);
     }
-    if (lane == 31) warp_sums[warp] = ic;
-    __syncthreads();
-    int before_c = carry[0], before_t = carry[1];
-    for (int w = 0; w < warp; ++w) before_c += warp_sums[w];
-    __syncthreads();
-    if (lane == 31) warp_sums[warp] = it;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) before_t += warp_sums[w];
-    const int first = before_c + ic - c;
-    if (i < bins) {
-      for (int j = 0; j < t; ++j) tiles[before_t + it - t + j] = make_int4(i < n_adapters ? i : -1, first + (j << shift), min(1 << shift, c - (j << shift)), 0);
-      count[i] = first;
-    }
-    __syncthreads();
-    if (tid == (int)blockDim.x - 1) { carry[0] = before_c + ic; carry[1] = before_t + it; }
-    __syncthreads();
+    count[i] = first;
   }
-  // (rows of an adapter in any order: no row's result depends on its place)
-  for (int r = tid; r < rows; r += blockDim.x) order[atomicAdd(&count[bin(r)], 1)] = r;
-  if (tid == 0) hdr[0] = carry[1];
+  __syncthreads();
+  for (int base = 0; base < rows; base += blockDim.x) {
+    const int at = count_rows(base + tid);
+    if (base + tid < rows) order[at] = base + tid;
+  }
+  if (tid == 0) { hdr[0] = next[2]; hdr[1] = next[1]; hdr[2] = next[3]; }
 }
 
 // ---- the products ---------------------------------------------------------------------------------------------------
 struct LoraArgs {
-  const __nv_bfloat16 *a, *b, *x, *y;
+  const uint4 *a, *b;
+  const __nv_bfloat16 *x, *y;
   __nv_bfloat16* out;
   const int* rank;
   const float* scale;
   const int* order;
-  const int4* tiles;
+  const int4 *tiles, *groups;
   const int* hdr;
-  int n_adapters, n, k, rows;
+  int *done, *err;
+  float* parts;
+  uint32_t* u;
+  int max_rows, max_tiles, n, k;
   int x_stride, y_stride, out_stride;
-  int most_parts;  // clusters that may share a tile's columns
 };
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -136,225 +147,324 @@ __device__ __forceinline__ float rest(float u) {
   const float hi = __bfloat162float(__float2bfloat16(u));
   return isfinite(hi) ? u - hi : 0.f;
 }
+// 16 bytes to shared memory, zeros where there is nothing to copy.
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_groups() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
 
+// ---- down: rings of chunks of 64 of K, a chunk [128 rows of x][128 bytes], 16-byte pieces of odd rows exchanged in halves, then A's -----------------
 template <int RS>
-struct Shape {
-  static constexpr int TM = most_tile_rows(RS), RC = RS > 64 ? 64 : RS, NT = RC / 8, KS = RS / 16;
-  static constexpr int MG = RS > 32 ? 1 : 2;          // groups of 16 rows at a time: registers
-  static constexpr int PAD = RC + 8, UPAD = RS + 8;   // strides without bank conflicts
-  static constexpr int kPart = kWarps * MG * 16 * PAD * 4, kHalves = 2 * TM * UPAD * 2;
-  static constexpr int kShared = (kPart > kHalves ? kPart : kHalves) + TM * RS * 4 + TM * 4;
+struct Down {
+  static constexpr int NT = RS / 8, CHUNK = (kTileRows + RS) * 128;
+  static constexpr int STAGES = RS == 64 ? 4 : RS > 64 ? 6 : 5, PER_SM = RS > 64 ? 1 : 2;
+  static constexpr int kShared = STAGES * CHUNK;
 };
 
 template <int RS>
-__global__ void __launch_bounds__(kThreads, 2) lora_kernel(const __grid_constant__ LoraArgs a) {
+__global__ void __launch_bounds__(kThreads, Down<RS>::PER_SM) lora_down_kernel(const __grid_constant__ LoraArgs a) {
   after_previous();
-  using Z = Shape<RS>;
-  extern __shared__ __align__(16) unsigned char smem[];
-  float* part = reinterpret_cast<float*>(smem);                       // [warp][row of the round][PAD]
-  __nv_bfloat16* halves = reinterpret_cast<__nv_bfloat16*>(smem);     // [hi, lo][row][UPAD], when the parts have been summed
-  float* u = reinterpret_cast<float*>(smem + (Z::kPart > Z::kHalves ? Z::kPart : Z::kHalves));  // [row][RS]: this CTA's share of K
-  int* row_of = reinterpret_cast<int*>(u + Z::TM * RS);
-  cg::cluster_group cluster = cg::this_cluster();
-  const int cta = cluster.block_rank(), clusters = gridDim.x / kCluster, me = blockIdx.x / kCluster;
+  using Z = Down<RS>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ int s_last;
+  const uint32_t ring = ptx::smem_u32(smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int n_tiles = a.hdr[0];
-  const int parts = max(1, min(a.most_parts, clusters / max(n_tiles, 1)));
-  const int each = (a.k + 64 * 32 - 1) / (64 * 32) * 32;  // a warp's share of K
-  const int k0 = (cta * kWarps + warp) * each, k1 = min(a.k, k0 + each);
+  const int n_items = a.hdr[0] * kSlices, n_few = a.hdr[2] * kSlices;
+  const int each = (a.k + 64 * 32 - 1) / (64 * 32) * 32, per_slice = 64 / kSlices * each, k_steps = (a.k + 31) / 32;  // 1/64 of K; a slice of it
 
-  for (int item = me; item < n_tiles * parts; item += clusters) {
-    const int4 tile = a.tiles[item / parts];
-    const int share = item % parts, count = tile.z, groups = (count + 15) / 16;
-    const int rank = tile.x >= 0 ? min(a.rank[tile.x], RS) : 0, rk = (rank + 15) / 16 * 16;
-    if (rank == 0 && a.out == a.y) continue;  // (the whole cluster)
-    for (int i = tid; i < Z::TM; i += kThreads) row_of[i] = i < count ? a.order[tile.y + i] : -1;
+  // The last block of a tile to come here adds its quarters up, times the scale.  Ranks that are padding have no part in it, whatever x holds.
+  auto finish = [&](int tile_at, const int4& tile) {
+    __threadfence();
     __syncthreads();
-    // ---- u: this warp's part of K, round by round of MG * 16 rows ----
-    if (rank > 0) {
-      const float scale = a.scale[tile.x];
-      for (int c0 = 0; c0 < rk; c0 += Z::RC) {
-        const __nv_bfloat16* aw = a.a + ((size_t)tile.x * RS + c0) * a.k;
-        const int nts = min(Z::NT, (rk - c0) / 8);
-        for (int m0 = 0; m0 < groups; m0 += Z::MG) {
-          float acc[Z::MG][Z::NT][4];
+    if (tid == 0) s_last = atomicAdd(&a.done[tile_at], 1) == kSlices - 1;
+    __syncthreads();
+    if (!s_last) return;
+    __threadfence();
+    const int rank = min(a.rank[tile.x], RS), per_row = (rank + 15) / 16 * 4;
+    const float scale = a.scale[tile.x];
+    for (int i = tid; i < tile.z * per_row; i += kThreads) {
+      const int row = i / per_row, c = (i - row * per_row) * 4;
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
+      float4 v[kSlices];
 #pragma unroll
-          for (int m = 0; m < Z::MG; ++m)
+      for (int q = 0; q < kSlices; ++q) v[q] = __ldcg(reinterpret_cast<const float4*>(a.parts + ((size_t)q * a.max_rows + tile.y + row) * RS + c));
 #pragma unroll
-            for (int j = 0; j < Z::NT; ++j) acc[m][j][0] = acc[m][j][1] = acc[m][j][2] = acc[m][j][3] = 0.f;
-          const __nv_bfloat16* xr[Z::MG][2];
+      for (int q = 0; q < kSlices; ++q) { s[0] += v[q].x; s[1] += v[q].y; s[2] += v[q].z; s[3] += v[q].w; }
 #pragma unroll
-          for (int m = 0; m < Z::MG; ++m)
+      for (int e = 0; e < 4; ++e) s[e] = c + e < rank ? s[e] * scale : 0.f;
+      uint32_t* to = a.u + ((((size_t)(tile.w + row / 16) * (RS / 16) + c / 16) * 2) * 32 + row % 8 * 4 + c % 16 / 4) * 4 + row % 16 / 8;
+      to[0] = pack(s[0], s[1]);
+      to[2] = pack(s[2], s[3]);
+      to[128] = pack(rest(s[0]), rest(s[1]));
+      to[130] = pack(rest(s[2]), rest(s[3]));
+    }
+    if (tid == 0) a.done[tile_at] = 0;
+  };
+
+  // ---- loads, ahead of the products and across items: this thread copies piece `piece` of rows row0, row0 + 32, ... ----
+  const int piece = tid & 7, row0 = tid >> 3;
+  const uint32_t x_to = ring + row0 * 128 + ((piece ^ ((row0 & 1) << 2)) << 4);
+  struct Cursor { int item, chunk, chunks, k0, rk; int4 tile; };
+  Cursor lc{};
+  const __nv_bfloat16* xp[kTileRows / 32];  // null: no such row
+  const uint4* ap = nullptr;
+  auto enter = [&](Cursor& c, int item) {  // the next item from `item` on that has something to do
+    for (;; item += gridDim.x) {
+      c.item = item;
+      if (item >= n_items) return;
+      c.tile = a.tiles[item / kSlices];
+      c.chunk = 0;
+      c.rk = c.tile.x >= 0 ? (min(a.rank[c.tile.x], RS) + 15) / 16 * 16 : 0;
+      c.k0 = item % kSlices * per_slice;
+      c.chunks = max(1, (min(a.k - c.k0, per_slice) + 63) / 64);
+      if (c.rk > 0) return;
+    }
+  };
+  auto enter_loads = [&](int item) {
+    enter(lc, item);
+    if (lc.item >= n_items) return;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int at = (m0 + m) * 16 + h * 8 + g, r = at < Z::TM ? row_of[at] : -1;
-              xr[m][h] = r >= 0 ? a.x + (size_t)r * a.x_stride : nullptr;
-            }
-#pragma unroll 2
-          for (int kk = k0 + 8 * t; kk - 8 * t < k1; kk += 32) {
-            const bool in = kk < k1;
-            const uint4 zero = make_uint4(0, 0, 0, 0);
-            uint4 xv[Z::MG][2], av[Z::NT];
+    for (int i = 0; i < kTileRows / 32; ++i) xp[i] = row0 + 32 * i < lc.tile.z ? a.x + (size_t)a.order[lc.tile.y + row0 + 32 * i] * a.x_stride + lc.k0 + piece * 8 : nullptr;
+    ap = a.a + ((size_t)lc.tile.x * k_steps + lc.k0 / 32) * (RS * 4);
+  };
+  uint32_t issued = 0, used = 0, load_slot = 0, use_slot = 0;
+  auto issue = [&]() {
+    if (lc.item < n_items) {
+      const int k = lc.chunk * 64;
+      const bool in = lc.k0 + k + piece * 8 < a.k;
+      const uint32_t to = load_slot * Z::CHUNK;
 #pragma unroll
-            for (int m = 0; m < Z::MG; ++m)
+      for (int i = 0; i < kTileRows / 32; ++i)
+        if (xp[i]) copy16(x_to + to + i * 32 * 128, in ? xp[i] + k : a.x, in);
 #pragma unroll
-              for (int h = 0; h < 2; ++h) xv[m][h] = in && xr[m][h] ? *reinterpret_cast<const uint4*>(xr[m][h] + kk) : zero;
+      for (int i = tid; i < RS * 8; i += kThreads)  // two steps of [8 ranks][lane]
+        if (i % (RS * 4) < lc.rk * 4) copy16(ring + to + kTileRows * 128 + i * 16, lc.k0 / 32 + lc.chunk * 2 + i / (RS * 4) < k_steps ? ap + lc.chunk * (RS * 8) + i : a.a, lc.k0 / 32 + lc.chunk * 2 + i / (RS * 4) < k_steps);
+      if (++lc.chunk == lc.chunks) enter_loads(lc.item + gridDim.x);
+    }
+    commit();
+    ++issued;
+    if (++load_slot == Z::STAGES) load_slot = 0;
+  };
+  enter_loads(blockIdx.x);
+  if (lc.item < n_items)
+    for (int i = 0; i < Z::STAGES - 1; ++i) issue();
+
+  Cursor c{};
+  for (enter(c, blockIdx.x); c.item < n_items; enter(c, c.item + gridDim.x)) {
+    float acc[Z::NT][4], sum[Z::NT][4];
 #pragma unroll
-            for (int j = 0; j < Z::NT; ++j) av[j] = in && j < nts ? *reinterpret_cast<const uint4*>(aw + (size_t)(j * 8 + g) * a.k + kk) : zero;
+    for (int j = 0; j < Z::NT; ++j)
 #pragma unroll
-            for (int j = 0; j < Z::NT; ++j) {
-              if (j >= nts) continue;
+      for (int e = 0; e < 4; ++e) acc[j][e] = sum[j][e] = 0.f;
+    const bool works = warp * 16 < c.tile.z;
+    const int nts = c.rk / 8, steps = each / 32;
+    int within = 0;
+    for (int chunk = 0; chunk < c.chunks; ++chunk) {
+      wait_groups<Z::STAGES - 2>();
+      __syncthreads();  // (the chunk is there, and the one before it has been used)
+      issue();
+      const uint32_t stage = ring + use_slot * Z::CHUNK, xa = stage + (warp * 16 + g) * 128, aw = stage + kTileRows * 128 + lane * 16;
+      if (++use_slot == Z::STAGES) use_slot = 0;
+      ++used;
+      if (!works) continue;
 #pragma unroll
-              for (int m = 0; m < Z::MG; ++m) {
-                mma(acc[m][j], xv[m][0].x, xv[m][1].x, xv[m][0].y, xv[m][1].y, av[j].x, av[j].y);
-                mma(acc[m][j], xv[m][0].z, xv[m][1].z, xv[m][0].w, xv[m][1].w, av[j].z, av[j].w);
-              }
-            }
-          }
-          float* mine = part + warp * Z::MG * 16 * Z::PAD;
+      for (int s = 0; s < 2; ++s) {
+        const uint32_t at = (uint32_t)((s * 4 + t) ^ ((g & 1) << 2)) << 4;
+        const uint4 va = lds16(xa + at), vb = lds16(xa + 8 * 128 + at);
 #pragma unroll
-          for (int m = 0; m < Z::MG; ++m)
-#pragma unroll
-            for (int j = 0; j < Z::NT; ++j) {
-              *reinterpret_cast<float2*>(mine + (m * 16 + g) * Z::PAD + j * 8 + 2 * t) = make_float2(acc[m][j][0], acc[m][j][1]);
-              *reinterpret_cast<float2*>(mine + (m * 16 + 8 + g) * Z::PAD + j * 8 + 2 * t) = make_float2(acc[m][j][2], acc[m][j][3]);
-            }
-          __syncthreads();
-          for (int i = tid; i < Z::MG * 16 * (Z::RC / 4); i += kThreads) {
-            const int row = i / (Z::RC / 4), c = i % (Z::RC / 4) * 4;
-            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-              const float4 v = *reinterpret_cast<const float4*>(part + (w * Z::MG * 16 + row) * Z::PAD + c);
-              s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
-            }
-            if (m0 * 16 + row < Z::TM) *reinterpret_cast<float4*>(u + (m0 * 16 + row) * RS + c0 + c) = s;
-          }
-          __syncthreads();
+        for (int j = 0; j < Z::NT; ++j) {
+          if (j >= nts) continue;
+          const uint4 w = lds16(aw + (s * Z::NT + j) * 512);
+          mma(acc[j], va.x, vb.x, va.y, vb.y, w.x, w.y);
+          mma(acc[j], va.z, vb.z, va.w, vb.w, w.z, w.w);
         }
-      }
-      // ---- the cluster's sum, as two bf16 numbers ----
-      const int per_row = rk / 4, quads = groups * 16 * per_row;
-      auto sum_of = [&](int i, uint2& hi, uint2& lo) {
-        const int row = i / per_row, c = (i - row * per_row) * 4;
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        if (++within == steps) {  // 1/64 of K is complete
+          within = 0;
 #pragma unroll
-        for (int r = 0; r < kCluster; ++r) {
-          const float4 v = *reinterpret_cast<const float4*>(cluster.map_shared_rank(u, r) + row * RS + c);
-          s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
-        }
+          for (int j = 0; j < Z::NT; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] = c + e < rank ? s[e] * scale : 0.f;  // (a padded rank has no part in it, whatever x holds)
-        hi = make_uint2(pack(s[0], s[1]), pack(s[2], s[3]));
-        lo = make_uint2(pack(rest(s[0]), rest(s[1])), pack(rest(s[2]), rest(s[3])));
-        return row * Z::UPAD + c;
-      };
-      cluster.sync();
-      const bool few = quads <= 512;
-      if (few) {  // every CTA sums all of it; nobody writes his share of K again before all have read it (below)
-        for (int i = tid; i < quads; i += kThreads) {
-          uint2 hi, lo;
-          const int at = sum_of(i, hi, lo);
-          *reinterpret_cast<uint2*>(halves + at) = hi;
-          *reinterpret_cast<uint2*>(halves + Z::TM * Z::UPAD + at) = lo;
+            for (int e = 0; e < 4; ++e) { sum[j][e] += acc[j][e]; acc[j][e] = 0.f; }
         }
-        __syncthreads();
-      } else {    // every CTA sums an eighth and hands it to all
-        const int from = (int)((long long)quads * cta / kCluster), to = (int)((long long)quads * (cta + 1) / kCluster);
-        for (int i = from + tid; i < to; i += kThreads) {
-          uint2 hi, lo;
-          const int at = sum_of(i, hi, lo);
-#pragma unroll
-          for (int r = 0; r < kCluster; ++r) {
-            __nv_bfloat16* there = cluster.map_shared_rank(halves, r);
-            *reinterpret_cast<uint2*>(there + at) = hi;
-            *reinterpret_cast<uint2*>(there + Z::TM * Z::UPAD + at) = lo;
-          }
-        }
-        cluster.sync();
       }
     }
-    // ---- out = y + u B^T: 32 columns a warp at a time; lane (g, t) has columns 8 t .. 8 t + 7 of rows g and g + 8 ----
-    const int chunks = (a.n + 31) / 32, ks = rk / 16;
-    for (int c = (share * kCluster + cta) * kWarps + warp; c < chunks; c += parts * kCluster * kWarps) {
-      uint2 bv[4][Z::KS];  // MMA column g of n-tile j is column 8 (g / 2) + 2 j + g % 2
-      const int n_lane = c * 32 + 8 * (g >> 1) + (g & 1);
+    if (works) {
+      float* parts = a.parts + ((size_t)(c.item % kSlices) * a.max_rows + c.tile.y) * RS;
+      const int ra = warp * 16 + g, rb = ra + 8;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < Z::NT; ++j) {
+        if (j >= nts) continue;
+        // (the last 1/64 of K may be cut short by the end of it)
+        if (ra < c.tile.z) *reinterpret_cast<float2*>(parts + (size_t)ra * RS + j * 8 + 2 * t) = make_float2(sum[j][0] + acc[j][0], sum[j][1] + acc[j][1]);
+        if (rb < c.tile.z) *reinterpret_cast<float2*>(parts + (size_t)rb * RS + j * 8 + 2 * t) = make_float2(sum[j][2] + acc[j][2], sum[j][3] + acc[j][3]);
+      }
+    }
+    finish(c.item / kSlices, c.tile);
+  }
+  wait_groups<0>();
+  __syncthreads();
+  // ---- tiles of few rows: the warps share the slice, straight from memory; the sums of its 1/64s of K are ... ----
+  constexpr int SHARE = 64 / kSlices / kWarps, PAD = RS + 8;  // 1/64s of a warp; floats between rows of their sums, [1/64][row][PAD] in place of the ring
+  float* sums = reinterpret_cast<float*>(smem);
+  for (int item = blockIdx.x + (n_items + gridDim.x - 1 - blockIdx.x) / gridDim.x * gridDim.x; item < n_items + n_few; item += gridDim.x) {
+    const int tile_at = a.max_tiles - 1 - (item - n_items) / kSlices, slice = (item - n_items) % kSlices;
+    const int4 tile = a.tiles[tile_at];
+    const int rank = tile.x >= 0 ? min(a.rank[tile.x], RS) : 0, nts = (rank + 15) / 16 * 2;
+    if (rank == 0) continue;
+    const bool on_a = g < tile.z, on_b = g + 8 < tile.z;
+    const __nv_bfloat16 *xa = a.x + (size_t)(on_a ? a.order[tile.y + g] : 0) * a.x_stride, *xb = a.x + (size_t)(on_b ? a.order[tile.y + 8 + g] : 0) * a.x_stride;
+    const uint4* aw = a.a + (size_t)tile.x * k_steps * (RS * 4) + lane;
+    auto load16 = [](const __nv_bfloat16* p, bool there) { return there ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0); };
+#pragma unroll(RS > 32 ? 1 : SHARE)
+    for (int i = 0; i < SHARE; ++i) {
+      const int part = warp * SHARE + i, k0 = slice * per_slice + part * each, k1 = min(a.k, k0 + each);
+      float acc[Z::NT][4];
 #pragma unroll
-        for (int s = 0; s < Z::KS; ++s)
-          bv[j][s] = s < ks && n_lane + 2 * j < a.n ? *reinterpret_cast<const uint2*>(a.b + ((size_t)tile.x * a.n + n_lane + 2 * j) * RS + s * 16 + 4 * t) : make_uint2(0, 0);
-      const int col = c * 32 + 8 * t;
-      auto load_y = [&](int m, uint4 (&v)[2]) {
+      for (int j = 0; j < Z::NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+#pragma unroll(RS > 32 ? 1 : 2)
+      for (int kk = k0; kk < k1; kk += 32) {
+        const bool in = kk + 8 * t < k1;
+        const uint4 va = load16(xa + kk + 8 * t, in && on_a), vb = load16(xb + kk + 8 * t, in && on_b);
+        uint4 w[Z::NT];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = m < groups ? row_of[m * 16 + h * 8 + g] : -1;
-          v[h] = r >= 0 && col < a.n ? *reinterpret_cast<const uint4*>(a.y + (size_t)r * a.y_stride + col) : make_uint4(0, 0, 0, 0);
+        for (int j = 0; j < Z::NT; ++j) w[j] = j < nts ? aw[(size_t)(kk / 32) * (RS * 4) + j * 32] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < Z::NT; ++j) {
+          if (j >= nts) continue;
+          mma(acc[j], va.x, vb.x, va.y, vb.y, w[j].x, w[j].y);
+          mma(acc[j], va.z, vb.z, va.w, vb.w, w[j].z, w[j].w);
         }
-      };
-      uint4 next[2];
-      load_y(0, next);
-      for (int m = 0; m < groups; ++m) {
-        uint4 yv[2] = {next[0], next[1]};
-        load_y(m + 1, next);
+      }
+      float* mine = sums + part * 16 * PAD;
+#pragma unroll
+      for (int j = 0; j < Z::NT; ++j) {
+        *reinterpret_cast<float2*>(mine + g * PAD + j * 8 + 2 * t) = make_float2(acc[j][0], acc[j][1]);
+        *reinterpret_cast<float2*>(mine + (8 + g) * PAD + j * 8 + 2 * t) = make_float2(acc[j][2], acc[j][3]);
+      }
+    }
+    __syncthreads();
+    // ... added in the order in which a warp by itself comes to them
+    for (int i = tid; i < tile.z * (RS / 4); i += kThreads) {
+      const int row = i / (RS / 4), e = i % (RS / 4) * 4;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int part = 0; part < 64 / kSlices; ++part) {
+        const float4 w = *reinterpret_cast<const float4*>(sums + (part * 16 + row) * PAD + e);
+        v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+      }
+      *reinterpret_cast<float4*>(a.parts + ((size_t)slice * a.max_rows + tile.y + row) * RS + e) = v;
+    }
+    finish(tile_at, tile);
+  }
+}
+
+// ---- up: 32 columns for a warp, steps of 32 rows ------------------------------------------------------------------------------------------------------
+// Its part of B stays in registers; lane (g, t) has columns 8 t .. 8 t + 7 of rows g and g + 8.  The warps of a block take neighbouring columns, so what
+// they read of y is contiguous and u comes from their L1.  Nothing passes through shared memory: with y by cp.async, u and B in bulk and warps for
+// that alone, those warps' issue was what everything waited for (1850 cycles for 32 rows of 256 columns, 1140 for their products).
+template <int RS>
+struct Up {
+  static constexpr int KS = RS / 16, COLS = kWarps * 32, PER_SM = RS == 16 ? 4 : RS == 32 ? 3 : RS == 64 ? 2 : 1;
+};
+
+// (Everything but u was there when the kernel ahead began, and that one lets this one start behind its own wait: only u is waited for.)
+template <int RS>
+__global__ void __launch_bounds__(kThreads, Up<RS>::PER_SM) lora_up_kernel(const __grid_constant__ LoraArgs a) {
+  using Z = Up<RS>;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int groups = a.hdr[1], col_blocks = (a.n + Z::COLS - 1) / Z::COLS, n_blocks = (a.n + 31) / 32;
+  const long long all = (long long)groups * col_blocks;
+  const int begin = (int)(all * blockIdx.x / gridDim.x), end = (int)(all * (blockIdx.x + 1) / gridDim.x);
+  if (begin < end) {
+    int block = begin / groups, at = begin - block * groups;  // range of columns, group
+    int4 group = a.groups[at];                                // {adapter, first place, rows, -}
+    auto row_of = [&](const int4& gr, int r) { return r < gr.z ? a.order[gr.y + r] : -1; };
+    auto load_y = [&](int row, int col) { return row >= 0 && col < a.n ? *reinterpret_cast<const uint4*>(a.y + (size_t)row * a.y_stride + col) : make_uint4(0, 0, 0, 0); };
+    int rows[2] = {row_of(group, g), row_of(group, g + 8)};
+    uint4 next[2] = {load_y(rows[0], (block * kWarps + warp) * 32 + 8 * t), load_y(rows[1], (block * kWarps + warp) * 32 + 8 * t)};
+    uint4 bv[Z::KS][2];
+    int c_block = -1, c_adapter = -1, ks = 0;
+    bool waited = false;
+    for (int s = begin; s < end; ++s) {
+      const int nb = block * kWarps + warp, col = nb * 32 + 8 * t, slot = at * (kGroupRows / 16);
+      const int4 now = group;
+      if (block != c_block || now.x != c_adapter) {
+        c_block = block; c_adapter = now.x;
+        ks = now.x >= 0 ? (min(a.rank[now.x], RS) + 15) / 16 : 0;
+        const uint4* bp = a.b + ((size_t)max(now.x, 0) * n_blocks + min(nb, n_blocks - 1)) * Z::KS * 64 + lane;
+#pragma unroll
+        for (int k = 0; k < Z::KS; ++k)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) bv[k][i] = k < ks ? bp[(k * 2 + i) * 32] : make_uint4(0, 0, 0, 0);
+      }
+      if (++at == groups) { at = 0; ++block; }
+      if (s + 1 < end) group = a.groups[at];
+      if (!waited) { after_previous(); waited = true; }
+#pragma unroll
+      for (int m = 0; m < kGroupRows; m += 16) {
+        const int to[2] = {rows[0], rows[1]};
+        const uint4 old[2] = {next[0], next[1]};
+        if (m + 16 < kGroupRows && m + 16 < now.z) {  // the next rows: of this group, or of the next one
+#pragma unroll
+          for (int h = 0; h < 2; ++h) { rows[h] = row_of(now, m + 16 + 8 * h + g); next[h] = load_y(rows[h], col); }
+        } else if (m < now.z) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) { rows[h] = s + 1 < end ? row_of(group, 8 * h + g) : -1; next[h] = load_y(rows[h], (block * kWarps + warp) * 32 + 8 * t); }
+        }
+        if (m >= now.z || (ks == 0 && a.out == a.y)) continue;
         float acc[4][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-        const __nv_bfloat16* ur = halves + (m * 16 + g) * Z::UPAD + 4 * t;
+        const uint4* up = reinterpret_cast<const uint4*>(a.u) + (size_t)(slot + m / 16) * Z::KS * 64 + lane;
 #pragma unroll
-        for (int s = 0; s < Z::KS; ++s) {
-          if (s >= ks) continue;
+        for (int k = 0; k < Z::KS; ++k) {
+          if (k >= ks) continue;
+          const uint4 u[2] = {__ldca(up + (k * 2) * 32), __ldca(up + (k * 2 + 1) * 32)};
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint2 up = *reinterpret_cast<const uint2*>(ur + half * Z::TM * Z::UPAD + s * 16);
-            const uint2 down = *reinterpret_cast<const uint2*>(ur + half * Z::TM * Z::UPAD + 8 * Z::UPAD + s * 16);
+          for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) mma(acc[j], up.x, down.x, up.y, down.y, bv[j][s].x, bv[j][s].y);
-          }
+            for (int i = 0; i < 2; ++i) {
+              mma(acc[2 * i], u[half].x, u[half].y, u[half].z, u[half].w, bv[k][i].x, bv[k][i].y);
+              mma(acc[2 * i + 1], u[half].x, u[half].y, u[half].z, u[half].w, bv[k][i].z, bv[k][i].w);
+            }
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int r = row_of[m * 16 + h * 8 + g];
-          if (r < 0 || col >= a.n) continue;
-          uint4 o = yv[h];
-          if (rank > 0) {
+          if (to[h] < 0 || col >= a.n) continue;
+          uint4 o = old[h];
+          if (ks > 0) {
             uint32_t* w = reinterpret_cast<uint32_t*>(&o);
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = pack(ptx::bf16_lo(w[j]) + acc[j][2 * h], ptx::bf16_hi(w[j]) + acc[j][2 * h + 1]);
           }
-          *reinterpret_cast<uint4*>(a.out + (size_t)r * a.out_stride + col) = o;
+          *reinterpret_cast<uint4*>(a.out + (size_t)to[h] * a.out_stride + col) = o;
         }
       }
+      if ((block != c_block || group.x != c_adapter) && group.x >= 0 && block * kWarps + warp < n_blocks && lane < RS / 2)  // the next step's B on its way to L2
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(a.b + ((size_t)group.x * n_blocks + block * kWarps + warp) * Z::KS * 64 + lane * 8));
     }
-    if (rank > 0) cluster.sync();  // (another CTA may still be reading this one's u)
-    else __syncthreads();
+  } else {
+    after_previous();
   }
 }
 
 template <int RS>
 b200_status launch(LoraArgs& a, int max_tiles, cudaStream_t s) {
-  using Z = Shape<RS>;
-  static int resident = 0;  // clusters that run at a time
-  if (resident == 0) {
-    B200_CUDA_TRY(cudaFuncSetAttribute(lora_kernel<RS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Z::kShared));
-    resident = std::max(1, ctas_in_clusters(lora_kernel<RS>, kCluster, 8, b200_sm_count(), kThreads, Z::kShared) / kCluster);
+  static bool configured = false;
+  if (!configured) {
+    B200_CUDA_TRY(cudaFuncSetAttribute(lora_down_kernel<RS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Down<RS>::kShared));
+    configured = true;
   }
-  a.most_parts = std::max(1, (a.n + 31) / 32 / (kCluster * kWarps));
-  const int clusters = (int)std::min<long long>(resident, (long long)max_tiles * a.most_parts);
-  cudaLaunchAttribute attr[2]{};
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = kCluster;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(clusters * kCluster));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Z::kShared;
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  (void)cudaLaunchKernelEx(&cfg, lora_kernel<RS>, a);
+  const long long sms = b200_sm_count(), items = (long long)max_tiles * ((a.n + Up<RS>::COLS - 1) / Up<RS>::COLS);
+  launch_after(lora_down_kernel<RS>, (unsigned)std::min<long long>((long long)max_tiles * kSlices, sms * Down<RS>::PER_SM), kThreads, Down<RS>::kShared, s, a);
+  B200_LAUNCH_CHECK();
+  launch_after(lora_up_kernel<RS>, (unsigned)std::min<long long>(items, sms * Up<RS>::PER_SM), kThreads, 0, s, a);
   B200_LAUNCH_CHECK();
   return B200_OK;
 }
@@ -377,8 +487,8 @@ extern "C" b200_status b200_lora_create(int32_t n_adapters, int32_t n, int32_t k
   if (st != B200_OK) return st;
   auto* l = new b200_lora();
   l->n_adapters = n_adapters; l->n = n; l->k = k; l->max_rank = max_rank;
-  l->rs = max_rank <= 16 ? 16 : max_rank <= 32 ? 32 : max_rank <= 64 ? 64 : 128;
-  const size_t a_bytes = (size_t)n_adapters * l->rs * k * 2, b_bytes = (size_t)n_adapters * l->rs * n * 2;
+  l->rs = rank_rows(max_rank);
+  const size_t a_bytes = n_adapters * l->a_units() * 16, b_bytes = n_adapters * l->b_units() * 16;
   cudaError_t e = cudaMalloc((void**)&l->a, a_bytes);
   if (e == cudaSuccess) e = cudaMalloc((void**)&l->b, b_bytes);
   if (e == cudaSuccess) e = cudaMalloc((void**)&l->rank, sizeof(int) * n_adapters);
@@ -410,11 +520,19 @@ extern "C" b200_status b200_lora_set(b200_lora* l, int32_t adapter, int32_t rank
   if (rank > 0 && (!h_a || !h_b)) { b200_set_error("lora: an adapter of rank %d without matrices", rank); return B200_ERR_INVALID_ARGUMENT; }
   b200_status st = b200_require_device();
   if (st != B200_OK) return st;
-  __nv_bfloat16 *a = l->a + (size_t)adapter * l->rs * l->k, *b = l->b + (size_t)adapter * l->rs * l->n;
-  B200_CUDA_TRY(cudaMemset(b, 0, (size_t)l->rs * l->n * 2));
-  if (rank > 0) {
-    B200_CUDA_TRY(cudaMemcpy(a, h_a, (size_t)rank * l->k * 2, cudaMemcpyHostToDevice));
-    B200_CUDA_TRY(cudaMemcpy2D(b, (size_t)l->rs * 2, h_b, (size_t)rank * 2, (size_t)rank * 2, l->n, cudaMemcpyHostToDevice));
+  if (rank > 0) {  // into the lanes' order
+    const uint16_t *ha = (const uint16_t*)h_a, *hb = (const uint16_t*)h_b;
+    const int rs = l->rs, ks = rs / 16;
+    std::vector<uint16_t> a(l->a_units() * 8, 0), b(l->b_units() * 8, 0);
+    for (int r = 0; r < rank; ++r)
+      for (int k = 0; k < l->k; ++k) a[((((size_t)(k / 32) * (rs / 8) + r / 8) * 32 + r % 8 * 4 + k % 32 / 8) * 8) + k % 8] = ha[(size_t)r * l->k + k];
+    for (int n = 0; n < l->n; ++n) {
+      const int c = n % 32, g = c / 8 * 2 + c % 2, j = c / 2 % 4;
+      for (int r = 0; r < rank; ++r)
+        b[(((((size_t)(n / 32) * ks + r / 16) * 2 + j / 2) * 32 + g * 4 + r % 16 / 4) * 2 + j % 2) * 4 + r % 4] = hb[(size_t)n * rank + r];
+    }
+    B200_CUDA_TRY(cudaMemcpy(l->a + adapter * l->a_units(), a.data(), a.size() * 2, cudaMemcpyHostToDevice));
+    B200_CUDA_TRY(cudaMemcpy(l->b + adapter * l->b_units(), b.data(), b.size() * 2, cudaMemcpyHostToDevice));
   }
   B200_CUDA_TRY(cudaMemcpy(l->scale + adapter, &scale, sizeof(float), cudaMemcpyHostToDevice));
   B200_CUDA_TRY(cudaMemcpy(l->rank + adapter, &rank, sizeof(int), cudaMemcpyHostToDevice));
@@ -436,7 +554,12 @@ extern "C" b200_status b200_lora_batch_create(int32_t max_rows, int32_t max_adap
   cudaError_t e = cudaMalloc((void**)&b->order, sizeof(int) * max_rows);
   if (e == cudaSuccess) e = cudaMalloc((void**)&b->tiles, sizeof(int4) * b->max_tiles);
   if (e == cudaSuccess) e = cudaMalloc((void**)&b->hdr, sizeof(int) * 4);
+  if (e == cudaSuccess) e = cudaMalloc((void**)&b->groups, sizeof(int4) * b->max_tiles);
+  if (e == cudaSuccess) e = cudaMalloc((void**)&b->done, sizeof(int) * b->max_tiles);
+  if (e == cudaSuccess) e = cudaMalloc((void**)&b->parts, sizeof(float) * kSlices * (size_t)max_rows * rank_rows(max_rank));
+  if (e == cudaSuccess) e = cudaMalloc((void**)&b->u, (size_t)b->max_tiles * kGroupRows * rank_rows(max_rank) * 4);
   if (e == cudaSuccess) e = cudaMemset(b->hdr, 0, sizeof(int) * 4);
+  if (e == cudaSuccess) e = cudaMemset(b->done, 0, sizeof(int) * b->max_tiles);
   if (e == cudaSuccess) e = cudaDeviceSynchronize();
   if (e != cudaSuccess) {
     b200_set_error("lora batch: %d rows: %s", max_rows, cudaGetErrorString(e));
@@ -450,7 +573,7 @@ extern "C" b200_status b200_lora_batch_create(int32_t max_rows, int32_t max_adap
 
 extern "C" void b200_lora_batch_destroy(b200_lora_batch* b) {
   if (!b) return;
-  for (void* p : {(void*)b->order, (void*)b->tiles, (void*)b->hdr}) if (p) cudaFree(p);
+  for (void* p : {(void*)b->order, (void*)b->tiles, (void*)b->hdr, (void*)b->groups, (void*)b->done, (void*)b->parts, (void*)b->u}) if (p) cudaFree(p);
   delete b;
 }
 
@@ -462,12 +585,19 @@ extern "C" b200_status b200_lora_plan(b200_lora_batch* b, const int32_t* d_row_a
   b->rows = rows;
   if (rows == 0) return B200_OK;
   launch_after(lora_plan_kernel, 1, rows <= 256 ? 256 : 1024, 0, (cudaStream_t)stream, d_row_adapter, rows, b->max_adapters,
-               most_tile_rows(b->max_rank), b->order, b->tiles, b->hdr);
+               b->max_tiles, b->order, b->tiles, b->groups, b->hdr);
   B200_LAUNCH_CHECK();
   return B200_OK;
 }
 
-extern "C" b200_status b200_lora_apply(const b200_lora* l, const b200_lora_batch* b, const void* d_x, int32_t x_stride, const void* d_y, int32_t y_stride,
+extern "C" b200_status b200_lora_error_word(b200_lora_batch* b, int32_t* out) {
+  if (!b || !out) { b200_set_error("lora batch: no handle, or no place for the word"); return B200_ERR_INVALID_ARGUMENT; }
+  B200_CUDA_TRY(cudaMemcpy(out, b->hdr + 3, sizeof(int), cudaMemcpyDeviceToHost));
+  if (*out != 0) B200_CUDA_TRY(cudaMemset(b->hdr + 3, 0, sizeof(int)));
+  return B200_OK;
+}
+
+extern "C" b200_status b200_lora_apply(const b200_lora* l, b200_lora_batch* b, const void* d_x, int32_t x_stride, const void* d_y, int32_t y_stride,
                                        void* d_out, int32_t out_stride, void* stream) {
   if (!l || !b) { b200_set_error("lora: no adapters, or no batch"); return B200_ERR_INVALID_ARGUMENT; }
   if (b->rows < 0) { b200_set_error("lora: the batch has no plan"); return B200_ERR_INVALID_ARGUMENT; }
@@ -479,15 +609,17 @@ extern "C" b200_status b200_lora_apply(const b200_lora* l, const b200_lora_batch
     b200_set_error("lora: rows start on 16 bytes, strides are multiples of 8 elements and hold a row; out is y itself or apart from it");
     return B200_ERR_INVALID_ARGUMENT;
   }
+  const int tiles = max_tiles_of(b->rows, b->max_adapters);
+  if ((long long)tiles * ((l->n + kWarps * 32 - 1) / (kWarps * 32)) > 0x7fffffff) { b200_set_error("lora: %d rows of %d columns in one call", b->rows, l->n); return B200_ERR_CAPACITY; }
   b200_status st = b200_require_device();
   if (st != B200_OK) return st;
   if (b->rows == 0) return B200_OK;
   LoraArgs a;
   a.a = l->a; a.b = l->b; a.x = (const __nv_bfloat16*)d_x; a.y = (const __nv_bfloat16*)d_y; a.out = (__nv_bfloat16*)d_out;
-  a.rank = l->rank; a.scale = l->scale; a.order = b->order; a.tiles = b->tiles; a.hdr = b->hdr;
-  a.n_adapters = l->n_adapters; a.n = l->n; a.k = l->k; a.rows = b->rows;
+  a.rank = l->rank; a.scale = l->scale; a.order = b->order; a.tiles = b->tiles; a.groups = b->groups; a.hdr = b->hdr; a.err = b->hdr + 3;
+  a.done = b->done; a.parts = b->parts; a.u = b->u;
+  a.max_rows = b->max_rows; a.max_tiles = b->max_tiles; a.n = l->n; a.k = l->k;
   a.x_stride = x_stride; a.y_stride = y_stride; a.out_stride = out_stride;
-  const int tiles = max_tiles_of(b->rows, b->max_adapters);
   cudaStream_t s = (cudaStream_t)stream;
   return l->rs == 16 ? launch<16>(a, tiles, s) : l->rs == 32 ? launch<32>(a, tiles, s) : l->rs == 64 ? launch<64>(a, tiles, s) : launch<128>(a, tiles, s);
 }

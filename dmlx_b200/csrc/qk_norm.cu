@@ -6,8 +6,10 @@
 // what is left goes to sincospif, which is exact about the 2 pi.
 //
 // A head is D / 8 lanes of eight neighbouring elements, so a warp takes 512 bytes (32 / (D / 8) heads) at once.  A pair (i, i + rot_dim / 2) lies
-// in two lanes at the same place, which a shuffle brings together; a pair (2 i, 2 i + 1) lies in one.  A warp has its row's cosines and sines in
-// registers for all the heads it takes, and takes as many of them as the number of rows allows (few rows: one load each).
+// in two lanes at the same place, and one shuffle of a word brings two partners; a pair (2 i, 2 i + 1) lies in a word.  Either way
+//   y = (x cos w - x' sin w') r,  r = 1 / sqrt(mean + eps),  x' the partner, sin with its sign,
+// so a head costs two packed operations per two elements beside the norm, with the products of angles and weights in registers for all heads that
+// a warp takes of its row.  The block's rows have their angles computed once, by all its threads.  Few rows: more warps for each.
 #include <cuda_bf16.h>
 #include <math.h>
 
@@ -34,132 +36,124 @@ struct NormRopeArgs {
   const int *positions, *row_seq;
   __nv_bfloat16 *q_out, *k_out;
   int q_out_stride, k_out_stride;
-  int rows, hq, hkv, rot, interleaved, parts;  // parts: warps that share a row
+  int rows, hq, hkv, rot, interleaved, block_rows;
   float eps;
   KvDev d;
   int layer;
   double turns[kMostPairs];  // frequency / (2 pi) of each pair
 };
 
-// PAGES: k goes into the row's page, and so does v.
-template <int D, bool PAGES>
-__global__ void __launch_bounds__(kWarps * 32) qk_norm_rope_kernel(const __grid_constant__ NormRopeArgs a) {
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 widen(uint32_t w) { return make_float2(ptx::bf16_lo(w), ptx::bf16_hi(w)); }
+
+// PAGES: k goes into the row's page, and so does v.  ROWS rows of a block, kWarps / ROWS warps for each, and gridDim.y blocks for the same rows.
+template <int D, bool PAGES, bool NEXT>
+__global__ void __launch_bounds__(kWarps * 32, 4) qk_norm_rope_kernel(const __grid_constant__ NormRopeArgs a) {
   after_previous();
   constexpr int LANES = D / 8, HEADS = 32 / LANES;  // lanes of a head; heads of a load
-  __shared__ double turns[kMostPairs];
-  if ((int)threadIdx.x < a.rot / 2) turns[threadIdx.x] = a.turns[threadIdx.x];
-  __syncthreads();
-  const int lane = threadIdx.x & 31, warp = blockIdx.x * kWarps + (threadIdx.x >> 5);
-  const int row = warp / a.parts, part = warp - row * a.parts;
-  if (row >= a.rows) return;
+  __shared__ float2 turn[kWarps * (D / 2)];         // [row of the block][pair] cosine, sine
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rows = a.block_rows, per_row = kWarps / rows;
+  const int row = blockIdx.x * rows + warp / per_row, parts = per_row * gridDim.y, part = blockIdx.y * per_row + warp % per_row;
   const int at = (lane % LANES) * 8, sub = lane / LANES;  // this lane's elements of a head; its head of a load
-  const int pos = a.positions[row];
-
-  float cs[8], sn[8];  // of this lane's elements; interleaved: of its four pairs
   const int half = a.rot / 2;
-  const bool turns_here = at < a.rot, second = !a.interleaved && at >= half;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    cs[e] = 1.f; sn[e] = 0.f;
-    if (!turns_here || (a.interleaved && e >= 4)) continue;
-    const double t = (double)pos * turns[a.interleaved ? at / 2 + e : (second ? at - half : at) + e];
-    sincospif((float)(2.0 * (t - rint(t))), &sn[e], &cs[e]);
-    if (second) sn[e] = -sn[e];
+  for (int i = threadIdx.x; i < rows * half; i += kWarps * 32) {
+    const int r = i / half, pair = i - r * half;
+    const double t = (double)(blockIdx.x * rows + r < a.rows ? a.positions[blockIdx.x * rows + r] : 0) * a.turns[pair];
+    float sn, cs;
+    sincospif((float)(2.0 * (t - rint(t))), &sn, &cs);
+    turn[r * half + pair] = make_float2(cs, sn);
   }
-  const int partner = (lane & ~(LANES - 1)) | (!turns_here || a.interleaved ? lane & (LANES - 1) : (second ? at - half : at + half) / 8);
-
-  float wq[8], wk[8];
-  auto weights = [&](const __nv_bfloat16* w, float (&f)[8]) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = 1.f;
-    if (!w) return;
-    const uint4 u = *reinterpret_cast<const uint4*>(w + at);
-    const uint32_t x[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) { f[2 * e] = ptx::bf16_lo(x[e]); f[2 * e + 1] = ptx::bf16_hi(x[e]); }
-  };
-  weights(a.q_weight, wq);
-  weights(a.k_weight, wk);
-
-  // a step whose reservation failed has no page for this row: nothing of it is written there (the error word is set)
-  size_t tile = 0;  // elements from the pool's start to this row in head 0 of its page
-  bool have_page = false;
-  if constexpr (PAGES) {
-    const int seq = a.row_seq[row], page_idx = pos / a.d.page_size;
-    have_page = pos >= 0 && seq >= 0 && seq < a.d.max_seqs && page_idx < a.d.seq_pages[seq];
-    if (have_page) {
-      const int page = a.d.block_table[(size_t)seq * a.d.max_pages_per_seq + page_idx];
-      tile = (((size_t)a.layer * a.d.n_pages + page) * a.hkv * a.d.page_size + (pos - page_idx * a.d.page_size)) * (size_t)D;
-    }
-  }
-  const int heads = a.hq + (PAGES ? 2 : 1) * a.hkv;
-  for (int h0 = part * HEADS; h0 < heads; h0 += kAhead * a.parts * HEADS) {
-    uint4 in[kAhead];
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int h = h0 + u * a.parts * HEADS + sub;
-      in[u] = make_uint4(0, 0, 0, 0);
-      if (h >= heads) continue;
-      const __nv_bfloat16* src = h < a.hq ? a.q + (size_t)row * a.q_stride + (size_t)h * D
-                                 : h < a.hq + a.hkv ? a.k + (size_t)row * a.k_stride + (size_t)(h - a.hq) * D
-                                                    : a.v + (size_t)row * a.v_stride + (size_t)(h - a.hq - a.hkv) * D;
-      in[u] = *reinterpret_cast<const uint4*>(src + at);
-    }
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int h = h0 + u * a.parts * HEADS + sub;
-      if (h0 + u * a.parts * HEADS >= heads) break;  // (the whole warp)
-      const uint32_t w[4] = {in[u].x, in[u].y, in[u].z, in[u].w};
-      float x[8], ss = 0.f;
+  __syncthreads();
+  if (row >= a.rows) return;
+  const bool turns_here = at < a.rot, second = !NEXT && at >= half;
+  const int partner = (lane & ~(LANES - 1)) | ((turns_here ? (second ? at - half : at + half) : at) / 8);
+  const uint32_t neighbours = turns_here ? 0x1032 : 0x3210;  // (what does not turn is its own partner: 0 times another infinite number is not 0)
+  // The row's heads, loads part, part + parts, ...: `src` and `dst` head 0 of the row, dst_head elements between heads there.
+  auto heads_of = [&](const __nv_bfloat16* src, int heads, const __nv_bfloat16* weight, __nv_bfloat16* dst, int dst_head, bool writes) {
+    float2 cw[4], sw[4];  // cosine times the weight of each of the lane's elements; sine, with its sign, times the partner's
+    {
+      const uint4 one = make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u);
+      const uint4 own = weight ? *reinterpret_cast<const uint4*>(weight + at) : one;
+      const uint4 other = NEXT || !weight ? own : *reinterpret_cast<const uint4*>(weight + (partner & (LANES - 1)) * 8);
+      const uint32_t wo[4] = {own.x, own.y, own.z, own.w}, wp[4] = {other.x, other.y, other.z, other.w};
+      const float2* tr = turn + (warp / per_row) * half;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[2 * e] = ptx::bf16_lo(w[e]);
-        x[2 * e + 1] = ptx::bf16_hi(w[e]);
-        ss = fmaf(x[2 * e], x[2 * e], fmaf(x[2 * e + 1], x[2 * e + 1], ss));
+        cw[e] = widen(wo[e]);
+        sw[e] = make_float2(0.f, 0.f);
+        if (!turns_here) continue;
+        if constexpr (NEXT) {
+          const float2 cs = tr[at / 2 + e];
+          sw[e] = make_float2(-cs.y * cw[e].y, cs.y * cw[e].x);
+          cw[e] = make_float2(cs.x * cw[e].x, cs.x * cw[e].y);
+        } else {
+          const float2 c0 = tr[(second ? at - half : at) + 2 * e], c1 = tr[(second ? at - half : at) + 2 * e + 1], p = widen(wp[e]);
+          const float sign = second ? 1.f : -1.f;
+          sw[e] = make_float2(sign * c0.y * p.x, sign * c1.y * p.y);
+          cw[e] = make_float2(c0.x * cw[e].x, c1.x * cw[e].y);
+        }
       }
+    }
+    int head = part * HEADS + sub;
+    const int step = parts * HEADS;
+    src += (size_t)head * D + at;
+    dst += (size_t)head * dst_head + at;
+    for (int h0 = part * HEADS; h0 < heads; h0 += kAhead * step) {  // (h0: the same in the whole warp)
+      uint4 in[kAhead];
 #pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const float r = rsqrtf(ss * (1.0f / D) + a.eps);
-      const bool is_q = h < a.hq;
+      for (int u = 0; u < kAhead; ++u) in[u] = head + u * step < heads ? *reinterpret_cast<const uint4*>(src + (size_t)(u * step) * D) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = x[e] * r * (is_q ? wq[e] : wk[e]);
-      float y[8];
-      if (a.interleaved) {
+      for (int u = 0; u < kAhead; ++u) {
+        if (h0 + u * step >= heads) break;
+        const uint32_t w[4] = {in[u].x, in[u].y, in[u].z, in[u].w};
+        float2 s2 = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s2 = fma2(widen(w[e]), widen(w[e]), s2);
+        float ss = s2.x + s2.y;
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float r = rsqrtf(ss * (1.0f / D) + a.eps);
+        uint4 out;
+        uint32_t* o = reinterpret_cast<uint32_t*>(&out);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          y[2 * e] = x[2 * e] * cs[e] - x[2 * e + 1] * sn[e];
-          y[2 * e + 1] = x[2 * e] * sn[e] + x[2 * e + 1] * cs[e];
+          const uint32_t other = NEXT ? __byte_perm(w[e], 0u, neighbours) : __shfl_sync(0xffffffffu, w[e], partner);
+          const float2 y = mul2(fma2(widen(other), sw[e], mul2(widen(w[e]), cw[e])), make_float2(r, r));
+          const __nv_bfloat162 p = __floats2bfloat162_rn(y.x, y.y);
+          o[e] = *reinterpret_cast<const uint32_t*>(&p);
         }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float other = __shfl_sync(0xffffffffu, x[e], partner);
-          y[e] = x[e] * cs[e] - other * sn[e];
-        }
+        if (writes && head + u * step < heads) *reinterpret_cast<uint4*>(dst + (size_t)(u * step) * dst_head) = out;
       }
-      if (!turns_here) {  // (0 times an infinite neighbour would not be 0)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = x[e];
-      }
-      uint4 out;
-      uint32_t* o = reinterpret_cast<uint32_t*>(&out);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const __nv_bfloat162 p = __floats2bfloat162_rn(y[2 * e], y[2 * e + 1]);
-        o[e] = *reinterpret_cast<const uint32_t*>(&p);
-      }
-      if (h >= heads) continue;
-      if (is_q) {
-        *reinterpret_cast<uint4*>(a.q_out + (size_t)row * a.q_out_stride + (size_t)h * D + at) = out;
-      } else if constexpr (PAGES) {
-        const bool is_v = h >= a.hq + a.hkv;
-        const int head = h - a.hq - (is_v ? a.hkv : 0);
-        __nv_bfloat16* pool = (__nv_bfloat16*)(is_v ? a.d.v_pool : a.d.k_pool) + tile + (size_t)head * a.d.page_size * D + at;
-        if (have_page) *reinterpret_cast<uint4*>(pool) = is_v ? in[u] : out;
-      } else {
-        *reinterpret_cast<uint4*>(a.k_out + (size_t)row * a.k_out_stride + (size_t)(h - a.hq) * D + at) = out;
-      }
+      head += kAhead * step;
+      src += (size_t)(kAhead * step) * D;
+      dst += (size_t)(kAhead * step) * dst_head;
     }
+  };
+  heads_of(a.q + (size_t)row * a.q_stride, a.hq, a.q_weight, a.q_out + (size_t)row * a.q_out_stride, D, true);
+  if constexpr (!PAGES) {
+    heads_of(a.k + (size_t)row * a.k_stride, a.hkv, a.k_weight, a.k_out + (size_t)row * a.k_out_stride, D, true);
+  } else {
+    // a step whose reservation failed has no page for this row: nothing of it is written there (the error word is set)
+    const int pos = a.positions[row], seq = a.row_seq[row], page_idx = pos / a.d.page_size;
+    const bool have_page = pos >= 0 && seq >= 0 && seq < a.d.max_seqs && page_idx < a.d.seq_pages[seq];
+    const int page = have_page ? a.d.block_table[(size_t)seq * a.d.max_pages_per_seq + page_idx] : 0, head_step = a.d.page_size * D;
+    const size_t tile = (((size_t)a.layer * a.d.n_pages + page) * a.hkv * a.d.page_size + (have_page ? pos - page_idx * a.d.page_size : 0)) * (size_t)D;
+    heads_of(a.k + (size_t)row * a.k_stride, a.hkv, a.k_weight, (__nv_bfloat16*)a.d.k_pool + tile, head_step, have_page);
+    if (have_page)
+      for (int h = part * HEADS + sub; h < a.hkv; h += parts * HEADS)
+        *reinterpret_cast<uint4*>((__nv_bfloat16*)a.d.v_pool + tile + (size_t)h * head_step + at) =
+            *reinterpret_cast<const uint4*>(a.v + (size_t)row * a.v_stride + (size_t)h * D + at);
   }
 }
 
@@ -186,21 +180,33 @@ b200_status fill(NormRopeArgs& a, const char* who, const b200_norm_rope* s, cons
   a.positions = d_positions; a.rows = rows; a.hq = s->n_q_heads; a.hkv = s->n_kv_heads;
   a.rot = s->rot_dim; a.interleaved = s->interleaved != 0; a.eps = s->eps;
   a.q_out = (__nv_bfloat16*)d_q_out; a.q_out_stride = q_out_stride;
-  for (int i = 0; i < s->rot_dim / 2; ++i) a.turns[i] = pow(s->theta, -2.0 * i / s->rot_dim) / (2.0 * M_PI);
+  // The frequencies of the last call's rotation: a model has one or two.
+  static thread_local struct { int rot = 0; double theta = 0.0, turns[kMostPairs]; } last;
+  if (last.rot != s->rot_dim || last.theta != s->theta) {
+    for (int i = 0; i < s->rot_dim / 2; ++i) last.turns[i] = pow(s->theta, -2.0 * i / s->rot_dim) / (2.0 * M_PI);
+    last.rot = s->rot_dim;
+    last.theta = s->theta;
+  }
+  std::copy(last.turns, last.turns + s->rot_dim / 2, a.turns);
   return B200_OK;
+}
+
+template <int D, bool PAGES>
+void launch_as(const NormRopeArgs& a, dim3 grid, cudaStream_t s) {
+  if (a.interleaved) launch_after(qk_norm_rope_kernel<D, PAGES, true>, grid, kWarps * 32, 0, s, a);
+  else launch_after(qk_norm_rope_kernel<D, PAGES, false>, grid, kWarps * 32, 0, s, a);
 }
 
 template <bool PAGES>
 b200_status launch(NormRopeArgs& a, int head_dim, cudaStream_t s) {
-  const int heads = a.hq + (PAGES ? 2 : 1) * a.hkv, loads = (heads * head_dim + 255) / 256;
-  // 32 warps per SM take the row's loads between them; with more rows than that a warp has whole rows
-  const int want = 32 * b200_sm_count();
-  a.parts = std::min(loads, std::max(1, (want + a.rows - 1) / a.rows));
-  const long long warps = (long long)a.rows * a.parts;
-  const unsigned grid = (unsigned)((warps + kWarps - 1) / kWarps);
-  if (head_dim == 64) launch_after(qk_norm_rope_kernel<64, PAGES>, grid, kWarps * 32, 0, s, a);
-  else if (head_dim == 128) launch_after(qk_norm_rope_kernel<128, PAGES>, grid, kWarps * 32, 0, s, a);
-  else launch_after(qk_norm_rope_kernel<256, PAGES>, grid, kWarps * 32, 0, s, a);
+  const int heads = 256 / head_dim, loads = std::max(1, std::max((a.hq + heads - 1) / heads, (a.hkv + heads - 1) / heads));
+  // warps for a row: enough that there are 32 on every SM, no more than the row has loads
+  const int want = std::min(loads, std::max(1, (32 * b200_sm_count() + a.rows - 1) / a.rows));
+  a.block_rows = want >= kWarps ? 1 : want > kWarps / 2 ? 1 : want > kWarps / 4 ? 2 : want > 1 ? 4 : 8;
+  const dim3 grid((a.rows + a.block_rows - 1) / a.block_rows, (want + kWarps - 1) / kWarps);
+  if (head_dim == 64) launch_as<64, PAGES>(a, grid, s);
+  else if (head_dim == 128) launch_as<128, PAGES>(a, grid, s);
+  else launch_as<256, PAGES>(a, grid, s);
   B200_LAUNCH_CHECK();
   return B200_OK;
 }

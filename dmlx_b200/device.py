@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import array
 import ctypes as C
+import math
 import operator
 from typing import List, Optional, Sequence
 
@@ -165,13 +166,15 @@ class PagedKVCache:
                          rot_dim: Optional[int] = None, interleaved: bool = False, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """b200_kv_norm_rope_append: qk_norm_rope with k and v going into the pages reserved for this step.  Returns q; on FP8 pools k is overwritten
         with the rotated keys."""
-        t, hq, d = q.shape
-        strides = _rows(q, t, hq, d), _rows(k, t, k.shape[1], d), _rows(v, t, k.shape[1], d)
-        q_out = q_out if q_out is not None else torch.empty((t, hq, d), dtype=q.dtype, device=q.device)
-        shape = _norm_rope_shape(q, k, q_weight, k_weight, eps, theta, rot_dim, interleaved)
-        _lib.check(lib.b200_kv_norm_rope_append(self._h, layer, C.byref(shape), q.data_ptr(), k.data_ptr(), v.data_ptr(), *strides, _ptr(q_weight),
-                                                _ptr(k_weight), _ptr(_ints(positions, t)), _ptr(_ints(row_seq, t)), t, q_out.data_ptr(),
-                                                _rows(q_out, t, hq, d), _stream()))
+        device = torch.cuda.current_device()
+        (t, hq, d), hkv = q.shape, k.shape[1]
+        q_shape, k_shape = (t, hq, d), (t, hkv, d)
+        strides = _rows(q, q_shape, device), _rows(k, k_shape, device), _rows(v, k_shape, device)
+        q_out = q.new_empty(q_shape) if q_out is None else q_out
+        shape = _lib.NormRope(hq, hkv, d, d if rot_dim is None else rot_dim, interleaved, eps, theta)
+        _lib.check(lib.b200_kv_norm_rope_append(self._h, layer, C.byref(shape), q.data_ptr(), k.data_ptr(), v.data_ptr(), *strides, _weight(q_weight, d, device),
+                                                _weight(k_weight, d, device), _ints(positions, t, device), _ints(row_seq, t, device), t, q_out.data_ptr(),
+                                                _rows(q_out, q_shape, device), _raw_stream(device)))
         return q_out
 
     def append(self, layer: int, k_rows: torch.Tensor, v_rows: torch.Tensor):
@@ -331,35 +334,37 @@ class LayeredKVCache(PagedKVCache):
         return out
 
 
-def _here(t: torch.Tensor) -> bool:
-    return t.is_cuda and t.device.index == torch.cuda.current_device()
+# (A stream object per call is 3 us of the host's time; a small call has ten.)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-def _rows(t: torch.Tensor, *shape) -> int:
-    """Checks bf16 rows on the device whose numbers lie one behind the other within a row (shape: None = any length); returns the elements between
-    rows."""
-    if not (_here(t) and t.dtype == torch.bfloat16 and t.dim() == len(shape) and all(want is None or have == want for have, want in zip(t.shape, shape))):
+def _rows(t: torch.Tensor, shape: tuple, device: int) -> int:
+    """Checks bf16 rows on the device whose numbers lie one behind the other within a row; returns the elements between rows."""
+    if t.dtype != torch.bfloat16 or t.shape != shape or t.get_device() != device:
         raise ValueError(f"expected bf16 rows of shape {shape} on the current device, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    inner = 1
-    for n, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-        if n > 1 and stride != inner:
+    inner = math.prod(shape[1:])
+    if t.is_contiguous():
+        return inner
+    width = 1
+    for n, stride in zip(reversed(shape[1:]), reversed(t.stride()[1:])):
+        if n > 1 and stride != width:
             raise ValueError(f"the numbers of a row are not contiguous: strides {t.stride()}")
-        inner *= n
-    return t.stride(0) if t.shape[0] > 1 else inner
+        width *= n
+    return t.stride(0) if shape[0] > 1 else inner
 
 
-def _ints(t: torch.Tensor, n: int) -> torch.Tensor:
-    if not (_here(t) and t.dtype == torch.int32 and tuple(t.shape) == (n,) and t.is_contiguous()):
+def _ints(t: torch.Tensor, n: int, device: int) -> int:
+    if t.dtype != torch.int32 or t.shape != (n,) or t.get_device() != device or not t.is_contiguous():
         raise ValueError(f"expected {n} contiguous int32 on the current device, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t
+    return t.data_ptr()
 
 
-def _norm_rope_shape(q: torch.Tensor, k: torch.Tensor, q_weight, k_weight, eps: float, theta: float, rot_dim: Optional[int], interleaved: bool):
-    d = q.shape[-1]
-    for w in (q_weight, k_weight):
-        if w is not None:
-            _rows(w, d)
-    return _lib.NormRope(q.shape[1], k.shape[1], d, d if rot_dim is None else rot_dim, int(interleaved), eps, theta)
+def _weight(w: Optional[torch.Tensor], d: int, device: int) -> Optional[int]:
+    if w is None:
+        return None
+    if w.dtype != torch.bfloat16 or w.shape != (d,) or w.get_device() != device or not w.is_contiguous():
+        raise ValueError(f"expected {d} contiguous bf16 weights on the current device, got {w.dtype} {tuple(w.shape)} on {w.device}")
+    return w.data_ptr()
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
@@ -367,14 +372,16 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, q_we
                  interleaved: bool = False, q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None):
     """b200_qk_norm_rope: RMSNorm of every head of q [T, Hq, D] and k [T, Hkv, D] (rows may be strided) and the rotation of its first rot_dim numbers
     (default: all) in one pass.  Returns (q, k) as new tensors, or q_out and k_out, which may be q and k themselves."""
-    t, hq, d = q.shape
-    q_stride, k_stride = _rows(q, t, hq, d), _rows(k, t, k.shape[1], d)
-    q_out = q_out if q_out is not None else torch.empty((t, hq, d), dtype=q.dtype, device=q.device)
-    k_out = k_out if k_out is not None else torch.empty((t, k.shape[1], d), dtype=k.dtype, device=k.device)
-    qo_stride, ko_stride = _rows(q_out, t, hq, d), _rows(k_out, t, k.shape[1], d)
-    shape = _norm_rope_shape(q, k, q_weight, k_weight, eps, theta, rot_dim, interleaved)
-    _lib.check(lib.b200_qk_norm_rope(C.byref(shape), q.data_ptr(), k.data_ptr(), q_stride, k_stride, _ptr(q_weight), _ptr(k_weight), _ptr(_ints(positions, t)),
-                                     t, q_out.data_ptr(), k_out.data_ptr(), qo_stride, ko_stride, _stream()))
+    device = torch.cuda.current_device()
+    (t, hq, d), hkv = q.shape, k.shape[1]
+    q_shape, k_shape = (t, hq, d), (t, hkv, d)
+    q_stride, k_stride = _rows(q, q_shape, device), _rows(k, k_shape, device)
+    q_out = q.new_empty(q_shape) if q_out is None else q_out
+    k_out = k.new_empty(k_shape) if k_out is None else k_out
+    shape = _lib.NormRope(hq, hkv, d, d if rot_dim is None else rot_dim, interleaved, eps, theta)
+    _lib.check(lib.b200_qk_norm_rope(C.byref(shape), q.data_ptr(), k.data_ptr(), q_stride, k_stride, _weight(q_weight, d, device), _weight(k_weight, d, device),
+                                     _ints(positions, t, device), t, q_out.data_ptr(), k_out.data_ptr(), _rows(q_out, q_shape, device),
+                                     _rows(k_out, k_shape, device), _raw_stream(device)))
     return q_out, k_out
 
 
@@ -385,7 +392,7 @@ class SharedPrefixAttention:
     def __init__(self, cache: PagedKVCache, max_rows: int):
         h = C.c_void_p()
         _lib.check(lib.b200_prefix_attn_create(cache._h, max_rows, C.byref(h)))
-        self._h, self.cache, self.rows = h.value, cache, None
+        self._h, self.cache, self.rows, self._heads = h.value, cache, None, (cache.cfg.n_q_heads, cache.cfg.head_dim)
 
     def close(self):
         if getattr(self, "_h", None) and lib is not None:
@@ -397,18 +404,17 @@ class SharedPrefixAttention:
 
     def plan(self, row_seq: torch.Tensor, row_ctx: torch.Tensor):
         """b200_prefix_attn_plan: row r is to see the first row_ctx[r] tokens of slot row_seq[r]."""
-        rows = row_seq.shape[0]
-        _lib.check(lib.b200_prefix_attn_plan(self._h, _ptr(_ints(row_seq, rows)), _ptr(_ints(row_ctx, rows)), rows, _stream()))
+        rows, device = row_seq.shape[0], torch.cuda.current_device()
+        _lib.check(lib.b200_prefix_attn_plan(self._h, _ints(row_seq, rows, device), _ints(row_ctx, rows, device), rows, _raw_stream(device)))
         self.rows = rows
 
     def run(self, layer: int, q: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """b200_prefix_attn_run: q [T, Hq, D] (rows may be strided), T the rows of the plan."""
-        c = self.cache.cfg
         if q.shape[0] != self.rows:
             raise ValueError(f"{q.shape[0]} rows, the plan has {self.rows}")
-        out = out if out is not None else torch.empty((self.rows, c.n_q_heads, c.head_dim), dtype=q.dtype, device=q.device)
-        strides = _rows(q, self.rows, c.n_q_heads, c.head_dim), _rows(out, self.rows, c.n_q_heads, c.head_dim)
-        _lib.check(lib.b200_prefix_attn_run(self._h, layer, q.data_ptr(), strides[0], out.data_ptr(), strides[1], _stream()))
+        device, shape = torch.cuda.current_device(), (self.rows, *self._heads)
+        out = q.new_empty(shape) if out is None else out
+        _lib.check(lib.b200_prefix_attn_run(self._h, layer, q.data_ptr(), _rows(q, shape, device), out.data_ptr(), _rows(out, shape, device), _raw_stream(device)))
         return out
 
 
@@ -444,9 +450,10 @@ class LoraAdapters:
         t = x.shape[0]
         if t != batch.rows:
             raise ValueError(f"{t} rows, the batch's plan has {batch.rows}")
-        out = out if out is not None else torch.empty((t, self.n), dtype=y.dtype, device=y.device)
-        strides = _rows(x, t, self.k), _rows(y, t, self.n), _rows(out, t, self.n)
-        _lib.check(lib.b200_lora_apply(self._h, batch._h, x.data_ptr(), strides[0], y.data_ptr(), strides[1], out.data_ptr(), strides[2], _stream()))
+        device, y_shape = torch.cuda.current_device(), (t, self.n)
+        out = y.new_empty(y_shape) if out is None else out
+        _lib.check(lib.b200_lora_apply(self._h, batch._h, x.data_ptr(), _rows(x, (t, self.k), device), y.data_ptr(), _rows(y, y_shape, device), out.data_ptr(),
+                                       _rows(out, y_shape, device), _raw_stream(device)))
         return out
 
 
@@ -466,10 +473,15 @@ class LoraBatch:
     def __del__(self):
         self.close()
 
+    def error_word(self) -> int:
+        out = C.c_int32()
+        _lib.check(lib.b200_lora_error_word(self._h, C.byref(out)))
+        return out.value
+
     def plan(self, row_adapter: torch.Tensor):
         """b200_lora_plan: the adapter of every row, -1 for none."""
-        rows = row_adapter.shape[0]
-        _lib.check(lib.b200_lora_plan(self._h, _ptr(_ints(row_adapter, rows)), rows, _stream()))
+        rows, device = row_adapter.shape[0], torch.cuda.current_device()
+        _lib.check(lib.b200_lora_plan(self._h, _ints(row_adapter, rows, device), rows, _raw_stream(device)))
         self.rows = rows
 
 
