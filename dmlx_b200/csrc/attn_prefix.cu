@@ -9,7 +9,7 @@
 // Four kernels.  The plan (one block, once per step) finds the tree by the first page that rows of a group have not compared yet: equal pages make
 // a group, its smallest common length a node.  Then, per layer:
 //   * nodes with more than 16 query rows per kv head: tcgen05.  An item is up to 256 query rows (row, head of the GQA group), a range of the
-//     node's pages, and a kv head; S = Q K^T into tensor memory, P = 2^(S - m) in bf16 in its place, O += P V with P read from there.  Every key is
+//     node's pages, and a kv head; S = Q K^T into tensor memory, P = 2^(S - m) in 16 bits in its place, O += P V with P read from there.  Every key is
 //     seen by every row, so there are no masks;
 //   * everything else, smaller nodes and the rows' own pages: a warp per item on mma.sync, 16 query rows, pages by TMA into rings of its own;
 //   * the join.
@@ -44,13 +44,13 @@ struct Node {
   int p0, p1;         // pages
 };
 struct Member { int row, slot; };  // a row of a node; the place of its first part
-struct ItemA { int node, tile, chunk, pad; };
-struct ItemB { int node, chunk; };  // node < 0: the own pages of row ~node
+struct alignas(16) ItemA { int seq, first, count, p0, p1, part, pad[2]; };  // pages of slot seq's table for `count` members from `first` on; their part behind `slot`
+struct alignas(16) ItemB { int seq, first, count, p0, p1, ctx, part, pad; };  // count 0: own pages of the row `first`, its part `part`, and ctx tokens that it sees; else members, as above
 
 enum { H_ITEMS_A = 0, H_ITEMS_B, H_PAGES_A, H_PAGES_B, H_NEXT_A, H_NEXT_B, H_NODES, H_WORKERS_A, H_COUNT = 16 };
 
 struct PlanDev {
-  int *hdr, *row_seq, *row_ctx, *row_from, *row_base, *own_slot, *member_node;
+  int *hdr, *row_seq, *row_ctx, *row_base, *member_node;
   Node* nodes;
   Member* members;
   ItemA* items_a;
@@ -285,12 +285,14 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
     for (int w = 0; w < warp; ++w) start += s.warp_sums[w];
     if (i < rows) {
       p.row_base[i] = start;
-      p.own_slot[i] = start + parts[i];
-      p.row_from[i] = from[i];
       depth[i] = start;
       if (own > 0) {
         const int at = atomicAdd(&s.next_b, own);
-        for (int c = 0; c < own; ++c) p.items_b[at + c] = ItemB{~i, c};
+        const int pages = ceil_div(p.row_ctx[i], d.page_size);
+        for (int c = 0; c < own; ++c) {
+          const int p0 = from[i] + c * min(len_b, pages);
+          p.items_b[at + c] = ItemB{p.row_seq[i], i, 0, p0, min(pages, p0 + min(len_b, pages)), p.row_ctx[i], start + parts[i] + c, 0};
+        }
       }
     }
     __syncthreads();
@@ -298,15 +300,22 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
     __syncthreads();
   }
   for (int at = tid; at < s.n_members; at += blockDim.x) p.members[at].slot += depth[p.members[at].row];
-  for (int i = tid; i < n_nodes; i += blockDim.x) {
+  // items of the nodes, a warp per node
+  for (int i = warp; i < n_nodes; i += blockDim.x / 32) {
     const Node n = p.nodes[i];
-    const int pages = n.p1 - n.p0;
-    if (is_large(n.count, group)) {
-      const int tiles = ceil_div(n.count, 2 * members), chunks = ceil_div(pages, len_a), at = atomicAdd(&s.next_a, tiles * chunks);
-      for (int c = 0; c < tiles * chunks; ++c) p.items_a[at + c] = ItemA{i, c % tiles, c / tiles, 0};
-    } else {
-      const int chunks = ceil_div(pages, len_b), at = atomicAdd(&s.next_b, chunks);
-      for (int c = 0; c < chunks; ++c) p.items_b[at + c] = ItemB{i, c};
+    const int pages = n.p1 - n.p0, large = is_large(n.count, group) ? 1 : 0, len = min(large ? len_a : len_b, pages), chunks = ceil_div(pages, len);
+    const int tiles = large ? ceil_div(n.count, 2 * members) : 1;
+    int at = 0;
+    if (lane == 0) at = atomicAdd(large ? &s.next_a : &s.next_b, tiles * chunks);
+    at = __shfl_sync(0xffffffffu, at, 0);
+    for (int c = lane; c < tiles * chunks; c += 32) {
+      const int tile = c % tiles, chunk = c / tiles, p0 = n.p0 + chunk * len, p1 = min(n.p1, p0 + len);
+      if (large) {
+        const int before = tile * 2 * members;
+        p.items_a[at + c] = ItemA{n.seq, n.first + before, min(2 * members, n.count - before), p0, p1, one_tile(n, tile, group) ? 2 * chunk : chunk, {0, 0}};
+      } else {
+        p.items_b[at + c] = ItemB{n.seq, n.first, n.count, p0, p1, 0x7fffffff, chunk, 0};
+      }
     }
   }
   __syncthreads();
@@ -391,61 +400,27 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-constexpr int kBWarps = 4;
 template <int D, bool FP8>
 struct ShapeB {
-  static constexpr int TILE = 32 * D * (FP8 ? 1 : 2);     // bytes of a page's K or V of one head
-  static constexpr int STAGES = FP8 ? 2 : (D == 128 ? 3 : 3);
-  static constexpr int PER_SM = FP8 ? 2 : (D == 128 ? 1 : 2);
-  static constexpr int QUEUE = 8;                         // items that a warp's loads may be ahead of its products
-  static constexpr size_t kShared = (size_t)kBWarps * STAGES * 2 * TILE + 1024 + sizeof(uint64_t) * kBWarps * STAGES + sizeof(int) * kBWarps * QUEUE;
+  static constexpr int TILE = 32 * D * (FP8 ? 1 : 2);  // bytes of a page's K or V of one head
+  static constexpr int WARPS = D == 64 ? 12 : 8, STAGES = FP8 || D == 64 ? 4 : 3;  // registers, then shared memory (a stage holds K or V of a page)
+  static constexpr int QUEUE = 8;                      // items that a warp's loads may be ahead of its products
+  static constexpr size_t kShared = (size_t)WARPS * STAGES * TILE + 1024 + sizeof(uint64_t) * WARPS * STAGES + sizeof(int) * WARPS * QUEUE;
 };
-
-struct WarpItem {
-  int head, seq, page_begin, page_end, ctx;  // ctx: of an own item; keys behind it are not seen
-  int rows, first;                           // rows < 0: the row `first` by itself; else `rows` members from `first` on
-  int chunk;
-};
-__device__ __forceinline__ WarpItem warp_item(const Args& a, int item) {
-  WarpItem it;
-  const int heads = a.d.n_kv_heads, n = item / heads, len = a.p.hdr[H_PAGES_B];
-  it.head = item - n * heads;
-  const ItemB b = a.p.items_b[n];
-  it.chunk = b.chunk;
-  int p0, p1;
-  if (b.node < 0) {
-    const int row = ~b.node;
-    it.first = row; it.rows = -1;
-    it.seq = a.p.row_seq[row];
-    it.ctx = a.p.row_ctx[row];
-    p0 = a.p.row_from[row];
-    p1 = (it.ctx + a.d.page_size - 1) / a.d.page_size;
-  } else {
-    const Node nd = a.p.nodes[b.node];
-    it.first = nd.first; it.rows = nd.count;
-    it.seq = nd.seq;
-    it.ctx = 0x7fffffff;
-    p0 = nd.p0;
-    p1 = nd.p1;
-  }
-  it.page_begin = p0 + (int)min((long long)b.chunk * len, (long long)(p1 - p0));
-  it.page_end = (int)min((long long)it.page_begin + len, (long long)p1);
-  return it;
-}
 
 // bf16: K and V as they are; FP8: the codes widened to f16 in registers (exact), K's dims and V's output columns in the order in which ldmatrix gives
 // the bytes, the page's K scale on the scores, its V scale (over the item's largest) on P.
 template <int D, bool FP8>
-__global__ void __launch_bounds__(kBWarps * 32, 1) prefix_warp_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(ShapeB<D, FP8>::WARPS * 32, 1) prefix_warp_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Args a) {
   wait_previous();
   using Z = ShapeB<D, FP8>;
   constexpr int TILE = Z::TILE, STAGES = Z::STAGES, KS = D / 16, NO = D / 8;
   extern __shared__ unsigned char smem_dyn[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~(uintptr_t)1023);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  unsigned char* tiles = smem + (size_t)warp * STAGES * 2 * TILE;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)kBWarps * STAGES * 2 * TILE) + warp * STAGES;
-  int* queue = reinterpret_cast<int*>(reinterpret_cast<uint64_t*>(smem + (size_t)kBWarps * STAGES * 2 * TILE) + kBWarps * STAGES) + warp * Z::QUEUE;
+  unsigned char* tiles = smem + (size_t)warp * STAGES * TILE;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)Z::WARPS * STAGES * TILE) + warp * STAGES;
+  int* queue = reinterpret_cast<int*>(reinterpret_cast<uint64_t*>(smem + (size_t)Z::WARPS * STAGES * TILE) + Z::WARPS * STAGES) + warp * Z::QUEUE;
   const int H = a.d.n_kv_heads, G = a.group, n_items = a.p.hdr[H_ITEMS_B] * H;
   if (lane == 0) {
     for (int s = 0; s < STAGES; ++s) ptx::mbar_init(&full[s], 1);
@@ -453,12 +428,12 @@ __global__ void __launch_bounds__(kBWarps * 32, 1) prefix_warp_kernel(const __gr
   }
   __syncwarp();
 
-  // ---- loads: the items come off a counter, pages ahead of the products ----
-  WarpItem p{};
-  int p_page = 0, p_ids = 0;
-  uint32_t taken = 0, loaded = 0;
-  bool p_more = true;
-  auto enter = [&]() {  // the next item's id into the queue (n_items: no more)
+  // ---- loads: the items come off a counter; K and V of page after page, ahead of the products ----
+  int p_head = 0, p_begin = 0, p_page = 0, p_end = 0, p_ids = 0, p_id = 0;
+  const int* p_table = nullptr;
+  uint32_t taken = 0, loaded = 0, load_slot = 0;
+  bool p_more = true, p_value = false;
+  auto enter = [&]() {  // the next item's number into the queue (-1: no more)
     int id = 0;
     if (lane == 0) id = atomicAdd(&a.p.hdr[H_NEXT_B], 1);
     id = __shfl_sync(0xffffffffu, id, 0);
@@ -466,50 +441,65 @@ __global__ void __launch_bounds__(kBWarps * 32, 1) prefix_warp_kernel(const __gr
     if (lane == 0) queue[taken % Z::QUEUE] = p_more ? id : -1;
     __syncwarp();
     ++taken;
-    if (p_more) { p = warp_item(a, id); p_page = p.page_begin; }
-  };
-  auto load_page = [&]() {
     if (!p_more) return;
-    const int rel = p_page - p.page_begin;
-    if ((rel & 31) == 0) p_ids = p_page + lane < p.page_end ? table_of(a, p.seq)[p_page + lane] : 0;
-    const int page = __shfl_sync(0xffffffffu, p_ids, rel & 31);
+    const ItemB it = a.p.items_b[id / H];
+    p_head = id % H;
+    p_table = table_of(a, it.seq);
+    p_begin = p_page = it.p0;
+    p_end = it.p1;
+  };
+  auto load_tile = [&]() {
+    if (!p_more) return;
+    if (!p_value) {
+      const int rel = p_page - p_begin;
+      if ((rel & 31) == 0) p_ids = p_page + lane < p_end ? p_table[p_page + lane] : 0;
+      p_id = __shfl_sync(0xffffffffu, p_ids, rel & 31);
+    }
     if (lane == 0) {
       ptx::fence_proxy_async_smem();
-      const uint32_t s = loaded % STAGES;
-      unsigned char* kd = tiles + (size_t)s * 2 * TILE;
-      const int row0 = (page * H + p.head) * 32;
-      ptx::mbar_expect_tx(&full[s], 2 * TILE);
+      const CUtensorMap* map = p_value ? &vmap : &kmap;
+      ptx::mbar_expect_tx(&full[load_slot], TILE);
 #pragma unroll
-      for (int b = 0; b < (FP8 ? 1 : D / 64); ++b) {
-        ptx::tma_load_3d(kd + b * 4096, &kmap, b * 64, row0, a.layer, &full[s]);
-        ptx::tma_load_3d(kd + TILE + b * 4096, &vmap, b * 64, row0, a.layer, &full[s]);
-      }
+      for (int b = 0; b < (FP8 ? 1 : D / 64); ++b) ptx::tma_load_3d(tiles + load_slot * TILE + b * 4096, map, b * 64, (p_id * H + p_head) * 32, a.layer, &full[load_slot]);
     }
     ++loaded;
-    if (++p_page >= p.page_end) enter();
+    if (++load_slot == STAGES) load_slot = 0;
+    if (p_value && ++p_page >= p_end) enter();
+    p_value = !p_value;
   };
   enter();
-  for (int i = 0; i < STAGES; ++i) load_page();
+  for (int i = 0; i < STAGES; ++i) load_tile();
 
   bool alive = true;
-  uint32_t used = 0;
+  uint32_t used = 0, use_slot = 0, use_lap = 0;
+  auto next_tile = [&]() {  // the address of the next tile in turn, when it is there
+    alive = ptx::mbar_wait(&full[use_slot], use_lap & 1u);
+    return ptx::smem_u32(tiles + use_slot * TILE);
+  };
+  auto done_tile = [&]() {
+    __syncwarp();
+    ++used;
+    if (++use_slot == STAGES) { use_slot = 0; ++use_lap; }
+    load_tile();
+  };
   const int ld_r = lane & 7, ld_m = lane >> 3;
   for (uint32_t n = 0; alive; ++n) {
     const int id = queue[n % Z::QUEUE];
     if (id < 0) break;
-    const WarpItem it = warp_item(a, id);
+    const ItemB it = a.p.items_b[id / H];
+    const int item_head = id % H;
     // a node of more than 16 query rows does not come here: its members are all in this item
-    const int members = it.rows < 0 ? 1 : it.rows;
+    const int members = max(it.count, 1);
     const bool low = members * G > 8;  // whether rows 8 to 15 of the tile are used
     int row[2], slot[2], qh[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = g + 8 * h, m = r / G;
       row[h] = slot[h] = -1;
-      qh[h] = it.head * G + r - m * G;
+      qh[h] = item_head * G + r - m * G;
       if (m < members) {
-        if (it.rows < 0) { row[h] = it.first; slot[h] = a.p.own_slot[it.first] + it.chunk; }
-        else { const Member mb = a.p.members[it.first + m]; row[h] = mb.row; slot[h] = mb.slot + it.chunk; }
+        if (it.count == 0) { row[h] = it.first; slot[h] = it.part; }
+        else { const Member mb = a.p.members[it.first + m]; row[h] = mb.row; slot[h] = mb.slot + it.part; }
       }
     }
     uint32_t qa[KS][4];
@@ -531,15 +521,15 @@ __global__ void __launch_bounds__(kBWarps * 32, 1) prefix_warp_kernel(const __gr
     float my_ks = 1.f, my_vr = 1.f, v_ref = 1.f;
     auto page_scales = [&](int page0) {  // lane i: the scales of page page0 + i
       my_ks = 0.f; my_vr = 0.f;
-      if (page0 + lane < it.page_end) {
-        const size_t at = ((size_t)a.layer * a.d.n_pages + table_of(a, it.seq)[page0 + lane]) * H + it.head;
+      if (page0 + lane < it.p1) {
+        const size_t at = ((size_t)a.layer * a.d.n_pages + table_of(a, it.seq)[page0 + lane]) * H + item_head;
         my_ks = a.d.k_scale[at];
         my_vr = a.d.v_scale[at];
       }
     };
     if constexpr (FP8) {
       v_ref = 0.f;
-      for (int base = it.page_begin; base < it.page_end; base += 32) { page_scales(base); v_ref = fmaxf(v_ref, my_vr); }
+      for (int base = it.p0; base < it.p1; base += 32) { page_scales(base); v_ref = fmaxf(v_ref, my_vr); }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) v_ref = fmaxf(v_ref, __shfl_xor_sync(0xffffffffu, v_ref, o));
     }
@@ -549,18 +539,16 @@ __global__ void __launch_bounds__(kBWarps * 32, 1) prefix_warp_kernel(const __gr
 #pragma unroll
     for (int j = 0; j < NO; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     float m_run[2] = {kNoScale, kNoScale}, l_run[2] = {0.f, 0.f};
-    for (int pg = it.page_begin; pg < it.page_end; ++pg) {
-      const uint32_t st = used % STAGES;
-      alive = ptx::mbar_wait(&full[st], (used / STAGES) & 1u);
+    for (int pg = it.p0; pg < it.p1; ++pg) {
+      const uint32_t kbase = next_tile();
       if (!alive) break;
       float ks = a.scale_log2, vr = 1.f;
       if constexpr (FP8) {
-        const int rel = pg - it.page_begin;
+        const int rel = pg - it.p0;
         if ((rel & 31) == 0) page_scales(pg);
         ks = __shfl_sync(0xffffffffu, my_ks, rel & 31) * a.scale_log2;
         vr = __shfl_sync(0xffffffffu, my_vr, rel & 31) * v_inv;
       }
-      const uint32_t kbase = ptx::smem_u32(tiles + (size_t)st * 2 * TILE), vbase = kbase + TILE;
       float sc[4][4];
 #pragma unroll
       for (int nt = 0; nt < 4; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
@@ -587,6 +575,7 @@ __global__ void __launch_bounds__(kBWarps * 32, 1) prefix_warp_kernel(const __gr
             mma<false>(sc[nt], qa[2 * kk + 1], b[2], b[3]);
           }
       }
+      done_tile();  // (the scores are in registers)
       const int left = it.ctx - pg * 32;  // keys of this page that are seen
       uint32_t pa[2][4];
       float corr[2] = {1.f, 1.f};
@@ -628,6 +617,8 @@ __global__ void __launch_bounds__(kBWarps * 32, 1) prefix_warp_kernel(const __gr
 #pragma unroll
         for (int j = 0; j < NO; ++j) { o[j][0] *= corr[0]; o[j][1] *= corr[0]; o[j][2] *= corr[1]; o[j][3] *= corr[1]; }
       }
+      const uint32_t vbase = next_tile();
+      if (!alive) break;
       const bool whole = left >= 32;  // else what lies behind the context may be anything, and 0 times it no number
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
@@ -664,9 +655,7 @@ __global__ void __launch_bounds__(kBWarps * 32, 1) prefix_warp_kernel(const __gr
           }
         }
       }
-      __syncwarp();
-      ++used;
-      load_page();
+      done_tile();
     }
     if (!alive) break;
 #pragma unroll
@@ -697,12 +686,15 @@ __global__ void __launch_bounds__(kBWarps * 32, 1) prefix_warp_kernel(const __gr
 }
 
 // ---- large nodes: tcgen05 ---------------------------------------------------------------------------------------------------
-// Warps 0-3 and 4-7: softmax, a thread per row of a tile; warp 8: loads of pages; warp 9: products; warps 12-15: the item's rows of q (rows of any
-// sequences, so by 16-byte copies), and on FP8 pools K and V to bf16.  An item of two tiles has both use every block of keys; one of one tile has its
-// blocks in turn to the two softmax groups, with sums and parts of their own.  The scores are read twice, for their maximum and for P, so that 512
-// threads have registers enough.  A row keeps its scale until a score is 2^kLate above it: all that a late scale costs is that the largest weight
-// is no longer 1, and so is rounded like the others.
-constexpr int kAThreads = 512;
+// Warps 0-7 and 8-15: softmax of a tile each, two threads a row (64 of a block's 128 keys); warp 16: loads of pages; warp 17: products; on FP8 pools warps
+// 18 and 19 widen the pages' codes to f16, which is exact, q and P being f16 there too.  An item of two tiles has both use every block of keys; one of one
+// tile has its blocks in turn to the two softmax groups, with sums and parts of their own.
+// A row keeps its scale until a score is 2^kLate above it, so that a block is one vote of its tile's threads and no exchange of maxima: all that a late
+// scale costs is that the largest weight is no longer 1, and so is rounded like the others.
+// (With one thread a row, two warps on each of the SM's quarters, a block of 128 keys took 4900 cycles: 3560 of softmax, which had nothing to hide its
+// latency behind, and 1350 until the next scores were there.)
+constexpr int kSoftWarps = 16, kLoadWarp = 16, kMmaWarp = 17, kWidenWarps = 2, kWiden = kWidenWarps * 32;
+__host__ __device__ constexpr int threads_a(bool fp8) { return (kMmaWarp + 1 + (fp8 ? kWidenWarps : 0)) * 32; }
 constexpr float kLate = 4.f;
 
 template <int D, bool FP8>
@@ -715,6 +707,7 @@ template <int D, bool FP8>
 struct SharedA {
   using Z = ShapeA<D, FP8>;
   uint64_t full[Z::SLOTS], free[Z::SLOTS], raw_full[4], raw_free[4], q_full, q_free, s_full[2], p_ready[2], o_full[2], item_full[2], item_free[2], drain;
+  float exchange[2][2][kTileRows];  // [tile][half of the keys]: a row's maximum, its sum
   int item[2][8];  // {kind, head, seq, first member, members, first page, last page + 1, chunk}; kind: tiles of rows, 0 = no more
   uint32_t tmem;
 };
@@ -722,6 +715,12 @@ struct SharedA {
 template <int D, bool FP8>
 constexpr size_t shared_a() { return 2 * ShapeA<D, FP8>::QBYTES + ShapeA<D, FP8>::SLOTS * ShapeA<D, FP8>::SLOT + ShapeA<D, FP8>::RAWS * ShapeA<D, FP8>::RAW + sizeof(SharedA<D, FP8>); }
 
+// Waits for the 256 softmax threads of tile g; whether any of them says so.
+__device__ __forceinline__ bool any_of_tile(int g, bool mine) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred.aligned q, %2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"(mine ? 1u : 0u), "r"(g + 1) : "memory");
+  return r != 0;
+}
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -729,7 +728,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 template <int D, bool FP8>
-__global__ void __launch_bounds__(kAThreads, 1) prefix_node_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(threads_a(FP8), 1) prefix_node_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Args a) {
   wait_previous();
   using Z = ShapeA<D, FP8>;
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -741,21 +740,21 @@ __global__ void __launch_bounds__(kAThreads, 1) prefix_node_kernel(const __grid_
   const int n_items = a.p.hdr[H_ITEMS_A] * a.d.n_kv_heads;
   if (n_items == 0) return;  // (the whole grid)
   if (threadIdx.x == 0) {
-    for (int s = 0; s < Z::SLOTS; ++s) { ptx::mbar_init(&sh.full[s], FP8 ? 128 : 1); ptx::mbar_init(&sh.free[s], 1); }
-    for (int s = 0; s < 4; ++s) { ptx::mbar_init(&sh.raw_full[s], 1); ptx::mbar_init(&sh.raw_free[s], 128); }
-    ptx::mbar_init(&sh.q_full, 128);
+    for (int s = 0; s < Z::SLOTS; ++s) { ptx::mbar_init(&sh.full[s], FP8 ? kWiden : 1); ptx::mbar_init(&sh.free[s], 1); }
+    for (int s = 0; s < 4; ++s) { ptx::mbar_init(&sh.raw_full[s], 1); ptx::mbar_init(&sh.raw_free[s], kWiden); }
+    ptx::mbar_init(&sh.q_full, kSoftWarps * 32);
     ptx::mbar_init(&sh.q_free, 1);
     for (int t = 0; t < 2; ++t) {
       ptx::mbar_init(&sh.s_full[t], 1);
-      ptx::mbar_init(&sh.p_ready[t], kTileRows);
+      ptx::mbar_init(&sh.p_ready[t], kSoftWarps * 16);
       ptx::mbar_init(&sh.o_full[t], 1);
       ptx::mbar_init(&sh.item_full[t], 1);
-      ptx::mbar_init(&sh.item_free[t], 13);  // products, eight warps of softmax, four of q
+      ptx::mbar_init(&sh.item_free[t], 1 + kSoftWarps + (FP8 ? kWidenWarps : 0));
     }
     ptx::mbar_init(&sh.drain, 1);
     ptx::mbar_fence_init();
   }
-  if (warp == 9) {
+  if (warp == kMmaWarp) {
     ptx::tmem_alloc(&sh.tmem, 512);
     ptx::tmem_relinquish();
   }
@@ -767,19 +766,17 @@ __global__ void __launch_bounds__(kAThreads, 1) prefix_node_kernel(const __grid_
   auto tmem_o = [&](int t) { return tmem + (uint32_t)(256 + t * D); };
   bool ok = (ptx::smem_u32(smem) & 1023) == 0;
   const int G = a.group, members = tile_members(G);
-  // The next item of the list into `it`; false at its end.  Everybody but the loads takes items from there in the same order.
-  auto next_item = [&](uint32_t n, int (&it)[8]) {
+  // The next item of the list into `it`.  Everybody but the loads takes items from there in the same order.
+  auto take_item = [&](uint32_t n, int (&it)[8]) {
     wait(&sh.item_full[n & 1u], (n >> 1) & 1u, ok);
-    ok = __all_sync(0xffffffffu, ok);
-    if (!ok) return false;
+    __syncwarp();
 #pragma unroll
     for (int i = 0; i < 8; ++i) it[i] = sh.item[n & 1u][i];
     __syncwarp();
     if (lane == 0) ptx::mbar_arrive(&sh.item_free[n & 1u]);
-    return it[0] != 0;
   };
 
-  if (warp == 8) {
+  if (warp == kLoadWarp) {
     // ---- pages; the warp stays together, lane 0 issues ----
     uint32_t loads = 0;
     constexpr int RING = FP8 ? 4 : Z::SLOTS;
@@ -788,29 +785,21 @@ __global__ void __launch_bounds__(kAThreads, 1) prefix_node_kernel(const __grid_
       wait(bar, parity, ok);
       ok = __all_sync(0xffffffffu, ok);
     };
-    const int chunk_pages = a.p.hdr[H_PAGES_A];
     for (uint32_t n = 0;; ++n) {
-      int id = 0;
-      if (lane == 0) id = atomicAdd(&a.p.hdr[H_NEXT_A], 1);
-      id = __shfl_sync(0xffffffffu, id, 0);
-      wait_all(&sh.item_free[n & 1u], ((n >> 1) & 1u) ^ 1u);
-      int kind = 0, head = 0, seq = 0, p0 = 0, p1 = 0;
-      if (ok && id < n_items) {
-        const ItemA it = a.p.items_a[id / a.d.n_kv_heads];
-        const Node nd = a.p.nodes[it.node];
-        const int before = it.tile * 2 * members, count = min(2 * members, nd.count - before);
-        head = id % a.d.n_kv_heads;
-        seq = nd.seq;
-        kind = count > members ? 2 : 1;
-        p0 = nd.p0 + it.chunk * chunk_pages;
-        p1 = (int)min((long long)p0 + chunk_pages, (long long)nd.p1);
-        if (lane == 0) {
-          int* to = sh.item[n & 1u];
-          to[1] = head; to[2] = seq; to[3] = nd.first + before; to[4] = count; to[5] = p0; to[6] = p1; to[7] = it.chunk;
-        }
+      int id = blockIdx.x;  // (the counter hands out what is behind the first round)
+      if (n > 0) {
+        if (lane == 0) id = gridDim.x + atomicAdd(&a.p.hdr[H_NEXT_A], 1);
+        id = __shfl_sync(0xffffffffu, id, 0);
       }
+      const bool there = id < n_items;
+      ItemA it{};
+      if (there) it = a.p.items_a[id / a.d.n_kv_heads];
+      const int head = id % a.d.n_kv_heads, seq = it.seq, p0 = it.p0, p1 = it.p1;
+      wait_all(&sh.item_free[n & 1u], ((n >> 1) & 1u) ^ 1u);
+      const int kind = ok && there ? (it.count > members ? 2 : 1) : 0;
       if (lane == 0) {
-        sh.item[n & 1u][0] = kind;
+        int* to = sh.item[n & 1u];
+        to[0] = kind; to[1] = head; to[2] = seq; to[3] = it.first; to[4] = it.count; to[5] = p0; to[6] = p1; to[7] = it.part;
         ptx::mbar_arrive(&sh.item_full[n & 1u]);
       }
       __syncwarp();
@@ -854,10 +843,11 @@ __global__ void __launch_bounds__(kAThreads, 1) prefix_node_kernel(const __grid_
       bool drained = true;
       for (uint32_t i = loads > (uint32_t)RING ? loads - RING : 0; i < loads; ++i) wait(&full[i % RING], (i / RING) & 1u, drained);
     }
-  } else if (warp == 9) {
+  } else if (warp == kMmaWarp) {
     // ---- products ----
     if (ptx::elect_one()) {
-      const uint32_t id_s = ptx::umma_idesc_bf16(kTileRows, kBlockKeys), id_o = ptx::umma_idesc_bf16(kTileRows, D) | ptx::kUmmaBMn;
+      constexpr uint32_t kF16 = ~((1u << 7) | (1u << 10));  // both operands
+      const uint32_t id_s = ptx::umma_idesc_bf16(kTileRows, kBlockKeys) & (FP8 ? kF16 : ~0u), id_o = (ptx::umma_idesc_bf16(kTileRows, D) | ptx::kUmmaBMn) & (FP8 ? kF16 : ~0u);
       const uint64_t q_desc = ptx::umma_desc_k_sw128(ptx::smem_u32(qbuf)), k_desc = ptx::umma_desc_k_sw128(ptx::smem_u32(ring));
       const uint64_t v_desc = ptx::umma_desc_mn_sw128(ptx::smem_u32(ring), kBlockKeys * 128);
       uint32_t n_p[2] = {0, 0}, n_q = 0, load0 = 0;  // softmaxes waited for; items; loads of the items before
@@ -951,194 +941,227 @@ __global__ void __launch_bounds__(kAThreads, 1) prefix_node_kernel(const __grid_
       ok = ok && fine;
     }
     __syncwarp();
-  } else if (warp >= 12) {
-    // ---- rows of q; FP8: operands from codes ----
-    const int me = threadIdx.x - 12 * 32;
-    uint32_t loads = 0;
-    int it[8];
-    for (uint32_t n = 0; next_item(n, it); ++n) {
-      wait(&sh.q_free, (n & 1u) ^ 1u, ok);
-      __syncwarp();
-      constexpr int PIECES = D / 8;  // 16-byte pieces of a row
-#pragma unroll 4
-      for (int i = me; i < it[0] * kTileRows * PIECES; i += 128) {
-        const int c = i % PIECES, r = i / PIECES % kTileRows, tile = i / (PIECES * kTileRows);
-        const int m = r / G, head = r - m * G, member = tile * members + m;
-        const bool there = m < members && member < it[4];
-        const int row = there ? a.p.members[it[3] + member].row : 0;
-        const __nv_bfloat16* src = a.q + (size_t)row * a.q_stride + (size_t)(it[1] * G + (there ? head : 0)) * D + c * 8;
-        const uint32_t dst = ptx::smem_u32(qbuf + tile * Z::QBYTES + (c >> 3) * (kTileRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-      }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      ptx::fence_proxy_async_smem();
-      ptx::mbar_arrive(&sh.q_full);
-      if constexpr (FP8) {
-        const int nb = (it[6] - it[5] + kBlockPages - 1) / kBlockPages;
-        for (int k = 0; k < 2 * nb; ++k, ++loads) {
-          const uint32_t from = loads % 4, to = loads % Z::SLOTS;
-          wait(&sh.raw_full[from], (loads / 4) & 1u, ok);
-          wait(&sh.free[to], ((loads / Z::SLOTS) & 1u) ^ 1u, ok);
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          const unsigned char* src = raw + from * Z::RAW + me * 128;  // a key per thread
-          unsigned char* dst = ring + to * Z::SLOT + me * 128;
-#pragma unroll
-          for (int c = 0; c < D / 16; ++c) {
-            const uint4 w = *reinterpret_cast<const uint4*>(src + ((c ^ (me & 7)) << 4));
-            const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-            uint32_t y[8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const uint32_t f16 = e4m3x2_to_f16x2(x[i] >> (16 * h));
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&f16));
-                y[2 * i + h] = pack_bf16(f.x, f.y);
-              }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int cc = 2 * c + h;
-              *reinterpret_cast<uint4*>(dst + (cc >> 3) * kBlockKeys * 128 + (((cc & 7) ^ (me & 7)) << 4)) = make_uint4(y[4 * h], y[4 * h + 1], y[4 * h + 2], y[4 * h + 3]);
-            }
-          }
-          ptx::fence_proxy_async_smem();
-          ptx::mbar_arrive(&sh.raw_free[from]);
-          ptx::mbar_arrive(&sh.full[to]);
-        }
-      }
-    }
-  } else if (warp < 8) {
-    // ---- softmax: a thread per row ----
-    const int g = warp >> 2, r = (warp & 3) * 32 + lane, m = r / G, head = r - m * G;
+  } else if (warp < kSoftWarps) {
+    // ---- the item's rows of q, then softmax: two threads per row ----
+    const int g = warp >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane, m = r / G, head = r - m * G;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     uint32_t n_s = 0, n_o = 0;
-    int it[8];
-    for (uint32_t n = 0; next_item(n, it); ++n) {
+    for (uint32_t n = 0;; ++n) {
+      int it[8];
+      take_item(n, it);
+      if (any_of_tile(g, !ok)) { ok = false; break; }  // (a tile's threads meet at barriers that wait without limit, so they leave together)
+      if (it[0] == 0) break;
+      wait(&sh.q_free, (n & 1u) ^ 1u, ok);
+      {
+        constexpr int PIECES = D / 8;  // 16-byte pieces of a row
+#pragma unroll
+        for (int i = threadIdx.x & 255; i < kTileRows * PIECES && g < it[0]; i += 256) {  // a tile's threads its rows: what they read at the end passes through there
+          const int c = i % PIECES, qr = i / PIECES, tile = g;
+          const int qm = qr / G, qh = qr - qm * G, member = tile * members + qm;
+          const bool there = qm < members && member < it[4];
+          const int row = there ? a.p.members[it[3] + member].row : 0;
+          const __nv_bfloat16* src = a.q + (size_t)row * a.q_stride + (size_t)(it[1] * G + (there ? qh : 0)) * D + c * 8;
+          const uint32_t dst = ptx::smem_u32(qbuf + tile * Z::QBYTES + (c >> 3) * (kTileRows * 128) + qr * 128 + (((c & 7) ^ (qr & 7)) << 4));
+          const uint4 w = there ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
+          uint32_t x[4] = {w.x, w.y, w.z, w.w};
+          if constexpr (FP8) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = pack_f16(ptx::bf16_lo(x[e]), ptx::bf16_hi(x[e]));
+          }
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+        }
+      }
+      ptx::fence_proxy_async_smem();
+      ptx::mbar_arrive(&sh.q_full);
       const bool alone = it[0] == 1;  // one tile of rows: the groups take the blocks in turn
       const int n_pages = it[6] - it[5], nb = (n_pages + kBlockPages - 1) / kBlockPages, member = (alone ? 0 : g * members) + m;
       const bool on = m < members && member < it[4];
+      const int slot = on ? a.p.members[it[3] + member].slot + it[7] + (alone ? g : 0) : 0;
       const int j0 = alone ? g : 0, step = alone ? 2 : 1;
-      float scale = kNoScale, l = 0.f;  // log2 units
-      float my_ks = 0.f, my_vs = 0.f;
+      float scale = kNoScale, l = 0.f;  // log2 units; the sum of this thread's keys
+      float my_ks = 0.f, my_vs = 0.f, v_ref = 1.f;
+      auto page_scales = [&](int page0) {  // lane i: the scales of page page0 + i of the item
+        my_ks = my_vs = 0.f;
+        if (page0 + lane < n_pages) {
+          const size_t at = ((size_t)a.layer * a.d.n_pages + table_of(a, it[2])[it[5] + page0 + lane]) * a.d.n_kv_heads + it[1];
+          my_ks = a.d.k_scale[at];
+          my_vs = a.d.v_scale[at];
+        }
+      };
+      if constexpr (FP8) {  // P is multiplied by a page's V scale over the item's largest
+        v_ref = 0.f;
+        for (int base = 0; base < n_pages; base += 32) { page_scales(base); v_ref = fmaxf(v_ref, my_vs); }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v_ref = fmaxf(v_ref, __shfl_xor_sync(0xffffffffu, v_ref, o));
+      }
+      const float v_inv = v_ref > 0.f ? 1.0f / v_ref : 0.f;
+      const uint32_t t_s = tmem_s(g) + lanes, t_o = tmem_o(g) + lanes + half * (D / 2);
       for (int j = j0; j < nb; j += step) {
-        const int pages = min(kBlockPages, n_pages - j * kBlockPages);
-        float ks[kBlockPages], vs[kBlockPages];
-        if constexpr (FP8) {  // lane i: the scales of page i of a run of 32
+        const int pages = min(kBlockPages, n_pages - j * kBlockPages) - 2 * half;  // of this thread's two that there are
+        float ks[2] = {a.scale_log2, a.scale_log2}, vs[2] = {1.f, 1.f};
+        if constexpr (FP8) {
           const int rel = j * kBlockPages;
-          if (j < j0 + step || (rel & 31) < kBlockPages * step) {
-            const int pg = (rel & ~31) + lane;
-            my_ks = my_vs = 0.f;
-            if (pg < n_pages) {
-              const size_t at = ((size_t)a.layer * a.d.n_pages + table_of(a, it[2])[it[5] + pg]) * a.d.n_kv_heads + it[1];
-              my_ks = a.d.k_scale[at];
-              my_vs = a.d.v_scale[at];
-            }
-          }
+          if (j < j0 + step || (rel & 31) < kBlockPages * step) page_scales(rel & ~31);
 #pragma unroll
-          for (int c = 0; c < kBlockPages; ++c) {
-            ks[c] = __shfl_sync(0xffffffffu, my_ks, (rel & 31) + c) * a.scale_log2;
-            vs[c] = __shfl_sync(0xffffffffu, my_vs, (rel & 31) + c);
+          for (int c = 0; c < 2; ++c) {
+            ks[c] = __shfl_sync(0xffffffffu, my_ks, (rel & 31) + 2 * half + c) * a.scale_log2;
+            vs[c] = __shfl_sync(0xffffffffu, my_vs, (rel & 31) + 2 * half + c) * v_inv;
           }
-        } else {
-#pragma unroll
-          for (int c = 0; c < kBlockPages; ++c) { ks[c] = a.scale_log2; vs[c] = 1.f; }
         }
         wait(&sh.s_full[g], n_s & 1u, ok);
         ++n_s;
         ptx::tc_fence_after_sync();
         __syncwarp();
-        const uint32_t t_s = tmem_s(g) + lanes, t_o = tmem_o(g) + lanes;
+        uint32_t u[2][32];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) ptx::tmem_ld32(t_s + half * 64 + c * 32, u[c]);
+        ptx::tmem_ld_wait();
+        if (pages < 2) {  // (columns behind the last page hold anything)
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            if (c >= pages) {
+              ks[c] = a.scale_log2;
+#pragma unroll
+              for (int i = 0; i < 32; ++i) u[c][i] = __float_as_uint(kHidden);
+            }
+        }
         float top = kHidden;
 #pragma unroll
-        for (int c = 0; c < kBlockPages; ++c) {
-          if (c >= pages) break;
-          uint32_t u[32];
-          ptx::tmem_ld32(t_s + c * 32, u);
-          ptx::tmem_ld_wait();
+        for (int c = 0; c < 2; ++c) {
           float mx[4] = {kHidden, kHidden, kHidden, kHidden};
 #pragma unroll
-          for (int i = 0; i < 32; ++i) mx[i & 3] = max_nan(mx[i & 3], __uint_as_float(u[i]));
+          for (int i = 0; i < 32; ++i) mx[i & 3] = max_nan(mx[i & 3], __uint_as_float(u[c][i]));
           top = max_nan(top, max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * ks[c]);
         }
-        // A score that is no number weighs nothing, as a hidden one does.
-        const bool odd = __any_sync(0xffffffffu, top != top);
-        if (odd) {
+        if (__any_sync(0xffffffffu, top != top)) {  // a score that is no number weighs nothing, as a hidden one does
           top = kHidden;
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float x = fmaxf(__uint_as_float(u[c][i]), kHidden);
+              u[c][i] = __float_as_uint(x);
+              top = fmaxf(top, x * ks[c]);
+            }
+        }
+        ptx::tc_fence_before_sync();
+        if (any_of_tile(g, top > scale + kLate)) {  // (behind it, too, all the tile's scores are in registers, and P may take their place)
+          sh.exchange[g][half][r] = top;
+          any_of_tile(g, false);
+          top = fmaxf(top, sh.exchange[g][half ^ 1][r]);
+          const bool late = top > scale + kLate;
+          const float corr = late ? ex2(scale - top) : 1.f;
+          if (late) scale = top;
+          l *= corr;
+          ptx::tc_fence_after_sync();
+          if (j != j0 && __any_sync(0xffffffffu, late)) {  // (the scores' arrival says that the product before them is done)
 #pragma unroll 1
-          for (int c = 0; c < pages; ++c) {
-            uint32_t u[32];
-            ptx::tmem_ld32(t_s + c * 32, u);
-            ptx::tmem_ld_wait();
-            float k2 = ks[0];
+            for (int c = 0; c < D / 2; c += 16) {
+              uint32_t w[16];
+              ptx::tmem_ld16(t_o + c, w);
+              ptx::tmem_ld_wait();
 #pragma unroll
-            for (int i = 1; i < kBlockPages; ++i) k2 = c == i ? ks[i] : k2;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(u[i]) * k2);
+              for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * corr);
+              ptx::tmem_st16(t_o + c, w);
+            }
           }
         }
-        const bool late = top > scale + kLate;
-        float corr = 1.f;
-        if (late) { corr = ex2(scale - top); scale = top; }
+        ptx::tc_fence_after_sync();
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         const float2 m2 = make_float2(-scale, -scale);
 #pragma unroll
-        for (int c = 0; c < kBlockPages; ++c) {
-          if (c >= pages) break;
-          uint32_t u[32], p[16];
-          ptx::tmem_ld32(t_s + c * 32, u);
-          ptx::tmem_ld_wait();
-          const float2 k2 = make_float2(ks[c], ks[c]);
+        for (int c = 0; c < 2; ++c) {
+          uint32_t p[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            float2 x = fma2(make_float2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])), k2, m2);
-            if (odd) x = make_float2(fmaxf(x.x, kHidden), fmaxf(x.y, kHidden));
+            const float2 x = fma2(make_float2(__uint_as_float(u[c][2 * i]), __uint_as_float(u[c][2 * i + 1])), make_float2(ks[c], ks[c]), m2);
             const float2 e = make_float2(ex2(x.x), ex2(x.y));
             sum[i & 1] = add2(sum[i & 1], e);
-            p[i] = FP8 ? pack_bf16(e.x * vs[c], e.y * vs[c]) : pack_bf16(e.x, e.y);
+            p[i] = FP8 ? pack_f16(e.x * vs[c], e.y * vs[c]) : pack_bf16(e.x, e.y);
           }
-          ptx::tmem_st16(t_s + c * 16, p);  // (over scores that have been read)
+          ptx::tmem_st16(t_s + half * 32 + c * 16, p);
         }
         const float2 both = add2(sum[0], sum[1]);
-        l = fmaf(l, corr, both.x + both.y);
-        if (j != j0 && __any_sync(0xffffffffu, late)) {  // (the scores' arrival says that the product before them is done)
-#pragma unroll
-          for (int c = 0; c < D; c += 32) {
-            uint32_t u[32];
-            ptx::tmem_ld32(t_o + c, u);
-            ptx::tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) * corr);
-            ptx::tmem_st32(t_o + c, u);
-          }
-        }
+        l += both.x + both.y;
         ptx::tmem_st_wait();
         ptx::tc_fence_before_sync();
         ptx::mbar_arrive(&sh.p_ready[g]);
       }
-      // ---- the row's part leaves ----
+      // ---- the row's part leaves, half of its columns from each thread ----
       if (j0 < nb) {
+        sh.exchange[g][half][r] = l;
+        any_of_tile(g, false);
+        l += sh.exchange[g][half ^ 1][r];
         wait(&sh.o_full[g], n_o & 1u, ok);
+        wait(&sh.q_free, n & 1u, ok);  // (all the item's scores have been computed: both groups' may come from the first tile)
         ++n_o;
         ptx::tc_fence_after_sync();
         __syncwarp();
-        size_t at = 0;
-        if (on) {
-          const int slot = a.p.members[it[3] + member].slot + (alone ? 2 * it[7] + g : it[7]);
-          at = (size_t)slot * a.n_q_heads + (size_t)it[1] * G + head;
-          *reinterpret_cast<float2*>(a.p.part_ml + at * 2) = make_float2(scale, l);
-        }
-        float* po = a.p.part_o + at * D;
+        const int q_head = it[1] * G + head;
+        if (on && half == 0) *reinterpret_cast<float2*>(a.p.part_ml + ((size_t)slot * a.n_q_heads + q_head) * 2) = make_float2(scale, l);
+        // 16 columns of 32 rows at a time through the tile's place for q (its products are done), so that four lanes write 64 bytes of a row
+        unsigned char* pass = qbuf + g * Z::QBYTES + (warp & 7) * 2048;
+        const int row4 = lane >> 2, piece4 = lane & 3;
 #pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          uint32_t u[32];
-          ptx::tmem_ld32(tmem_o(g) + lanes + c, u);
+        for (int c = 0; c < D / 2; c += 16) {
+          uint32_t w[16];
+          ptx::tmem_ld16(t_o + c, w);
           ptx::tmem_ld_wait();
-          if (on) {
+          if constexpr (FP8) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(po + c + i) = make_uint4(u[i], u[i + 1], u[i + 2], u[i + 3]);
+            for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * v_ref);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(pass + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int from = row4 + 8 * i;  // a row of this warp
+            const int to_slot = __shfl_sync(0xffffffffu, on ? slot : -1, from), to_head = __shfl_sync(0xffffffffu, q_head, from);
+            const uint4 v = *reinterpret_cast<const uint4*>(pass + from * 64 + ((piece4 ^ ((from >> 1) & 3)) << 4));
+            if (to_slot >= 0) *reinterpret_cast<uint4*>(a.p.part_o + ((size_t)to_slot * a.n_q_heads + to_head) * D + half * (D / 2) + c + piece4 * 4) = v;
+          }
+          __syncwarp();
+        }
+        ptx::fence_proxy_async_smem();
+        ptx::tc_fence_before_sync();
+        any_of_tile(g, false);  // (the sums have been read before the next maxima take their place)
+      }
+    }
+  } else if constexpr (FP8) {
+    // ---- operands from codes: two keys per thread ----
+    const int me = threadIdx.x - (kMmaWarp + 1) * 32;
+    uint32_t loads = 0;
+    for (uint32_t n = 0;; ++n) {
+      int it[8];
+      take_item(n, it);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok || it[0] == 0) break;
+      const int nb = (it[6] - it[5] + kBlockPages - 1) / kBlockPages;
+      for (int k = 0; k < 2 * nb; ++k, ++loads) {
+        const uint32_t from = loads % 4, to = loads % Z::SLOTS;
+        wait(&sh.raw_full[from], (loads / 4) & 1u, ok);
+        wait(&sh.free[to], ((loads / Z::SLOTS) & 1u) ^ 1u, ok);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+#pragma unroll
+        for (int key = me; key < kBlockKeys; key += kWiden) {
+          const unsigned char* src = raw + from * Z::RAW + key * 128;
+          unsigned char* dst = ring + to * Z::SLOT + key * 128;
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) {
+            const uint4 w = *reinterpret_cast<const uint4*>(src + ((c ^ (key & 7)) << 4));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t lo = h ? w.z : w.x, hi = h ? w.w : w.y;
+              const int cc = 2 * c + h;
+              *reinterpret_cast<uint4*>(dst + (cc >> 3) * kBlockKeys * 128 + (((cc & 7) ^ (key & 7)) << 4)) =
+                  make_uint4(e4m3x2_to_f16x2(lo), e4m3x2_to_f16x2(lo >> 16), e4m3x2_to_f16x2(hi), e4m3x2_to_f16x2(hi >> 16));
+            }
           }
         }
-        ptx::tc_fence_before_sync();
+        ptx::fence_proxy_async_smem();
+        ptx::mbar_arrive(&sh.raw_free[from]);
+        ptx::mbar_arrive(&sh.full[to]);
       }
     }
   }
@@ -1146,7 +1169,7 @@ __global__ void __launch_bounds__(kAThreads, 1) prefix_node_kernel(const __grid_
   ptx::tc_fence_before_sync();
   __syncthreads();
   ptx::tc_fence_after_sync();
-  if (warp == 9) ptx::tmem_dealloc(tmem, 512);
+  if (warp == kMmaWarp) ptx::tmem_dealloc(tmem, 512);
 }
 
 // ---- the join: a warp per (row, query head) -----------------------------------------------------------------------------------
@@ -1219,9 +1242,9 @@ b200_status launch_layer(const b200_kv* kv, const Args& a, cudaStream_t s) {
     B200_CUDA_TRY((cudaFuncSetAttribute(prefix_warp_kernel<D, FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ShapeB<D, FP8>::kShared)));
     configured = true;
   }
-  launch_after(prefix_node_kernel<D, FP8>, b200_sm_count(), kAThreads, shared_nodes, s, kv->kmap, kv->vmap, a);
+  launch_after(prefix_node_kernel<D, FP8>, b200_sm_count(), threads_a(FP8), shared_nodes, s, kv->kmap, kv->vmap, a);
   B200_LAUNCH_CHECK();
-  launch_after(prefix_warp_kernel<D, FP8>, b200_sm_count() * ShapeB<D, FP8>::PER_SM, kBWarps * 32, ShapeB<D, FP8>::kShared, s, kv->kmap, kv->vmap, a);
+  launch_after(prefix_warp_kernel<D, FP8>, b200_sm_count(), ShapeB<D, FP8>::WARPS * 32, ShapeB<D, FP8>::kShared, s, kv->kmap, kv->vmap, a);
   B200_LAUNCH_CHECK();
   launch_after(prefix_join_kernel<D>, (a.rows * a.n_q_heads + 7) / 8, 256, 0, s, a);
   B200_LAUNCH_CHECK();
@@ -1253,7 +1276,7 @@ extern "C" b200_status b200_prefix_attn_create(b200_kv* kv, int32_t max_rows, b2
   size_t bytes = 0;
   auto place = [&](size_t n) { const size_t at = bytes; bytes += (n + 255) / 256 * 256; return at; };
   const size_t r = max_rows, slots = p.max_slots;
-  const size_t hdr = place(sizeof(int) * H_COUNT), seq = place(4 * r), ctx = place(4 * r), from = place(4 * r), base = place(4 * (r + 1)), own = place(4 * r);
+  const size_t hdr = place(sizeof(int) * H_COUNT), seq = place(4 * r), ctx = place(4 * r), base = place(4 * (r + 1));
   const size_t nodes = place(sizeof(Node) * (kLevels * r / 2 + 1)), members = place(sizeof(Member) * kLevels * r), of_node = place(4 * kLevels * r);
   const size_t items_a = place(sizeof(ItemA) * slots), items_b = place(sizeof(ItemB) * slots);
   const size_t part_o = place(sizeof(float) * slots * c.n_q_heads * c.head_dim), part_ml = place(sizeof(float) * 2 * slots * c.n_q_heads);
@@ -1267,8 +1290,8 @@ extern "C" b200_status b200_prefix_attn_create(b200_kv* kv, int32_t max_rows, b2
     return B200_ERR_CUDA;
   }
   char* b = (char*)h->buf;
-  p.hdr = (int*)(b + hdr); p.row_seq = (int*)(b + seq); p.row_ctx = (int*)(b + ctx); p.row_from = (int*)(b + from); p.row_base = (int*)(b + base);
-  p.own_slot = (int*)(b + own); p.nodes = (Node*)(b + nodes); p.members = (Member*)(b + members); p.member_node = (int*)(b + of_node);
+  p.hdr = (int*)(b + hdr); p.row_seq = (int*)(b + seq); p.row_ctx = (int*)(b + ctx); p.row_base = (int*)(b + base);
+  p.nodes = (Node*)(b + nodes); p.members = (Member*)(b + members); p.member_node = (int*)(b + of_node);
   p.items_a = (ItemA*)(b + items_a); p.items_b = (ItemB*)(b + items_b); p.part_o = (float*)(b + part_o); p.part_ml = (float*)(b + part_ml);
   *out = h;
   return B200_OK;
@@ -1297,9 +1320,9 @@ extern "C" b200_status b200_prefix_attn_plan(b200_prefix_attn* h, const int32_t*
   }
   const b200_kv_config& c = h->kv->cfg;
   const bool fp8 = c.kv_dtype != B200_KV_BF16;
-  const int per_sm = fp8 ? ShapeB<128, true>::PER_SM : c.head_dim == 128 ? ShapeB<128, false>::PER_SM : ShapeB<64, false>::PER_SM;
+  const int warps = fp8 ? ShapeB<128, true>::WARPS : c.head_dim == 128 ? ShapeB<128, false>::WARPS : ShapeB<64, false>::WARPS;
   launch_after(prefix_plan_kernel, 1, rows <= 256 ? 256 : 1024, shared, (cudaStream_t)stream, h->kv->dev, h->p, d_row_seq, d_row_ctx, rows, hash,
-               c.n_q_heads / c.n_kv_heads, b200_sm_count(), b200_sm_count() * per_sm * kBWarps);
+               c.n_q_heads / c.n_kv_heads, b200_sm_count(), b200_sm_count() * warps);
   B200_LAUNCH_CHECK();
   return B200_OK;
 }
