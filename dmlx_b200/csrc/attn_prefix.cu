@@ -31,6 +31,7 @@ namespace {
 
 constexpr int kMaxRows = 4096;
 constexpr int kLevels = 3;        // nodes that a row may go through
+constexpr int kItemUnits = 44;    // of an item of the tensor-core kernel, beside its blocks
 constexpr int kMinPages = 2;      // of a node: below that a part of its own costs more than it saves
 constexpr int kWarpRows = 16;     // query rows of an item of the warps' kernel
 constexpr int kBlockKeys = 128, kBlockPages = 4, kTileRows = 128;
@@ -47,7 +48,7 @@ struct Member { int row, slot; };  // a row of a node; the place of its first pa
 struct alignas(16) ItemA { int seq, first, count, p0, p1, part, pad[2]; };  // pages of slot seq's table for `count` members from `first` on; their part behind `slot`
 struct alignas(16) ItemB { int seq, first, count, p0, p1, ctx, part, pad; };  // count 0: own pages of the row `first`, its part `part`, and ctx tokens that it sees; else members, as above
 
-enum { H_ITEMS_A = 0, H_ITEMS_B, H_PAGES_A, H_PAGES_B, H_NEXT_A, H_NEXT_B, H_NODES, H_WORKERS_A, H_COUNT = 16 };
+enum { H_ITEMS_A = 0, H_ITEMS_B, H_NEXT_A, H_NEXT_B, H_WORKERS_A, H_COUNT = 16 };  // H_WORKERS_A: blocks that work on the large nodes
 
 struct PlanDev {
   int *hdr, *row_seq, *row_ctx, *row_base, *member_node;
@@ -68,21 +69,22 @@ __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; 
 // Parts of a row of a node: a chunk gives one, or two where the item has one tile of rows and its blocks of keys go to the two softmax groups in turn.
 __device__ __forceinline__ bool is_large(int count, int group) { return count * group > kWarpRows; }
 __device__ __forceinline__ bool one_tile(const Node& n, int tile, int group) { return n.count - tile * 2 * tile_members(group) <= tile_members(group); }
+__device__ __forceinline__ int even_length(int pages, int len) { return ceil_div(ceil_div(pages, ceil_div(pages, len)), kBlockPages) * kBlockPages; }  // of as many chunks
 __device__ __forceinline__ int large_parts(int pages, int len, bool one) {  // len: pages of a chunk, a multiple of kBlockPages
   const int chunks = ceil_div(pages, len), last = pages - (chunks - 1) * len;
   return one ? 2 * chunks - (last <= kBlockPages ? 1 : 0) : chunks;
 }
 
-constexpr int kLengthsA = 7;  // pages of a chunk: all, 256, 128, 64, 32, 16, 8
-__device__ __forceinline__ int length_a(int k) { return k == 0 ? 1 << 28 : 512 >> k; }
+constexpr int kLengthsA = 12;  // pages of a chunk: all, 256, 192, 128, 96, ..., 12, 8
+__device__ __forceinline__ int length_a(int k) { return k == 0 ? 1 << 28 : k & 1 ? 512 >> (k + 1) / 2 : 384 >> k / 2; }
 constexpr int kLengthsB = 6;  // all, 32, 16, 8, 4, 2
 __device__ __forceinline__ int length_b(int k) { return k == 0 ? 1 << 28 : 64 >> k; }
 
 struct PlanShared {
-  int n_nodes, n_members, more, over, warp_sums[32], carry;
+  int n_nodes, n_members, more, warp_sums[32], carry;
   int max_a[kLengthsA], items_a[kLengthsA], units_a[kLengthsA], slots_a[kLengthsA];
   int items_b[kLengthsB], slots_b[kLengthsB];
-  int pick_a, pick_b, next_a, next_b;
+  int units_b, workers_a, pick_a, pick_b, next_a, next_b;
 };
 
 // Common pages of two sequences that agree up to `lo` (at least one page behind it too): a search in steps of 16 probes.
@@ -104,7 +106,7 @@ __device__ __forceinline__ int common_pages(const int* a, const int* b, int lo, 
 }
 
 __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, const int* row_seq, const int* row_ctx, int rows, int hash_size, int group,
-                                                           int workers, int warps) {
+                                                           int workers, int warps, float per_page) {
   after_previous();
   extern __shared__ __align__(16) unsigned char dyn[];
   unsigned long long* keys = reinterpret_cast<unsigned long long*>(dyn);  // [hash_size]
@@ -200,7 +202,7 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
   // ---- lengths of chunks ----
   if (tid < kLengthsA) { s.max_a[tid] = 0; s.items_a[tid] = 0; s.units_a[tid] = 0; s.slots_a[tid] = 0; }
   if (tid < kLengthsB) { s.items_b[tid] = 0; s.slots_b[tid] = 0; }
-  if (tid == 0) { s.next_a = 0; s.next_b = 0; s.carry = 0; }
+  if (tid == 0) { s.next_a = 0; s.next_b = 0; s.carry = 0; s.units_b = 0; }
   __syncthreads();
   const int n_nodes = s.n_nodes, members = tile_members(group), warp_members = kWarpRows / group;
   for (int i = tid; i < n_nodes; i += blockDim.x) {
@@ -211,11 +213,11 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
       const bool one = last <= members;
 #pragma unroll
       for (int k = 0; k < kLengthsA; ++k) {
-        // eighths of a block: two tiles of rows count 8, one 5; an item's fill, drain and way out 12
-        const int len = length_a(k), chunks = ceil_div(pages, len), blocks = ceil_div(pages, kBlockPages);
-        atomicMax(&s.max_a[k], (tiles > 1 || !one ? 8 : 5) * min(blocks, len / kBlockPages) + 12);
+        // eighths of a block: two tiles of rows count 8, one 5 (4060 cycles); an item's fill, drain and way out kItemUnits (22000)
+        const int len = even_length(pages, length_a(k)), chunks = ceil_div(pages, len), blocks = ceil_div(pages, kBlockPages);
+        atomicMax(&s.max_a[k], (tiles > 1 || !one ? 8 : 5) * min(blocks, len / kBlockPages) + kItemUnits);
         atomicAdd(&s.items_a[k], tiles * chunks);
-        atomicAdd(&s.units_a[k], (8 * (tiles - (one ? 1 : 0)) + (one ? 5 : 0)) * blocks + 12 * tiles * chunks);
+        atomicAdd(&s.units_a[k], (8 * (tiles - (one ? 1 : 0)) + (one ? 5 : 0)) * blocks + kItemUnits * tiles * chunks);
         atomicAdd(&s.slots_a[k], (n.count - (one ? last : 0)) * large_parts(pages, len, false) + (one ? last : 0) * large_parts(pages, len, true));
       }
     } else {
@@ -225,31 +227,48 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
         atomicAdd(&s.items_b[k], ceil_div(n.count, warp_members) * chunks);
         atomicAdd(&s.slots_b[k], n.count * chunks);
       }
+      atomicAdd(&s.units_b, ceil_div(n.count, warp_members) * pages);
     }
   }
-  int own_chunks[kLengthsB] = {};
+  int own_chunks[kLengthsB] = {}, own_pages = 0;
   for (int i = tid; i < rows; i += blockDim.x) {
     const int pages = ceil_div(p.row_ctx[i], d.page_size) - from[i];
 #pragma unroll
     for (int k = 0; k < kLengthsB; ++k) own_chunks[k] += ceil_div(pages, length_b(k));
+    own_pages += pages;
   }
 #pragma unroll
   for (int k = 0; k < kLengthsB; ++k) {
     const int c = __reduce_add_sync(0xffffffffu, own_chunks[k]);
     if (lane == 0) { atomicAdd(&s.items_b[k], c); atomicAdd(&s.slots_b[k], c); }
   }
+  own_pages = __reduce_add_sync(0xffffffffu, own_pages);
+  if (lane == 0) atomicAdd(&s.units_b, own_pages);
   __syncthreads();
-  if (tid == 0) {
-    const int heads = d.n_kv_heads;
-    int pick = 0;
-    long long best = 0;
-    for (int k = 0; k < kLengthsA; ++k) {  // the shortest estimated time of those whose parts fit
-      if (k > 0 && s.slots_a[k] + s.slots_b[0] > p.max_slots) continue;
-      const long long share = (long long)s.units_a[k] * heads / workers, waves = ((long long)s.items_a[k] * heads + workers - 1) / workers;
-      const long long cost = max(max((long long)s.max_a[k], share), waves * s.max_a[k] * 7 / 8) + s.slots_a[k] / 64;
-      if (k == 0 || cost < best) { best = cost; pick = k; }
+  if (warp == 0) {
+    // The rest runs beside the large nodes, on the SMs that they leave and on theirs when they are done.  Of an SM it takes 2.3 units an item and
+    // `per_page` a page (0.6 us and, of 128 dims in 16 bits, 0.2, on 37 to 74 SMs), and half as much again when all SMs do this at once, which the memory bounds.
+    // Chunks in some rounds of the blocks that the nodes get; the shortest estimated time of those whose parts fit, a lane per choice of the two.
+    const float rest = ((float)s.units_b * per_page + 2.3f * s.items_b[0]) * d.n_kv_heads;
+    float best = 3e38f;
+    int choice = 0;
+    for (int c = lane; c < 4 * kLengthsA; c += 32) {
+      const int k = c >> 2, items = s.items_a[k] * d.n_kv_heads, rounds = max(ceil_div(items, workers), 1) + (c & 3), mine = max(ceil_div(items, rounds), 1);
+      const float nodes = fmaxf((float)s.units_a[k] * d.n_kv_heads / mine, 0.875f * rounds * s.max_a[k]);
+      const float cost = nodes + fmaxf(rest - (workers - mine) * nodes, 0.f) * 1.5f / workers + s.slots_a[k] * 0.025f;
+      if ((k == 0 || s.slots_a[k] + s.slots_b[0] <= p.max_slots) && cost < best) { best = cost; choice = k << 16 | mine; }
     }
-    s.pick_a = pick;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float other = __shfl_xor_sync(0xffffffffu, best, o);
+      const int theirs = __shfl_xor_sync(0xffffffffu, choice, o);
+      if (other < best || (other == best && theirs < choice)) { best = other; choice = theirs; }
+    }
+    if (lane == 0) { s.pick_a = choice >> 16; s.workers_a = choice & 0xffff; }
+  }
+  __syncwarp();
+  if (tid == 0) {
+    const int heads = d.n_kv_heads, pick = s.pick_a;
     int pick_b = 0;  // the longest chunks that give every warp about two items, if their parts fit
     for (int k = 1; k < kLengthsB; ++k) {
       if (s.slots_a[pick] + s.slots_b[k] > p.max_slots) break;
@@ -266,7 +285,7 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
       const Node n = p.nodes[p.member_node[at]];
       const int row = p.members[at].row, pages = n.p1 - n.p0;
       p.members[at].slot = parts[row];
-      parts[row] += is_large(n.count, group) ? large_parts(pages, len_a, one_tile(n, (at - n.first) / (2 * members), group)) : ceil_div(pages, len_b);
+      parts[row] += is_large(n.count, group) ? large_parts(pages, even_length(pages, len_a), one_tile(n, (at - n.first) / (2 * members), group)) : ceil_div(pages, len_b);
     }
     __syncthreads();
   }
@@ -303,7 +322,7 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
   // items of the nodes, a warp per node
   for (int i = warp; i < n_nodes; i += blockDim.x / 32) {
     const Node n = p.nodes[i];
-    const int pages = n.p1 - n.p0, large = is_large(n.count, group) ? 1 : 0, len = min(large ? len_a : len_b, pages), chunks = ceil_div(pages, len);
+    const int pages = n.p1 - n.p0, large = is_large(n.count, group) ? 1 : 0, len = large ? even_length(pages, len_a) : min(len_b, pages), chunks = ceil_div(pages, len);
     const int tiles = large ? ceil_div(n.count, 2 * members) : 1;
     int at = 0;
     if (lane == 0) at = atomicAdd(large ? &s.next_a : &s.next_b, tiles * chunks);
@@ -323,12 +342,9 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
     p.row_base[rows] = s.carry;
     p.hdr[H_ITEMS_A] = s.next_a;
     p.hdr[H_ITEMS_B] = s.next_b;
-    p.hdr[H_PAGES_A] = len_a;
-    p.hdr[H_PAGES_B] = len_b;
     p.hdr[H_NEXT_A] = 0;
     p.hdr[H_NEXT_B] = 0;
-    p.hdr[H_NODES] = n_nodes;
-    p.hdr[H_WORKERS_A] = workers;
+    p.hdr[H_WORKERS_A] = s.workers_a;
   }
 }
 
@@ -411,8 +427,7 @@ struct ShapeB {
 // bf16: K and V as they are; FP8: the codes widened to f16 in registers (exact), K's dims and V's output columns in the order in which ldmatrix gives
 // the bytes, the page's K scale on the scores, its V scale (over the item's largest) on P.
 template <int D, bool FP8>
-__global__ void __launch_bounds__(ShapeB<D, FP8>::WARPS * 32, 1) prefix_warp_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Args a) {
-  wait_previous();
+__device__ __forceinline__ void warp_items(const CUtensorMap& kmap, const CUtensorMap& vmap, const Args& a) {
   using Z = ShapeB<D, FP8>;
   constexpr int TILE = Z::TILE, STAGES = Z::STAGES, KS = D / 16, NO = D / 8;
   extern __shared__ unsigned char smem_dyn[];
@@ -682,7 +697,13 @@ __global__ void __launch_bounds__(ShapeB<D, FP8>::WARPS * 32, 1) prefix_warp_ker
     for (uint32_t i = first > used ? first : used; i < loaded; ++i) ptx::mbar_wait(&full[i % STAGES], (i / STAGES) & 1u);
     if (lane == 0) atomicExch(a.d.state + ST_ATTN_ERR, B200_ERR_DEVICE_FLAGGED);
   }
-  let_next_start();
+}
+// The kernel ahead, the nodes', waits for all that is before it and then lets this one start, on the SMs that it leaves and later on its own.  Neither
+// reads what the other writes, and the waits here are for copies of its own, so this one waits for the nodes' only at its end: what follows waits for this one alone.
+template <int D, bool FP8>
+__global__ void __launch_bounds__(ShapeB<D, FP8>::WARPS * 32, 1) prefix_warp_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Args a) {
+  warp_items<D, FP8>(kmap, vmap, a);
+  wait_previous();
 }
 
 // ---- large nodes: tcgen05 ---------------------------------------------------------------------------------------------------
@@ -715,10 +736,10 @@ struct SharedA {
 template <int D, bool FP8>
 constexpr size_t shared_a() { return 2 * ShapeA<D, FP8>::QBYTES + ShapeA<D, FP8>::SLOTS * ShapeA<D, FP8>::SLOT + ShapeA<D, FP8>::RAWS * ShapeA<D, FP8>::RAW + sizeof(SharedA<D, FP8>); }
 
-// Waits for the 256 softmax threads of tile g; whether any of them says so.
-__device__ __forceinline__ bool any_of_tile(int g, bool mine) {
+// Waits for `count` threads, of whole warps, at barrier `id`; whether any of them says so.
+__device__ __forceinline__ bool any_of(int id, int count, bool mine) {
   uint32_t r;
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred.aligned q, %2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"(mine ? 1u : 0u), "r"(g + 1) : "memory");
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred.aligned q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"(mine ? 1u : 0u), "r"(id), "r"(count) : "memory");
   return r != 0;
 }
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -729,7 +750,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 
 template <int D, bool FP8>
 __global__ void __launch_bounds__(threads_a(FP8), 1) prefix_node_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Args a) {
-  wait_previous();
+  after_previous();  // (the warps' kernel takes the SMs that this one leaves)
   using Z = ShapeA<D, FP8>;
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char* qbuf = smem;                    // [tile][box][128 rows][128 B]
@@ -738,7 +759,8 @@ __global__ void __launch_bounds__(threads_a(FP8), 1) prefix_node_kernel(const __
   SharedA<D, FP8>& sh = *reinterpret_cast<SharedA<D, FP8>*>(raw + Z::RAWS * Z::RAW);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n_items = a.p.hdr[H_ITEMS_A] * a.d.n_kv_heads;
-  if (n_items == 0) return;  // (the whole grid)
+  const int workers = a.p.hdr[H_WORKERS_A];
+  if (n_items == 0 || (int)blockIdx.x >= workers) return;  // (whole blocks)
   if (threadIdx.x == 0) {
     for (int s = 0; s < Z::SLOTS; ++s) { ptx::mbar_init(&sh.full[s], FP8 ? kWiden : 1); ptx::mbar_init(&sh.free[s], 1); }
     for (int s = 0; s < 4; ++s) { ptx::mbar_init(&sh.raw_full[s], 1); ptx::mbar_init(&sh.raw_free[s], kWiden); }
@@ -788,7 +810,7 @@ __global__ void __launch_bounds__(threads_a(FP8), 1) prefix_node_kernel(const __
     for (uint32_t n = 0;; ++n) {
       int id = blockIdx.x;  // (the counter hands out what is behind the first round)
       if (n > 0) {
-        if (lane == 0) id = gridDim.x + atomicAdd(&a.p.hdr[H_NEXT_A], 1);
+        if (lane == 0) id = workers + atomicAdd(&a.p.hdr[H_NEXT_A], 1);
         id = __shfl_sync(0xffffffffu, id, 0);
       }
       const bool there = id < n_items;
@@ -881,7 +903,7 @@ __global__ void __launch_bounds__(threads_a(FP8), 1) prefix_node_kernel(const __
           wait(&sh.p_ready[t], n_p[t] & 1u, ok);
           ++n_p[t];
           ptx::tc_fence_after_sync();
-          for (int k = 0; k < steps; ++k) ptx::umma_bf16_tmem_a(tmem_o(t), tmem_s(t) + k * 8, v0 + k * (2048 >> 4), id_o, first && k == 0 ? 0u : 1u);
+          for (int k = 0; k < steps; ++k) ptx::umma_bf16_tmem_a(tmem_o(t), tmem_s(t) + (k >> 2) * 64 + (k & 3) * 8, v0 + k * (2048 >> 4), id_o, first && k == 0 ? 0u : 1u);
         };
         if (kind == 2) {
           arrived(0);
@@ -943,32 +965,43 @@ __global__ void __launch_bounds__(threads_a(FP8), 1) prefix_node_kernel(const __
     __syncwarp();
   } else if (warp < kSoftWarps) {
     // ---- the item's rows of q, then softmax: two threads per row ----
-    const int g = warp >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane, m = r / G, head = r - m * G;
+    const int g = warp >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane, m = r / G, head = r - m * G, pair = 1 + (warp >> 3) * 4 + (warp & 3);
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     uint32_t n_s = 0, n_o = 0;
     for (uint32_t n = 0;; ++n) {
       int it[8];
       take_item(n, it);
-      if (any_of_tile(g, !ok)) { ok = false; break; }  // (a tile's threads meet at barriers that wait without limit, so they leave together)
+      if (any_of(9 + g, 256, !ok)) { ok = false; break; }  // (a tile's threads meet at barriers that wait without limit, so they leave together)
       if (it[0] == 0) break;
       wait(&sh.q_free, (n & 1u) ^ 1u, ok);
       {
         constexpr int PIECES = D / 8;  // 16-byte pieces of a row
+        constexpr int EACH = kTileRows * PIECES / 256;  // of a thread, all under way at once
+        if (g < it[0]) {
+          uint4 w[EACH];
+          int row[EACH];
 #pragma unroll
-        for (int i = threadIdx.x & 255; i < kTileRows * PIECES && g < it[0]; i += 256) {  // a tile's threads its rows: what they read at the end passes through there
-          const int c = i % PIECES, qr = i / PIECES, tile = g;
-          const int qm = qr / G, qh = qr - qm * G, member = tile * members + qm;
-          const bool there = qm < members && member < it[4];
-          const int row = there ? a.p.members[it[3] + member].row : 0;
-          const __nv_bfloat16* src = a.q + (size_t)row * a.q_stride + (size_t)(it[1] * G + (there ? qh : 0)) * D + c * 8;
-          const uint32_t dst = ptx::smem_u32(qbuf + tile * Z::QBYTES + (c >> 3) * (kTileRows * 128) + qr * 128 + (((c & 7) ^ (qr & 7)) << 4));
-          const uint4 w = there ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
-          uint32_t x[4] = {w.x, w.y, w.z, w.w};
-          if constexpr (FP8) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = pack_f16(ptx::bf16_lo(x[e]), ptx::bf16_hi(x[e]));
+          for (int e = 0; e < EACH; ++e) {
+            const int qm = ((threadIdx.x & 255) + e * 256) / PIECES / G, qh = ((threadIdx.x & 255) + e * 256) / PIECES - qm * G, member = g * members + qm;
+            row[e] = qm < members && member < it[4] ? a.p.members[it[3] + member].row * G + qh : -1;
           }
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+#pragma unroll
+          for (int e = 0; e < EACH; ++e) {
+            const int c = threadIdx.x % PIECES, at = max(row[e], 0) / G;
+            const __nv_bfloat16* src = a.q + (size_t)at * a.q_stride + (size_t)(it[1] * G + max(row[e], 0) - at * G) * D + c * 8;
+            w[e] = row[e] >= 0 ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
+          }
+#pragma unroll
+          for (int e = 0; e < EACH; ++e) {
+            const int c = threadIdx.x % PIECES, qr = ((threadIdx.x & 255) + e * 256) / PIECES;
+            const uint32_t dst = ptx::smem_u32(qbuf + g * Z::QBYTES + (c >> 3) * (kTileRows * 128) + qr * 128 + (((c & 7) ^ (qr & 7)) << 4));
+            uint32_t x[4] = {w[e].x, w[e].y, w[e].z, w[e].w};
+            if constexpr (FP8) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x[i] = pack_f16(ptx::bf16_lo(x[i]), ptx::bf16_hi(x[i]));
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+          }
         }
       }
       ptx::fence_proxy_async_smem();
@@ -1045,9 +1078,9 @@ __global__ void __launch_bounds__(threads_a(FP8), 1) prefix_node_kernel(const __
             }
         }
         ptx::tc_fence_before_sync();
-        if (any_of_tile(g, top > scale + kLate)) {  // (behind it, too, all the tile's scores are in registers, and P may take their place)
+        if (any_of(pair, 64, top > scale + kLate)) {
           sh.exchange[g][half][r] = top;
-          any_of_tile(g, false);
+          any_of(pair, 64, false);
           top = fmaxf(top, sh.exchange[g][half ^ 1][r]);
           const bool late = top > scale + kLate;
           const float corr = late ? ex2(scale - top) : 1.f;
@@ -1079,7 +1112,7 @@ __global__ void __launch_bounds__(threads_a(FP8), 1) prefix_node_kernel(const __
             sum[i & 1] = add2(sum[i & 1], e);
             p[i] = FP8 ? pack_f16(e.x * vs[c], e.y * vs[c]) : pack_bf16(e.x, e.y);
           }
-          ptx::tmem_st16(t_s + half * 32 + c * 16, p);
+          ptx::tmem_st16(t_s + half * 64 + c * 16, p);  // (over scores of its own that are in registers)
         }
         const float2 both = add2(sum[0], sum[1]);
         l += both.x + both.y;
@@ -1089,10 +1122,10 @@ __global__ void __launch_bounds__(threads_a(FP8), 1) prefix_node_kernel(const __
       }
       // ---- the row's part leaves, half of its columns from each thread ----
       if (j0 < nb) {
-        sh.exchange[g][half][r] = l;
-        any_of_tile(g, false);
-        l += sh.exchange[g][half ^ 1][r];
         wait(&sh.o_full[g], n_o & 1u, ok);
+        sh.exchange[g][half][r] = l;  // (the sums are there, so all threads have read the last maxima)
+        any_of(pair, 64, false);
+        l += sh.exchange[g][half ^ 1][r];
         wait(&sh.q_free, n & 1u, ok);  // (all the item's scores have been computed: both groups' may come from the first tile)
         ++n_o;
         ptx::tc_fence_after_sync();
@@ -1102,6 +1135,12 @@ __global__ void __launch_bounds__(threads_a(FP8), 1) prefix_node_kernel(const __
         // 16 columns of 32 rows at a time through the tile's place for q (its products are done), so that four lanes write 64 bytes of a row
         unsigned char* pass = qbuf + g * Z::QBYTES + (warp & 7) * 2048;
         const int row4 = lane >> 2, piece4 = lane & 3;
+        int to_slot[4], to_head[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // of rows row4 + 8 i of this warp
+          to_slot[i] = __shfl_sync(0xffffffffu, on ? slot : -1, row4 + 8 * i);
+          to_head[i] = __shfl_sync(0xffffffffu, q_head, row4 + 8 * i);
+        }
 #pragma unroll
         for (int c = 0; c < D / 2; c += 16) {
           uint32_t w[16];
@@ -1116,16 +1155,15 @@ __global__ void __launch_bounds__(threads_a(FP8), 1) prefix_node_kernel(const __
           __syncwarp();
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int from = row4 + 8 * i;  // a row of this warp
-            const int to_slot = __shfl_sync(0xffffffffu, on ? slot : -1, from), to_head = __shfl_sync(0xffffffffu, q_head, from);
+            const int from = row4 + 8 * i;
             const uint4 v = *reinterpret_cast<const uint4*>(pass + from * 64 + ((piece4 ^ ((from >> 1) & 3)) << 4));
-            if (to_slot >= 0) *reinterpret_cast<uint4*>(a.p.part_o + ((size_t)to_slot * a.n_q_heads + to_head) * D + half * (D / 2) + c + piece4 * 4) = v;
+            if (to_slot[i] >= 0) *reinterpret_cast<uint4*>(a.p.part_o + ((size_t)to_slot[i] * a.n_q_heads + to_head[i]) * D + half * (D / 2) + c + piece4 * 4) = v;
           }
           __syncwarp();
         }
         ptx::fence_proxy_async_smem();
         ptx::tc_fence_before_sync();
-        any_of_tile(g, false);  // (the sums have been read before the next maxima take their place)
+        any_of(9 + g, 256, false);  // (all of it has left before the next q takes its place)
       }
     }
   } else if constexpr (FP8) {
@@ -1322,7 +1360,7 @@ extern "C" b200_status b200_prefix_attn_plan(b200_prefix_attn* h, const int32_t*
   const bool fp8 = c.kv_dtype != B200_KV_BF16;
   const int warps = fp8 ? ShapeB<128, true>::WARPS : c.head_dim == 128 ? ShapeB<128, false>::WARPS : ShapeB<64, false>::WARPS;
   launch_after(prefix_plan_kernel, 1, rows <= 256 ? 256 : 1024, shared, (cudaStream_t)stream, h->kv->dev, h->p, d_row_seq, d_row_ctx, rows, hash,
-               c.n_q_heads / c.n_kv_heads, b200_sm_count(), b200_sm_count() * warps);
+               c.n_q_heads / c.n_kv_heads, b200_sm_count(), b200_sm_count() * warps, fp8 ? 1.15f : c.head_dim == 128 ? 0.75f : 0.4f);
   B200_LAUNCH_CHECK();
   return B200_OK;
 }
