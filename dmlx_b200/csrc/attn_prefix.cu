@@ -831,6 +831,8 @@ __global__ void __launch_bounds__(threads_a(FP8), 1) prefix_node_kernel(const __
       int ids = p0 + lane < p1 ? table[p0 + lane] : 0, more = 0;
       for (int pg = p0; pg < p1 && ok; pg += kBlockPages) {
         const int rel = pg - p0;
+        if (n == 0 && rel == kBlockPages) wait_all(&sh.q_full, 0);  // (at the start all blocks load at once; q comes before what can wait)
+        if (!ok) break;
         if ((rel & 31) == 0) {
           if (rel > 0) ids = more;
           more = pg + 32 + lane < p1 ? table[pg + 32 + lane] : 0;
