@@ -67,7 +67,7 @@ __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; 
 
 // ---- the plan ------------------------------------------------------------------------------------------------------------
 // Parts of a row of a node: a chunk gives one, or two where the item has one tile of rows and its blocks of keys go to the two softmax groups in turn.
-__device__ __forceinline__ bool is_large(int count, int group) { return count * group > kWarpRows; }
+__host__ __device__ __forceinline__ bool is_large(int count, int group) { return count * group > kWarpRows; }
 __device__ __forceinline__ bool one_tile(const Node& n, int tile, int group) { return n.count - tile * 2 * tile_members(group) <= tile_members(group); }
 __device__ __forceinline__ int even_length(int pages, int len) { return ceil_div(ceil_div(pages, ceil_div(pages, len)), kBlockPages) * kBlockPages; }  // of as many chunks
 __device__ __forceinline__ int large_parts(int pages, int len, bool one) {  // len: pages of a chunk, a multiple of kBlockPages
@@ -142,30 +142,50 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
     if (tid == 0) s.more = 0;
     __syncthreads();
     level_first[levels] = s.n_members;
-    for (int i = tid; i < rows; i += blockDim.x) {
-      entry[i] = -1;
-      if (depth[i] >= full[i]) continue;
-      const int page = d.block_table[(size_t)p.row_seq[i] * d.max_pages_per_seq + depth[i]];
-      const unsigned long long key = (unsigned long long)(unsigned)grp[i] << 32 | (unsigned)page;
-      unsigned at = ((unsigned)page * 2654435761u ^ (unsigned)grp[i] * 40503u) & (hash_size - 1);
-      for (int probe = 0; probe < hash_size; ++probe) {
-        const unsigned long long had = atomicCAS(&keys[at], kEmpty, key);
-        if (had == kEmpty || had == key) break;
-        at = (at + 1) & (hash_size - 1);
+    for (int base = 0; base < rows; base += blockDim.x) {
+      const int i = base + tid;
+      const bool on = i < rows && depth[i] < full[i];
+      if (i < rows) entry[i] = -1;
+      unsigned long long key = kEmpty;
+      if (on) key = (unsigned long long)(unsigned)grp[i] << 32 | (unsigned)d.block_table[(size_t)p.row_seq[i] * d.max_pages_per_seq + depth[i]];
+      // the lanes that agree with the first of them go in as one
+      const unsigned active = __ballot_sync(0xffffffffu, on);
+      if (active == 0) continue;
+      const int lead = __ffs(active) - 1;
+      const unsigned long long first = __shfl_sync(0xffffffffu, key, lead);
+      const unsigned alike = __ballot_sync(0xffffffffu, on && key == first);
+      const bool mine = alike >> lane & 1u;
+      unsigned at = 0;
+      if (on && (!mine || lane == lead)) {
+        at = ((unsigned)key * 2654435761u ^ (unsigned)(key >> 32) * 40503u) & (hash_size - 1);
+        for (int probe = 0; probe < hash_size; ++probe) {
+          const unsigned long long had = atomicCAS(&keys[at], kEmpty, key);
+          if (had == kEmpty || had == key) break;
+          at = (at + 1) & (hash_size - 1);
+        }
+        atomicMin(&leader[at], i);  // (the first lane has the smallest row of its group)
+        atomicAdd(&count[at], mine ? __popc(alike) : 1);
       }
-      entry[i] = (int)at;
-      atomicMin(&leader[at], i);
-      atomicAdd(&count[at], 1);
+      const unsigned of_lead = __shfl_sync(0xffffffffu, at, lead);
+      if (on) entry[i] = (int)(mine ? of_lead : at);
     }
     __syncthreads();
-    for (int i = tid; i < rows; i += blockDim.x) {
-      const int e = entry[i];
-      if (e < 0 || count[e] < 2) continue;
-      const int l = leader[e];
-      const int have = l == i ? full[i]
-                              : common_pages(d.block_table + (size_t)p.row_seq[i] * d.max_pages_per_seq, d.block_table + (size_t)p.row_seq[l] * d.max_pages_per_seq,
-                                             depth[i] + 1, min(full[i], full[l]));
-      atomicMin(&common[e], have);
+    for (int base = 0; base < rows; base += blockDim.x) {
+      const int i = base + tid, e = i < rows ? entry[i] : -1;
+      const bool on = e >= 0 && count[max(e, 0)] >= 2;
+      int have = 0x7fffffff;
+      if (on) {
+        const int l = leader[e];
+        have = l == i ? full[i]
+                      : common_pages(d.block_table + (size_t)p.row_seq[i] * d.max_pages_per_seq, d.block_table + (size_t)p.row_seq[l] * d.max_pages_per_seq,
+                                     depth[i] + 1, min(full[i], full[l]));
+      }
+      const unsigned active = __ballot_sync(0xffffffffu, on);
+      if (active == 0) continue;
+      const int lead = __ffs(active) - 1, first = __shfl_sync(0xffffffffu, e, lead);
+      const bool mine = on && e == first;
+      const int least = __reduce_min_sync(0xffffffffu, mine ? have : 0x7fffffff);
+      if (on && (!mine || lane == lead)) atomicMin(&common[e], mine ? least : have);
     }
     __syncthreads();
     for (int i = tid; i < rows; i += blockDim.x) {
@@ -205,29 +225,23 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
   if (tid == 0) { s.next_a = 0; s.next_b = 0; s.carry = 0; s.units_b = 0; }
   __syncthreads();
   const int n_nodes = s.n_nodes, members = tile_members(group), warp_members = kWarpRows / group;
-  for (int i = tid; i < n_nodes; i += blockDim.x) {
-    const Node n = p.nodes[i];
-    const int pages = n.p1 - n.p0;
+  for (int u = tid; u < n_nodes * kLengthsA; u += blockDim.x) {  // a thread per node and length
+    const Node n = p.nodes[u / kLengthsA];
+    const int k = u % kLengthsA, pages = n.p1 - n.p0;
     if (is_large(n.count, group)) {
       const int tiles = ceil_div(n.count, 2 * members), last = n.count - (tiles - 1) * 2 * members;
       const bool one = last <= members;
-#pragma unroll
-      for (int k = 0; k < kLengthsA; ++k) {
-        // eighths of a block: two tiles of rows count 8, one 5 (4060 cycles); an item's fill, drain and way out kItemUnits (22000)
-        const int len = even_length(pages, length_a(k)), chunks = ceil_div(pages, len), blocks = ceil_div(pages, kBlockPages);
-        atomicMax(&s.max_a[k], (tiles > 1 || !one ? 8 : 5) * min(blocks, len / kBlockPages) + kItemUnits);
-        atomicAdd(&s.items_a[k], tiles * chunks);
-        atomicAdd(&s.units_a[k], (8 * (tiles - (one ? 1 : 0)) + (one ? 5 : 0)) * blocks + kItemUnits * tiles * chunks);
-        atomicAdd(&s.slots_a[k], (n.count - (one ? last : 0)) * large_parts(pages, len, false) + (one ? last : 0) * large_parts(pages, len, true));
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < kLengthsB; ++k) {
-        const int chunks = ceil_div(pages, length_b(k));
-        atomicAdd(&s.items_b[k], ceil_div(n.count, warp_members) * chunks);
-        atomicAdd(&s.slots_b[k], n.count * chunks);
-      }
-      atomicAdd(&s.units_b, ceil_div(n.count, warp_members) * pages);
+      // eighths of a block: two tiles of rows count 8, one 5 (4000 cycles); an item's fill, drain and way out kItemUnits (22000)
+      const int len = even_length(pages, length_a(k)), chunks = ceil_div(pages, len), blocks = ceil_div(pages, kBlockPages);
+      atomicMax(&s.max_a[k], (tiles > 1 || !one ? 8 : 5) * min(blocks, len / kBlockPages) + kItemUnits);
+      atomicAdd(&s.items_a[k], tiles * chunks);
+      atomicAdd(&s.units_a[k], (8 * (tiles - (one ? 1 : 0)) + (one ? 5 : 0)) * blocks + kItemUnits * tiles * chunks);
+      atomicAdd(&s.slots_a[k], (n.count - (one ? last : 0)) * large_parts(pages, len, false) + (one ? last : 0) * large_parts(pages, len, true));
+    } else if (k < kLengthsB) {
+      const int chunks = ceil_div(pages, length_b(k)), tiles = ceil_div(n.count, warp_members);
+      atomicAdd(&s.items_b[k], tiles * chunks);
+      atomicAdd(&s.slots_b[k], n.count * chunks);
+      if (k == 0) atomicAdd(&s.units_b, tiles * pages);
     }
   }
   int own_chunks[kLengthsB] = {}, own_pages = 0;
@@ -250,12 +264,14 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
     // `per_page` a page (0.6 us and, of 128 dims in 16 bits, 0.2, on 37 to 74 SMs), and half as much again when all SMs do this at once, which the memory bounds.
     // Chunks in some rounds of the blocks that the nodes get; the shortest estimated time of those whose parts fit, a lane per choice of the two.
     const float rest = ((float)s.units_b * per_page + 2.3f * s.items_b[0]) * d.n_kv_heads;
+    const float per_worker = __fdividef(1.5f, workers);
+    auto share_up = [](int a, int b) { return __float2int_ru(__fdividef((float)a, (float)b)); };  // (a little too much or too little does no harm)
     float best = 3e38f;
     int choice = 0;
     for (int c = lane; c < 4 * kLengthsA; c += 32) {
-      const int k = c >> 2, items = s.items_a[k] * d.n_kv_heads, rounds = max(ceil_div(items, workers), 1) + (c & 3), mine = max(ceil_div(items, rounds), 1);
-      const float nodes = fmaxf((float)s.units_a[k] * d.n_kv_heads / mine, 0.875f * rounds * s.max_a[k]);
-      const float cost = nodes + fmaxf(rest - (workers - mine) * nodes, 0.f) * 1.5f / workers + s.slots_a[k] * 0.025f;
+      const int k = c >> 2, items = s.items_a[k] * d.n_kv_heads, rounds = max(share_up(items, workers), 1) + (c & 3), mine = min(max(share_up(items, rounds), 1), workers);
+      const float nodes = fmaxf(__fdividef((float)s.units_a[k] * d.n_kv_heads, mine), 0.875f * rounds * s.max_a[k]);
+      const float cost = nodes + fmaxf(rest - (workers - mine) * nodes, 0.f) * per_worker + s.slots_a[k] * 0.025f;
       if ((k == 0 || s.slots_a[k] + s.slots_b[0] <= p.max_slots) && cost < best) { best = cost; choice = k << 16 | mine; }
     }
 #pragma unroll
@@ -264,18 +280,11 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
       const int theirs = __shfl_xor_sync(0xffffffffu, choice, o);
       if (other < best || (other == best && theirs < choice)) { best = other; choice = theirs; }
     }
-    if (lane == 0) { s.pick_a = choice >> 16; s.workers_a = choice & 0xffff; }
-  }
-  __syncwarp();
-  if (tid == 0) {
-    const int heads = d.n_kv_heads, pick = s.pick_a;
-    int pick_b = 0;  // the longest chunks that give every warp about two items, if their parts fit
-    for (int k = 1; k < kLengthsB; ++k) {
-      if (s.slots_a[pick] + s.slots_b[k] > p.max_slots) break;
-      pick_b = k;
-      if ((long long)s.items_b[k] * heads >= 2LL * warps) break;
-    }
-    s.pick_b = pick_b;
+    // Of the rest, the longest chunks that give every warp about two items, if their parts fit.
+    const int pick = choice >> 16, k = min(lane, kLengthsB - 1);
+    const unsigned stop = __ballot_sync(0xffffffffu, lane > 0 && (lane >= kLengthsB - 1 || (long long)s.items_b[k] * d.n_kv_heads >= 2LL * warps));
+    const unsigned over = __ballot_sync(0xffffffffu, lane > 0 && (lane >= kLengthsB || s.slots_a[pick] + s.slots_b[k] > p.max_slots));
+    if (lane == 0) { s.pick_a = pick; s.workers_a = choice & 0xffff; s.pick_b = min(__ffs(stop) - 1, __ffs(over) - 2); }
   }
   __syncthreads();
   const int len_a = length_a(s.pick_a), len_b = length_b(s.pick_b);
@@ -353,6 +362,7 @@ struct Args {
   KvDev d;
   PlanDev p;
   int layer, rows, n_q_heads, group;
+  bool nodes;  // whether the kernel of the large nodes is ahead of the warps'
   const __nv_bfloat16* q;
   int q_stride;
   __nv_bfloat16* out;
@@ -702,6 +712,7 @@ __device__ __forceinline__ void warp_items(const CUtensorMap& kmap, const CUtens
 // reads what the other writes, and the waits here are for copies of its own, so this one waits for the nodes' only at its end: what follows waits for this one alone.
 template <int D, bool FP8>
 __global__ void __launch_bounds__(ShapeB<D, FP8>::WARPS * 32, 1) prefix_warp_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Args a) {
+  if (!a.nodes) wait_previous();
   warp_items<D, FP8>(kmap, vmap, a);
   wait_previous();
 }
@@ -1282,8 +1293,10 @@ b200_status launch_layer(const b200_kv* kv, const Args& a, cudaStream_t s) {
     B200_CUDA_TRY((cudaFuncSetAttribute(prefix_warp_kernel<D, FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ShapeB<D, FP8>::kShared)));
     configured = true;
   }
-  launch_after(prefix_node_kernel<D, FP8>, b200_sm_count(), threads_a(FP8), shared_nodes, s, kv->kmap, kv->vmap, a);
-  B200_LAUNCH_CHECK();
+  if (a.nodes) {
+    launch_after(prefix_node_kernel<D, FP8>, b200_sm_count(), threads_a(FP8), shared_nodes, s, kv->kmap, kv->vmap, a);
+    B200_LAUNCH_CHECK();
+  }
   launch_after(prefix_warp_kernel<D, FP8>, b200_sm_count(), ShapeB<D, FP8>::WARPS * 32, ShapeB<D, FP8>::kShared, s, kv->kmap, kv->vmap, a);
   B200_LAUNCH_CHECK();
   launch_after(prefix_join_kernel<D>, (a.rows * a.n_q_heads + 7) / 8, 256, 0, s, a);
@@ -1384,6 +1397,7 @@ extern "C" b200_status b200_prefix_attn_run(b200_prefix_attn* h, int32_t layer, 
   if (h->rows == 0) return B200_OK;
   Args a;
   a.d = kv->dev; a.p = h->p; a.layer = layer; a.rows = h->rows; a.n_q_heads = c.n_q_heads; a.group = c.n_q_heads / c.n_kv_heads;
+  a.nodes = is_large(h->rows, a.group);  // (else no node is: the least rows take one launch less)
   a.q = (const __nv_bfloat16*)d_q; a.q_stride = q_stride; a.out = (__nv_bfloat16*)d_out; a.out_stride = out_stride;
   a.scale_log2 = 1.4426950408889634f / sqrtf((float)c.head_dim);
   cudaStream_t s = (cudaStream_t)stream;
