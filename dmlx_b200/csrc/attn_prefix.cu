@@ -714,6 +714,7 @@ template <int D, bool FP8>
 __global__ void __launch_bounds__(ShapeB<D, FP8>::WARPS * 32, 1) prefix_warp_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Args a) {
   if (!a.nodes) wait_previous();
   warp_items<D, FP8>(kmap, vmap, a);
+  let_next_start();
   wait_previous();
 }
 
@@ -1250,16 +1251,16 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const __grid_constant_
     mm = m_new;
 #pragma unroll
     for (int e = 0; e < V; ++e) acc[e] *= corr;
-    for (int c = 0; c < n; c += 4) {
-      float v[4][V];
+    for (int c = 0; c < n; c += 8) {
+      float v[8][V];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 8; ++i) {
         const float* src = po + (size_t)(base + min(c + i, n - 1)) * a.n_q_heads * D;
         if constexpr (V == 4) { const float4 f = *reinterpret_cast<const float4*>(src); v[i][0] = f.x; v[i][1] = f.y; v[i][2] = f.z; v[i][3] = f.w; }
         else { const float2 f = *reinterpret_cast<const float2*>(src); v[i][0] = f.x; v[i][1] = f.y; }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 8; ++i) {
         const float wi = __shfl_sync(0xffffffffu, w, (c + i) & 31);
         if (c + i >= n) continue;
 #pragma unroll
