@@ -308,7 +308,6 @@ _sig("b200_lora_destroy", None, vp)
 _sig("b200_lora_set", i32, vp, i32, i32, f32, vp, vp)
 _sig("b200_lora_batch_create", i32, i32, i32, i32, P(vp))
 _sig("b200_lora_batch_destroy", None, vp)
-_sig("b200_lora_error_word", i32, vp, P(i32))
 _sig("b200_lora_plan", i32, vp, vp, i32, vp)
 _sig("b200_lora_apply", i32, vp, vp, vp, i32, vp, i32, vp, i32, vp)
 _sig("b200_kv_create_layers", i32, P(KvConfig), P(KvLayer), P(vp))

@@ -20,6 +20,7 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <new>
 
 #include "common.h"
 #include "kv_pool.cuh"
@@ -1321,7 +1322,8 @@ extern "C" b200_status b200_prefix_attn_create(b200_kv* kv, int32_t max_rows, b2
   }
   b200_status st = b200_require_device();
   if (st != B200_OK) return st;
-  auto* h = new b200_prefix_attn();
+  auto* h = new (std::nothrow) b200_prefix_attn();
+  if (!h) { b200_set_error("prefix attention: out of host memory"); return B200_ERR_CAPACITY; }
   h->kv = kv; h->max_rows = max_rows;
   // A row has at most kLevels nodes of one or two parts, and its own pages; beyond that, room for the chunks of few rows.
   PlanDev& p = h->p;

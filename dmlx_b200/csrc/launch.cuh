@@ -9,6 +9,10 @@
 // So the bodies of two kernels of a stream never overlap, and as a kernel ends only after its own wait did, the wait of the next one covers all
 // that came before.
 //
+// A kernel behind one that passes `let_next_start` only after its own wait may go further: all that is older than that one has ended when it starts, so
+// it may read that, and work on what the one ahead has no part in, and waits for the one ahead's results where it needs them, at its end at the latest
+// (lora_up_kernel, prefix_warp_kernel).
+//
 // No kernel's input is `const T* __restrict__`: a kernel runs from its early start on, so what the one ahead writes changes within its lifetime, and
 // the qualifier would let the compiler load it ahead of the wait (no other pointer reaches the object, so the wait's "memory" clobber would not
 // stand in the way) or through the read-only path.  Memory that is only written may be `__restrict__`, so that loads are not held back by stores,

@@ -3,9 +3,13 @@
 // The plan sorts a batch's rows by adapter and cuts each adapter's rows into tiles.  Then two kernels per projection:
 //   * down: an item is a tile and a quarter of K, u = A x in f32, a warp for 16 rows; the block that is the last of its tile adds the quarters up;
 //   * up: out = y + u B^T by steps of 32 rows of an adapter and 256 columns, of which every block has an equal share.
-// Both are bound by what they read and write once (x and A; y, B and out), so what they multiply comes through rings in shared memory, loads of later
-// items under way while the present one is multiplied (cp.async; the rows of a tile may lie anywhere).  The second kernel's blocks are on their SMs,
-// with y and B on the way, when the first one ends.
+// Both are bound by what they read and write once (x and A; y, B and out).  The first kernel's operands come through a ring in shared memory, loads of
+// later items under way while the present one is multiplied (cp.async; the rows of a tile may lie anywhere), or straight into registers where a tile
+// has few rows; the second kernel's go straight into registers.  Its blocks are on their SMs, with y and B on the way, when the first one ends.
+//
+// Measured, everything in HBM: 256 rows of 64 adapters of rank 16 at 4096 -> 6144, 12.1 us (2.5 in the plan); 1583 rows of 33 adapters of rank up to 64
+// at 4096 -> 28672, 110 us, 2.3 TB/s of what it cannot do without; 8192 rows of 5 of rank 32 at 14336 -> 4096, 94 us, 4.0 TB/s: 60 us of them are the
+// first product's, which reads x at 3.9 TB/s.
 //
 // The products run on mma.sync m16n8k16.  A lane takes 16 neighbouring bytes of a row of x as its places of K in two MMAs, four neighbouring ranks
 // as its places in one of the second product, and eight neighbouring columns of y as its places of N.  A, B and u lie in memory as the lanes take
@@ -17,7 +21,8 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
-#include <vector>
+#include <memory>
+#include <new>
 
 #include "common.h"
 #include "launch.cuh"
@@ -37,7 +42,7 @@ struct b200_lora {
 
 // The rows of a step by adapter: order[max_rows]; tiles of {adapter or -1, first place in order, rows, first slot} (those of many rows from the front
 // on, those of few from the back); groups of 32 rows of an adapter {adapter, first place, rows, -}, each two slots of 16; header {tiles of many rows,
-// groups, tiles of few, error word}.  And what goes from the first product to the second.
+// groups, tiles of few}.  And what goes from the first product to the second.
 struct b200_lora_batch {
   int max_rows = 0, max_adapters = 0, max_rank = 0, max_tiles = 0, rows = -1;
   int* order = nullptr;
@@ -54,7 +59,7 @@ namespace {
 constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kSlices = 4;        // of K
 constexpr int kFewRows = 16;      // of a tile whose slice of K the warps of a block share
-constexpr int kMaxAdapters = 4096, kMaxRank = 128, kTileRows = 128, kGroupRows = 32;
+constexpr int kMaxAdapters = 4096, kMaxRank = 128, kMaxWidth = 1 << 24, kTileRows = 128, kGroupRows = 32;
 constexpr int kEnoughTiles = 74;  // half the SMs (a tile is four items of the first product): beyond that, larger tiles rather than more of them
 
 int rank_rows(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
@@ -127,7 +132,7 @@ struct LoraArgs {
   const int* order;
   const int4 *tiles, *groups;
   const int* hdr;
-  int *done, *err;
+  int* done;
   float* parts;
   uint32_t* u;
   int max_rows, max_tiles, n, k;
@@ -234,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, Down<RS>::PER_SM) lora_down_kernel(c
     for (int i = 0; i < kTileRows / 32; ++i) xp[i] = row0 + 32 * i < lc.tile.z ? a.x + (size_t)a.order[lc.tile.y + row0 + 32 * i] * a.x_stride + lc.k0 + piece * 8 : nullptr;
     ap = a.a + ((size_t)lc.tile.x * k_steps + lc.k0 / 32) * (RS * 4);
   };
-  uint32_t issued = 0, used = 0, load_slot = 0, use_slot = 0;
+  uint32_t load_slot = 0, use_slot = 0;
   auto issue = [&]() {
     if (lc.item < n_items) {
       const int k = lc.chunk * 64;
@@ -249,7 +254,6 @@ __global__ void __launch_bounds__(kThreads, Down<RS>::PER_SM) lora_down_kernel(c
       if (++lc.chunk == lc.chunks) enter_loads(lc.item + gridDim.x);
     }
     commit();
-    ++issued;
     if (++load_slot == Z::STAGES) load_slot = 0;
   };
   enter_loads(blockIdx.x);
@@ -272,7 +276,6 @@ __global__ void __launch_bounds__(kThreads, Down<RS>::PER_SM) lora_down_kernel(c
       issue();
       const uint32_t stage = ring + use_slot * Z::CHUNK, xa = stage + (warp * 16 + g) * 128, aw = stage + kTileRows * 128 + lane * 16;
       if (++use_slot == Z::STAGES) use_slot = 0;
-      ++used;
       if (!works) continue;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
@@ -309,7 +312,7 @@ __global__ void __launch_bounds__(kThreads, Down<RS>::PER_SM) lora_down_kernel(c
   }
   wait_groups<0>();
   __syncthreads();
-  // ---- tiles of few rows: the warps share the slice, straight from memory; the sums of its 1/64s of K are ... ----
+  // ---- tiles of few rows: the warps share the slice, straight from memory; the sums of its 1/64s of K go to shared memory ----
   constexpr int SHARE = 64 / kSlices / kWarps, PAD = RS + 8;  // 1/64s of a warp; floats between rows of their sums, [1/64][row][PAD] in place of the ring
   float* sums = reinterpret_cast<float*>(smem);
   for (int item = blockIdx.x + (n_items + gridDim.x - 1 - blockIdx.x) / gridDim.x * gridDim.x; item < n_items + n_few; item += gridDim.x) {
@@ -349,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, Down<RS>::PER_SM) lora_down_kernel(c
       }
     }
     __syncthreads();
-    // ... added in the order in which a warp by itself comes to them
+    // added in the order in which a warp by itself comes to them
     for (int i = tid; i < tile.z * (RS / 4); i += kThreads) {
       const int row = i / (RS / 4), e = i % (RS / 4) * 4;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -482,10 +485,14 @@ extern "C" b200_status b200_lora_create(int32_t n_adapters, int32_t n, int32_t k
     b200_set_error("lora: %d adapters of rank %d (at most %d, and %d)", n_adapters, max_rank, kMaxAdapters, kMaxRank);
     return B200_ERR_INVALID_ARGUMENT;
   }
-  if (n <= 0 || k <= 0 || n % 8 != 0 || k % 8 != 0) { b200_set_error("lora: a projection of %d x %d (multiples of 8)", n, k); return B200_ERR_INVALID_ARGUMENT; }
+  if (n <= 0 || k <= 0 || n % 8 != 0 || k % 8 != 0 || n > kMaxWidth || k > kMaxWidth) {
+    b200_set_error("lora: a projection of %d x %d (multiples of 8, at most %d)", n, k, kMaxWidth);
+    return B200_ERR_INVALID_ARGUMENT;
+  }
   b200_status st = b200_require_device();
   if (st != B200_OK) return st;
-  auto* l = new b200_lora();
+  auto* l = new (std::nothrow) b200_lora();
+  if (!l) { b200_set_error("lora: out of host memory"); return B200_ERR_CAPACITY; }
   l->n_adapters = n_adapters; l->n = n; l->k = k; l->max_rank = max_rank;
   l->rs = rank_rows(max_rank);
   const size_t a_bytes = n_adapters * l->a_units() * 16, b_bytes = n_adapters * l->b_units() * 16;
@@ -523,7 +530,9 @@ extern "C" b200_status b200_lora_set(b200_lora* l, int32_t adapter, int32_t rank
   if (rank > 0) {  // into the lanes' order
     const uint16_t *ha = (const uint16_t*)h_a, *hb = (const uint16_t*)h_b;
     const int rs = l->rs, ks = rs / 16;
-    std::vector<uint16_t> a(l->a_units() * 8, 0), b(l->b_units() * 8, 0);
+    const size_t a_size = l->a_units() * 8, b_size = l->b_units() * 8;
+    std::unique_ptr<uint16_t[]> a(new (std::nothrow) uint16_t[a_size]()), b(new (std::nothrow) uint16_t[b_size]());
+    if (!a || !b) { b200_set_error("lora: out of host memory for an adapter of %d x %d", l->n, l->k); return B200_ERR_CAPACITY; }
     for (int r = 0; r < rank; ++r)
       for (int k = 0; k < l->k; ++k) a[((((size_t)(k / 32) * (rs / 8) + r / 8) * 32 + r % 8 * 4 + k % 32 / 8) * 8) + k % 8] = ha[(size_t)r * l->k + k];
     for (int n = 0; n < l->n; ++n) {
@@ -531,8 +540,8 @@ extern "C" b200_status b200_lora_set(b200_lora* l, int32_t adapter, int32_t rank
       for (int r = 0; r < rank; ++r)
         b[(((((size_t)(n / 32) * ks + r / 16) * 2 + j / 2) * 32 + g * 4 + r % 16 / 4) * 2 + j % 2) * 4 + r % 4] = hb[(size_t)n * rank + r];
     }
-    B200_CUDA_TRY(cudaMemcpy(l->a + adapter * l->a_units(), a.data(), a.size() * 2, cudaMemcpyHostToDevice));
-    B200_CUDA_TRY(cudaMemcpy(l->b + adapter * l->b_units(), b.data(), b.size() * 2, cudaMemcpyHostToDevice));
+    B200_CUDA_TRY(cudaMemcpy(l->a + adapter * l->a_units(), a.get(), a_size * 2, cudaMemcpyHostToDevice));
+    B200_CUDA_TRY(cudaMemcpy(l->b + adapter * l->b_units(), b.get(), b_size * 2, cudaMemcpyHostToDevice));
   }
   B200_CUDA_TRY(cudaMemcpy(l->scale + adapter, &scale, sizeof(float), cudaMemcpyHostToDevice));
   B200_CUDA_TRY(cudaMemcpy(l->rank + adapter, &rank, sizeof(int), cudaMemcpyHostToDevice));
@@ -549,7 +558,8 @@ extern "C" b200_status b200_lora_batch_create(int32_t max_rows, int32_t max_adap
   }
   b200_status st = b200_require_device();
   if (st != B200_OK) return st;
-  auto* b = new b200_lora_batch();
+  auto* b = new (std::nothrow) b200_lora_batch();
+  if (!b) { b200_set_error("lora batch: out of host memory"); return B200_ERR_CAPACITY; }
   b->max_rows = max_rows; b->max_adapters = max_adapters; b->max_rank = max_rank; b->max_tiles = max_tiles_of(max_rows, max_adapters);
   cudaError_t e = cudaMalloc((void**)&b->order, sizeof(int) * max_rows);
   if (e == cudaSuccess) e = cudaMalloc((void**)&b->tiles, sizeof(int4) * b->max_tiles);
@@ -590,13 +600,6 @@ extern "C" b200_status b200_lora_plan(b200_lora_batch* b, const int32_t* d_row_a
   return B200_OK;
 }
 
-extern "C" b200_status b200_lora_error_word(b200_lora_batch* b, int32_t* out) {
-  if (!b || !out) { b200_set_error("lora batch: no handle, or no place for the word"); return B200_ERR_INVALID_ARGUMENT; }
-  B200_CUDA_TRY(cudaMemcpy(out, b->hdr + 3, sizeof(int), cudaMemcpyDeviceToHost));
-  if (*out != 0) B200_CUDA_TRY(cudaMemset(b->hdr + 3, 0, sizeof(int)));
-  return B200_OK;
-}
-
 extern "C" b200_status b200_lora_apply(const b200_lora* l, b200_lora_batch* b, const void* d_x, int32_t x_stride, const void* d_y, int32_t y_stride,
                                        void* d_out, int32_t out_stride, void* stream) {
   if (!l || !b) { b200_set_error("lora: no adapters, or no batch"); return B200_ERR_INVALID_ARGUMENT; }
@@ -616,7 +619,7 @@ extern "C" b200_status b200_lora_apply(const b200_lora* l, b200_lora_batch* b, c
   if (b->rows == 0) return B200_OK;
   LoraArgs a;
   a.a = l->a; a.b = l->b; a.x = (const __nv_bfloat16*)d_x; a.y = (const __nv_bfloat16*)d_y; a.out = (__nv_bfloat16*)d_out;
-  a.rank = l->rank; a.scale = l->scale; a.order = b->order; a.tiles = b->tiles; a.groups = b->groups; a.hdr = b->hdr; a.err = b->hdr + 3;
+  a.rank = l->rank; a.scale = l->scale; a.order = b->order; a.tiles = b->tiles; a.groups = b->groups; a.hdr = b->hdr;
   a.done = b->done; a.parts = b->parts; a.u = b->u;
   a.max_rows = b->max_rows; a.max_tiles = b->max_tiles; a.n = l->n; a.k = l->k;
   a.x_stride = x_stride; a.y_stride = y_stride; a.out_stride = out_stride;

@@ -473,11 +473,6 @@ class LoraBatch:
     def __del__(self):
         self.close()
 
-    def error_word(self) -> int:
-        out = C.c_int32()
-        _lib.check(lib.b200_lora_error_word(self._h, C.byref(out)))
-        return out.value
-
     def plan(self, row_adapter: torch.Tensor):
         """b200_lora_plan: the adapter of every row, -1 for none."""
         rows, device = row_adapter.shape[0], torch.cuda.current_device()

@@ -552,7 +552,7 @@ b200_status b200_qmm_static_scratch(const b200_qweight* w, const void* d_x, int3
  * its plan: steps that may run at the same time (two captured graphs on two streams) have a batch handle each. */
 typedef struct b200_lora b200_lora;
 typedef struct b200_lora_batch b200_lora_batch;
-/* Up to 4096 adapters of rank up to 128; n and k multiples of 8.  All start without matrices (rank 0). */
+/* Up to 4096 adapters of rank up to 128; n and k multiples of 8 up to 2^24.  All start without matrices (rank 0). */
 b200_status b200_lora_create(int32_t n_adapters, int32_t n, int32_t k, int32_t max_rank, b200_lora** out);
 void b200_lora_destroy(b200_lora* l);
 /* Host pointers, bf16: A [rank, k], B [n, rank]; rank 0 takes the adapter out.  Synchronous; no step that uses this adapter may be in flight. */
@@ -561,8 +561,6 @@ b200_status b200_lora_batch_create(int32_t max_rows, int32_t max_adapters, int32
 void b200_lora_batch_destroy(b200_lora_batch* b);
 /* d_row_adapter [rows]: the adapter of every row; a number that is none (-1) leaves the row as it is, and so does an adapter of rank 0. */
 b200_status b200_lora_plan(b200_lora_batch* b, const int32_t* d_row_adapter, int32_t rows, void* stream);
-/* Reads and clears the batch's error word: 0, or B200_ERR_DEVICE_FLAGGED where a kernel's bounded wait ran out (its outputs are then not complete). */
-b200_status b200_lora_error_word(b200_lora_batch* b, int32_t* out);
 /* Over the rows of the batch's plan, bf16, strides in elements (multiples of 8, rows start on 16 bytes).  d_out may be d_y (rows without an adapter
  * are then not touched); otherwise the two do not overlap and rows without an adapter are copied.  Same bits for a row whatever shares its batch. */
 b200_status b200_lora_apply(const b200_lora* l, b200_lora_batch* b, const void* d_x, int32_t x_stride, const void* d_y, int32_t y_stride,
