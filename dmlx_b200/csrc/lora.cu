@@ -368,12 +368,14 @@ __global__ void __launch_bounds__(kThreads, Down<RS>::PER_SM) lora_down_kernel(c
 }
 
 // ---- up: 32 columns for a warp, steps of 32 rows ------------------------------------------------------------------------------------------------------
-// Its part of B stays in registers; lane (g, t) has columns 8 t .. 8 t + 7 of rows g and g + 8.  The warps of a block take neighbouring columns, so what
-// they read of y is contiguous and u comes from their L1.  Nothing passes through shared memory: with y by cp.async, u and B in bulk and warps for
-// that alone, those warps' issue was what everything waited for (1850 cycles for 32 rows of 256 columns, 1140 for their products).
+// Its part of B stays in registers; lane (g, t) has columns 8 t .. 8 t + 7 of rows g, g + 8, g + 16 and g + 24.  The warps of a block take neighbouring
+// columns, so what they read of y is contiguous and u comes from their L1.  Nothing passes through shared memory: with y by cp.async, u and B in bulk
+// and warps for that alone, those warps' issue was what everything waited for (1850 cycles for 32 rows of 256 columns, 1140 for their products).
+// What bounds it is how many bytes are on their way: 2 KB of y a warp, a step of 32 rows ahead (1583 rows of rank 64 to 28672 columns 70 us; 16 rows
+// ahead, and B loaded before the next y instead of behind it, 88), and blocks per SM as the registers for that allow.
 template <int RS>
 struct Up {
-  static constexpr int KS = RS / 16, COLS = kWarps * 32, PER_SM = RS == 16 ? 4 : RS == 32 ? 3 : RS == 64 ? 2 : 1;
+  static constexpr int KS = RS / 16, COLS = kWarps * 32, PER_SM = RS == 16 ? 3 : RS <= 64 ? 2 : 1;
 };
 
 // (Everything but u was there when the kernel ahead began, and that one lets this one start behind its own wait: only u is waited for.)
@@ -385,46 +387,59 @@ __global__ void __launch_bounds__(kThreads, Up<RS>::PER_SM) lora_up_kernel(const
   const long long all = (long long)groups * col_blocks;
   const int begin = (int)(all * blockIdx.x / gridDim.x), end = (int)(all * (blockIdx.x + 1) / gridDim.x);
   if (begin < end) {
-    int block = begin / groups, at = begin - block * groups;  // range of columns, group
-    int4 group = a.groups[at];                                // {adapter, first place, rows, -}
-    auto row_of = [&](const int4& gr, int r) { return r < gr.z ? a.order[gr.y + r] : -1; };
-    auto load_y = [&](int row, int col) { return row >= 0 && col < a.n ? *reinterpret_cast<const uint4*>(a.y + (size_t)row * a.y_stride + col) : make_uint4(0, 0, 0, 0); };
-    int rows[2] = {row_of(group, g), row_of(group, g + 8)};
-    uint4 next[2] = {load_y(rows[0], (block * kWarps + warp) * 32 + 8 * t), load_y(rows[1], (block * kWarps + warp) * 32 + 8 * t)};
+    // Ahead of the step at hand: y of the next one, the rows' numbers of the one behind it, and the group behind that.
+    struct Place { int block, at; };  // range of columns, group
+    auto behind = [&](Place p) { return ++p.at == groups ? Place{p.block + 1, 0} : p; };
+    auto group_of = [&](int s, const Place& p) { return s < end ? a.groups[p.at] : make_int4(-1, 0, 0, 0); };  // {adapter, first place, rows, -}
+    auto rows_of = [&](const int4& gr, int (&r)[4]) {  // g, g + 8, g + 16, g + 24 of the group; -1: none
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = g + 8 * i < gr.z ? a.order[gr.y + g + 8 * i] : -1;
+    };
+    auto load_y = [&](const int (&r)[4], int block, uint4 (&y)[4]) {
+      const int col = (block * kWarps + warp) * 32 + 8 * t;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = r[i] >= 0 && col < a.n ? *reinterpret_cast<const uint4*>(a.y + (size_t)r[i] * a.y_stride + col) : make_uint4(0, 0, 0, 0);
+    };
+    Place p0{begin / groups, 0}, p1, p2;
+    p0.at = begin - p0.block * groups;
+    p1 = behind(p0);
+    p2 = behind(p1);
+    int4 g0 = group_of(begin, p0), g1 = group_of(begin + 1, p1), g2 = group_of(begin + 2, p2);
+    int r0[4], r1[4];
+    uint4 y0[4];
+    rows_of(g0, r0);
+    rows_of(g1, r1);
+    load_y(r0, p0.block, y0);
+    auto ranks_of = [&](int adapter) { return adapter >= 0 ? (min(a.rank[adapter], RS) + 15) / 16 : 0; };  // in sixteens
+    auto load_b = [&](int adapter, int block, int ks, uint4 (&v)[Z::KS][2]) {
+      const uint4* bp = a.b + ((size_t)max(adapter, 0) * n_blocks + min(block * kWarps + warp, n_blocks - 1)) * Z::KS * 64 + lane;
+#pragma unroll
+      for (int k = 0; k < Z::KS; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) v[k][i] = k < ks ? bp[(k * 2 + i) * 32] : make_uint4(0, 0, 0, 0);
+    };
     uint4 bv[Z::KS][2];
-    int c_block = -1, c_adapter = -1, ks = 0;
-    bool waited = false;
+    int ks = ranks_of(g0.x);
+    load_b(g0.x, p0.block, ks, bv);
     for (int s = begin; s < end; ++s) {
-      const int nb = block * kWarps + warp, col = nb * 32 + 8 * t, slot = at * (kGroupRows / 16);
-      const int4 now = group;
-      if (block != c_block || now.x != c_adapter) {
-        c_block = block; c_adapter = now.x;
-        ks = now.x >= 0 ? (min(a.rank[now.x], RS) + 15) / 16 : 0;
-        const uint4* bp = a.b + ((size_t)max(now.x, 0) * n_blocks + min(nb, n_blocks - 1)) * Z::KS * 64 + lane;
+      const int col = (p0.block * kWarps + warp) * 32 + 8 * t, slot = p0.at * (kGroupRows / 16);
+      const bool other = s + 1 < end && (g1.x != g0.x || p1.block != p0.block);  // another part of B is next
+      if (other && g1.x >= 0 && p1.block * kWarps + warp < n_blocks && lane < RS / 2)  // on its way to L2
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(a.b + ((size_t)g1.x * n_blocks + p1.block * kWarps + warp) * Z::KS * 64 + lane * 8));
+      uint4 y1[4];
+      load_y(r1, p1.block, y1);
+      int r2[4];
+      rows_of(g2, r2);
+      const Place p3 = behind(p2);
+      const int4 g3 = group_of(s + 3, p3);
+      if (s == begin) after_previous();
 #pragma unroll
-        for (int k = 0; k < Z::KS; ++k)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) bv[k][i] = k < ks ? bp[(k * 2 + i) * 32] : make_uint4(0, 0, 0, 0);
-      }
-      if (++at == groups) { at = 0; ++block; }
-      if (s + 1 < end) group = a.groups[at];
-      if (!waited) { after_previous(); waited = true; }
-#pragma unroll
-      for (int m = 0; m < kGroupRows; m += 16) {
-        const int to[2] = {rows[0], rows[1]};
-        const uint4 old[2] = {next[0], next[1]};
-        if (m + 16 < kGroupRows && m + 16 < now.z) {  // the next rows: of this group, or of the next one
-#pragma unroll
-          for (int h = 0; h < 2; ++h) { rows[h] = row_of(now, m + 16 + 8 * h + g); next[h] = load_y(rows[h], col); }
-        } else if (m < now.z) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) { rows[h] = s + 1 < end ? row_of(group, 8 * h + g) : -1; next[h] = load_y(rows[h], (block * kWarps + warp) * 32 + 8 * t); }
-        }
-        if (m >= now.z || (ks == 0 && a.out == a.y)) continue;
+      for (int m = 0; m < kGroupRows / 16; ++m) {
+        if (m * 16 >= g0.z || (ks == 0 && a.out == a.y)) continue;
         float acc[4][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-        const uint4* up = reinterpret_cast<const uint4*>(a.u) + (size_t)(slot + m / 16) * Z::KS * 64 + lane;
+        const uint4* up = reinterpret_cast<const uint4*>(a.u) + (size_t)(slot + m) * Z::KS * 64 + lane;
 #pragma unroll
         for (int k = 0; k < Z::KS; ++k) {
           if (k >= ks) continue;
@@ -439,18 +454,24 @@ __global__ void __launch_bounds__(kThreads, Up<RS>::PER_SM) lora_up_kernel(const
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          if (to[h] < 0 || col >= a.n) continue;
-          uint4 o = old[h];
+          if (r0[2 * m + h] < 0 || col >= a.n) continue;
+          uint4 o = y0[2 * m + h];
           if (ks > 0) {
             uint32_t* w = reinterpret_cast<uint32_t*>(&o);
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = pack(ptx::bf16_lo(w[j]) + acc[j][2 * h], ptx::bf16_hi(w[j]) + acc[j][2 * h + 1]);
           }
-          *reinterpret_cast<uint4*>(a.out + (size_t)to[h] * a.out_stride + col) = o;
+          *reinterpret_cast<uint4*>(a.out + (size_t)r0[2 * m + h] * a.out_stride + col) = o;
         }
       }
-      if ((block != c_block || group.x != c_adapter) && group.x >= 0 && block * kWarps + warp < n_blocks && lane < RS / 2)  // the next step's B on its way to L2
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(a.b + ((size_t)group.x * n_blocks + block * kWarps + warp) * Z::KS * 64 + lane * 8));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { r0[i] = r1[i]; r1[i] = r2[i]; y0[i] = y1[i]; }
+      if (other) {
+        ks = ranks_of(g1.x);
+        load_b(g1.x, p1.block, ks, bv);
+      }
+      p0 = p1; p1 = p2; p2 = p3;
+      g0 = g1; g1 = g2; g2 = g3;
     }
   } else {
     after_previous();
