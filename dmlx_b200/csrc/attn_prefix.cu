@@ -13,9 +13,13 @@
 //     seen by every row, so there are no masks;
 //   * everything else, smaller nodes and the rows' own pages: a warp per item on mma.sync, 16 query rows, pages by TMA into rings of its own;
 //   * the join.
+// The first two run at the same time: the plan gives the nodes as many SMs as lets both end together.
 //
-// The tensor-core kernel is bound by the exponentials and the products, 2048 cycles each for 128 keys and 256 query rows; the warps' kernel by the
-// stream of pages.
+// Of 128 keys and 256 query rows the tensor-core kernel's exponentials and its products take 2048 cycles each; a block of both takes 3750, since a tile's
+// next scores wait for its last product (P lies where they go) and the two tiles overlap only in part; an item has 22000 more around its blocks, for q,
+// the first pages and 128 KB of parts.  The warps' kernel is bound by the stream of pages.  Measured per layer, 32 query heads on 8, 128 dims, pages in
+// HBM: 256 rows behind 8192 shared tokens with up to 512 of their own 86 us (one after the other 110: 52 the nodes' on all SMs, 51 the warps', 10 the
+// join), 64 rows behind 2048 28 us, 128 rows behind 4096 on FP8 pages 38 us; plans 11 to 14 us.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
@@ -402,6 +406,9 @@ __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, bool& ok) {
 __device__ __forceinline__ const int* table_of(const Args& a, int seq) { return a.d.block_table + (size_t)seq * a.d.max_pages_per_seq; }
 
 // ---- everything but the large nodes: a warp per item ------------------------------------------------------------------------
+// 16 query rows are all that mma.sync needs for one tile, and the pages of few rows come as fast as the memory gives them: about 2180 pages of 8 heads, 285 MB
+// in K and V, 51 us on all SMs, 5.6 TB/s; 59 us on 92 of them, 68 on 74.  K and V are loads of their own, so that a warp's next page is on its way before
+// this one's values have been used.
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
@@ -723,10 +730,11 @@ __global__ void __launch_bounds__(ShapeB<D, FP8>::WARPS * 32, 1) prefix_warp_ker
 // Warps 0-7 and 8-15: softmax of a tile each, two threads a row (64 of a block's 128 keys); warp 16: loads of pages; warp 17: products; on FP8 pools warps
 // 18 and 19 widen the pages' codes to f16, which is exact, q and P being f16 there too.  An item of two tiles has both use every block of keys; one of one
 // tile has its blocks in turn to the two softmax groups, with sums and parts of their own.
-// A row keeps its scale until a score is 2^kLate above it, so that a block is one vote of its tile's threads and no exchange of maxima: all that a late
-// scale costs is that the largest weight is no longer 1, and so is rounded like the others.
-// (With one thread a row, two warps on each of the SM's quarters, a block of 128 keys took 4900 cycles: 3560 of softmax, which had nothing to hide its
-// latency behind, and 1350 until the next scores were there.)
+// A row keeps its scale until a score is 2^kLate above it, so that a block is one vote of the two warps of a row and no exchange of maxima: all that a
+// late scale costs is that the largest weight is no longer 1, and so is rounded like the others.
+// (256 rows behind 8192 tokens, on all SMs: 52 us.  With one thread a row, two warps on each of the SM's quarters, 61: 3560 cycles of softmax had nothing
+// to hide their latency behind.  64 keys at a time into two places of tensor memory, the next scores ahead of the softmax, 63, since products of 64
+// columns take longer per key; a row in four lanes of one warp, with nothing to agree on, 56; a warp of products for each tile slows both, 82 for 66.)
 constexpr int kSoftWarps = 16, kLoadWarp = 16, kMmaWarp = 17, kWidenWarps = 2, kWiden = kWidenWarps * 32;
 __host__ __device__ constexpr int threads_a(bool fp8) { return (kMmaWarp + 1 + (fp8 ? kWidenWarps : 0)) * 32; }
 constexpr float kLate = 4.f;

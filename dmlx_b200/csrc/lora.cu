@@ -7,8 +7,8 @@
 // later items under way while the present one is multiplied (cp.async; the rows of a tile may lie anywhere), or straight into registers where a tile
 // has few rows; the second kernel's go straight into registers.  Its blocks are on their SMs, with y and B on the way, when the first one ends.
 //
-// Measured, everything in HBM: 256 rows of 64 adapters of rank 16 at 4096 -> 6144, 12.1 us (2.5 in the plan); 1583 rows of 33 adapters of rank up to 64
-// at 4096 -> 28672, 110 us, 2.3 TB/s of what it cannot do without; 8192 rows of 5 of rank 32 at 14336 -> 4096, 94 us, 4.0 TB/s: 60 us of them are the
+// Measured, everything in HBM: 256 rows of 64 adapters of rank 16 at 4096 -> 6144, 12.9 us (and 3.1 for the plan); 1583 rows of 33 adapters of rank up to 64
+// at 4096 -> 28672, 93 us, 2.8 TB/s of what it cannot do without; 8192 rows of 5 of rank 32 at 14336 -> 4096, 94 us, 4.0 TB/s: 60 us of them are the
 // first product's, which reads x at 3.9 TB/s.
 //
 // The products run on mma.sync m16n8k16.  A lane takes 16 neighbouring bytes of a row of x as its places of K in two MMAs, four neighbouring ranks
