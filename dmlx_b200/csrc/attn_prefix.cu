@@ -1001,17 +1001,18 @@ __global__ void __launch_bounds__(threads_a(FP8), 1) prefix_node_kernel(const __
         constexpr int PIECES = D / 8;  // 16-byte pieces of a row
         constexpr int EACH = kTileRows * PIECES / 256;  // of a thread, all under way at once
         if (g < it[0]) {
+          const int by_group = 65536 / a.group + 1;  // x * by_group >> 16 is x / G up to 127
           uint4 w[EACH];
           int row[EACH];
 #pragma unroll
           for (int e = 0; e < EACH; ++e) {
-            const int qm = ((threadIdx.x & 255) + e * 256) / PIECES / G, qh = ((threadIdx.x & 255) + e * 256) / PIECES - qm * G, member = g * members + qm;
-            row[e] = qm < members && member < it[4] ? a.p.members[it[3] + member].row * G + qh : -1;
+            const int qr = ((threadIdx.x & 255) + e * 256) / PIECES, qm = qr * by_group >> 16, member = g * members + qm;
+            row[e] = qm < members && member < it[4] ? a.p.members[it[3] + member].row : -1;
           }
 #pragma unroll
           for (int e = 0; e < EACH; ++e) {
-            const int c = threadIdx.x % PIECES, at = max(row[e], 0) / G;
-            const __nv_bfloat16* src = a.q + (size_t)at * a.q_stride + (size_t)(it[1] * G + max(row[e], 0) - at * G) * D + c * 8;
+            const int qr = ((threadIdx.x & 255) + e * 256) / PIECES, qh = qr - (qr * by_group >> 16) * G;
+            const __nv_bfloat16* src = a.q + (size_t)max(row[e], 0) * a.q_stride + (size_t)(it[1] * G + qh) * D + (threadIdx.x % PIECES) * 8;
             w[e] = row[e] >= 0 ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
           }
 #pragma unroll
