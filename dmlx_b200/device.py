@@ -404,14 +404,16 @@ class SharedPrefixAttention:
 
     def plan(self, row_seq: torch.Tensor, row_ctx: torch.Tensor):
         """b200_prefix_attn_plan: row r is to see the first row_ctx[r] tokens of slot row_seq[r]."""
+        if self.cache._h is None:
+            raise ValueError("the pool is closed")
         rows, device = row_seq.shape[0], torch.cuda.current_device()
         _lib.check(lib.b200_prefix_attn_plan(self._h, _ints(row_seq, rows, device), _ints(row_ctx, rows, device), rows, _raw_stream(device)))
         self.rows = rows
 
     def run(self, layer: int, q: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """b200_prefix_attn_run: q [T, Hq, D] (rows may be strided), T the rows of the plan."""
-        if q.shape[0] != self.rows:
-            raise ValueError(f"{q.shape[0]} rows, the plan has {self.rows}")
+        if q.shape[0] != self.rows or self.cache._h is None:
+            raise ValueError("the pool is closed" if self.cache._h is None else f"{q.shape[0]} rows, the plan has {self.rows}")
         device, shape = torch.cuda.current_device(), (self.rows, *self._heads)
         out = q.new_empty(shape) if out is None else out
         _lib.check(lib.b200_prefix_attn_run(self._h, layer, q.data_ptr(), _rows(q, shape, device), out.data_ptr(), _rows(out, shape, device), _raw_stream(device)))

@@ -2,7 +2,12 @@
 
 Tolerance, per number: half a step of bf16 of the result, 2^-8 of it; the weights are rounded to bf16 before their product, 2^-8 of each, so 2^-8 of
 E = sum p |v| / sum p; and a score is off by its f32 sum, (d / 16 + 2) 2^-22 of S = |q| |k| / sqrt(d), and by its exponent's argument and the
-exponential, 2^-20 together for |scores| up to 16 or S: a weight and the sum by twice that, relative."""
+exponential, 2^-20 together for |scores| up to 16 or S: a weight and the sum by twice that, relative.
+
+On 8-bit pages a weight, times its page's V scale over the largest of a run of pages, is rounded to f16, whose numbers below 2^-14 are 2^-24 apart: what is
+small is off by up to 2^-25 instead, of the row's largest weight in the part, which is 1 or more, as is therefore the part's sum.  It multiplies the
+code and that largest scale, so the part is off by 2^-25 max(scale) sum |code| at most, and what parts are joined to by no more than the worst of them
+(their shares add up to 1).  Where the token that has nearly all the weight holds a zero, this is more than all the above."""
 import ctypes as C
 import math
 
@@ -44,8 +49,17 @@ def _held(cache, layer, slots):
     return held
 
 
+def _value_codes(cache, layer, slot):
+    """|code| [tokens, heads, dims] of a slot's values on 8-bit pages, and their scales [tokens, heads]."""
+    raw = [[torch.from_numpy(x) for x in cache.page_raw(layer, p)] for p in cache.block_table(slot)]
+    codes = [v.view(torch.float8_e4m3fn).double().abs().permute(1, 0, 2) for _, v, _, _ in raw]
+    scales = [vs.double()[None].expand(v.shape[1], -1) for _, v, _, vs in raw]
+    return torch.cat(codes or [torch.zeros((0, cache.cfg.n_kv_heads, cache.cfg.head_dim))]).cuda(), torch.cat(scales or [torch.zeros((0, cache.cfg.n_kv_heads))]).cuda()
+
+
 def _want(cache, layer, q, row_seq, row_ctx):
     held = _held(cache, layer, {s for s in row_seq if 0 <= s < cache.cfg.max_seqs})
+    small = {s: _value_codes(cache, layer, s) for s in held} if cache.cfg.kv_dtype != 0 else {}
     t, hq, d = q.shape
     group = hq // cache.cfg.n_kv_heads
     want, tol = torch.zeros(q.shape, dtype=torch.float64, device="cuda"), torch.zeros(q.shape, dtype=torch.float64, device="cuda")
@@ -58,7 +72,10 @@ def _want(cache, layer, q, row_seq, row_ctx):
         p = torch.softmax(scores, 1)
         want[r] = torch.einsum("ht,thd->hd", p, v)
         e = torch.einsum("ht,thd->hd", p, v.abs())
-        tol[r] = 2.0 ** -8 * want[r].abs() + (2.0 ** -8 + 2 * ((d / 16 + 2) * 2.0 ** -22 * top[:, None] + 2.0 ** -20 * (top[:, None] / 16).clamp(min=1))) * e
+        if cache.cfg.kv_dtype != 0:
+            codes, scales = (x[:n] for x in small[s])
+            tol[r] += (2.0 ** -25 * scales.amax(0)[:, None] * codes.sum(0)).repeat_interleave(group, 0)
+        tol[r] += 2.0 ** -8 * want[r].abs() + (2.0 ** -8 + 2 * ((d / 16 + 2) * 2.0 ** -22 * top[:, None] + 2.0 ** -20 * (top[:, None] / 16).clamp(min=1))) * e
     return want, tol
 
 
@@ -300,6 +317,49 @@ def test_plans_follow_the_pages():
         ctx = [cache.seq_len(s) for s in slots]
         q = _random(len(slots), 8, 128, seed=20 + n, scale=2.0)
         _check(_run(cache, q, slots, ctx, handle=handle), *_want(cache, 0, q, slots, ctx))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_handle_through_batches_of_many_and_few_rows(fp8):
+    """16 query rows at most and more than that take other kernels; one handle, plans and layers in turn, captured and replayed too."""
+    from dmlx_b200 import device as dev
+
+    cache, slots, ctx = _tree(dev, 36, 700, 0, 0, [1, 64, 130], 8, 2, 128, fp8, layers=2)
+    handle = dev.SharedPrefixAttention(cache, 40)
+    for n, rows in enumerate((36, 4, 1, 5, 36, 3)):
+        row_seq, row_ctx = _ints(*slots[:rows]), _ints(*ctx[:rows])
+        q = [_random(rows, 8, 128, seed=10 * n + layer, scale=2.0) for layer in range(2)]
+        handle.plan(row_seq, row_ctx)
+        got = [handle.run(layer, q[layer]) for layer in range(2)]
+        graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            handle.plan(row_seq, row_ctx)
+            again = [handle.run(layer, q[layer]) for layer in range(2)]
+        for _ in range(2):
+            graph.replay()
+        torch.cuda.synchronize()
+        for layer in range(2):
+            want, tol = _want(cache, layer, q[layer], slots[:rows], ctx[:rows])
+            _check(got[layer], want, tol)
+            _check(again[layer], want, tol)
+    assert cache.error_word() == 0
+
+
+@pytest.mark.gpu
+def test_a_closed_pool_is_refused():
+    from dmlx_b200 import device as dev
+
+    cache, slots, ctx = _tree(dev, 2, 64, 0, 0, [1], 4, 1, 64)
+    handle = dev.SharedPrefixAttention(cache, 4)
+    handle.plan(_ints(*slots), _ints(*ctx))
+    cache.close()
+    with pytest.raises(ValueError):
+        handle.run(0, _random(2, 4, 64, seed=1))
+    with pytest.raises(ValueError):
+        handle.plan(_ints(*slots), _ints(*ctx))
+    handle.close()
 
 
 @pytest.mark.gpu
