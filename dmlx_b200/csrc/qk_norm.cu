@@ -11,8 +11,9 @@
 // so a head costs two packed operations per two elements beside the norm, with the products of angles and weights in registers for all heads that
 // a warp takes of its row.  The block's rows have their angles computed once, by all its threads.  Few rows: more warps for each.
 //
-// Bound by what it reads and writes: 8192 rows of 32 + 8 heads of 128 take 36.6 us, 4.6 TB/s (kAhead loads in flight a warp, 32 warps per SM; 64 warps 41,
-// 128 warps 49, loads a round ahead in registers 52, requested into L2 ahead 39); 257 rows of 16 + 4 heads of 64 take 3.1 us, one row 3.7, a launch's latency.
+// Bound by what it reads and writes: 8192 rows of 32 + 8 heads of 128 take 34.6 us, 4.8 TB/s (kAhead loads in flight a warp, 32 warps per SM, the first of
+// them ahead of the angles, else 36.0; 64 warps 41, 128 warps 49, every round's loads ahead 52, requested into L2 ahead 39); 257 rows of 16 + 4 heads of 64
+// take 2.9 us, one row 3.5, a launch's latency.
 #include <cuda_bf16.h>
 #include <math.h>
 
@@ -70,6 +71,15 @@ __global__ void __launch_bounds__(kWarps * 32, 4) qk_norm_rope_kernel(const __gr
   const int row = blockIdx.x * rows + warp / per_row, parts = per_row * gridDim.y, part = blockIdx.y * per_row + warp % per_row;
   const int at = (lane % LANES) * 8, sub = lane / LANES;  // this lane's elements of a head; its head of a load
   const int half = a.rot / 2;
+  const int head0 = part * HEADS + sub, step = parts * HEADS;
+  // The first loads of q are on their way while the angles are computed.
+  uint4 in[kAhead];
+  auto load = [&](const __nv_bfloat16* src, int head, int heads) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) in[u] = head + u * step < heads ? *reinterpret_cast<const uint4*>(src + (size_t)(u * step) * D) : make_uint4(0, 0, 0, 0);
+  };
+  const int first = head0 * D + at;
+  load(a.q + (size_t)min(row, a.rows - 1) * a.q_stride + first, head0, a.hq);
   for (int i = threadIdx.x; i < rows * half; i += kWarps * 32) {
     const int r = i / half, pair = i - r * half;
     const double t = (double)(blockIdx.x * rows + r < a.rows ? a.positions[blockIdx.x * rows + r] : 0) * a.turns[pair];
@@ -83,7 +93,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) qk_norm_rope_kernel(const __gr
   const int partner = (lane & ~(LANES - 1)) | ((turns_here ? (second ? at - half : at + half) : at) / 8);
   const uint32_t neighbours = turns_here ? 0x1032 : 0x3210;  // (what does not turn is its own partner: 0 times another infinite number is not 0)
   // The row's heads, loads part, part + parts, ...: `src` and `dst` head 0 of the row, dst_head elements between heads there.
-  auto heads_of = [&](const __nv_bfloat16* src, int heads, const __nv_bfloat16* weight, __nv_bfloat16* dst, int dst_head, bool writes) {
+  auto heads_of = [&](const __nv_bfloat16* src, int heads, const __nv_bfloat16* weight, __nv_bfloat16* dst, int dst_head, bool writes, bool loaded) {
     float2 cw[4], sw[4];  // cosine times the weight of each of the lane's elements; sine, with its sign, times the partner's
     {
       const uint4 one = make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u);
@@ -108,14 +118,11 @@ __global__ void __launch_bounds__(kWarps * 32, 4) qk_norm_rope_kernel(const __gr
         }
       }
     }
-    int head = part * HEADS + sub;
-    const int step = parts * HEADS;
-    src += (size_t)head * D + at;
+    int head = head0;
+    src += first;
     dst += (size_t)head * dst_head + at;
     for (int h0 = part * HEADS; h0 < heads; h0 += kAhead * step) {  // (h0: the same in the whole warp)
-      uint4 in[kAhead];
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) in[u] = head + u * step < heads ? *reinterpret_cast<const uint4*>(src + (size_t)(u * step) * D) : make_uint4(0, 0, 0, 0);
+      if (!loaded || h0 != part * HEADS) load(src, head, heads);
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         if (h0 + u * step >= heads) break;
@@ -143,16 +150,16 @@ __global__ void __launch_bounds__(kWarps * 32, 4) qk_norm_rope_kernel(const __gr
       dst += (size_t)(kAhead * step) * dst_head;
     }
   };
-  heads_of(a.q + (size_t)row * a.q_stride, a.hq, a.q_weight, a.q_out + (size_t)row * a.q_out_stride, D, true);
+  heads_of(a.q + (size_t)row * a.q_stride, a.hq, a.q_weight, a.q_out + (size_t)row * a.q_out_stride, D, true, true);
   if constexpr (!PAGES) {
-    heads_of(a.k + (size_t)row * a.k_stride, a.hkv, a.k_weight, a.k_out + (size_t)row * a.k_out_stride, D, true);
+    heads_of(a.k + (size_t)row * a.k_stride, a.hkv, a.k_weight, a.k_out + (size_t)row * a.k_out_stride, D, true, false);
   } else {
     // a step whose reservation failed has no page for this row: nothing of it is written there (the error word is set)
     const int pos = a.positions[row], seq = a.row_seq[row], page_idx = pos / a.d.page_size;
     const bool have_page = pos >= 0 && seq >= 0 && seq < a.d.max_seqs && page_idx < a.d.seq_pages[seq];
     const int page = have_page ? a.d.block_table[(size_t)seq * a.d.max_pages_per_seq + page_idx] : 0, head_step = a.d.page_size * D;
     const size_t tile = (((size_t)a.layer * a.d.n_pages + page) * a.hkv * a.d.page_size + (have_page ? pos - page_idx * a.d.page_size : 0)) * (size_t)D;
-    heads_of(a.k + (size_t)row * a.k_stride, a.hkv, a.k_weight, (__nv_bfloat16*)a.d.k_pool + tile, head_step, have_page);
+    heads_of(a.k + (size_t)row * a.k_stride, a.hkv, a.k_weight, (__nv_bfloat16*)a.d.k_pool + tile, head_step, have_page, false);
     if (have_page)
       for (int h = part * HEADS + sub; h < a.hkv; h += parts * HEADS)
         *reinterpret_cast<uint4*>((__nv_bfloat16*)a.d.v_pool + tile + (size_t)h * head_step + at) =
