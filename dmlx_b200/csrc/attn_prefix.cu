@@ -36,7 +36,7 @@ namespace {
 
 constexpr int kMaxRows = 4096;
 constexpr int kLevels = 3;        // nodes that a row may go through
-constexpr int kItemUnits = 44;    // of an item of the tensor-core kernel, beside its blocks
+constexpr int kItemUnits = 44, kBlockUnits = 10, kTileUnits = 6;  // of time, of the tensor-core kernel
 constexpr int kMinPages = 2;      // of a node: below that a part of its own costs more than it saves
 constexpr int kWarpRows = 16;     // query rows of an item of the warps' kernel
 constexpr int kBlockKeys = 128, kBlockPages = 4, kTileRows = 128;
@@ -89,7 +89,7 @@ struct PlanShared {
   int n_nodes, n_members, more, warp_sums[32], carry;
   int max_a[kLengthsA], items_a[kLengthsA], units_a[kLengthsA], slots_a[kLengthsA];
   int items_b[kLengthsB], slots_b[kLengthsB];
-  int units_b, workers_a, pick_a, pick_b, next_a, next_b;
+  int units_b, longest_b, workers_a, pick_a, pick_b, next_a, next_b;
 };
 
 // Common pages of two sequences that agree up to `lo` (at least one page behind it too): a search in steps of 16 probes.
@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
   // ---- lengths of chunks ----
   if (tid < kLengthsA) { s.max_a[tid] = 0; s.items_a[tid] = 0; s.units_a[tid] = 0; s.slots_a[tid] = 0; }
   if (tid < kLengthsB) { s.items_b[tid] = 0; s.slots_b[tid] = 0; }
-  if (tid == 0) { s.next_a = 0; s.next_b = 0; s.carry = 0; s.units_b = 0; }
+  if (tid == 0) { s.next_a = 0; s.next_b = 0; s.carry = 0; s.units_b = 0; s.longest_b = 0; }
   __syncthreads();
   const int n_nodes = s.n_nodes, members = tile_members(group), warp_members = kWarpRows / group;
   for (int u = tid; u < n_nodes * kLengthsA; u += blockDim.x) {  // a thread per node and length
@@ -236,25 +236,26 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
     if (is_large(n.count, group)) {
       const int tiles = ceil_div(n.count, 2 * members), last = n.count - (tiles - 1) * 2 * members;
       const bool one = last <= members;
-      // eighths of a block: two tiles of rows count 8, one 5 (4000 cycles); an item's fill, drain and way out kItemUnits (22000)
+      // in units of 500 cycles: a block of two tiles of rows kBlockUnits, of one kTileUnits, with the memory busy beside; an item's fill, drain and way out kItemUnits
       const int len = even_length(pages, length_a(k)), chunks = ceil_div(pages, len), blocks = ceil_div(pages, kBlockPages);
-      atomicMax(&s.max_a[k], (tiles > 1 || !one ? 8 : 5) * min(blocks, len / kBlockPages) + kItemUnits);
+      atomicMax(&s.max_a[k], (tiles > 1 || !one ? kBlockUnits : kTileUnits) * min(blocks, len / kBlockPages) + kItemUnits);
       atomicAdd(&s.items_a[k], tiles * chunks);
-      atomicAdd(&s.units_a[k], (8 * (tiles - (one ? 1 : 0)) + (one ? 5 : 0)) * blocks + kItemUnits * tiles * chunks);
+      atomicAdd(&s.units_a[k], (kBlockUnits * (tiles - (one ? 1 : 0)) + (one ? kTileUnits : 0)) * blocks + kItemUnits * tiles * chunks);
       atomicAdd(&s.slots_a[k], (n.count - (one ? last : 0)) * large_parts(pages, len, false) + (one ? last : 0) * large_parts(pages, len, true));
     } else if (k < kLengthsB) {
       const int chunks = ceil_div(pages, length_b(k)), tiles = ceil_div(n.count, warp_members);
       atomicAdd(&s.items_b[k], tiles * chunks);
       atomicAdd(&s.slots_b[k], n.count * chunks);
-      if (k == 0) atomicAdd(&s.units_b, tiles * pages);
+      if (k == 0) { atomicAdd(&s.units_b, tiles * pages); atomicMax(&s.longest_b, pages); }
     }
   }
-  int own_chunks[kLengthsB] = {}, own_pages = 0;
+  int own_chunks[kLengthsB] = {}, own_pages = 0, longest = 0;
   for (int i = tid; i < rows; i += blockDim.x) {
     const int pages = ceil_div(p.row_ctx[i], d.page_size) - from[i];
 #pragma unroll
     for (int k = 0; k < kLengthsB; ++k) own_chunks[k] += ceil_div(pages, length_b(k));
     own_pages += pages;
+    longest = max(longest, pages);
   }
 #pragma unroll
   for (int k = 0; k < kLengthsB; ++k) {
@@ -262,22 +263,26 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
     if (lane == 0) { atomicAdd(&s.items_b[k], c); atomicAdd(&s.slots_b[k], c); }
   }
   own_pages = __reduce_add_sync(0xffffffffu, own_pages);
-  if (lane == 0) atomicAdd(&s.units_b, own_pages);
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  if (lane == 0) { atomicAdd(&s.units_b, own_pages); atomicMax(&s.longest_b, longest); }
   __syncthreads();
   if (warp == 0) {
-    // The rest runs beside the large nodes, on the SMs that they leave and on theirs when they are done.  Of an SM it takes 2.3 units an item and
-    // `per_page` a page (0.6 us and, of 128 dims in 16 bits, 0.2, on 37 to 74 SMs), and half as much again when all SMs do this at once, which the memory bounds.
-    // Chunks in some rounds of the blocks that the nodes get; the shortest estimated time of those whose parts fit, a lane per choice of the two.
-    const float rest = ((float)s.units_b * per_page + 2.3f * s.items_b[0]) * d.n_kv_heads;
-    const float per_worker = __fdividef(1.5f, workers);
-    auto share_up = [](int a, int b) { return __float2int_ru(__fdividef((float)a, (float)b)); };  // (a little too much or too little does no harm)
+    // Lengths of both kinds of chunks, and how many blocks work on the nodes, by the shortest estimated time of those whose parts fit; a lane per choice.
+    // The rest runs beside the nodes, on the SMs that they leave and on theirs when they are done.  Of an SM it takes 2.3 units an item and `per_page` a
+    // page (0.6 us and, of 128 dims in 16 bits, 0.2), up to two thirds of the SMs, whose loads are all that the memory gives; the last items end one by one.
+    const float of_item = per_page * __fdividef(warps, workers) * 0.6f, most = 0.68f * workers, heads = d.n_kv_heads;
+    auto share_up = [](float a, float b) { return __float2int_ru(__fdividef(a, b)); };  // (a little too much or too little does no harm)
     float best = 3e38f;
     int choice = 0;
-    for (int c = lane; c < 4 * kLengthsA; c += 32) {
-      const int k = c >> 2, items = s.items_a[k] * d.n_kv_heads, rounds = max(share_up(items, workers), 1) + (c & 3), mine = min(max(share_up(items, rounds), 1), workers);
-      const float nodes = fmaxf(__fdividef((float)s.units_a[k] * d.n_kv_heads, mine), 0.875f * rounds * s.max_a[k]);
-      const float cost = nodes + fmaxf(rest - (workers - mine) * nodes, 0.f) * per_worker + s.slots_a[k] * 0.025f;
-      if ((k == 0 || s.slots_a[k] + s.slots_b[0] <= p.max_slots) && cost < best) { best = cost; choice = k << 16 | mine; }
+    for (int c = lane; c < kLengthsA * 2 * kLengthsB; c += 32) {
+      const int k = c / (2 * kLengthsB), b = c % kLengthsB, slots = s.slots_a[k] + s.slots_b[b];
+      const float items = s.items_a[k] * heads, rounds = max(share_up(items, workers), 1) + c / kLengthsB % 2;
+      const int mine = min(max(share_up(items, rounds), 1), workers);
+      const float nodes = fmaxf(__fdividef(s.units_a[k] * heads, mine), 0.875f * rounds * s.max_a[k]);
+      const float rest = (s.units_b * per_page + 2.3f * s.items_b[b]) * heads, rate = fmaxf(fminf(workers - mine, most), 0.01f), beside = __fdividef(rest, rate);
+      const float pages = fminf(beside, nodes + __fdividef(fmaxf(rest - nodes * rate, 0.f), most)) + of_item * min(length_b(b), s.longest_b);
+      const float cost = fmaxf(nodes, pages) + 0.025f * slots;
+      if ((slots <= p.max_slots || (k == 0 && b == 0)) && cost < best) { best = cost; choice = (k * kLengthsB + b) << 16 | mine; }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -285,11 +290,7 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
       const int theirs = __shfl_xor_sync(0xffffffffu, choice, o);
       if (other < best || (other == best && theirs < choice)) { best = other; choice = theirs; }
     }
-    // Of the rest, the longest chunks that give every warp about two items, if their parts fit.
-    const int pick = choice >> 16, k = min(lane, kLengthsB - 1);
-    const unsigned stop = __ballot_sync(0xffffffffu, lane > 0 && (lane >= kLengthsB - 1 || (long long)s.items_b[k] * d.n_kv_heads >= 2LL * warps));
-    const unsigned over = __ballot_sync(0xffffffffu, lane > 0 && (lane >= kLengthsB || s.slots_a[pick] + s.slots_b[k] > p.max_slots));
-    if (lane == 0) { s.pick_a = pick; s.workers_a = choice & 0xffff; s.pick_b = min(__ffs(stop) - 1, __ffs(over) - 2); }
+    if (lane == 0) { s.pick_a = (choice >> 16) / kLengthsB; s.pick_b = (choice >> 16) % kLengthsB; s.workers_a = choice & 0xffff; }
   }
   __syncthreads();
   const int len_a = length_a(s.pick_a), len_b = length_b(s.pick_b);
