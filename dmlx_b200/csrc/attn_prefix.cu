@@ -271,6 +271,7 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
     // The rest runs beside the nodes, on the SMs that they leave and on theirs when they are done.  Of an SM it takes 2.3 units an item and `per_page` a
     // page (0.6 us and, of 128 dims in 16 bits, 0.2), up to two thirds of the SMs, whose loads are all that the memory gives; the last items end one by one.
     const float of_item = per_page * __fdividef(warps, workers) * 0.6f, most = 0.68f * workers, heads = d.n_kv_heads;
+    const float of_slot = 6e-6f * d.n_kv_heads * group * d.head_dim;  // written and read again
     auto share_up = [](float a, float b) { return __float2int_ru(__fdividef(a, b)); };  // (a little too much or too little does no harm)
     float best = 3e38f;
     int choice = 0;
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
       const float nodes = fmaxf(__fdividef(s.units_a[k] * heads, mine), 0.875f * rounds * s.max_a[k]);
       const float rest = (s.units_b * per_page + 2.3f * s.items_b[b]) * heads, rate = fmaxf(fminf(workers - mine, most), 0.01f), beside = __fdividef(rest, rate);
       const float pages = fminf(beside, nodes + __fdividef(fmaxf(rest - nodes * rate, 0.f), most)) + of_item * min(length_b(b), s.longest_b);
-      const float cost = fmaxf(nodes, pages) + 0.025f * slots;
+      const float cost = fmaxf(nodes, pages) + of_slot * slots;
       if ((slots <= p.max_slots || (k == 0 && b == 0)) && cost < best) { best = cost; choice = (k * kLengthsB + b) << 16 | mine; }
     }
 #pragma unroll
