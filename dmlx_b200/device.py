@@ -170,7 +170,7 @@ class PagedKVCache:
         (t, hq, d), hkv = q.shape, k.shape[1]
         q_shape, k_shape = (t, hq, d), (t, hkv, d)
         strides = _rows(q, q_shape, device), _rows(k, k_shape, device), _rows(v, k_shape, device)
-        q_out = q.new_empty(q_shape) if q_out is None else q_out
+        q_out = torch.empty_like(q) if q_out is None else q_out
         shape = _lib.NormRope(hq, hkv, d, d if rot_dim is None else rot_dim, interleaved, eps, theta)
         _lib.check(lib.b200_kv_norm_rope_append(self._h, layer, C.byref(shape), q.data_ptr(), k.data_ptr(), v.data_ptr(), *strides, _weight(q_weight, d, device),
                                                 _weight(k_weight, d, device), _ints(positions, t, device), _ints(row_seq, t, device), t, q_out.data_ptr(),
@@ -376,8 +376,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, q_we
     (t, hq, d), hkv = q.shape, k.shape[1]
     q_shape, k_shape = (t, hq, d), (t, hkv, d)
     q_stride, k_stride = _rows(q, q_shape, device), _rows(k, k_shape, device)
-    q_out = q.new_empty(q_shape) if q_out is None else q_out
-    k_out = k.new_empty(k_shape) if k_out is None else k_out
+    q_out = torch.empty_like(q) if q_out is None else q_out
+    k_out = torch.empty_like(k) if k_out is None else k_out
     shape = _lib.NormRope(hq, hkv, d, d if rot_dim is None else rot_dim, interleaved, eps, theta)
     _lib.check(lib.b200_qk_norm_rope(C.byref(shape), q.data_ptr(), k.data_ptr(), q_stride, k_stride, _weight(q_weight, d, device), _weight(k_weight, d, device),
                                      _ints(positions, t, device), t, q_out.data_ptr(), k_out.data_ptr(), _rows(q_out, q_shape, device),
@@ -415,7 +415,7 @@ class SharedPrefixAttention:
         if q.shape[0] != self.rows or self.cache._h is None:
             raise ValueError("the pool is closed" if self.cache._h is None else f"{q.shape[0]} rows, the plan has {self.rows}")
         device, shape = torch.cuda.current_device(), (self.rows, *self._heads)
-        out = q.new_empty(shape) if out is None else out
+        out = torch.empty_like(q) if out is None else out
         _lib.check(lib.b200_prefix_attn_run(self._h, layer, q.data_ptr(), _rows(q, shape, device), out.data_ptr(), _rows(out, shape, device), _raw_stream(device)))
         return out
 
@@ -453,7 +453,7 @@ class LoraAdapters:
         if t != batch.rows:
             raise ValueError(f"{t} rows, the batch's plan has {batch.rows}")
         device, y_shape = torch.cuda.current_device(), (t, self.n)
-        out = y.new_empty(y_shape) if out is None else out
+        out = torch.empty_like(y) if out is None else out
         _lib.check(lib.b200_lora_apply(self._h, batch._h, x.data_ptr(), _rows(x, (t, self.k), device), y.data_ptr(), _rows(y, y_shape, device), out.data_ptr(),
                                        _rows(out, y_shape, device), _raw_stream(device)))
         return out
