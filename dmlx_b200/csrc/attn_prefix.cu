@@ -18,8 +18,8 @@
 // Of 128 keys and 256 query rows the tensor-core kernel's exponentials and its products take 2048 cycles each; a block of both takes 3750, since a tile's
 // next scores wait for its last product (P lies where they go) and the two tiles overlap only in part; an item has 22000 more around its blocks, for q,
 // the first pages and 128 KB of parts.  The warps' kernel is bound by the stream of pages.  Measured per layer, 32 query heads on 8, 128 dims, pages in
-// HBM: 256 rows behind 8192 shared tokens with up to 512 of their own 86 us (one after the other 110: 52 the nodes' on all SMs, 51 the warps', 10 the
-// join), 64 rows behind 2048 28 us, 128 rows behind 4096 on FP8 pages 38 us; plans 11 to 14 us.
+// HBM: 256 rows behind 8192 shared tokens with up to 512 of their own 88 us (one after the other 110: 52 the nodes' on all SMs, 51 the warps', 10 the
+// join), 64 rows behind 2048 28 us, 128 rows behind 4096 on FP8 pages 39.5 us; plans 11 to 15 us.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
@@ -50,7 +50,7 @@ struct Node {
   int p0, p1;         // pages
 };
 struct Member { int row, slot; };  // a row of a node; the place of its first part
-struct alignas(16) ItemA { int seq, first, count, p0, p1, part, pad[2]; };  // pages of slot seq's table for `count` members from `first` on; their part behind `slot`
+struct alignas(16) ItemA { int seq, first, count, p0, p1, part, tiles, pad; };  // pages of slot seq's table for `count` members from `first` on; their part behind `slot`
 struct alignas(16) ItemB { int seq, first, count, p0, p1, ctx, part, pad; };  // count 0: own pages of the row `first`, its part `part`, and ctx tokens that it sees; else members, as above
 
 enum { H_ITEMS_A = 0, H_ITEMS_B, H_NEXT_A, H_NEXT_B, H_WORKERS_A, H_COUNT = 16 };  // H_WORKERS_A: blocks that work on the large nodes
@@ -71,9 +71,12 @@ __host__ __device__ constexpr int tile_members(int group) { return kTileRows / g
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 // ---- the plan ------------------------------------------------------------------------------------------------------------
-// Parts of a row of a node: a chunk gives one, or two where the item has one tile of rows and its blocks of keys go to the two softmax groups in turn.
+// A large node's rows in items of equal size, of one tile if all of them fit, else of two each: how many parts a row has depends on the node alone, not on
+// its place among the members, which atomics hand out.  A chunk gives a row one part, or two where the item's one tile of rows has its blocks of keys go to
+// the two softmax groups in turn.
 __host__ __device__ __forceinline__ bool is_large(int count, int group) { return count * group > kWarpRows; }
-__device__ __forceinline__ bool one_tile(const Node& n, int tile, int group) { return n.count - tile * 2 * tile_members(group) <= tile_members(group); }
+__device__ __forceinline__ bool one_tile(const Node& n, int group) { return n.count <= tile_members(group); }
+__device__ __forceinline__ int items_of(const Node& n, int group) { return ceil_div(n.count, 2 * tile_members(group)); }  // of a chunk
 __device__ __forceinline__ int even_length(int pages, int len) { return ceil_div(ceil_div(pages, ceil_div(pages, len)), kBlockPages) * kBlockPages; }  // of as many chunks
 __device__ __forceinline__ int large_parts(int pages, int len, bool one) {  // len: pages of a chunk, a multiple of kBlockPages
   const int chunks = ceil_div(pages, len), last = pages - (chunks - 1) * len;
@@ -229,19 +232,19 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
   if (tid < kLengthsB) { s.items_b[tid] = 0; s.slots_b[tid] = 0; }
   if (tid == 0) { s.next_a = 0; s.next_b = 0; s.carry = 0; s.units_b = 0; s.longest_b = 0; }
   __syncthreads();
-  const int n_nodes = s.n_nodes, members = tile_members(group), warp_members = kWarpRows / group;
+  const int n_nodes = s.n_nodes, warp_members = kWarpRows / group;
   for (int u = tid; u < n_nodes * kLengthsA; u += blockDim.x) {  // a thread per node and length
     const Node n = p.nodes[u / kLengthsA];
     const int k = u % kLengthsA, pages = n.p1 - n.p0;
     if (is_large(n.count, group)) {
-      const int tiles = ceil_div(n.count, 2 * members), last = n.count - (tiles - 1) * 2 * members;
-      const bool one = last <= members;
       // in units of 500 cycles: a block of two tiles of rows kBlockUnits, of one kTileUnits, with the memory busy beside; an item's fill, drain and way out kItemUnits
-      const int len = even_length(pages, length_a(k)), chunks = ceil_div(pages, len), blocks = ceil_div(pages, kBlockPages);
-      atomicMax(&s.max_a[k], (tiles > 1 || !one ? kBlockUnits : kTileUnits) * min(blocks, len / kBlockPages) + kItemUnits);
+      const bool one = one_tile(n, group);
+      const int len = even_length(pages, length_a(k)), chunks = ceil_div(pages, len), blocks = ceil_div(pages, kBlockPages), of_block = one ? kTileUnits : kBlockUnits;
+      const int tiles = items_of(n, group);
+      atomicMax(&s.max_a[k], of_block * min(blocks, len / kBlockPages) + kItemUnits);
       atomicAdd(&s.items_a[k], tiles * chunks);
-      atomicAdd(&s.units_a[k], (kBlockUnits * (tiles - (one ? 1 : 0)) + (one ? kTileUnits : 0)) * blocks + kItemUnits * tiles * chunks);
-      atomicAdd(&s.slots_a[k], (n.count - (one ? last : 0)) * large_parts(pages, len, false) + (one ? last : 0) * large_parts(pages, len, true));
+      atomicAdd(&s.units_a[k], tiles * (of_block * blocks + kItemUnits * chunks));
+      atomicAdd(&s.slots_a[k], n.count * large_parts(pages, len, one));
     } else if (k < kLengthsB) {
       const int chunks = ceil_div(pages, length_b(k)), tiles = ceil_div(n.count, warp_members);
       atomicAdd(&s.items_b[k], tiles * chunks);
@@ -301,7 +304,7 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
       const Node n = p.nodes[p.member_node[at]];
       const int row = p.members[at].row, pages = n.p1 - n.p0;
       p.members[at].slot = parts[row];
-      parts[row] += is_large(n.count, group) ? large_parts(pages, even_length(pages, len_a), one_tile(n, (at - n.first) / (2 * members), group)) : ceil_div(pages, len_b);
+      parts[row] += is_large(n.count, group) ? large_parts(pages, even_length(pages, len_a), one_tile(n, group)) : ceil_div(pages, len_b);
     }
     __syncthreads();
   }
@@ -339,15 +342,14 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
   for (int i = warp; i < n_nodes; i += blockDim.x / 32) {
     const Node n = p.nodes[i];
     const int pages = n.p1 - n.p0, large = is_large(n.count, group) ? 1 : 0, len = large ? even_length(pages, len_a) : min(len_b, pages), chunks = ceil_div(pages, len);
-    const int tiles = large ? ceil_div(n.count, 2 * members) : 1;
+    const int tiles = large ? items_of(n, group) : 1, each = ceil_div(n.count, tiles), one = one_tile(n, group) ? 1 : 0;
     int at = 0;
     if (lane == 0) at = atomicAdd(large ? &s.next_a : &s.next_b, tiles * chunks);
     at = __shfl_sync(0xffffffffu, at, 0);
     for (int c = lane; c < tiles * chunks; c += 32) {
       const int tile = c % tiles, chunk = c / tiles, p0 = n.p0 + chunk * len, p1 = min(n.p1, p0 + len);
       if (large) {
-        const int before = tile * 2 * members;
-        p.items_a[at + c] = ItemA{n.seq, n.first + before, min(2 * members, n.count - before), p0, p1, one_tile(n, tile, group) ? 2 * chunk : chunk, {0, 0}};
+        p.items_a[at + c] = ItemA{n.seq, n.first + tile * each, min(each, n.count - tile * each), p0, p1, one ? 2 * chunk : chunk, one ? 1 : 2, 0};
       } else {
         p.items_b[at + c] = ItemB{n.seq, n.first, n.count, p0, p1, 0x7fffffff, chunk, 0};
       }
@@ -842,7 +844,7 @@ __global__ void __launch_bounds__(threads_a(FP8), 1) prefix_node_kernel(const __
       if (there) it = a.p.items_a[id / a.d.n_kv_heads];
       const int head = id % a.d.n_kv_heads, seq = it.seq, p0 = it.p0, p1 = it.p1;
       wait_all(&sh.item_free[n & 1u], ((n >> 1) & 1u) ^ 1u);
-      const int kind = ok && there ? (it.count > members ? 2 : 1) : 0;
+      const int kind = ok && there ? it.tiles : 0;
       if (lane == 0) {
         int* to = sh.item[n & 1u];
         to[0] = kind; to[1] = head; to[2] = seq; to[3] = it.first; to[4] = it.count; to[5] = p0; to[6] = p1; to[7] = it.part;

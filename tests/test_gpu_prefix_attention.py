@@ -348,6 +348,22 @@ def test_a_handle_through_batches_of_many_and_few_rows(fp8):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,hq,hkv,d,fp8", [(70, 32, 4, 128, False), (70, 32, 4, 128, True), (33, 8, 2, 64, False), (65, 64, 4, 64, False), (9, 8, 2, 128, False)])
+def test_a_row_s_bits_do_not_depend_on_its_place(rows, hq, hkv, d, fp8):
+    """Plans made again, and of the rows in another order: which rows share a tile differs, no result does."""
+    from dmlx_b200 import device as dev
+
+    cache, slots, ctx = _tree(dev, rows, 650, 0, 0, [1, 40, 90], hq, hkv, d, fp8)
+    q = _random(rows, hq, d, seed=4, scale=2.0)
+    handle = dev.SharedPrefixAttention(cache, rows)
+    first = _run(cache, q, slots, ctx, handle=handle)
+    for turn in range(6):
+        order = torch.randperm(rows, generator=torch.Generator().manual_seed(turn)).tolist() if turn % 2 else list(range(rows))
+        again = _run(cache, q[order], [slots[i] for i in order], [ctx[i] for i in order], handle=handle)
+        assert torch.equal(again, first[order])
+
+
+@pytest.mark.gpu
 def test_a_closed_pool_is_refused():
     from dmlx_b200 import device as dev
 
