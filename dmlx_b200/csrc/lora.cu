@@ -60,13 +60,12 @@ constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kSlices = 4;        // of K
 constexpr int kFewRows = 16;      // of a tile whose slice of K the warps of a block share
 constexpr int kMaxAdapters = 4096, kMaxRank = 128, kMaxWidth = 1 << 24, kTileRows = 128, kGroupRows = 32;
-constexpr int kEnoughTiles = 74;  // half the SMs (a tile is four items of the first product): beyond that, larger tiles rather than more of them
 
 int rank_rows(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
 
 // ---- the plan ------------------------------------------------------------------------------------------------------
 // Places, tiles and groups are handed out as the atomics come: no row's result depends on its place, its tile or its block.
-__global__ void __launch_bounds__(1024) lora_plan_kernel(const int* row_adapter, int rows, int n_adapters, int max_tiles, int* __restrict__ order,
+__global__ void __launch_bounds__(1024) lora_plan_kernel(const int* row_adapter, int rows, int n_adapters, int max_tiles, int enough_tiles, int* __restrict__ order,
                                                          int4* __restrict__ tiles, int4* __restrict__ groups, int* __restrict__ hdr) {
   after_previous();
   __shared__ int count[kMaxAdapters + 1], total[4], next[4];  // next: place, group, tile of many rows, tile of few
@@ -101,7 +100,7 @@ __global__ void __launch_bounds__(1024) lora_plan_kernel(const int* row_adapter,
   }
   __syncthreads();
   int shift = 4;
-  while ((1 << shift) < kTileRows && total[shift - 4] > kEnoughTiles) ++shift;
+  while ((1 << shift) < kTileRows && total[shift - 4] > enough_tiles) ++shift;
   for (int i = tid; i < bins; i += blockDim.x) {
     const int c = count[i];
     if (c == 0) continue;
@@ -615,8 +614,11 @@ extern "C" b200_status b200_lora_plan(b200_lora_batch* b, const int32_t* d_row_a
   if (st != B200_OK) return st;
   b->rows = rows;
   if (rows == 0) return B200_OK;
+  // A tile is kSlices items of the first product: beyond one for each of its blocks, larger tiles rather than more of them (2097 rows of two adapters of
+  // rank 128, one block per SM, at 14336 -> 4096: 99 us; with room for two blocks per SM, so smaller tiles, 166).
+  const int enough = b200_sm_count() * (b->max_rank > 64 ? Down<128>::PER_SM : Down<64>::PER_SM) / kSlices;
   launch_after(lora_plan_kernel, 1, rows <= 256 ? 256 : 1024, 0, (cudaStream_t)stream, d_row_adapter, rows, b->max_adapters,
-               b->max_tiles, b->order, b->tiles, b->groups, b->hdr);
+               b->max_tiles, enough, b->order, b->tiles, b->groups, b->hdr);
   B200_LAUNCH_CHECK();
   return B200_OK;
 }
