@@ -763,8 +763,10 @@ struct SharedA {
 template <int D, bool FP8>
 constexpr size_t shared_a() { return 2 * ShapeA<D, FP8>::QBYTES + ShapeA<D, FP8>::SLOTS * ShapeA<D, FP8>::SLOT + ShapeA<D, FP8>::RAWS * ShapeA<D, FP8>::RAW + sizeof(SharedA<D, FP8>); }
 
-// Waits for `count` threads, of whole warps, at barrier `id`; whether any of them says so.
+// Waits for `count` threads, of whole warps, at barrier `id`; whether any of them says so.  (The barrier is `.aligned` and has no limit: a warp's lanes
+// come to it together, also out of a wait that each of them polls for itself.)
 __device__ __forceinline__ bool any_of(int id, int count, bool mine) {
+  __syncwarp();
   uint32_t r;
   asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred.aligned q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"(mine ? 1u : 0u), "r"(id), "r"(count) : "memory");
   return r != 0;

@@ -117,6 +117,43 @@ def _tree(dev, rows, system, docs, doc, own, hq, hkv, d, fp8=False, layers=1, se
     return cache, slots, [cache.seq_len(s) for s in slots]
 
 
+class _Device:
+    """`count` 32-bit words of device memory from `address` on."""
+
+    def __init__(self, address, count):
+        self.__cuda_array_interface__ = dict(shape=(count,), typestr="<i4", data=(address, False), version=3)
+
+
+def _plan_of(handle):
+    """What the handle's last plan made of the large nodes, {items per kv head, other items, blocks that work on them} and the items {slot, first member, members,
+    first page, last page + 1, part, tiles of rows, -}, read behind the handle's pointers: pool, {rows, rows}, memory, header, five arrays, items."""
+    words = (C.c_uint64 * 12).from_address(handle._h)
+    torch.cuda.synchronize()
+    header = torch.as_tensor(_Device(words[3], 5), device="cuda").tolist()
+    items = torch.as_tensor(_Device(words[10], 8 * max(header[0], 1)), device="cuda").view(-1, 8)[:header[0]].tolist()
+    return dict(large=header[0], other=header[1], workers=header[4], items=items)
+
+
+def _forest(dev, docs, hq, hkv, d, fp8, seed=0):
+    """Documents of their own, (rows, pages) each, every row with one token more.  Keys grow along a document, so that the largest score comes late, and values differ
+    by 4^4 between pages; (cache, slots, contexts)."""
+    pages, rows = max(p for _, p in docs) + 1, sum(r for r, _ in docs)
+    cache = dev.PagedKVCache(1, hkv, d, sum(p for _, p in docs) + rows + 8, len(docs) + rows, pages, hq, max_rows=max(32 * pages, rows), kv_dtype=dev.KV_FP8_E4M3 if fp8 else dev.KV_BF16)
+    slots = []
+    for i, (count, of_doc) in enumerate(docs):
+        tokens = 32 * of_doc
+        cache.reserve(torch.tensor([[i, tokens, 0, 0]], dtype=torch.int32, device="cuda"))
+        k, v = _random(tokens, hkv, d, seed=seed + i), _random(tokens, hkv, d, seed=seed + 1000 + i)
+        k *= torch.linspace(0.02, 2.5, tokens, device="cuda").bfloat16()[:, None, None]
+        v *= (4.0 ** ((torch.arange(tokens, device="cuda") // 32 * 7 + i) % 5 - 2)).bfloat16()[:, None, None]
+        cache.append(0, k, v)
+        for _ in range(count):
+            slots.append(len(docs) + len(slots))
+            cache.fork(i, slots[-1], tokens)
+    _append(cache, {s: 1 for s in slots}, seed + 2000)
+    return cache, slots, [cache.seq_len(s) for s in slots]
+
+
 CASES = [  # rows, system, docs, doc, own tokens, hq, hkv, d, fp8
     (1, 0, 0, 0, [1], 4, 1, 64, False),
     (1, 0, 0, 0, [1000], 8, 2, 128, False),
@@ -450,6 +487,26 @@ def test_a_step_s_attention_half():
     for r, s in enumerate(slots):
         held_k, held_v = cache.gather(0, s)
         assert torch.equal(held_k[-1], rows_k[r]) and torch.equal(held_v[-1], v[r])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pages", [(9, 13, 22, 41, 5), (37, 40, 33, 35)])
+@pytest.mark.parametrize("d,fp8", [(128, False), (128, True), (64, False)])
+def test_blocks_that_take_items_of_both_kinds_in_turn(pages, d, fp8):
+    """More items of large nodes than SMs, whatever lengths the plan picks (25 nodes of 8 kv heads): of one tile of rows (4 of 8 query heads) and of two (17)."""
+    from dmlx_b200 import device as dev
+
+    cache, slots, ctx = _forest(dev, [((4, 17)[i % 2], pages[i % len(pages)]) for i in range(25)], 64, 8, d, fp8)
+    q = _random(len(slots), 64, d, seed=9)
+    handle = dev.SharedPrefixAttention(cache, len(slots))
+    got = _run(cache, q, slots, ctx, handle=handle)
+    plan = _plan_of(handle)
+    assert plan["large"] * 8 > plan["workers"] > 0 and {it[6] for it in plan["items"]} == {1, 2}
+    for tiles in (1, 2):  # pages that end inside a block of four, and more blocks than there are places for keys and values
+        lengths = [it[4] - it[3] for it in plan["items"] if it[6] == tiles]
+        assert max(lengths) > (32 if min(pages) > 32 else 16) and any(n % 4 for n in lengths)
+    _check(got, *_want(cache, 0, q, slots, ctx))
+    assert torch.equal(got, handle.run(0, q))
 
 
 def test_what_is_refused():
