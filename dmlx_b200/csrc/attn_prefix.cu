@@ -512,7 +512,8 @@ __device__ __forceinline__ void warp_items(const CUtensorMap& kmap, const CUtens
   bool alive = true;
   uint32_t used = 0, use_slot = 0, use_lap = 0;
   auto next_tile = [&]() {  // the address of the next tile in turn, when it is there
-    alive = ptx::mbar_wait(&full[use_slot], use_lap & 1u);
+    // (each lane polls for itself: what follows wants the whole warp, whether the tile came or not)
+    alive = __all_sync(0xffffffffu, ptx::mbar_wait(&full[use_slot], use_lap & 1u));
     return ptx::smem_u32(tiles + use_slot * TILE);
   };
   auto done_tile = [&]() {

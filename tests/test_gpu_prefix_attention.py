@@ -509,6 +509,28 @@ def test_blocks_that_take_items_of_both_kinds_in_turn(pages, d, fp8):
     assert torch.equal(got, handle.run(0, q))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,hq,hkv,fp8", [(128, 32, 8, False), (128, 48, 3, True), (64, 8, 8, False)])
+def test_warps_that_take_many_items_in_turn(d, hq, hkv, fp8):
+    """Rows that share nothing, of one page to several: more items than the chip has warps for them, so that each takes the pages of several through its ring."""
+    from dmlx_b200 import device as dev
+
+    rows = 1300
+    cache = dev.PagedKVCache(1, hkv, d, 4 * rows, rows, 6, hq, max_rows=2048, kv_dtype=dev.KV_FP8_E4M3 if fp8 else dev.KV_BF16)
+    counts = [(1, 40, 32, 65, 7, 129)[i % 6] for i in range(rows)]
+    for lo in range(0, rows, 40):
+        _append(cache, {s: counts[s] for s in range(lo, min(lo + 40, rows))}, lo)
+    q = _random(rows, hq, d, seed=3, scale=2.0)
+    slots = list(range(rows))
+    handle = dev.SharedPrefixAttention(cache, rows)
+    got = _run(cache, q, slots, counts, handle=handle)
+    plan = _plan_of(handle)
+    assert plan["large"] == 0 and plan["other"] * hkv > 12 * torch.cuda.get_device_properties(0).multi_processor_count
+    some = list(range(0, rows, 7))
+    _check(got[some], *_want(cache, 0, q[some], [slots[i] for i in some], [counts[i] for i in some]))
+    assert torch.equal(got, handle.run(0, q))
+
+
 def test_what_is_refused():
     from dmlx_b200 import _lib
 
