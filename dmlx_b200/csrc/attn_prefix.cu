@@ -1100,15 +1100,22 @@ __global__ void __launch_bounds__(threads_a(FP8), 1) prefix_node_kernel(const __
           top = max_nan(top, max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * ks[c]);
         }
         if (__any_sync(0xffffffffu, top != top)) {  // a score that is no number weighs nothing, as a hidden one does
-          top = kHidden;
+          const bool none = top != top;
+          top = none ? kHidden : top;
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+          for (int c = 0; c < 2; ++c) {
+            if (none) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float x = fmaxf(__uint_as_float(u[c][i]), kHidden);
-              u[c][i] = __float_as_uint(x);
-              top = fmaxf(top, x * ks[c]);
+              for (int i = 0; i < 32; ++i) {
+                // (on 8-bit pages behind the page's scale, which would make so little of kHidden that it is above kNoScale)
+                const float x = fmaxf(FP8 ? __uint_as_float(u[c][i]) * ks[c] : __uint_as_float(u[c][i]), kHidden);
+                u[c][i] = __float_as_uint(x);
+                top = fmaxf(top, FP8 ? x : x * ks[c]);
+              }
+              if (FP8) ks[c] = 1.f;
             }
+          }
+          __syncwarp();
         }
         ptx::tc_fence_before_sync();
         if (any_of(pair, 64, top > scale + kLate)) {

@@ -531,6 +531,49 @@ def test_warps_that_take_many_items_in_turn(d, hq, hkv, fp8):
     assert torch.equal(got, handle.run(0, q))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [20, 3])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_scores_that_are_no_numbers_weigh_nothing(rows, fp8):
+    """A query that is no number, and keys: all of the first four pages for one kv head and some of later ones, of a node of many rows and of one of few."""
+    from dmlx_b200 import device as dev
+
+    cache, slots, ctx = _tree(dev, rows, 700, 0, 0, [3, 40], 8, 2, 128, fp8)
+    q = _random(rows, 8, 128, seed=5, scale=2.0)
+    want, tol = _want(cache, 0, q, slots, ctx)
+    bad = q.clone()
+    bad[1, 3, 7], bad[2, 6] = float("nan"), float("nan")
+    got = _run(cache, bad, slots, ctx)
+    fine = torch.ones(rows, 8, dtype=torch.bool, device="cuda")
+    fine[1, 3] = fine[2, 6] = False
+    assert bool(((got.double() - want).abs() <= tol)[fine].all())
+    assert not bool(got[1, 3].any()) and not bool(got[2, 6].any())
+    # keys of the second kv head
+    table, hidden = cache.block_table(slots[0]), torch.zeros(700, dtype=torch.bool)
+    for at, tokens in [(i, range(32)) for i in range(4)] + [(6, (0, 9, 31)), (20, (5,))]:
+        k, v, ks, vs = cache.page_raw(0, table[at])
+        for t in tokens:
+            k[1, t, t % 128] = 0x7F if fp8 else 0x7FC0
+            hidden[32 * at + t] = True
+        cache.page_load(0, table[at], k, v, ks, vs)
+    held = _held(cache, 0, set(slots))
+    got = _run(cache, q, slots, ctx)
+    assert bool(((got.double() - want).abs() <= tol)[:, :4].all())
+    for r, s in enumerate(slots):
+        k, v = (x[:ctx[r], 1] for x in held[s])
+        there = torch.ones(ctx[r], dtype=torch.bool, device="cuda")
+        there[:700] = ~hidden.cuda()
+        assert bool(k[~there].isnan().any(1).all()) and bool(k[there].isfinite().all())
+        scores = q[r, 4:].double() @ k[there].T / math.sqrt(128)
+        top = (q[r, 4:].double().abs() @ k[there].abs().T).amax(1, keepdim=True) / math.sqrt(128)
+        p = torch.softmax(scores, 1)
+        of_row = 2.0 ** -8 * (p @ v[there]).abs() + (2.0 ** -8 + 2 * (10 * 2.0 ** -22 * top + 2.0 ** -20 * (top / 16).clamp(min=1))) * (p @ v[there].abs())
+        if fp8:
+            codes, scales = (x[:ctx[r], 1] for x in _value_codes(cache, 0, s))
+            of_row += 2.0 ** -25 * scales.amax() * codes.sum(0)
+        assert bool(((got[r, 4:].double() - p @ v[there]).abs() <= of_row).all())
+
+
 def test_what_is_refused():
     from dmlx_b200 import _lib
 
