@@ -53,7 +53,7 @@ struct Member { int row, slot; };  // a row of a node; the place of its first pa
 struct alignas(16) ItemA { int seq, first, count, p0, p1, part, tiles, pad; };  // pages of slot seq's table for `count` members from `first` on; their part behind `slot`
 struct alignas(16) ItemB { int seq, first, count, p0, p1, ctx, part, pad; };  // count 0: own pages of the row `first`, its part `part`, and ctx tokens that it sees; else members, as above
 
-enum { H_ITEMS_A = 0, H_ITEMS_B, H_NEXT_A, H_NEXT_B, H_WORKERS_A, H_COUNT = 16 };  // H_WORKERS_A: blocks that work on the large nodes
+enum { H_ITEMS_A = 0, H_ITEMS_B, H_NEXT_A, H_NEXT_B, H_WORKERS_A, H_ROWS, H_COUNT = 16 };  // H_WORKERS_A: blocks that work on the large nodes; H_ROWS: of the plan
 
 struct PlanDev {
   int *hdr, *row_seq, *row_ctx, *row_base, *member_node;
@@ -363,6 +363,7 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
     p.hdr[H_NEXT_A] = 0;
     p.hdr[H_NEXT_B] = 0;
     p.hdr[H_WORKERS_A] = s.workers_a;
+    p.hdr[H_ROWS] = rows;
   }
 }
 
@@ -370,7 +371,7 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
 struct Args {
   KvDev d;
   PlanDev p;
-  int layer, rows, n_q_heads, group;
+  int layer, rows, n_q_heads, group;  // rows of q and out; the plan of a graph's launches may come to have others (row numbers that q lacks are not read)
   bool nodes;  // whether the kernel of the large nodes is ahead of the warps'
   const __nv_bfloat16* q;
   int q_stride;
@@ -541,6 +542,7 @@ __device__ __forceinline__ void warp_items(const CUtensorMap& kmap, const CUtens
         if (it.count == 0) { row[h] = it.first; slot[h] = it.part; }
         else { const Member mb = a.p.members[it.first + m]; row[h] = mb.row; slot[h] = mb.slot + it.part; }
       }
+      if (row[h] >= a.rows) row[h] = -1;
     }
     uint32_t qa[KS][4];
 #pragma unroll
@@ -1017,6 +1019,7 @@ __global__ void __launch_bounds__(threads_a(FP8), 1) prefix_node_kernel(const __
           for (int e = 0; e < EACH; ++e) {
             const int qr = ((threadIdx.x & 255) + e * 256) / PIECES, qm = qr * by_group >> 16, member = g * members + qm;
             row[e] = qm < members && member < it[4] ? a.p.members[it[3] + member].row : -1;
+            if (row[e] >= a.rows) row[e] = -1;
           }
 #pragma unroll
           for (int e = 0; e < EACH; ++e) {
@@ -1256,8 +1259,12 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const __grid_constant_
   after_previous();
   const int u = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (blockIdx.x == 0 && threadIdx.x == 0) { a.p.hdr[H_NEXT_A] = 0; a.p.hdr[H_NEXT_B] = 0; }  // for the next layer
-  if (u >= a.rows * a.n_q_heads || a.d.state[ST_ATTN_ERR] != 0) return;
   const int row = u / a.n_q_heads, qh = u - row * a.n_q_heads;
+  if (!a.nodes && a.p.hdr[H_ITEMS_A] > 0) {  // a plan of more rows than the launches are for
+    if (blockIdx.x == 0 && threadIdx.x == 0) atomicExch(a.d.state + ST_ATTN_ERR, B200_ERR_INVALID_ARGUMENT);
+    return;
+  }
+  if (row >= min(a.rows, a.p.hdr[H_ROWS]) || a.d.state[ST_ATTN_ERR] != 0) return;
   const int s0 = a.p.row_base[row], s1 = a.p.row_base[row + 1];
   constexpr int V = D / 32;
   const float2* ml = reinterpret_cast<const float2*>(a.p.part_ml) + qh;

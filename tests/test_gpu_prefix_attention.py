@@ -574,6 +574,46 @@ def test_scores_that_are_no_numbers_weigh_nothing(rows, fp8):
         assert bool(((got[r, 4:].double() - p @ v[there]).abs() <= of_row).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+def test_captured_layers_behind_plans_of_other_rows(fp8):
+    """Layers in a graph without their plan: of more rows, of fewer, of rows for which a launch more would be needed, and of a plan that has not run."""
+    from dmlx_b200 import _lib
+    from dmlx_b200 import device as dev
+
+    cache, slots, ctx = _tree(dev, 40, 400, 0, 0, [1, 64, 130], 8, 2, 128, fp8)
+    q = _random(40, 8, 128, seed=2, scale=2.0)
+    handle, out = dev.SharedPrefixAttention(cache, 64), torch.zeros((40, 8, 128), dtype=torch.bfloat16, device="cuda")
+    plan = lambda rows: handle.plan(_ints(*slots[:rows]), _ints(*ctx[:rows]))  # noqa: E731
+    unplanned, row_seq, row_ctx = torch.cuda.CUDAGraph(), _ints(*slots[:20]), _ints(*ctx[:20])
+    with torch.cuda.graph(unplanned):
+        handle.plan(row_seq, row_ctx)
+        handle.run(0, q[:20], out=out[:20])
+    out.fill_(7)
+    handle.run(0, q[:20], out=out[:20])  # the plan was captured, and has not run
+    assert cache.error_word() == 0 and bool((out == 7).all())
+    graphs = {}
+    for rows in (20, 4):
+        plan(rows)
+        handle.run(0, q[:rows], out=out[:rows])
+        torch.cuda.synchronize()
+        graphs[rows] = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graphs[rows]):
+            handle.run(0, q[:rows], out=out[:rows])
+    want, tol = _want(cache, 0, q, slots, ctx)
+    for captured, planned in ((20, 40), (20, 8), (20, 20), (4, 2), (4, 3), (4, 40), (4, 4)):
+        plan(planned)
+        out.fill_(7)
+        graphs[captured].replay()
+        both = min(captured, planned)
+        if (captured, planned) == (4, 40):
+            assert cache.error_word() == _lib.ERR_INVALID_ARGUMENT
+            both = 0
+        assert cache.error_word() == 0
+        _check(out[:both], want[:both], tol[:both])
+        assert bool((out[both:] == 7).all())
+
+
 def test_what_is_refused():
     from dmlx_b200 import _lib
 
