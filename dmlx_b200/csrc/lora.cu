@@ -134,7 +134,7 @@ struct LoraArgs {
   int* done;
   float* parts;
   uint32_t* u;
-  int max_rows, max_tiles, n, k;
+  int max_rows, max_tiles, rows, n, k;  // rows: of x, y and out; the plan of a graph's launches may come to have others
   int x_stride, y_stride, out_stride;
 };
 
@@ -235,7 +235,10 @@ __global__ void __launch_bounds__(kThreads, Down<RS>::PER_SM) lora_down_kernel(c
     enter(lc, item);
     if (lc.item >= n_items) return;
 #pragma unroll
-    for (int i = 0; i < kTileRows / 32; ++i) xp[i] = row0 + 32 * i < lc.tile.z ? a.x + (size_t)a.order[lc.tile.y + row0 + 32 * i] * a.x_stride + lc.k0 + piece * 8 : nullptr;
+    for (int i = 0; i < kTileRows / 32; ++i) {
+      const int row = row0 + 32 * i < lc.tile.z ? a.order[lc.tile.y + row0 + 32 * i] : a.rows;
+      xp[i] = row < a.rows ? a.x + (size_t)row * a.x_stride + lc.k0 + piece * 8 : nullptr;
+    }
     ap = a.a + ((size_t)lc.tile.x * k_steps + lc.k0 / 32) * (RS * 4);
   };
   uint32_t load_slot = 0, use_slot = 0;
@@ -319,8 +322,9 @@ __global__ void __launch_bounds__(kThreads, Down<RS>::PER_SM) lora_down_kernel(c
     const int4 tile = a.tiles[tile_at];
     const int rank = tile.x >= 0 ? min(a.rank[tile.x], RS) : 0, nts = (rank + 15) / 16 * 2;
     if (rank == 0) continue;
-    const bool on_a = g < tile.z, on_b = g + 8 < tile.z;
-    const __nv_bfloat16 *xa = a.x + (size_t)(on_a ? a.order[tile.y + g] : 0) * a.x_stride, *xb = a.x + (size_t)(on_b ? a.order[tile.y + 8 + g] : 0) * a.x_stride;
+    const int row_a = g < tile.z ? a.order[tile.y + g] : a.rows, row_b = g + 8 < tile.z ? a.order[tile.y + 8 + g] : a.rows;
+    const bool on_a = row_a < a.rows, on_b = row_b < a.rows;
+    const __nv_bfloat16 *xa = a.x + (size_t)(on_a ? row_a : 0) * a.x_stride, *xb = a.x + (size_t)(on_b ? row_b : 0) * a.x_stride;
     const uint4* aw = a.a + (size_t)tile.x * k_steps * (RS * 4) + lane;
     auto load16 = [](const __nv_bfloat16* p, bool there) { return there ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0); };
 #pragma unroll(RS > 32 ? 1 : SHARE)
@@ -392,7 +396,10 @@ __global__ void __launch_bounds__(kThreads, Up<RS>::PER_SM) lora_up_kernel(const
     auto group_of = [&](int s, const Place& p) { return s < end ? a.groups[p.at] : make_int4(-1, 0, 0, 0); };  // {adapter, first place, rows, -}
     auto rows_of = [&](const int4& gr, int (&r)[4]) {  // g, g + 8, g + 16, g + 24 of the group; -1: none
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] = g + 8 * i < gr.z ? a.order[gr.y + g + 8 * i] : -1;
+      for (int i = 0; i < 4; ++i) {
+        r[i] = g + 8 * i < gr.z ? a.order[gr.y + g + 8 * i] : -1;
+        if (r[i] >= a.rows) r[i] = -1;
+      }
     };
     auto load_y = [&](const int (&r)[4], int block, uint4 (&y)[4]) {
       const int col = (block * kWarps + warp) * 32 + 8 * t;
@@ -644,7 +651,7 @@ extern "C" b200_status b200_lora_apply(const b200_lora* l, b200_lora_batch* b, c
   a.a = l->a; a.b = l->b; a.x = (const __nv_bfloat16*)d_x; a.y = (const __nv_bfloat16*)d_y; a.out = (__nv_bfloat16*)d_out;
   a.rank = l->rank; a.scale = l->scale; a.order = b->order; a.tiles = b->tiles; a.groups = b->groups; a.hdr = b->hdr;
   a.done = b->done; a.parts = b->parts; a.u = b->u;
-  a.max_rows = b->max_rows; a.max_tiles = b->max_tiles; a.n = l->n; a.k = l->k;
+  a.max_rows = b->max_rows; a.max_tiles = b->max_tiles; a.rows = b->rows; a.n = l->n; a.k = l->k;
   a.x_stride = x_stride; a.y_stride = y_stride; a.out_stride = out_stride;
   cudaStream_t s = (cudaStream_t)stream;
   return l->rs == 16 ? launch<16>(a, tiles, s) : l->rs == 32 ? launch<32>(a, tiles, s) : l->rs == 64 ? launch<64>(a, tiles, s) : launch<128>(a, tiles, s);

@@ -550,7 +550,8 @@ b200_status b200_qmm_static_scratch(const b200_qweight* w, const void* d_x, int3
  * requests share (b200_qmm on the same x), A_a [rank, k] and B_a [n, rank] are bf16, sums are f32, the result is rounded once.
  * A b200_lora holds the adapters of one projection, a b200_lora_batch the rows of a step in the order of their adapters: it is planned once per
  * step (device, asynchronous) and used by every projection of every layer whose handle has as many adapters.  A batch handle is the workspace of
- * its plan: steps that may run at the same time (two captured graphs on two streams) have a batch handle each. */
+ * its plan: steps that may run at the same time (two captured graphs on two streams) have a batch handle each.  Layers that a graph holds without their
+ * plan work on the rows that both they and the plan ahead have. */
 typedef struct b200_lora b200_lora;
 typedef struct b200_lora_batch b200_lora_batch;
 /* Up to 4096 adapters of rank up to 128; n and k multiples of 8 up to 2^24.  All start without matrices (rank 0). */

@@ -201,6 +201,34 @@ def test_graphs_with_batches_of_their_own_on_two_streams():
             _check(side[4], *_want(host, *of))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("captured,few,many", [(40, 7, 60), (1600, 900, 2000)])
+def test_captured_layers_behind_plans_of_other_rows(captured, few, many):
+    """Layers in a graph without their plan work on the rows that both have, and leave what lies behind as it was."""
+    from dmlx_b200 import device as dev
+
+    n, k = 264, 640
+    w, host = _adapters(dev, 2, n, k, 32, [30, 32])
+    row_adapter = (torch.arange(many, dtype=torch.int32) * 7 % 5 - 1).clamp(max=1)
+    x, y = _rows(many, k, 1), _rows(many, n, 2)
+    ids, dx, dy, out = row_adapter.cuda(), x.cuda(), y.cuda(), torch.zeros((many, n), dtype=torch.bfloat16, device="cuda")
+    dx[captured:], dy[captured:] = float("nan"), float("nan")
+    batch, graph = dev.LoraBatch(many, 2, 32), torch.cuda.CUDAGraph()
+    batch.plan(ids[:captured])
+    w.apply(batch, dx[:captured], dy[:captured], out=out[:captured])
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        w.apply(batch, dx[:captured], dy[:captured], out=out[:captured])
+    want, tol = _want(host, row_adapter.tolist(), x, y)
+    for planned in (many, few, captured):
+        batch.plan(ids[:planned])
+        out.fill_(7)
+        graph.replay()
+        both = min(planned, captured)
+        _check(out[:both], want[:both], tol[:both])
+        assert bool((out[both:] == 7).all())
+
+
 def test_what_is_refused():
     from dmlx_b200 import _lib
 
