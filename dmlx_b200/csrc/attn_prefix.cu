@@ -135,7 +135,8 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(KvDev d, PlanDev p, c
   for (int i = tid; i < rows; i += blockDim.x) {
     const int seq = row_seq[i];
     const bool there = seq >= 0 && seq < d.max_seqs;
-    const int ctx = there ? min(max(row_ctx[i], 0), d.max_pages_per_seq * d.page_size) : 0;
+    // (behind its pages a slot's table names what it had before: rows that ask for it would agree there with rows that they share nothing with before)
+    const int ctx = there ? min(max(row_ctx[i], 0), d.seq_pages[seq] * d.page_size) : 0;
     p.row_seq[i] = there ? seq : 0;
     p.row_ctx[i] = ctx;
     full[i] = ctx / d.page_size;

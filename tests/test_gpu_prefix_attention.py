@@ -614,6 +614,24 @@ def test_captured_layers_behind_plans_of_other_rows(fp8):
         assert bool((out[both:] == 7).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [2, 16])
+def test_a_context_beyond_a_slot_s_pages_is_that_row_s_matter_alone(group):
+    """A slot whose table still names pages that it has given up, and a row (of padding, say) that asks for them, ahead of rows that share what the slot still has."""
+    from dmlx_b200 import device as dev
+
+    cache = dev.PagedKVCache(1, 2, 128, 64, 8, 12, 2 * group, max_rows=512)
+    _append(cache, {0: 320}, 1)
+    for s in (1, 2, 3):
+        cache.fork(0, s, 320)
+    cache.rollback(1, 64)
+    _append(cache, {1: 96}, 2)
+    cache.rollback(3, 0)
+    row_seq, row_ctx, held = [1, 0, 2, 3, 0], [320, 320, 320, 320, 319], [160, 320, 320, 0, 319]
+    q = _random(5, 2 * group, 128, seed=3, scale=2.0)
+    _check(_run(cache, q, row_seq, row_ctx), *_want(cache, 0, q, row_seq, held))
+
+
 def test_what_is_refused():
     from dmlx_b200 import _lib
 
