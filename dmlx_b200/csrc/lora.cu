@@ -396,15 +396,13 @@ __global__ void __launch_bounds__(kThreads, Up<RS>::PER_SM) lora_up_kernel(const
     auto group_of = [&](int s, const Place& p) { return s < end ? a.groups[p.at] : make_int4(-1, 0, 0, 0); };  // {adapter, first place, rows, -}
     auto rows_of = [&](const int4& gr, int (&r)[4]) {  // g, g + 8, g + 16, g + 24 of the group; -1: none
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        r[i] = g + 8 * i < gr.z ? a.order[gr.y + g + 8 * i] : -1;
-        if (r[i] >= a.rows) r[i] = -1;
-      }
+      for (int i = 0; i < 4; ++i) r[i] = g + 8 * i < gr.z ? a.order[gr.y + g + 8 * i] : -1;
     };
+    auto there = [&](int r) { return (unsigned)r < (unsigned)a.rows; };  // (asked where a row is used: its number is under way until then)
     auto load_y = [&](const int (&r)[4], int block, uint4 (&y)[4]) {
       const int col = (block * kWarps + warp) * 32 + 8 * t;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = r[i] >= 0 && col < a.n ? *reinterpret_cast<const uint4*>(a.y + (size_t)r[i] * a.y_stride + col) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < 4; ++i) y[i] = there(r[i]) && col < a.n ? *reinterpret_cast<const uint4*>(a.y + (size_t)r[i] * a.y_stride + col) : make_uint4(0, 0, 0, 0);
     };
     Place p0{begin / groups, 0}, p1, p2;
     p0.at = begin - p0.block * groups;
@@ -460,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, Up<RS>::PER_SM) lora_up_kernel(const
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          if (r0[2 * m + h] < 0 || col >= a.n) continue;
+          if (!there(r0[2 * m + h]) || col >= a.n) continue;
           uint4 o = y0[2 * m + h];
           if (ks > 0) {
             uint32_t* w = reinterpret_cast<uint32_t*>(&o);
