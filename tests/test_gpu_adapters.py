@@ -229,6 +229,90 @@ def test_captured_layers_behind_plans_of_other_rows(captured, few, many):
         assert bool((out[both:] == 7).all())
 
 
+class _Device:
+    """`count` 32-bit words of device memory from `address` on."""
+
+    def __init__(self, address, count):
+        self.__cuda_array_interface__ = dict(shape=(count,), typestr="<i4", data=(address, False), version=3)
+
+
+def _tiles_of(batch):
+    """Rows of the tiles that the batch's last plan made, those of many rows and those of few, read behind the handle's pointers: five numbers, order, tiles, header."""
+    words, numbers = (C.c_uint64 * 6).from_address(batch._h), (C.c_int32 * 4).from_address(batch._h)
+    torch.cuda.synchronize()
+    many, _, few = torch.as_tensor(_Device(words[5], 3), device="cuda").tolist()
+    tiles = torch.as_tensor(_Device(words[4], 4 * numbers[3]), device="cuda").view(-1, 4).tolist()
+    return [t[2] for t in tiles[:many]], [t[2] for t in tiles[numbers[3] - few:]]
+
+
+def _want_of_many(host, row_adapter, x, y):
+    """_want, an adapter's rows at once."""
+    want, tol = y.double().clone(), torch.zeros(y.shape, dtype=torch.float64)
+    for slot, (a, b, s) in host.items():
+        at = (row_adapter == slot).nonzero()[:, 0]
+        xr = x[at].double()
+        u, big = xr @ a.T, xr.abs() @ a.T.abs()
+        delta = s * (u @ b.T)
+        tol[at] = abs(s) * (((x.shape[1] / 16 + 80) * 2.0 ** -22 * big + (2.0 ** -17 + (a.shape[0] / 8 + 16) * 2.0 ** -22) * u.abs()) @ b.T.abs())
+        tol[at] += 2.0 ** -22 * (y[at].double().abs() + delta.abs())
+        want[at] += delta
+    return want, tol + 2.0 ** -8 * want.abs()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,ranks,max_rank,n,k,tile", [
+    (3000, [16, 9], 16, 1032, 4104, 64),
+    (3000, [32, 20], 32, 72, 4104, 64),
+    (3000, [64, 40], 64, 72, 2120, 64),
+    (2000, [128, 80], 128, 72, 2120, 64),
+    (9700, [16, 16, 5], 16, 72, 2120, 128),
+    (9700, [30, 17], 32, 40, 4104, 128),
+    (9900, [64, 33, 48], 64, 264, 4104, 128),
+    (5300, [128, 65, 100], 128, 136, 4104, 128),
+])
+def test_tiles_of_many_rows(rows, ranks, max_rank, n, k, tile):
+    """Tiles of 64 and 128 rows, the last one of an adapter ragged, K of several steps a 64th that ends inside one; of 128 rows more shares of tiles than blocks run at
+    once, so that a block's loads go on into its next one."""
+    from dmlx_b200 import device as dev
+
+    w, host = _adapters(dev, len(ranks), n, k, max_rank, ranks)
+    row_adapter = torch.randint(0, len(ranks), (rows,), generator=torch.Generator().manual_seed(rows)).to(torch.int32)
+    row_adapter[5:rows:97] = -1
+    x, y = _rows(rows, k, 1), _rows(rows, n, 2)
+    batch = dev.LoraBatch(rows, len(ranks), max_rank)
+    batch.plan(row_adapter.cuda())
+    many, _ = _tiles_of(batch)
+    assert max(many) == tile and any(t % 16 for t in many)
+    if tile == 128:
+        assert 4 * len(many) > torch.cuda.get_device_properties(0).multi_processor_count * (1 if max_rank > 64 else 2)
+    got = w.apply(batch, x.cuda(), y.cuda())
+    _check(got, *_want_of_many(host, row_adapter, x, y))
+    assert torch.equal(got.cpu()[row_adapter < 0], y[row_adapter < 0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ranks,max_rank", [([64, 16, 40, 8, 33], 64), ([16, 3], 16), ([20, 32], 32), ([128, 65], 128)])
+def test_a_row_s_bits_do_not_depend_on_the_size_of_its_tile(ranks, max_rank):
+    """The same rows in tiles of 128, of 64, and of up to 16 rows, whose operands come another way."""
+    from dmlx_b200 import device as dev
+
+    n, k, rows = 136, 4104, 6000
+    w, _ = _adapters(dev, len(ranks), n, k, max_rank, ranks)
+    g = torch.Generator().manual_seed(5)
+    row_adapter = torch.randint(0, len(ranks), (rows,), generator=g).to(torch.int32).cuda()
+    x, y = _rows(rows, k, 6).cuda(), _rows(rows, n, 7).cuda()
+    batch = dev.LoraBatch(rows, len(ranks), max_rank)
+    batch.plan(row_adapter)
+    assert max(_tiles_of(batch)[0]) == 128
+    whole = w.apply(batch, x, y)
+    for count, largest in ((2000 if max_rank > 64 else 3000, 64), (300, 16), (17, 16), (1, 1)):
+        some = torch.randperm(rows, generator=g)[:count].cuda()
+        batch.plan(row_adapter[some].contiguous())
+        many, few = _tiles_of(batch)
+        assert max(many + few) <= largest and (largest <= 16) == (not many)
+        assert torch.equal(w.apply(batch, x[some], y[some]), whole[some]), count
+
+
 def test_what_is_refused():
     from dmlx_b200 import _lib
 
