@@ -632,6 +632,33 @@ def test_a_context_beyond_a_slot_s_pages_is_that_row_s_matter_alone(group):
     _check(_run(cache, q, row_seq, row_ctx), *_want(cache, 0, q, row_seq, held))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("each", [1, 6])
+def test_trees_deeper_than_the_plan_goes(each, fp8):
+    """Texts that go on from one another seven times, `each` rows behind every one; some go on by a page, which is too little for a node of its own."""
+    from dmlx_b200 import device as dev
+
+    lengths = [70, 130, 33, 96, 200, 32, 64]
+    cache = dev.PagedKVCache(1, 2, 128, 400, 8 + 7 * each, 32, 8, max_rows=1024, kv_dtype=dev.KV_FP8_E4M3 if fp8 else dev.KV_BF16)
+    slots, texts = [], 0
+    for level, n in enumerate(lengths):
+        if level:
+            cache.fork(level - 1, level, texts)
+        _append(cache, {level: n}, level)
+        texts += n
+        for i in range(each):
+            slots.append(8 + len(slots))
+            cache.fork(level, slots[-1], texts)
+            if i % 3 != 2:
+                _append(cache, {slots[-1]: 1 + 40 * i}, 100 + len(slots))
+    order = torch.randperm(len(slots), generator=torch.Generator().manual_seed(1)).tolist()
+    slots = [slots[i] for i in order] + [6, 0]
+    ctx = [cache.seq_len(s) for s in slots]
+    q = _random(len(slots), 8, 128, seed=4, scale=2.0)
+    _check(_run(cache, q, slots, ctx), *_want(cache, 0, q, slots, ctx))
+
+
 def test_what_is_refused():
     from dmlx_b200 import _lib
 
