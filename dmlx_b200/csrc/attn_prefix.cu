@@ -1261,12 +1261,13 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const __grid_constant_
   const int u = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (blockIdx.x == 0 && threadIdx.x == 0) { a.p.hdr[H_NEXT_A] = 0; a.p.hdr[H_NEXT_B] = 0; }  // for the next layer
   const int row = u / a.n_q_heads, qh = u - row * a.n_q_heads;
-  if (!a.nodes && a.p.hdr[H_ITEMS_A] > 0) {  // a plan of more rows than the launches are for
+  // (all on their way together; there is room for the places of a.rows rows whatever the plan)
+  const int planned = a.p.hdr[H_ROWS], large = a.p.hdr[H_ITEMS_A], error = a.d.state[ST_ATTN_ERR], s0 = a.p.row_base[min(row, a.rows)], s1 = a.p.row_base[min(row + 1, a.rows)];
+  if (!a.nodes && large > 0) {  // a plan of more rows than the launches are for
     if (blockIdx.x == 0 && threadIdx.x == 0) atomicExch(a.d.state + ST_ATTN_ERR, B200_ERR_INVALID_ARGUMENT);
     return;
   }
-  if (row >= min(a.rows, a.p.hdr[H_ROWS]) || a.d.state[ST_ATTN_ERR] != 0) return;
-  const int s0 = a.p.row_base[row], s1 = a.p.row_base[row + 1];
+  if (row >= min(a.rows, planned) || error != 0) return;
   constexpr int V = D / 32;
   const float2* ml = reinterpret_cast<const float2*>(a.p.part_ml) + qh;
   const float* po = a.p.part_o + (size_t)qh * D + lane * V;
