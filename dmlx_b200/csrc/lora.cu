@@ -7,9 +7,9 @@
 // later items under way while the present one is multiplied (cp.async; the rows of a tile may lie anywhere), or straight into registers where a tile
 // has few rows; the second kernel's go straight into registers.  Its blocks are on their SMs, with y and B on the way, when the first one ends.
 //
-// Measured, everything in HBM: 256 rows of 64 adapters of rank 16 at 4096 -> 6144, 12.9 us (and 3.1 for the plan); 1583 rows of 33 adapters of rank up to 64
-// at 4096 -> 28672, 93 us, 2.8 TB/s of what it cannot do without; 8192 rows of 5 of rank 32 at 14336 -> 4096, 94 us, 4.0 TB/s: 60 us of them are the
-// first product's, which reads x at 3.9 TB/s.
+// Measured: 256 rows of 64 adapters of rank 16 at 4096 -> 6144, 16.5 us from HBM and 12.7 from L2 (and 3.3 for the plan); 1583 rows of 33 adapters of rank up
+// to 64 at 4096 -> 28672, 92 to 95 us, 2.7 TB/s of what it cannot do without; 8192 rows of 5 of rank 32 at 14336 -> 4096, 93 to 95 us, 4.0 TB/s: 60 us of them
+// are the first product's, which reads x at 3.9 TB/s.
 //
 // The products run on mma.sync m16n8k16.  A lane takes 16 neighbouring bytes of a row of x as its places of K in two MMAs, four neighbouring ranks
 // as its places in one of the second product, and eight neighbouring columns of y as its places of N.  A, B and u lie in memory as the lanes take
@@ -398,11 +398,13 @@ __global__ void __launch_bounds__(kThreads, Up<RS>::PER_SM) lora_up_kernel(const
 #pragma unroll
       for (int i = 0; i < 4; ++i) r[i] = g + 8 * i < gr.z ? a.order[gr.y + g + 8 * i] : -1;
     };
-    auto there = [&](int r) { return (unsigned)r < (unsigned)a.rows; };  // (asked where a row is used: its number is under way until then)
+    // (Whether the call has a row is asked where it is used, its number being under way until then.  Another load in place of one that is left out: with the
+    // condition widened, 1583 rows of rank 128 to 28672 columns took 217 us for 207.)
+    auto there = [&](int r) { return (unsigned)r < (unsigned)a.rows; };
     auto load_y = [&](const int (&r)[4], int block, uint4 (&y)[4]) {
       const int col = (block * kWarps + warp) * 32 + 8 * t;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = there(r[i]) && col < a.n ? *reinterpret_cast<const uint4*>(a.y + (size_t)r[i] * a.y_stride + col) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < 4; ++i) y[i] = r[i] >= 0 && col < a.n ? *reinterpret_cast<const uint4*>(a.y + (size_t)min(r[i], a.rows - 1) * a.y_stride + col) : make_uint4(0, 0, 0, 0);
     };
     Place p0{begin / groups, 0}, p1, p2;
     p0.at = begin - p0.block * groups;
@@ -428,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, Up<RS>::PER_SM) lora_up_kernel(const
     for (int s = begin; s < end; ++s) {
       const int col = (p0.block * kWarps + warp) * 32 + 8 * t, slot = p0.at * (kGroupRows / 16);
       const bool other = s + 1 < end && (g1.x != g0.x || p1.block != p0.block);  // another part of B is next
-      if (other && g1.x >= 0 && p1.block * kWarps + warp < n_blocks && lane < RS / 2)  // on its way to L2
+      if (other && g1.x >= 0 && p1.block * kWarps + warp < n_blocks && lane < RS / 2)  // on its way to L2, as it is laid out: all RS ranks, of 128 the first 64
         asm volatile("prefetch.global.L2 [%0];" ::"l"(a.b + ((size_t)g1.x * n_blocks + p1.block * kWarps + warp) * Z::KS * 64 + lane * 8));
       uint4 y1[4];
       load_y(r1, p1.block, y1);
