@@ -19,7 +19,7 @@
 // next scores wait for its last product (P lies where they go) and the two tiles overlap only in part; an item has 22000 more around its blocks, for q,
 // the first pages and 128 KB of parts.  The warps' kernel is bound by the stream of pages.  Measured per layer, 32 query heads on 8, 128 dims, pages in
 // HBM: 256 rows behind 8192 shared tokens with up to 512 of their own 88 us (one after the other 110: 52 the nodes' on all SMs, 51 the warps', 10 the
-// join), 64 rows behind 2048 28 us, 128 rows behind 4096 on FP8 pages 39.5 us; plans 11 to 15 us.
+// join), 64 rows behind 2048 28 us, 128 rows behind 4096 on FP8 pages 39.5 us; plans 11 to 16 us.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 

@@ -349,11 +349,13 @@ b200_status b200_paged_attn_prefill(b200_kv* kv, int32_t layer, const void* d_q,
 /* Attention of a batch whose sequences share pages (b200_kv_fork, prefix sharing): the contract of b200_paged_attn_decode, with every page that
  * several rows see read and multiplied once for all of them (no reference counterpart).  The plan, once per step, finds on the device what the rows'
  * page tables have in common and copies the row arrays; the layers of the step then take q, [q heads][head_dim] rows of bf16 with strides in
- * elements (multiples of 8, rows on 16 bytes), and out likewise.  A row of context 0, or of a slot that is none, gets zeros, and no row sees more than the
- * pages that its slot holds when the plan runs.  Rows of any order, which no result depends on; a slot may have several.  A plan is valid until pages are reserved, released or forked.  A handle belongs to one pool, which outlives it, and is the
- * workspace of its plan: steps that may run at the same time have a handle each.  Layers that a graph holds without their plan work on the rows that both it and the
- * plan ahead have; where theirs are so few (16 query rows per kv head) that no launch is there for what a larger plan found, nothing is written and the pool's error word
- * is set (INVALID_ARGUMENT).  Up to 4096 rows, 16 query heads per kv head; bf16 pools, and FP8 pools of head_dim 128. */
+ * elements (multiples of 8, rows on 16 bytes), and out likewise.  A row of context 0, or of a slot that is none, gets zeros, and no row sees more than
+ * the pages that its slot holds when the plan runs.  Rows of any order, which no result depends on; a slot may have several.  What rows share is used
+ * up to three branchings of their tree, and pages behind those count as a row's own.  A plan is valid until pages are reserved, released or forked.
+ * A handle belongs to one pool, which outlives it, and is the workspace of its plan: steps that may run at the same time have a handle each.  Layers
+ * that a graph holds without their plan work on the rows that both they and the plan ahead have; where theirs are so few (16 query rows per kv head)
+ * that no launch is there for what a larger plan found, nothing is written and the pool's error word is set (INVALID_ARGUMENT).  Up to 4096 rows, 16
+ * query heads per kv head; bf16 pools, and FP8 pools of head_dim 128. */
 typedef struct b200_prefix_attn b200_prefix_attn;
 b200_status b200_prefix_attn_create(b200_kv* kv, int32_t max_rows, b200_prefix_attn** out);
 void b200_prefix_attn_destroy(b200_prefix_attn* h);
