@@ -620,7 +620,10 @@ extern "C" b200_status b200_lora_plan(b200_lora_batch* b, const int32_t* d_row_a
   b200_status st = b200_require_device();
   if (st != B200_OK) return st;
   b->rows = rows;
-  if (rows == 0) return B200_OK;
+  if (rows == 0) {  // (for layers in a graph: none of their rows are there)
+    B200_CUDA_TRY(cudaMemsetAsync(b->hdr, 0, sizeof(int) * 4, (cudaStream_t)stream));
+    return B200_OK;
+  }
   // A tile is kSlices items of the first product: beyond one for each of its blocks, larger tiles rather than more of them (2097 rows of two adapters of
   // rank 128, one block per SM, at 14336 -> 4096: 99 us; with room for two blocks per SM, so smaller tiles, 166).
   const int enough = b200_sm_count() * (b->max_rank > 64 ? Down<128>::PER_SM : Down<64>::PER_SM) / kSlices;
