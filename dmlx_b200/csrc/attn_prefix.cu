@@ -1399,7 +1399,10 @@ extern "C" b200_status b200_prefix_attn_plan(b200_prefix_attn* h, const int32_t*
   b200_status st = b200_require_device();
   if (st != B200_OK) return st;
   h->rows = rows;
-  if (rows == 0) return B200_OK;
+  if (rows == 0) {  // (for layers in a graph: none of their rows are there)
+    B200_CUDA_TRY(cudaMemsetAsync(h->p.hdr, 0, sizeof(int) * H_COUNT, (cudaStream_t)stream));
+    return B200_OK;
+  }
   int hash = 64;
   while (hash < rows || (hash < 2 * rows && hash < 4096)) hash *= 2;
   const size_t shared = (size_t)hash * (8 + 4 * 4) + (size_t)rows * 4 * 6;
