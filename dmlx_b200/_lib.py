@@ -19,7 +19,7 @@ if not os.path.exists(LIB_PATH):
 
 lib = C.CDLL(LIB_PATH)
 
-u64, u32, i32, f32, f64 = C.c_uint64, C.c_uint32, C.c_int32, C.c_float, C.c_double
+u64, i64, u32, i32, f32, f64 = C.c_uint64, C.c_int64, C.c_uint32, C.c_int32, C.c_float, C.c_double
 vp = C.c_void_p
 P = C.POINTER
 
@@ -310,6 +310,22 @@ _sig("b200_lora_batch_create", i32, i32, i32, i32, P(vp))
 _sig("b200_lora_batch_destroy", None, vp)
 _sig("b200_lora_plan", i32, vp, vp, i32, vp)
 _sig("b200_lora_apply", i32, vp, vp, vp, i32, vp, i32, vp, i32, vp)
+
+
+class ResidualNormShape(C.Structure):
+    _fields_ = [(n, i32) for n in ("n", "h_f32", "y_f32", "gate_sigmoid")] + [("scale", f32), ("eps", f32)]
+
+
+_sig("b200_i8_weight_create", i32, i32, i32, vp, vp, P(vp))
+_sig("b200_i8_weight_create_gated", i32, i32, i32, vp, vp, vp, vp, P(vp))
+_sig("b200_i8_weight_destroy", None, vp)
+_sig("b200_i8_rows_create", i32, i32, i32, i32, P(vp))
+_sig("b200_i8_rows_destroy", None, vp)
+_sig("b200_i8_quantize", i32, vp, vp, i64, i32, i32, vp)
+_sig("b200_i8_rows_get", i32, vp, vp, vp, vp)
+_sig("b200_i8_mm", i32, vp, vp, vp, i64, i32, vp, vp, i64, i32, vp)
+_sig("b200_i8_ffn", i32, vp, vp, vp, vp, i64, i32, i32, vp, i64, vp)
+_sig("b200_residual_norm", i32, P(ResidualNormShape), vp, i64, vp, i64, vp, i64, vp, vp, i32, vp, i64, vp, i64, vp, vp)
 _sig("b200_kv_create_layers", i32, P(KvConfig), P(KvLayer), P(vp))
 _sig("b200_argmax_f32", i32, vp, i32, i32, vp, vp)
 _sig("b200_qmm_f32", i32, vp, vp, i32, vp, i32, i32, i32, vp)

@@ -1,0 +1,514 @@
+// Products of rows and weights in 8-bit integers, and the gated feed-forward block made of them:
+//   y[t][n] = (sum_k q[t][k] w[n][k]) scale[n] step[t] + bias[n],   q[t][k] = round(127 x[t][k] / max_k |x[t][k]|),  step[t] = max_k |x[t][k]| / 127.
+//
+// The sums are exact (int32 on tcgen05.mma kind::i8), so neither the order of K nor what shares a tile changes a bit of a row.
+#include <cuda_bf16.h>
+#include <math.h>
+
+#include <algorithm>
+#include <new>
+
+#include "common.h"
+#include "i8.cuh"
+#include "launch.cuh"
+#include "ptx.cuh"
+#include "qmm.cuh"
+#include "rows.cuh"
+
+namespace {
+
+// ---- rows into 8 bits ----------------------------------------------------------------------------------------------------
+// A block per row, or a warp for rows of up to 32 * 8 * NV columns; the row waits in registers while its largest is looked for.  Bound by
+// what it reads and writes.
+template <typename T>
+struct QuantizeArgs {
+  const T* x;
+  long long x_stride;
+  signed char* q;
+  float* scale;
+  int rows, k, chunks, aligned;
+};
+
+// NV: vectors of eight columns of a thread; 0: any number, the row is read twice.  WARP: a warp for a row.
+template <typename T, int NV, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : 1024) i8_quantize_kernel(QuantizeArgs<T> a) {
+  after_previous();
+  __shared__ uint32_t part[32];
+  const int threads = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
+  const int row = WARP ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+  if (row >= a.rows) return;
+  const T* x = a.x + (size_t)row * a.x_stride;
+  const int vectors = a.chunks * (kI8Chunk / 8);
+  Eight<T> keep[NV > 0 ? NV : 1];
+  uint32_t most = 0u;
+  if constexpr (NV > 0) {
+#pragma unroll
+    for (int u = 0; u < NV; ++u) keep[u] = load_eight(x, (t + u * threads) * 8, a.k, a.aligned);
+#pragma unroll
+    for (int u = 0; u < NV; ++u) most = most_of(most, keep[u]);
+  } else {
+    for (int v = t; v < vectors; v += threads) {
+      keep[0] = load_eight(x, v * 8, a.k, a.aligned);
+      most = most_of(most, keep[0]);
+    }
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  if constexpr (!WARP) {
+    if ((t & 31) == 0) part[t >> 5] = most;
+    __syncthreads();
+    most = __reduce_max_sync(0xffffffffu, (t & 31) < (threads >> 5) ? part[t & 31] : 0u);
+  }
+  const I8Scale s = I8Scale::of(__uint_as_float(most));
+  if (t == 0) a.scale[row] = s.step();
+  auto put = [&](int v, const Eight<T>& raw) {
+    float f[8];
+    widen(raw, f);
+    i8_store8(a.q, row, v * 8, a.chunks, s, f);
+  };
+  if constexpr (NV > 0) {
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+      if (t + u * threads < vectors) put(t + u * threads, keep[u]);
+  } else {
+    for (int v = t; v < vectors; v += threads) {
+      keep[0] = load_eight(x, v * 8, a.k, a.aligned);
+      put(v, keep[0]);
+    }
+  }
+}
+
+template <typename T>
+b200_status quantize(const T* x, long long x_stride, int rows, int k, const I8RowsDev& to, cudaStream_t s) {
+  QuantizeArgs<T> a;
+  a.x = x; a.x_stride = x_stride; a.q = to.q; a.scale = to.scale; a.rows = rows; a.k = k; a.chunks = i8_chunks(k);
+  a.aligned = ((uintptr_t)x & 15) == 0 && x_stride * sizeof(T) % 16 == 0;
+  const int vectors = a.chunks * (kI8Chunk / 8);
+  if (vectors <= 32 * 4) {
+    const int warps = rows >= 8 * b200_sm_count() ? 8 : 1;
+    const unsigned grid = (unsigned)((rows + warps - 1) / warps);
+    if (vectors <= 32 * 1) launch_after(i8_quantize_kernel<T, 1, true>, grid, warps * 32, 0, s, a);
+    else if (vectors <= 32 * 2) launch_after(i8_quantize_kernel<T, 2, true>, grid, warps * 32, 0, s, a);
+    else launch_after(i8_quantize_kernel<T, 4, true>, grid, warps * 32, 0, s, a);
+  } else if (vectors <= 4 * 1024) {
+    // few rows: more threads, each with fewer loads to wait for
+    const int nv = vectors <= 1024 && rows <= 2 * b200_sm_count() ? 1 : vectors <= 2048 && rows <= 2 * b200_sm_count() ? 2 : 4;
+    const int threads = (vectors + 32 * nv - 1) / (32 * nv) * 32;
+    if (nv == 1) launch_after(i8_quantize_kernel<T, 1, false>, rows, threads, 0, s, a);
+    else if (nv == 2) launch_after(i8_quantize_kernel<T, 2, false>, rows, threads, 0, s, a);
+    else launch_after(i8_quantize_kernel<T, 4, false>, rows, threads, 0, s, a);
+  } else {
+    launch_after(i8_quantize_kernel<T, 0, false>, rows, 1024, 0, s, a);
+  }
+  B200_LAUNCH_CHECK();
+  return B200_OK;
+}
+
+// ---- what the handles hold, into and out of its order -----------------------------------------------------------------------
+// A thread for sixteen columns of a row of the laid-out weight.
+__global__ void i8_lay_out_kernel(const signed char* src, const float* scales, int n, int k, int chunks, int tile0, int tile_step, int tiles, signed char* __restrict__ q,
+                                  float* __restrict__ scale) {
+  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  const int per_row = chunks * 8;
+  const long long row = i / per_row;
+  const int piece = (int)(i - row * per_row);
+  if (row >= (long long)tiles * kI8Tile) return;
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+  if (row < n)
+    for (int e = 0; e < 16; ++e)
+      if (piece * 16 + e < k) w[e / 4] |= (uint32_t)(unsigned char)src[(size_t)row * k + piece * 16 + e] << (8 * (e % 4));
+  const int to = (int)(tile0 + row / kI8Tile * tile_step), r = (int)(row % kI8Tile);
+  *reinterpret_cast<uint4*>(q + ((size_t)to * chunks + piece / 8) * kI8Block + r * kI8Chunk + (((piece % 8) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+  if (piece == 0) scale[(size_t)to * kI8Tile + r] = row < n ? scales[row] : 0.f;
+}
+
+__global__ void i8_rows_get_kernel(I8RowsDev from, int rows, int k, int chunks, signed char* __restrict__ q, float* __restrict__ steps) {
+  after_previous();
+  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= (long long)rows * k) return;
+  const int row = (int)(i / k), c = (int)(i - (long long)row * k);
+  if (q) q[i] = from.q[i8_at(row, c, chunks)];
+  if (steps && c == 0) steps[row] = from.scale[row];
+}
+
+// ---- products ----------------------------------------------------------------------------------------------------------------
+struct MmArgs {
+  const signed char* w;
+  const float* w_scale;
+  const signed char* q;
+  const float* step;
+  const float* bias;
+  void* y;
+  long long y_stride;
+  int* err;
+  int rows, n, chunks, tiles, tn, stages;
+  int y_f32, act;  // (a feed-forward block's inner rows are f32)
+};
+
+// D[tmem] (+)= A B of signed 8-bit integers, 32-bit sums.
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Instruction descriptor: signed 8-bit A and B (both K-major), 32-bit sums, tile m x n.
+__device__ __forceinline__ uint32_t idesc_i8(uint32_t m, uint32_t n) { return 2u << 4 | 1u << 7 | 1u << 10 | (n >> 3) << 17 | (m >> 4) << 24; }
+
+__device__ __forceinline__ float activated(int act, float g) {
+  if (act == B200_ACT_SILU) return g / (1.0f + __expf(-g));
+  if (act == B200_ACT_GELU) return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
+  // 0.5 g (1 + tanh z) = g / (1 + e^-2z)
+  return g / (1.0f + __expf(-1.5957691216057308f * (g + 0.044715f * g * g * g)));
+}
+
+// A weight tile (gated: the gate's and up's tile of the same channels) by up to tn rows per CTA.  The weights are the MMA's M, the rows its N, so that few
+// rows waste nothing; a lane of tensor memory is a channel.  Warp 0 loads, warp 1 multiplies, four bring the sums to the output.
+constexpr int kStreamThreads = 192;
+
+template <bool GATED>
+__global__ void __launch_bounds__(kStreamThreads) i8_stream_kernel(MmArgs a) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  constexpr int W = GATED ? 2 : 1;
+  const int S = a.stages, stage_bytes = W * kI8Block + a.tn * kI8Chunk;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)S * stage_bytes);
+  uint64_t* done = full + S;
+  uint64_t* sums = done + S;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sums + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tile = blockIdx.x, t0 = blockIdx.y * a.tn, rows_here = min(a.tn, a.rows - t0), n_here = (rows_here + 15) / 16 * 16;
+  uint32_t cols = 32;
+  while (cols < (uint32_t)(W * a.tn)) cols *= 2;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      ptx::mbar_init(&full[s], 1);
+      ptx::mbar_init(&done[s], 1);
+    }
+    ptx::mbar_init(sums, 1);
+    ptx::mbar_fence_init();
+  }
+  __syncthreads();
+  auto load_weights = [&](int i, int s) {
+    ptx::mbar_expect_tx(&full[s], W * kI8Block + n_here * kI8Chunk);
+    for (int h = 0; h < W; ++h)
+      ptx::bulk_g2s(smem + (size_t)s * stage_bytes + h * kI8Block, a.w + ((size_t)(tile * W + h) * a.chunks + i) * kI8Block, kI8Block, &full[s]);
+  };
+  auto load_rows = [&](int i, int s) {  // (a tile of 256 rows is two of the layout's)
+    for (int r = 0; r < n_here; r += kI8Tile) {
+      const int row = t0 + r;
+      ptx::bulk_g2s(smem + (size_t)s * stage_bytes + W * kI8Block + r * kI8Chunk, a.q + ((size_t)(row / kI8Tile) * a.chunks + i) * kI8Block + row % kI8Tile * kI8Chunk,
+                    min(kI8Tile, n_here - r) * kI8Chunk, &full[s]);
+    }
+  };
+  const int ahead = min(S, a.chunks);  // weights asked for before the kernels ahead have ended
+  if (threadIdx.x == 0)
+    for (int i = 0; i < ahead; ++i) load_weights(i, i);
+  wait_previous();
+  if (warp == 1) {
+    ptx::tmem_alloc(tmem_slot, cols);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  ptx::tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  bool ok = true;
+  if (warp == 0) {
+    if (lane == 0) {
+      int s = 0, issued = 0;
+      uint32_t ph = 1;
+      for (int i = 0; i < a.chunks; ++i) {
+        if (i >= ahead) {
+          ok = ptx::mbar_wait(&done[s], ph);
+          if (!ok) break;
+          load_weights(i, s);
+        }
+        load_rows(i, s);
+        ++issued;
+        if (++s == S) { s = 0; ph ^= 1u; }
+      }
+      let_next_start();
+      if (!ok)  // copies are on their way into this memory
+        for (int i = max(0, issued - S); i < issued; ++i) ptx::mbar_wait(&full[i % S], (i / S) & 1);
+    }
+  } else if (warp == 1) {
+    if (ptx::elect_one()) {
+      const uint32_t idesc = idesc_i8(kI8Tile, n_here);
+      int s = 0;
+      uint32_t ph = 0;
+      for (int i = 0; i < a.chunks; ++i) {
+        ok = ptx::mbar_wait(&full[s], ph);
+        if (!ok) break;
+        ptx::tc_fence_after_sync();
+        const uint32_t at = ptx::smem_u32(smem + (size_t)s * stage_bytes);
+        const uint64_t db = ptx::umma_desc_k_sw128(at + W * kI8Block);
+#pragma unroll
+        for (int h = 0; h < W; ++h) {
+          const uint64_t da = ptx::umma_desc_k_sw128(at + h * kI8Block);
+#pragma unroll
+          for (int k4 = 0; k4 < 4; ++k4) umma_i8(tmem + h * a.tn, da + 2 * k4, db + 2 * k4, idesc, (i > 0 || k4 > 0) ? 1u : 0u);
+        }
+        ptx::umma_commit(&done[s]);
+        if (++s == S) { s = 0; ph ^= 1u; }
+      }
+      ptx::umma_commit(sums);
+      if (!ok) ptx::mbar_wait(sums, 0);
+    }
+    __syncwarp();
+  } else {
+    ok = ptx::mbar_wait(sums, 0);
+    ok = __all_sync(0xffffffffu, ok);
+    if (ok) {
+      ptx::tc_fence_after_sync();
+      const int quarter = warp & 3, channel = tile * kI8Tile + quarter * 32 + lane;
+      const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
+      const size_t scale_at = (size_t)tile * W * kI8Tile + quarter * 32 + lane;
+      const float ws = a.w_scale[scale_at], us = GATED ? a.w_scale[scale_at + kI8Tile] : 0.f;
+      const float bias = !GATED && a.bias && channel < a.n ? a.bias[channel] : 0.f;
+      for (int c0 = 0; c0 < rows_here; c0 += 16) {
+        uint32_t v[16], u[16];
+        ptx::tmem_ld16(acc + c0, v);
+        if constexpr (GATED) ptx::tmem_ld16(acc + a.tn + c0, u);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          if (c0 + j >= rows_here || channel >= a.n) continue;
+          const size_t row = t0 + c0 + j, at = row * a.y_stride + channel;
+          const float step = a.step[row];
+          float y = (float)(int)v[j] * ws * step + bias;
+          if constexpr (GATED) y = activated(a.act, y) * ((float)(int)u[j] * us * step);
+          if (GATED || a.y_f32) reinterpret_cast<float*>(a.y)[at] = y;
+          else reinterpret_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16(y);
+        }
+      }
+    }
+  }
+  if (!ok) atomicExch(a.err, B200_ERR_DEVICE_FLAGGED);
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) ptx::tmem_dealloc(tmem, cols);
+}
+
+template <bool GATED>
+b200_status launch_product(MmArgs& a, cudaStream_t s) {
+  static bool configured = false;
+  constexpr int kShared = 112 * 1024, W = GATED ? 2 : 1;  // two CTAs on an SM
+  if (!configured) {
+    B200_CUDA_TRY(cudaFuncSetAttribute(i8_stream_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared));
+    configured = true;
+  }
+  const int most = GATED ? 128 : 256;
+  a.tn = 16;
+  while (a.tn < most && a.tn < a.rows) a.tn *= 2;
+  const int stage = W * kI8Block + a.tn * kI8Chunk;
+  a.stages = std::min(a.chunks, (kShared - 2048) / stage);
+  launch_after(i8_stream_kernel<GATED>, dim3(a.tiles / W, (a.rows + a.tn - 1) / a.tn), kStreamThreads, (size_t)a.stages * stage + 2048, s, a);
+  B200_LAUNCH_CHECK();
+  return B200_OK;
+}
+
+b200_status product(const b200_i8_weight* w, const I8RowsDev& x, int rows, const float* bias, int act, void* y, long long y_stride, int y_f32, cudaStream_t s) {
+  MmArgs a{};
+  b200_status st = b200_qmm_ensure_err_word(&a.err);
+  if (st != B200_OK) return st;
+  a.w = w->q; a.w_scale = w->scale; a.q = x.q; a.step = x.scale; a.bias = bias; a.y = y; a.y_stride = y_stride; a.y_f32 = y_f32; a.act = act;
+  a.rows = rows; a.n = w->n; a.chunks = w->chunks; a.tiles = w->tiles;
+  return w->gated ? launch_product<true>(a, s) : launch_product<false>(a, s);
+}
+
+// ---- handles -------------------------------------------------------------------------------------------------------------------
+b200_status create_weight(int n, int k, bool gated, const int8_t* const* q, const float* const* scales, b200_i8_weight** out) {
+  if (!out) { b200_set_error("i8 weight: no place for the handle"); return B200_ERR_INVALID_ARGUMENT; }
+  *out = nullptr;
+  const int parts = gated ? 2 : 1;
+  for (int p = 0; p < parts; ++p)
+    if (!q[p] || !scales[p]) { b200_set_error("i8 weight: no numbers, or no scales"); return B200_ERR_INVALID_ARGUMENT; }
+  if (n <= 0 || k <= 0 || n > 1 << 24 || k > kI8MaxK) { b200_set_error("i8 weight: %d x %d (at most %d x %d)", n, k, 1 << 24, kI8MaxK); return B200_ERR_INVALID_ARGUMENT; }
+  b200_status st = b200_require_device();
+  if (st != B200_OK) return st;
+  int* err = nullptr;
+  st = b200_qmm_ensure_err_word(&err);  // (not in the first product, which may be captured)
+  if (st != B200_OK) return st;
+  auto* w = new (std::nothrow) b200_i8_weight();
+  if (!w) { b200_set_error("i8 weight: out of host memory"); return B200_ERR_CAPACITY; }
+  const int tiles = (n + kI8Tile - 1) / kI8Tile;
+  w->n = n; w->k = k; w->gated = gated; w->tiles = tiles * parts; w->chunks = i8_chunks(k);
+  cudaError_t e = cudaDeviceSynchronize();  // (the numbers may be another stream's work)
+  if (e == cudaSuccess) e = cudaMalloc((void**)&w->q, (size_t)w->tiles * w->chunks * kI8Block);
+  if (e == cudaSuccess) e = cudaMalloc((void**)&w->scale, sizeof(float) * (size_t)w->tiles * kI8Tile);
+  int device = 0;
+  if (e == cudaSuccess) e = cudaGetDevice(&device);
+  void *q_copy = nullptr, *scale_copy = nullptr;
+  for (int p = 0; p < parts && e == cudaSuccess; ++p) {
+    auto here = [&](const void* from, size_t bytes, void*& copy) -> const void* {  // in this device's memory
+      cudaPointerAttributes at{};
+      if (cudaPointerGetAttributes(&at, from) == cudaSuccess && at.type == cudaMemoryTypeDevice && at.device == device) return from;
+      cudaGetLastError();
+      if (!copy) e = cudaMalloc(&copy, bytes);
+      if (e == cudaSuccess) e = cudaMemcpy(copy, from, bytes, cudaMemcpyDefault);
+      return copy;
+    };
+    const void* q_here = here(q[p], (size_t)n * k, q_copy);
+    const void* scale_here = e == cudaSuccess ? here(scales[p], sizeof(float) * (size_t)n, scale_copy) : nullptr;
+    if (e != cudaSuccess) break;
+    const long long pieces = (long long)tiles * kI8Tile * w->chunks * 8;
+    i8_lay_out_kernel<<<(unsigned)((pieces + 255) / 256), 256>>>((const signed char*)q_here, (const float*)scale_here, n, k, w->chunks, p, parts, tiles, w->q, w->scale);
+    ++g_b200_launch_counter;
+    e = cudaGetLastError();
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+  }
+  if (q_copy) cudaFree(q_copy);
+  if (scale_copy) cudaFree(scale_copy);
+  if (e != cudaSuccess) {
+    b200_set_error("i8 weight: %d x %d: %s", n, k, cudaGetErrorString(e));
+    cudaGetLastError();
+    b200_i8_weight_destroy(w);
+    return B200_ERR_CUDA;
+  }
+  *out = w;
+  return B200_OK;
+}
+
+// The checks of x and the rows that a product reads.
+b200_status take_rows(const char* who, b200_i8_rows* r, const void* d_x, int64_t x_stride, int32_t rows, int32_t k, cudaStream_t s) {
+  if (rows < 0 || rows > r->max_rows) { b200_set_error("%s: %d rows, the handle is for %d", who, rows, r->max_rows); return rows < 0 ? B200_ERR_INVALID_ARGUMENT : B200_ERR_CAPACITY; }
+  if (k > r->max_k) { b200_set_error("%s: rows of %d columns, the handle is for %d", who, k, r->max_k); return B200_ERR_CAPACITY; }
+  if (rows == 0) {  // (whether x is there or not)
+    r->rows = 0;
+    r->k = k;
+    return B200_OK;
+  }
+  if (!d_x) {
+    if (r->rows != rows || r->k != k) {
+      b200_set_error("%s: %d rows of %d columns, the handle holds %d of %d", who, rows, k, std::max(0, r->rows), r->k);
+      return B200_ERR_INVALID_ARGUMENT;
+    }
+    return B200_OK;
+  }
+  if (rows > 1 && x_stride < k) { b200_set_error("%s: rows of %d columns %lld apart", who, k, (long long)x_stride); return B200_ERR_INVALID_ARGUMENT; }
+  if (((uintptr_t)d_x & 1) != 0) { b200_set_error("%s: x is not on a number's boundary", who); return B200_ERR_INVALID_ARGUMENT; }
+  b200_status st = quantize((const __nv_bfloat16*)d_x, x_stride, rows, k, r->x, s);
+  if (st == B200_OK) { r->rows = rows; r->k = k; }
+  return st;
+}
+
+b200_status check_out(const char* who, const void* d_y, int64_t y_stride, int32_t rows, int32_t n, int size) {
+  if (rows > 0 && (!d_y || ((uintptr_t)d_y & (size - 1)) != 0 || (rows > 1 && y_stride < n))) {
+    b200_set_error("%s: no place for %d rows of %d columns", who, rows, n);
+    return B200_ERR_INVALID_ARGUMENT;
+  }
+  return B200_OK;
+}
+
+}  // namespace
+
+extern "C" b200_status b200_i8_weight_create(int32_t n, int32_t k, const int8_t* q, const float* scales, b200_i8_weight** out) {
+  return create_weight(n, k, false, &q, &scales, out);
+}
+
+extern "C" b200_status b200_i8_weight_create_gated(int32_t n, int32_t k, const int8_t* gate_q, const float* gate_scales, const int8_t* up_q, const float* up_scales,
+                                                   b200_i8_weight** out) {
+  const int8_t* q[2] = {gate_q, up_q};
+  const float* scales[2] = {gate_scales, up_scales};
+  return create_weight(n, k, true, q, scales, out);
+}
+
+extern "C" void b200_i8_weight_destroy(b200_i8_weight* w) {
+  if (!w) return;
+  for (void* p : {(void*)w->q, (void*)w->scale}) if (p) cudaFree(p);
+  delete w;
+}
+
+extern "C" b200_status b200_i8_rows_create(int32_t max_rows, int32_t max_k, int32_t max_hidden, b200_i8_rows** out) {
+  if (!out) { b200_set_error("i8 rows: no place for the handle"); return B200_ERR_INVALID_ARGUMENT; }
+  *out = nullptr;
+  if (max_rows <= 0 || max_rows > 1 << 24 || max_k <= 0 || max_k > kI8MaxK || max_hidden < 0 || max_hidden > kI8MaxK) {
+    b200_set_error("i8 rows: %d rows of %d columns, %d inside a block (at most %d, %d and %d)", max_rows, max_k, max_hidden, 1 << 24, kI8MaxK, kI8MaxK);
+    return B200_ERR_INVALID_ARGUMENT;
+  }
+  b200_status st = b200_require_device();
+  if (st != B200_OK) return st;
+  auto* r = new (std::nothrow) b200_i8_rows();
+  if (!r) { b200_set_error("i8 rows: out of host memory"); return B200_ERR_CAPACITY; }
+  r->max_rows = max_rows; r->max_k = max_k; r->max_hidden = max_hidden; r->h_stride = (max_hidden + 7) / 8 * 8;
+  const size_t tiles = (max_rows + kI8Tile - 1) / kI8Tile;
+  cudaError_t e = cudaSuccess;
+  auto make = [&](I8RowsDev& d, int k) {
+    const size_t bytes = tiles * i8_chunks(k) * kI8Block;
+    if (e == cudaSuccess) e = cudaMalloc((void**)&d.q, bytes);
+    if (e == cudaSuccess) e = cudaMalloc((void**)&d.scale, sizeof(float) * tiles * kI8Tile);
+    if (e == cudaSuccess) e = cudaMemset(d.q, 0, bytes);
+    if (e == cudaSuccess) e = cudaMemset(d.scale, 0, sizeof(float) * tiles * kI8Tile);
+  };
+  make(r->x, max_k);
+  if (max_hidden > 0) {
+    make(r->hidden, max_hidden);
+    if (e == cudaSuccess) e = cudaMalloc((void**)&r->h, sizeof(float) * (size_t)max_rows * r->h_stride);
+  }
+  if (e == cudaSuccess) e = cudaDeviceSynchronize();
+  if (e != cudaSuccess) {
+    b200_set_error("i8 rows: %d rows of %d columns, %d inside a block: %s", max_rows, max_k, max_hidden, cudaGetErrorString(e));
+    cudaGetLastError();
+    b200_i8_rows_destroy(r);
+    return B200_ERR_CUDA;
+  }
+  *out = r;
+  return B200_OK;
+}
+
+extern "C" void b200_i8_rows_destroy(b200_i8_rows* r) {
+  if (!r) return;
+  for (void* p : {(void*)r->x.q, (void*)r->x.scale, (void*)r->hidden.q, (void*)r->hidden.scale, (void*)r->h}) if (p) cudaFree(p);
+  delete r;
+}
+
+extern "C" b200_status b200_i8_quantize(b200_i8_rows* r, const void* d_x, int64_t x_stride, int32_t rows, int32_t k, void* stream) {
+  if (!r || k <= 0 || (rows > 0 && !d_x)) { b200_set_error("i8 quantize: no handle, or no rows"); return B200_ERR_INVALID_ARGUMENT; }
+  b200_status st = b200_require_device();
+  if (st != B200_OK) return st;
+  return take_rows("i8 quantize", r, d_x, x_stride, rows, k, (cudaStream_t)stream);
+}
+
+extern "C" b200_status b200_i8_rows_get(const b200_i8_rows* r, void* d_q, float* d_steps, void* stream) {
+  if (!r || r->rows < 0) { b200_set_error("i8 rows: nothing there"); return B200_ERR_INVALID_ARGUMENT; }
+  b200_status st = b200_require_device();
+  if (st != B200_OK) return st;
+  if (r->rows == 0 || (!d_q && !d_steps)) return B200_OK;
+  const long long numbers = (long long)r->rows * r->k;
+  launch_after(i8_rows_get_kernel, (unsigned)((numbers + 255) / 256), 256, 0, (cudaStream_t)stream, r->x, r->rows, r->k, i8_chunks(r->k), (signed char*)d_q, d_steps);
+  B200_LAUNCH_CHECK();
+  return B200_OK;
+}
+
+extern "C" b200_status b200_i8_mm(const b200_i8_weight* w, b200_i8_rows* r, const void* d_x, int64_t x_stride, int32_t rows, const float* d_bias, void* d_y,
+                                  int64_t y_stride, int32_t y_f32, void* stream) {
+  if (!w || !r) { b200_set_error("i8 mm: no weight, or no rows"); return B200_ERR_INVALID_ARGUMENT; }
+  if (w->gated) { b200_set_error("i8 mm: the weight is a feed-forward block's gate and up"); return B200_ERR_INVALID_ARGUMENT; }
+  b200_status st = check_out("i8 mm", d_y, y_stride, rows, w->n, y_f32 ? 4 : 2);
+  if (st == B200_OK) st = b200_require_device();
+  if (st == B200_OK) st = take_rows("i8 mm", r, d_x, x_stride, rows, w->k, (cudaStream_t)stream);
+  if (st != B200_OK || rows == 0) return st;
+  return product(w, r->x, rows, d_bias, 0, d_y, y_stride, y_f32 != 0, (cudaStream_t)stream);
+}
+
+extern "C" b200_status b200_i8_ffn(const b200_i8_weight* gate_up, const b200_i8_weight* down, b200_i8_rows* r, const void* d_x, int64_t x_stride, int32_t rows,
+                                   int32_t activation, void* d_y, int64_t y_stride, void* stream) {
+  if (!gate_up || !down || !r) { b200_set_error("i8 ffn: no weights, or no rows"); return B200_ERR_INVALID_ARGUMENT; }
+  if (!gate_up->gated || down->gated || down->k != gate_up->n) {
+    b200_set_error("i8 ffn: %s weight of %d channels in front of %s of %d columns", gate_up->gated ? "a gated" : "a plain", gate_up->n, down->gated ? "a gated one" : "one", down->k);
+    return B200_ERR_INVALID_ARGUMENT;
+  }
+  if (activation < B200_ACT_SILU || activation > B200_ACT_GELU_TANH) { b200_set_error("i8 ffn: activation %d", activation); return B200_ERR_INVALID_ARGUMENT; }
+  if (down->k > r->max_hidden) { b200_set_error("i8 ffn: %d channels inside the block, the handle is for %d", down->k, r->max_hidden); return B200_ERR_CAPACITY; }
+  b200_status st = check_out("i8 ffn", d_y, y_stride, rows, down->n, 2);
+  if (st == B200_OK) st = b200_require_device();
+  if (st == B200_OK) st = take_rows("i8 ffn", r, d_x, x_stride, rows, gate_up->k, (cudaStream_t)stream);
+  if (st != B200_OK || rows == 0) return st;
+  cudaStream_t s = (cudaStream_t)stream;
+  st = product(gate_up, r->x, rows, nullptr, activation, r->h, r->h_stride, 0, s);
+  if (st == B200_OK) st = quantize(r->h, r->h_stride, rows, down->k, r->hidden, s);
+  if (st == B200_OK) st = product(down, r->hidden, rows, nullptr, 0, d_y, y_stride, 0, s);
+  return st;
+}

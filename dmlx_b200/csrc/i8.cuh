@@ -1,0 +1,131 @@
+// Rows and weights in 8-bit integers: how they lie in memory, and how a row becomes one (i8.cu multiplies them, residual_norm.cu makes rows too).
+//
+// Both are [tile of 128 rows][block of 128 columns][row][128 bytes], a block 16 KiB in one piece: what a stage of the matmul kernels takes with one bulk copy.
+// The 16-byte chunks of a row are permuted by the row's place in its group of eight (the 128-byte swizzle that the MMAs read).  Columns behind the last are
+// zero.  Rows behind the last hold whatever they held: their products go nowhere.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "dmlx_b200.h"
+#include "ptx.cuh"
+
+constexpr int kI8Tile = 128;              // rows of a tile
+constexpr int kI8Chunk = 128;             // columns of a block
+constexpr int kI8Block = kI8Tile * kI8Chunk;
+constexpr int kI8MaxK = 131072;           // 127 * 128 * 131072 < 2^31: a sum fits 32 bits whatever it is made of
+
+struct I8RowsDev {
+  signed char* q;  // [row tile][chunks][128][128], swizzled
+  float* scale;    // [row]
+};
+
+struct b200_i8_rows {
+  int max_rows = 0, max_k = 0, max_hidden = 0;
+  int rows = -1, k = 0;                 // what it holds; -1: nothing yet
+  I8RowsDev x{}, hidden{};
+  // [max_rows][h_stride]: the feed-forward block's inner rows until their largest is known.  In bf16 the products behind them were 1e-2 off (what is
+  // rounded twice goes to another of 255 numbers one time in twenty, and a rounded largest moves a row's every step).
+  float* h = nullptr;
+  int h_stride = 0;
+};
+
+struct b200_i8_weight {
+  int n = 0, k = 0, tiles = 0, chunks = 0;
+  bool gated = false;                   // tiles alternate: 128 channels of the gate, the same 128 of up
+  signed char* q = nullptr;             // [tile][chunks][128][128], swizzled
+  float* scale = nullptr;               // [tiles * 128]
+};
+
+inline int i8_chunks(int k) { return (k + kI8Chunk - 1) / kI8Chunk; }
+
+#ifdef __CUDACC__
+// Where column c of a row lies.
+__device__ __forceinline__ size_t i8_at(int row, int c, int chunks) {
+  const int r = row % kI8Tile;
+  return ((size_t)(row / kI8Tile) * chunks + c / kI8Chunk) * kI8Block + r * kI8Chunk + ((((c % kI8Chunk) >> 4) ^ (r & 7)) << 4) + (c & 15);
+}
+
+// A row's numbers as multiples of most / 127, most = its largest magnitude.  The quotient 127 x / most is rounded to the nearest, halves to the even, as if
+// it were exact: the product with the rounded 127 / most is at most 2^-15 off, and where that could decide, the division is made.  (For x of bf16 127 x is
+// exact, and the division rounds correctly: halves are numbers of f32, so it can reach one but not cross it, and nothing is left to chance.)
+struct I8Scale {
+  float most, inv;
+  static __device__ __forceinline__ I8Scale of(float m) { return I8Scale{m, __fdiv_rn(127.0f, m)}; }
+  __device__ __forceinline__ float step() const { return __fdiv_rn(most, 127.0f); }
+  __device__ __forceinline__ bool plain() const { return most > 0.f && most < __int_as_float(0x7f800000); }  // else all zeros: a row of nothing, or one without numbers
+  __device__ __forceinline__ int quantize(float x) const {
+    const float t = x * inv;
+    float r = rintf(t);
+    if (!(fabsf(t - r) < 0.4999f)) {
+      const float down = most > 1e30f ? 0.00390625f : 1.0f;  // (127 times the largest numbers is none of f32)
+      r = rintf(__fdiv_rn(127.0f * (x * down), most * down));
+    }
+    return (int)r;
+  }
+};
+// Eight neighbouring numbers of a row as they lie in memory, those behind the last as zeros.
+template <typename T>
+struct Eight { uint4 r[sizeof(T) / 2]; };
+
+template <typename T>
+__device__ __forceinline__ Eight<T> load_eight(const T* p, int c, int n, bool fit) {
+  Eight<T> e;
+  if (fit && c + 8 <= n) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) e.r[i] = reinterpret_cast<const uint4*>(p + c)[i];
+  } else {
+    T v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i < n ? p[c + i] : T(0.f);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 4) w[j] = __float_as_uint(v[4 * i + j]);
+        else w[j] = (uint32_t)__bfloat16_as_ushort(v[2 * j]) | (uint32_t)__bfloat16_as_ushort(v[2 * j + 1]) << 16;
+      }
+      e.r[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  return e;
+}
+__device__ __forceinline__ void widen(const Eight<__nv_bfloat16>& e, float (&v)[8]) {
+  const uint32_t w[4] = {e.r[0].x, e.r[0].y, e.r[0].z, e.r[0].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = ptx::bf16_lo(w[i]);
+    v[2 * i + 1] = ptx::bf16_hi(w[i]);
+  }
+}
+__device__ __forceinline__ void widen(const Eight<float>& e, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    v[4 * i] = __uint_as_float(e.r[i].x); v[4 * i + 1] = __uint_as_float(e.r[i].y);
+    v[4 * i + 2] = __uint_as_float(e.r[i].z); v[4 * i + 3] = __uint_as_float(e.r[i].w);
+  }
+}
+// The largest magnitude of m and eight numbers, as bits: what is no number is the largest of all.
+__device__ __forceinline__ uint32_t most_of(uint32_t m, const Eight<__nv_bfloat16>& e) {
+  const uint4& r = e.r[0];
+  const uint32_t a = __vmaxu2(__vmaxu2(r.x & 0x7fff7fffu, r.y & 0x7fff7fffu), __vmaxu2(r.z & 0x7fff7fffu, r.w & 0x7fff7fffu));
+  return max(m, max(a << 16, a & 0xffff0000u));
+}
+__device__ __forceinline__ uint32_t most_of(uint32_t m, const Eight<float>& e) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) m = max(max(max(m, e.r[i].x & 0x7fffffffu), max(e.r[i].y & 0x7fffffffu, e.r[i].z & 0x7fffffffu)), e.r[i].w & 0x7fffffffu);
+  return m;
+}
+
+// Eight neighbouring columns, the first a multiple of eight.
+__device__ __forceinline__ void i8_store8(signed char* q, int row, int c, int chunks, const I8Scale& s, const float (&v)[8]) {
+  uint32_t w[2] = {0u, 0u};
+  if (s.plain()) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e / 4] |= ((uint32_t)s.quantize(v[e]) & 0xffu) << (8 * (e % 4));
+  }
+  *reinterpret_cast<uint2*>(q + i8_at(row, c, chunks)) = make_uint2(w[0], w[1]);
+}
+#endif

@@ -4167,6 +4167,12 @@ b200_status b200_qmm_error_words_async(int32_t* h_out, void* stream) {
 
 const int* b200_qmm_err_word_device() { return g_err; }
 
+b200_status b200_qmm_ensure_err_word(int** out) {
+  b200_status st = ensure_state(0);
+  *out = g_err;
+  return st;
+}
+
 b200_status b200_qmm_static_error_word_async(int32_t* h_out, void* stream) {
   *h_out = 0;
   if (int* se = static_err_of_current_device()) B200_CUDA_TRY(cudaMemcpyAsync(h_out, se, sizeof(int), cudaMemcpyDeviceToHost, (cudaStream_t)stream));

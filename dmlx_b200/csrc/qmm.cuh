@@ -104,5 +104,7 @@ b200_status b200_qmm_grouped_from_tokens(const b200_qweight* w, const void* d_to
 b200_status b200_qmm_error_words_async(int32_t* h_out, void* stream);
 // The first of these two words on the device; null before the first matmul.
 const int* b200_qmm_err_word_device();
+// The same, made if it is not there yet (allocates: not in a captured call).
+b200_status b200_qmm_ensure_err_word(int** out);
 // The second one, copied as above where there is one.
 b200_status b200_qmm_static_error_word_async(int32_t* h_out, void* stream);

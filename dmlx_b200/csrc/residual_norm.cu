@@ -1,0 +1,210 @@
+// The norms behind and before a block with its gate and its factor on the residual, in one pass over the rows:
+//   p = y r(y) w_post (or y), times the gate or its sigmoid;  h' = h + scale p;  x = h' r(h') w_norm (or h'),  r(v) = 1 / sqrt(mean(v^2) + eps).
+//
+// A row waits in registers, a block of threads for it (a warp where it is short, eight rows to a block), and two rounds of sums: |y|^2, then |h'|^2
+// together with the largest |h' w_norm|, from which the 8-bit form's step follows without a third (r > 0, and rounding keeps the order).  x is made of h'
+// before its rounding.  f32 in between, one rounding for each result.  Bound by what it reads and writes.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "common.h"
+#include "i8.cuh"
+#include "launch.cuh"
+#include "ptx.cuh"
+#include "rows.cuh"
+
+namespace {
+
+struct ResidualNormArgs {
+  const void *h, *y;
+  const __nv_bfloat16 *gate, *post_w, *norm_w;
+  void* h_out;
+  __nv_bfloat16* x_out;
+  I8RowsDev q;
+  long long h_stride, y_stride, gate_stride, h_out_stride, x_out_stride;
+  int rows, n, chunks, sigmoid;
+  int fit;  // bits: which rows may be read and written in vectors of eight
+  float scale, eps;
+};
+enum { kFitH = 1, kFitY = 2, kFitGate = 4, kFitPost = 8, kFitNorm = 16, kFitHOut = 32, kFitXOut = 64 };
+
+template <typename T>
+__device__ __forceinline__ void store_eight(T* p, int c, int n, bool fit, const float (&v)[8]) {
+  if (fit && c + 8 <= n) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(p + c) = make_float4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<float4*>(p + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&b);
+      }
+      *reinterpret_cast<uint4*>(p + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < n) st(p + c + i, v[i]);
+  }
+}
+
+// NV vectors of eight columns for each thread.  WARP: a warp for a row.  (1024 threads with 32 numbers each have 64 registers: half of a row's y is
+// still in its 16 bits while h comes.)
+template <typename H, typename Y, int NV, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const __grid_constant__ ResidualNormArgs a) {
+  after_previous();
+  __shared__ float part[3][32];
+  const int threads = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
+  const int row = WARP ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+  if (row >= a.rows) return;
+  auto column = [&](int u) { return (t + u * threads) * 8; };
+  auto whole = [&](float v, float* p) {  // the row's sum
+    v = warp_sum(v);
+    if constexpr (!WARP) {
+      if ((t & 31) == 0) p[t >> 5] = v;
+      __syncthreads();
+      v = warp_sum((t & 31) < (threads >> 5) ? p[t & 31] : 0.f);
+    }
+    return v;
+  };
+  const H* h = (const H*)a.h + (size_t)row * a.h_stride;
+  const Y* y = (const Y*)a.y + (size_t)row * a.y_stride;
+  Eight<Y> yr[NV];
+  Eight<H> hr[NV];
+#pragma unroll
+  for (int u = 0; u < NV; ++u) yr[u] = load_eight(y, column(u), a.n, a.fit & kFitY);
+#pragma unroll
+  for (int u = 0; u < NV; ++u) hr[u] = load_eight(h, column(u), a.n, a.fit & kFitH);
+  float ry = 1.f;
+  if (a.post_w) {
+    float ss = 0.f;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      float v[8];
+      widen(yr[u], v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
+    }
+    ry = rsqrtf(whole(ss, part[0]) / (float)a.n + a.eps);
+  }
+  float x[NV][8];
+  float ss = 0.f;
+  uint32_t most = 0u;
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    const int c = column(u);
+    float p[8], w[8];
+    widen(yr[u], p);
+    if (a.post_w) {
+      widen(load_eight(a.post_w, c, a.n, a.fit & kFitPost), w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[e] = p[e] * ry * w[e];
+    }
+    if (a.gate) {
+      widen(load_eight(a.gate + (size_t)row * a.gate_stride, c, a.n, a.fit & kFitGate), w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[e] *= a.sigmoid ? __fdividef(1.0f, 1.0f + __expf(-w[e])) : w[e];
+    }
+    widen(hr[u], w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[u][e] = fmaf(a.scale, p[e], w[e]);
+      ss = fmaf(x[u][e], x[u][e], ss);  // (behind the last column all is zero)
+    }
+    if (c < a.n) store_eight((H*)a.h_out + (size_t)row * a.h_out_stride, c, a.n, a.fit & kFitHOut, x[u]);
+    if (a.norm_w) {
+      widen(load_eight(a.norm_w, c, a.n, a.fit & kFitNorm), w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[u][e] *= w[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(x[u][e]) & 0x7fffffffu);
+  }
+  if (!a.x_out && !a.q.q) return;
+  float r = 1.f;
+  most = __reduce_max_sync(0xffffffffu, most);
+  if constexpr (!WARP) {
+    if ((t & 31) == 0) part[2][t >> 5] = __uint_as_float(most);
+  }
+  if (a.norm_w || !WARP) r = whole(ss, part[1]);
+  r = a.norm_w ? rsqrtf(r / (float)a.n + a.eps) : 1.f;
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[u][e] *= r;
+    if (a.x_out && column(u) < a.n) store_eight(a.x_out + (size_t)row * a.x_out_stride, column(u), a.n, a.fit & kFitXOut, x[u]);
+  }
+  if (!a.q.q) return;
+  if constexpr (!WARP) most = __reduce_max_sync(0xffffffffu, (t & 31) < (threads >> 5) ? __float_as_uint(part[2][t & 31]) : 0u);
+  const I8Scale s = I8Scale::of(__uint_as_float(most) * r);
+  if (t == 0) a.q.scale[row] = s.step();
+#pragma unroll
+  for (int u = 0; u < NV; ++u)
+    if (column(u) < a.chunks * kI8Chunk) i8_store8(a.q.q, row, column(u), a.chunks, s, x[u]);
+}
+
+template <typename H, typename Y>
+b200_status launch(const ResidualNormArgs& a, cudaStream_t s) {
+  const int vectors = a.chunks * (kI8Chunk / 8);
+  if (vectors <= 32 * 2) {
+    const int warps = a.rows >= 8 * b200_sm_count() ? 8 : 1;
+    const unsigned grid = (unsigned)((a.rows + warps - 1) / warps);
+    if (vectors <= 32) launch_after(residual_norm_kernel<H, Y, 1, true>, grid, warps * 32, 0, s, a);
+    else launch_after(residual_norm_kernel<H, Y, 2, true>, grid, warps * 32, 0, s, a);
+  } else {
+    // few rows: more threads, each with fewer loads to wait for
+    const bool few = a.rows <= 2 * b200_sm_count();
+    const int nv = vectors <= 1024 && few ? 1 : vectors <= 2048 ? 2 : 4;
+    const int threads = (vectors + 32 * nv - 1) / (32 * nv) * 32;
+    if (nv == 1) launch_after(residual_norm_kernel<H, Y, 1, false>, a.rows, threads, 0, s, a);
+    else if (nv == 2) launch_after(residual_norm_kernel<H, Y, 2, false>, a.rows, threads, 0, s, a);
+    else launch_after(residual_norm_kernel<H, Y, 4, false>, a.rows, threads, 0, s, a);
+  }
+  B200_LAUNCH_CHECK();
+  return B200_OK;
+}
+
+constexpr int kMostColumns = 32768;  // 1024 threads of four vectors
+
+}  // namespace
+
+extern "C" b200_status b200_residual_norm(const b200_residual_norm_shape* shape, const void* d_h, int64_t h_stride, const void* d_y, int64_t y_stride,
+                                          const void* d_gate, int64_t gate_stride, const void* d_post_weight, const void* d_norm_weight, int32_t rows, void* d_h_out,
+                                          int64_t h_out_stride, void* d_x_out, int64_t x_out_stride, b200_i8_rows* q_out, void* stream) {
+  if (!shape || rows < 0) { b200_set_error("residual norm: no shape, or %d rows", rows); return B200_ERR_INVALID_ARGUMENT; }
+  const int n = shape->n;
+  if (n <= 0 || n > kMostColumns) { b200_set_error("residual norm: rows of %d columns (at most %d)", n, kMostColumns); return B200_ERR_UNSUPPORTED; }
+  if (!(shape->eps >= 0.f)) { b200_set_error("residual norm: eps %g", (double)shape->eps); return B200_ERR_INVALID_ARGUMENT; }
+  const int h_size = shape->h_f32 ? 4 : 2, y_size = shape->y_f32 ? 4 : 2;
+  auto holds = [&](const void* p, int64_t stride, int size) { return p && ((uintptr_t)p & (size - 1)) == 0 && (rows <= 1 || stride >= n); };
+  if (rows > 0 && (!holds(d_h, h_stride, h_size) || !holds(d_y, y_stride, y_size) || !holds(d_h_out, h_out_stride, h_size) || (d_x_out && !holds(d_x_out, x_out_stride, 2)) ||
+                   (d_gate && gate_stride != 0 && !holds(d_gate, gate_stride, 2)) || (((uintptr_t)d_gate | (uintptr_t)d_post_weight | (uintptr_t)d_norm_weight) & 1) != 0 ||
+                   (d_h_out == d_h && rows > 1 && h_out_stride != h_stride))) {
+    b200_set_error("residual norm: rows of %d columns, each on a number's boundary, strides that hold a row; h_out is h itself or apart from it", n);
+    return B200_ERR_INVALID_ARGUMENT;
+  }
+  if (q_out && (rows > q_out->max_rows || n > q_out->max_k)) {
+    b200_set_error("residual norm: %d rows of %d columns, the 8-bit rows are for %d of %d", rows, n, q_out->max_rows, q_out->max_k);
+    return B200_ERR_CAPACITY;
+  }
+  b200_status st = b200_require_device();
+  if (st != B200_OK) return st;
+  if (q_out) { q_out->rows = rows; q_out->k = n; }
+  if (rows == 0) return B200_OK;
+  ResidualNormArgs a{};
+  a.h = d_h; a.y = d_y; a.gate = (const __nv_bfloat16*)d_gate; a.post_w = (const __nv_bfloat16*)d_post_weight; a.norm_w = (const __nv_bfloat16*)d_norm_weight;
+  a.h_out = d_h_out; a.x_out = (__nv_bfloat16*)d_x_out;
+  if (q_out) a.q = q_out->x;
+  a.h_stride = h_stride; a.y_stride = y_stride; a.gate_stride = gate_stride; a.h_out_stride = h_out_stride; a.x_out_stride = x_out_stride;
+  a.rows = rows; a.n = n; a.chunks = i8_chunks(n); a.sigmoid = shape->gate_sigmoid != 0; a.scale = shape->scale; a.eps = shape->eps;
+  auto fits = [&](const void* p, int64_t stride, int size, int bit) { return ((uintptr_t)p & 15) == 0 && (rows <= 1 || stride * size % 16 == 0) ? bit : 0; };
+  a.fit = fits(d_h, h_stride, h_size, kFitH) | fits(d_y, y_stride, y_size, kFitY) | fits(d_gate, gate_stride, 2, kFitGate) | fits(d_post_weight, 0, 2, kFitPost) |
+          fits(d_norm_weight, 0, 2, kFitNorm) | fits(d_h_out, h_out_stride, h_size, kFitHOut) | fits(d_x_out, x_out_stride, 2, kFitXOut);
+  cudaStream_t s = (cudaStream_t)stream;
+  if (shape->h_f32) return shape->y_f32 ? launch<float, float>(a, s) : launch<float, __nv_bfloat16>(a, s);
+  return shape->y_f32 ? launch<__nv_bfloat16, float>(a, s) : launch<__nv_bfloat16, __nv_bfloat16>(a, s);
+}

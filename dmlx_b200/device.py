@@ -338,10 +338,10 @@ class LayeredKVCache(PagedKVCache):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-def _rows(t: torch.Tensor, shape: tuple, device: int) -> int:
-    """Checks bf16 rows on the device whose numbers lie one behind the other within a row; returns the elements between rows."""
-    if t.dtype != torch.bfloat16 or t.shape != shape or t.get_device() != device:
-        raise ValueError(f"expected bf16 rows of shape {shape} on the current device, got {t.dtype} {tuple(t.shape)} on {t.device}")
+def _rows(t: torch.Tensor, shape: tuple, device: int, dtype: torch.dtype = torch.bfloat16) -> int:
+    """Checks rows of a type (bf16) on the device whose numbers lie one behind the other within a row; returns the elements between rows."""
+    if t.dtype != dtype or t.shape != shape or t.get_device() != device:
+        raise ValueError(f"expected {str(dtype)[6:]} rows of shape {shape} on the current device, got {t.dtype} {tuple(t.shape)} on {t.device}")
     inner = math.prod(shape[1:])
     if t.is_contiguous():
         return inner
@@ -480,6 +480,138 @@ class LoraBatch:
         rows, device = row_adapter.shape[0], torch.cuda.current_device()
         _lib.check(lib.b200_lora_plan(self._h, _ints(row_adapter, rows, device), rows, _raw_stream(device)))
         self.rows = rows
+
+
+class I8Weight:
+    """A projection's weight in 8 bits (b200_i8_weight): q int8 [n, k], a scale f32 for each of n; wherever they lie."""
+
+    def __init__(self, q: torch.Tensor, scales: torch.Tensor):
+        self._make(lib.b200_i8_weight_create, False, (q, scales))
+
+    @classmethod
+    def gated(cls, gate_q: torch.Tensor, gate_scales: torch.Tensor, up_q: torch.Tensor, up_scales: torch.Tensor) -> "I8Weight":
+        """The gate and the up projection of a feed-forward block, for i8_ffn."""
+        self = cls.__new__(cls)
+        self._make(lib.b200_i8_weight_create_gated, True, (gate_q, gate_scales), (up_q, up_scales))
+        return self
+
+    def _make(self, create, is_gated: bool, *parts):
+        n, k = parts[0][0].shape
+        kept = []
+        for q, scales in parts:
+            if q.dtype != torch.int8 or scales.dtype != torch.float32 or tuple(q.shape) != (n, k) or tuple(scales.shape) != (n,):
+                raise ValueError(f"expected int8 [{n}, {k}] and f32 [{n}], got {q.dtype} {tuple(q.shape)} and {scales.dtype} {tuple(scales.shape)}")
+            kept += [q.detach().contiguous(), scales.detach().contiguous()]
+        h = C.c_void_p()
+        _lib.check(create(n, k, *(t.data_ptr() for t in kept), C.byref(h)))
+        self._h, self.n, self.k, self.is_gated = h.value, n, k, is_gated
+
+    def close(self):
+        if getattr(self, "_h", None) and lib is not None:
+            lib.b200_i8_weight_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        self.close()
+
+
+class I8Rows:
+    """The rows of a step in 8 bits, a scale for each, and the workspace of the products that read them (b200_i8_rows).  max_hidden: the widest
+    feed-forward block that takes them."""
+
+    def __init__(self, max_rows: int, max_k: int, max_hidden: int = 0):
+        h = C.c_void_p()
+        _lib.check(lib.b200_i8_rows_create(max_rows, max_k, max_hidden, C.byref(h)))
+        self._h, self.max_rows, self.rows, self.k = h.value, max_rows, None, None
+
+    def close(self):
+        if getattr(self, "_h", None) and lib is not None:
+            lib.b200_i8_rows_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        self.close()
+
+    def quantize(self, x: torch.Tensor):
+        """b200_i8_quantize: x [T, k] bf16 (rows may be strided)."""
+        (t, k), device = x.shape, torch.cuda.current_device()
+        _lib.check(lib.b200_i8_quantize(self._h, x.data_ptr(), _rows(x, (t, k), device), t, k, _raw_stream(device)))
+        self.rows, self.k = t, k
+
+    def get(self):
+        """b200_i8_rows_get: (q int8 [T, k], steps f32 [T]); a row is q * step."""
+        device = torch.cuda.current_device()
+        q, steps = torch.empty((self.rows or 0, self.k or 0), dtype=torch.int8, device="cuda"), torch.empty(self.rows or 0, dtype=torch.float32, device="cuda")
+        _lib.check(lib.b200_i8_rows_get(self._h, q.data_ptr(), steps.data_ptr(), _raw_stream(device)))
+        return q, steps
+
+    def _take(self, x: Optional[torch.Tensor], k: int, device: int):
+        """(address, stride, rows) of x, or of what is there already."""
+        if x is None:
+            if self.k != k:
+                raise ValueError(f"the handle holds {'nothing' if self.k is None else f'rows of {self.k} columns'}, the weight has {k}")
+            return None, 0, self.rows
+        t = x.shape[0]
+        return x.data_ptr(), _rows(x, (t, k), device), t
+
+
+def _out_rows(out: Optional[torch.Tensor], t: int, n: int, dtype: torch.dtype, device: int):
+    """(out, stride): a new tensor, or the caller's (rows may be strided)."""
+    if out is None:
+        return torch.empty((t, n), dtype=dtype, device="cuda"), n
+    return out, _rows(out, (t, n), device, dtype)
+
+
+def i8_mm(w: I8Weight, rows: I8Rows, x: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+          f32: bool = False) -> torch.Tensor:
+    """b200_i8_mm: rows times w, scaled, plus a bias f32 [n]; bf16, or f32.  x [T, k] bf16 is brought into `rows` first; without it the rows there are taken."""
+    device = torch.cuda.current_device()
+    at, stride, t = rows._take(x, w.k, device)
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (w.n,) or bias.get_device() != device or not bias.is_contiguous()):
+        raise ValueError(f"expected a bias of {w.n} contiguous f32 on the current device, got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
+    out, out_stride = _out_rows(out, t, w.n, torch.float32 if f32 else torch.bfloat16, device)
+    _lib.check(lib.b200_i8_mm(w._h, rows._h, at, stride, t, None if bias is None else bias.data_ptr(), out.data_ptr(), out_stride, f32, _raw_stream(device)))
+    rows.rows, rows.k = t, w.k
+    return out
+
+
+ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
+
+
+def i8_ffn(gate_up: I8Weight, down: I8Weight, rows: I8Rows, x: Optional[torch.Tensor] = None, activation: str = "silu",
+           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """b200_i8_ffn: down(act(gate x) * (up x)), the rows in 8 bits in front of each product.  x as in i8_mm."""
+    device = torch.cuda.current_device()
+    at, stride, t = rows._take(x, gate_up.k, device)
+    out, out_stride = _out_rows(out, t, down.n, torch.bfloat16, device)
+    _lib.check(lib.b200_i8_ffn(gate_up._h, down._h, rows._h, at, stride, t, ACTIVATIONS[activation], out.data_ptr(), out_stride, _raw_stream(device)))
+    rows.rows, rows.k = t, gate_up.k
+    return out
+
+
+def residual_norm(h: torch.Tensor, y: torch.Tensor, norm_weight: Optional[torch.Tensor] = None, post_weight: Optional[torch.Tensor] = None,
+                  gate: Optional[torch.Tensor] = None, gate_sigmoid: bool = False, scale: float = 1.0, eps: float = 1e-5, h_out: Optional[torch.Tensor] = None,
+                  x_out: Optional[torch.Tensor] = None, rows: Optional[I8Rows] = None):
+    """b200_residual_norm: h + scale * gate * norm(y), and the norm of that for the next block.  h, y [T, n] bf16 or f32, gate bf16 [n] or [T, n] (rows may be
+    strided), a weight that is None is no norm.  Returns (h, x): x bf16, or None where it goes into `rows` in 8 bits.  h_out may be h."""
+    device, shape = torch.cuda.current_device(), tuple(h.shape)
+    t, n = shape
+    h_out = torch.empty(shape, dtype=h.dtype, device="cuda") if h_out is None else h_out
+    if rows is None and x_out is None:
+        x_out = torch.empty(shape, dtype=torch.bfloat16, device="cuda")
+    gate_stride = 0
+    if gate is not None:
+        gate_stride = _rows(gate, shape, device) if gate.dim() == 2 else (_weight(gate, n, device), 0)[1]
+    f32 = torch.float32
+    as_c = _lib.ResidualNormShape(n, h.dtype == f32, y.dtype == f32, gate_sigmoid, scale, eps)
+    kind = lambda v: f32 if v.dtype == f32 else torch.bfloat16  # noqa: E731
+    _lib.check(lib.b200_residual_norm(C.byref(as_c), h.data_ptr(), _rows(h, shape, device, kind(h)), y.data_ptr(), _rows(y, shape, device, kind(y)),
+                                      None if gate is None else gate.data_ptr(), gate_stride, _weight(post_weight, n, device), _weight(norm_weight, n, device), t,
+                                      h_out.data_ptr(), _rows(h_out, shape, device, kind(h)), None if x_out is None else x_out.data_ptr(),
+                                      0 if x_out is None else _rows(x_out, shape, device), None if rows is None else rows._h, _raw_stream(device)))
+    if rows is not None:
+        rows.rows, rows.k = t, n
+    return h_out, x_out
 
 
 def set_attn_pages_per_chunk(n: int):

@@ -1,0 +1,246 @@
+"""The norms behind and before a block with its gate and its factor on the residual, against a plain form in 64 bits.
+
+u = 2^-24.  A sum of squares is 32 additions of a thread and ten of warps, 45 u of it with the squares', so 23 u of its root; rsqrt 4 u, mean and eps 2 u; the products with
+the weight and with the gate 3 u; the gate's sigmoid 2^-20 (its exponential is off by 2 + 1.16 |z| of its last place, |z| up to 9 here, its reciprocal by
+two).  So scale * p is off by 2^-18 of itself at most, h' by that and u of |h| + |scale p|.  The second norm adds 2^-18 of its own, and what h' is off by:
+through the root no more than the norm of its errors over its own.  Rounding: half a step of bf16, 2^-8."""
+import pytest
+import torch
+
+
+def _make(rows, n, seed, h_f32=False, y_f32=False):
+    g = torch.Generator().manual_seed(seed)
+    rnd = lambda *s: torch.randn(s, generator=g)  # noqa: E731
+    as_ = lambda t, f32: t if f32 else t.bfloat16()  # noqa: E731
+    return dict(h=as_(3 * rnd(rows, n), h_f32), y=as_(rnd(rows, n), y_f32), post=(1 + 0.2 * rnd(n)).bfloat16(), norm=(1 + 0.2 * rnd(n)).bfloat16(),
+                gate_row=(rnd(rows, n)).bfloat16(), gate=(0.5 + 0.3 * rnd(n)).bfloat16())
+
+
+def _want(h, y, post, norm, gate, sigmoid, scale, eps):
+    """(h', its tolerance, x, its tolerance) before any rounding of the results."""
+    r = lambda v: (v.square().mean(-1, keepdim=True) + eps).rsqrt()  # noqa: E731
+    p = y.double()
+    if post is not None:
+        p = p * r(p) * post.double()
+    if gate is not None:
+        p = p * (torch.sigmoid(gate.double()) if sigmoid else gate.double())
+    p = scale * p
+    out = h.double() + p
+    h_tol = 2.0 ** -18 * p.abs() + 2.0 ** -23 * (h.double().abs() + p.abs())
+    if norm is None:
+        return out, h_tol, out, h_tol
+    w = norm.double() * r(out)
+    x = out * w
+    size = out.square().sum(-1, keepdim=True).sqrt().clamp(min=1e-300)
+    return out, h_tol, x, w.abs() * h_tol + x.abs() * (2.0 ** -18 + h_tol.square().sum(-1, keepdim=True).sqrt() / size)
+
+
+def _check(got, want, tol):
+    if got.dtype == torch.bfloat16:
+        tol = tol + 2.0 ** -8 * want.abs()
+    off = (got.double().cpu() - want).abs()
+    assert bool((off <= tol).all()), float((off - tol).max())
+
+
+def _cuda(t):
+    return None if t is None else t.cuda()
+
+
+SHAPES = [(1, 1), (1, 4096), (2, 7), (3, 128), (5, 129), (64, 256), (33, 512), (1300, 512), (40, 513), (400, 1000), (7, 2880), (300, 4096), (320, 5003), (2, 8192), (310, 8200),
+          (3, 16384), (300, 16384), (2, 16392), (5, 20001), (2, 32768)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n", SHAPES)
+@pytest.mark.parametrize("h_f32,y_f32,post,gate,sigmoid", [(False, False, True, None, False), (True, False, True, "gate", False), (False, True, False, "gate_row", True),
+                                                           (True, True, True, "gate_row", False), (False, False, False, None, False)])
+def test_norms(rows, n, h_f32, y_f32, post, gate, sigmoid):
+    from dmlx_b200 import device as dev
+
+    c = _make(rows, n, rows + n, h_f32, y_f32)
+    post_w, gate_w, scale, eps = c["post"] if post else None, c[gate] if gate else None, 0.22, 1e-5
+    want = _want(c["h"], c["y"], post_w, c["norm"], gate_w, sigmoid, scale, eps)
+    h, x = dev.residual_norm(c["h"].cuda(), c["y"].cuda(), c["norm"].cuda(), post_weight=_cuda(post_w), gate=_cuda(gate_w), gate_sigmoid=sigmoid, scale=scale, eps=eps)
+    assert h.dtype == c["h"].dtype and x.dtype == torch.bfloat16
+    _check(h, want[0], want[1])
+    _check(x, want[2], want[3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n", [(1, 4096), (5, 130), (700, 256), (1300, 500), (300, 4096), (320, 5003), (3, 17000)])
+@pytest.mark.parametrize("normed", [True, False])
+def test_into_8_bits(rows, n, normed):
+    """A number is half a step off at most, and the step is what the row's largest over 127 says, to two more roundings."""
+    from dmlx_b200 import device as dev
+
+    c = _make(rows, n, n)
+    norm = c["norm"] if normed else None
+    h_want, h_tol, x, tol = _want(c["h"], c["y"], c["post"], norm, None, False, 0.5, 1e-6)
+    held = dev.I8Rows(rows + 1, n + 5)
+    h, none = dev.residual_norm(c["h"].cuda(), c["y"].cuda(), _cuda(norm), post_weight=c["post"].cuda(), scale=0.5, eps=1e-6, rows=held)
+    assert none is None
+    _check(h, h_want, h_tol)
+    q, steps = held.get()
+    q, steps = q.cpu().double(), steps.cpu().double()[:, None]
+    most = x.abs().amax(1, keepdim=True)
+    off = (steps * 127 - most).abs()
+    assert bool((off <= tol.amax(1, keepdim=True) + 2.0 ** -22 * most).all())
+    assert bool(((q * steps - x).abs() <= 0.5 * steps + tol + 2.0 ** -20 * most).all()) and bool((q.abs().amax(1) == 127).all())
+    # both forms at once are the same
+    other = dev.I8Rows(rows, n)
+    h2, x2 = dev.residual_norm(c["h"].cuda(), c["y"].cuda(), _cuda(norm), post_weight=c["post"].cuda(), scale=0.5, eps=1e-6, rows=other,
+                               x_out=torch.empty((rows, n), dtype=torch.bfloat16, device="cuda"))
+    _check(x2, x, tol)
+    assert torch.equal(h, h2) and torch.equal(other.get()[0].cpu().double(), q)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("at", [0, 8, 1, 3])
+@pytest.mark.parametrize("h_f32", [False, True])
+def test_strides_places_and_what_lies_around(at, h_f32):
+    from dmlx_b200 import device as dev
+
+    rows, n, more = 37, 520, 24
+    c = _make(rows, n + more, 3, h_f32)
+    cut = lambda t: t[..., at:at + n]  # noqa: E731
+    want = _want(cut(c["h"]), cut(c["y"]), cut(c["post"]), cut(c["norm"]), cut(c["gate_row"]), False, -1.5, 1e-5)
+    h, y, gate = c["h"].cuda(), c["y"].cuda(), c["gate_row"].cuda()
+    out, x_out = torch.full((rows + 2, n + more), 7.0, dtype=h.dtype, device="cuda"), torch.full((rows + 2, n + more), 7.0, dtype=torch.bfloat16, device="cuda")
+    dev.residual_norm(cut(h), cut(y), cut(c["norm"].cuda()), post_weight=cut(c["post"].cuda()), gate=cut(gate), scale=-1.5, h_out=cut(out[:rows]), x_out=cut(x_out[:rows]))
+    _check(cut(out[:rows]), want[0], want[1])
+    _check(cut(x_out[:rows]), want[2], want[3])
+    for t in (out, x_out):
+        assert bool((t[rows:] == 7).all()) and bool((t[:, :at] == 7).all()) and bool((t[:, at + n:] == 7).all())
+    assert torch.equal(h.cpu(), c["h"]) and torch.equal(y.cpu(), c["y"]) and torch.equal(gate.cpu(), c["gate_row"])
+    # into h itself, the same bits
+    dev.residual_norm(cut(h), cut(y), cut(c["norm"].cuda()), post_weight=cut(c["post"].cuda()), gate=cut(gate), scale=-1.5, h_out=cut(h), x_out=cut(x_out[:rows]))
+    assert torch.equal(cut(h), cut(out[:rows]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [200, 4096])
+def test_rows_that_hold_no_number_and_rows_of_nothing(n):
+    from dmlx_b200 import device as dev
+
+    rows = 9
+    c = _make(rows, n, 5)
+    run = lambda h, y, held=None: dev.residual_norm(h.cuda(), y.cuda(), c["norm"].cuda(), post_weight=c["post"].cuda(), scale=0.3, rows=held)  # noqa: E731
+    good = run(c["h"], c["y"])
+    h, y = c["h"].clone(), c["y"].clone()
+    y[1, 3], h[4, 0], y[6, n - 1] = float("nan"), float("inf"), -float("inf")
+    h[7], y[7] = 0, 0
+    bad = run(h, y)
+    rest = [0, 2, 3, 5, 8]
+    for g, b in zip(good, bad):
+        assert torch.equal(g[rest], b[rest])
+        assert bool(b[1].isnan().all()) and bool((b[7] == 0).all())
+    assert bool(bad[1][4].isnan().any()) and bool(bad[1][6].isnan().all())
+    held = dev.I8Rows(rows, n)
+    run(h, y, held)
+    q, steps = held.get()
+    assert bool((q[[1, 4, 6, 7]] == 0).all()) and float(steps[7]) == 0 and not bool(steps[[1, 4, 6]].isfinite().any())
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    from dmlx_b200 import device as dev
+
+    rows, n, stride = 2, 136, 2 ** 31 + 64
+    c = _make(rows, n, 6)
+    far = lambda: torch.empty(stride + n, dtype=torch.bfloat16, device="cuda").as_strided((rows, n), (stride, 1))  # noqa: E731
+    h, y, out, x = far(), far(), far(), far()
+    h.copy_(c["h"])
+    y.copy_(c["y"])
+    dev.residual_norm(h, y, c["norm"].cuda(), scale=0.3, h_out=out, x_out=x)
+    want = _want(c["h"], c["y"], None, c["norm"], None, False, 0.3, 1e-5)
+    _check(out.contiguous(), want[0], want[1])
+    _check(x.contiguous(), want[2], want[3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 40, 500])
+def test_the_half_of_a_layer_in_a_graph(rows):
+    """Norms into 8 bits, the feed-forward block, norms for the next block: replayed, the bits of the calls one by one; and against a layer in 64 bits that quantises
+    nothing, whose products' errors are then those of 8 bits (half a step of 127 of a largest of five deviations, three times over, spread over a row: a cosine of
+    0.999 leaves four times that)."""
+    from dmlx_b200 import device as dev
+
+    n, f = 768, 1280
+    g = torch.Generator().manual_seed(rows)
+
+    def weight(n, k):
+        w = torch.randn((n, k), generator=g) * k ** -0.5
+        s = w.abs().amax(1) / 127
+        return torch.round(w / s[:, None]).to(torch.int8), s
+
+    gate, up, down = weight(f, n), weight(f, n), weight(n, f)
+    gate_up, down_w = dev.I8Weight.gated(*gate, *up), dev.I8Weight(*down)
+    c = _make(rows, n, 7)
+    held = dev.I8Rows(rows, n, f)
+    h, y, post, norm = c["h"].cuda(), c["y"].cuda(), c["post"].cuda(), c["norm"].cuda()
+
+    def half():
+        h1, _ = dev.residual_norm(h, y, norm, post_weight=post, scale=0.4, rows=held)
+        return dev.residual_norm(h1, dev.i8_ffn(gate_up, down_w, held), norm, post_weight=post, scale=0.4)
+
+    half()
+    torch.cuda.synchronize()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=stream):
+        replayed = half()
+    c2 = _make(rows, n, 8)
+    h.copy_(c2["h"])
+    y.copy_(c2["y"])
+    graph.replay()
+    torch.cuda.synchronize()
+    once = half()
+    for a, b in zip(replayed, once):
+        assert torch.equal(a, b)
+    w64 = [q.double() * s.double()[:, None] for q, s in (gate, up, down)]
+    h1, _, x, _ = _want(c2["h"], c2["y"], c["post"], c["norm"], None, False, 0.4, 1e-5)
+    inner = torch.nn.functional.silu(x @ w64[0].T) * (x @ w64[1].T)
+    h2, _, x2, _ = _want(h1, inner @ w64[2].T, c["post"], c["norm"], None, False, 0.4, 1e-5)
+    for got, want in zip(once, (h2, x2)):
+        assert float(torch.nn.functional.cosine_similarity(got.double().cpu().flatten(), want.flatten(), 0)) > 0.999
+
+
+@pytest.mark.gpu
+def test_refusals():
+    from dmlx_b200 import _lib
+    from dmlx_b200 import device as dev
+
+    c = {k: v.cuda() for k, v in _make(4, 64, 9).items()}
+    h, y, norm = c["h"], c["y"], c["norm"]
+    for call in (lambda: dev.residual_norm(h, y[:3], norm), lambda: dev.residual_norm(h, y, norm[:32]), lambda: dev.residual_norm(h.half(), y, norm),
+                 lambda: dev.residual_norm(h, y, norm.float()), lambda: dev.residual_norm(h, y, norm, gate=c["gate"][:3]),
+                 lambda: dev.residual_norm(h, y, norm, gate=c["gate_row"].float()), lambda: dev.residual_norm(h, y, norm, h_out=h.float()), lambda: dev.residual_norm(h.cpu(), y, norm)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(_lib.B200Error) as e:
+        dev.residual_norm(h, y, norm, rows=dev.I8Rows(3, 64))
+    assert e.value.status == _lib.ERR_CAPACITY
+    with pytest.raises(_lib.B200Error):
+        dev.residual_norm(h, y, norm, eps=-1.0)
+    wide = torch.zeros((1, 32769), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(_lib.B200Error) as e:
+        dev.residual_norm(wide, wide)
+    assert e.value.status == _lib.ERR_UNSUPPORTED
+    none = torch.empty((0, 64), dtype=torch.bfloat16, device="cuda")
+    assert dev.residual_norm(none, none, norm)[0].shape == (0, 64)
+
+
+def test_refusals_without_a_device():
+    import ctypes as C
+
+    from dmlx_b200 import _lib
+
+    run = lambda shape, rows=1, p=64, stride=8: _lib.lib.b200_residual_norm(shape and C.byref(shape), p, stride, p, stride, None, 0, None, None, rows, p, stride, None, 0, None, None)  # noqa: E731
+    bad = _lib.ERR_INVALID_ARGUMENT
+    assert run(None) == bad
+    assert run(_lib.ResidualNormShape(8, 0, 0, 0, 1.0, 1e-5), rows=-1) == bad
+    assert run(_lib.ResidualNormShape(0, 0, 0, 0, 1.0, 1e-5)) == _lib.ERR_UNSUPPORTED
+    assert run(_lib.ResidualNormShape(32769, 0, 0, 0, 1.0, 1e-5)) == _lib.ERR_UNSUPPORTED
+    assert run(_lib.ResidualNormShape(8, 0, 0, 0, 1.0, float("nan"))) == bad
+    assert run(_lib.ResidualNormShape(8, 0, 0, 0, 1.0, 1e-5), p=None) == bad
+    assert run(_lib.ResidualNormShape(8, 1, 0, 0, 1.0, 1e-5), p=66) == bad
+    assert run(_lib.ResidualNormShape(8, 0, 0, 0, 1.0, 1e-5), rows=2, stride=7) == bad
