@@ -140,7 +140,7 @@ struct MmArgs {
   void* y;
   long long y_stride;
   int* err;
-  int rows, n, chunks, tiles, tn, stages;
+  int rows, n, chunks, tiles, tn, stages, shares;
   int y_f32, act;  // (a feed-forward block's inner rows are f32)
 };
 
@@ -163,9 +163,31 @@ __device__ __forceinline__ float activated(int act, float g) {
   return g / (1.0f + __expf(-1.5957691216057308f * (g + 0.044715f * g * g * g)));
 }
 
-// A weight tile (gated: the gate's and up's tile of the same channels) by up to tn rows per CTA.  The weights are the MMA's M, the rows its N, so that few
-// rows waste nothing; a lane of tensor memory is a channel.  Warp 0 loads, warp 1 multiplies, four bring the sums to the output.
-constexpr int kStreamThreads = 192;
+// One output of a product; in a feed-forward block `u` is up's sum, and the gate's goes through the activation.
+template <bool GATED>
+__device__ __forceinline__ float output_of(const MmArgs& a, int sum, int up, float ws, float us, float step, float bias) {
+  const float y = (float)sum * ws * step + bias;
+  if constexpr (GATED) return activated(a.act, y) * ((float)up * us * step);
+  else return y;
+}
+
+// ---- up to a few hundred rows: streams of weights ----
+// A weight tile (gated: the gate's and up's tile of the same channels) by up to tn rows and a share of K per CTA.  The weights are the MMA's M, the rows
+// its N, so that few rows waste nothing; a lane of tensor memory is a channel.  Warp 0 loads, warp 1 multiplies, four bring the sums to the output.
+// Bound by the weights, which come at the rate of memory only if every SM asks for them: a cluster of up to eight CTAs shares K (as many as still run at
+// the same time, two CTAs on an SM), and each CTA adds up, over the cluster's shared memory, a share of the rows.
+constexpr int kStreamThreads = 192, kStreamShared = 112 * 1024, kMostShares = 8;
+
+__device__ __forceinline__ int load_of_rank(uint32_t addr, uint32_t rank) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(ptx::map_to_rank(addr, rank)) : "memory");
+  return v;
+}
+
+// The rows that a CTA of the cluster brings to the output: CTA q the q-th so many.
+__host__ __device__ constexpr int rows_per_rank(int tn, int rows_here, int shares) {
+  return tn <= 32 ? (rows_here + shares - 1) / shares : ((rows_here + shares - 1) / shares + 15) / 16 * 16;
+}
 
 template <bool GATED>
 __global__ void __launch_bounds__(kStreamThreads) i8_stream_kernel(MmArgs a) {
@@ -178,9 +200,11 @@ __global__ void __launch_bounds__(kStreamThreads) i8_stream_kernel(MmArgs a) {
   uint64_t* sums = done + S;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sums + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tile = blockIdx.x, t0 = blockIdx.y * a.tn, rows_here = min(a.tn, a.rows - t0), n_here = (rows_here + 15) / 16 * 16;
-  uint32_t cols = 32;
-  while (cols < (uint32_t)(W * a.tn)) cols *= 2;
+  const int shares = a.shares, rank = shares > 1 ? (int)ptx::cluster_rank() : 0;
+  const int tile = blockIdx.x / shares, t0 = blockIdx.y * a.tn, rows_here = min(a.tn, a.rows - t0), n_here = (rows_here + 15) / 16 * 16;
+  const int per_share = (a.chunks + shares - 1) / shares, chunk0 = rank * per_share, chunks = min(per_share, a.chunks - chunk0);  // (never none)
+  uint32_t cols = 32;  // (the sums' 16 columns from any row on are there; from 64 rows on shares begin at a multiple of 16)
+  while (cols < (uint32_t)(W * a.tn + (a.tn <= 32 ? 16 : 0))) cols *= 2;
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       ptx::mbar_init(&full[s], 1);
@@ -193,16 +217,16 @@ __global__ void __launch_bounds__(kStreamThreads) i8_stream_kernel(MmArgs a) {
   auto load_weights = [&](int i, int s) {
     ptx::mbar_expect_tx(&full[s], W * kI8Block + n_here * kI8Chunk);
     for (int h = 0; h < W; ++h)
-      ptx::bulk_g2s(smem + (size_t)s * stage_bytes + h * kI8Block, a.w + ((size_t)(tile * W + h) * a.chunks + i) * kI8Block, kI8Block, &full[s]);
+      ptx::bulk_g2s(smem + (size_t)s * stage_bytes + h * kI8Block, a.w + ((size_t)(tile * W + h) * a.chunks + chunk0 + i) * kI8Block, kI8Block, &full[s]);
   };
   auto load_rows = [&](int i, int s) {  // (a tile of 256 rows is two of the layout's)
     for (int r = 0; r < n_here; r += kI8Tile) {
       const int row = t0 + r;
-      ptx::bulk_g2s(smem + (size_t)s * stage_bytes + W * kI8Block + r * kI8Chunk, a.q + ((size_t)(row / kI8Tile) * a.chunks + i) * kI8Block + row % kI8Tile * kI8Chunk,
-                    min(kI8Tile, n_here - r) * kI8Chunk, &full[s]);
+      ptx::bulk_g2s(smem + (size_t)s * stage_bytes + W * kI8Block + r * kI8Chunk,
+                    a.q + ((size_t)(row / kI8Tile) * a.chunks + chunk0 + i) * kI8Block + row % kI8Tile * kI8Chunk, min(kI8Tile, n_here - r) * kI8Chunk, &full[s]);
     }
   };
-  const int ahead = min(S, a.chunks);  // weights asked for before the kernels ahead have ended
+  const int ahead = min(S, chunks);  // weights asked for before the kernels ahead have ended
   if (threadIdx.x == 0)
     for (int i = 0; i < ahead; ++i) load_weights(i, i);
   wait_previous();
@@ -215,11 +239,17 @@ __global__ void __launch_bounds__(kStreamThreads) i8_stream_kernel(MmArgs a) {
   ptx::tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
   bool ok = true;
+  const int quarter = warp & 3, channel = tile * kI8Tile + quarter * 32 + lane;
+  const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
+  const int per_rank = rows_per_rank(a.tn, rows_here, shares);
+  auto first_of = [&](int q) { return min(rows_here, q * per_rank); };
+  int* parts = reinterpret_cast<int*>(smem);  // [gate, up][row of another's][channel]: this CTA's sums for the others, where the stages were
+  const int mine0 = first_of(rank), mine1 = first_of(rank + 1);
   if (warp == 0) {
     if (lane == 0) {
       int s = 0, issued = 0;
       uint32_t ph = 1;
-      for (int i = 0; i < a.chunks; ++i) {
+      for (int i = 0; i < chunks; ++i) {
         if (i >= ahead) {
           ok = ptx::mbar_wait(&done[s], ph);
           if (!ok) break;
@@ -233,12 +263,13 @@ __global__ void __launch_bounds__(kStreamThreads) i8_stream_kernel(MmArgs a) {
       if (!ok)  // copies are on their way into this memory
         for (int i = max(0, issued - S); i < issued; ++i) ptx::mbar_wait(&full[i % S], (i / S) & 1);
     }
+    __syncwarp();
   } else if (warp == 1) {
     if (ptx::elect_one()) {
       const uint32_t idesc = idesc_i8(kI8Tile, n_here);
       int s = 0;
       uint32_t ph = 0;
-      for (int i = 0; i < a.chunks; ++i) {
+      for (int i = 0; i < chunks; ++i) {
         ok = ptx::mbar_wait(&full[s], ph);
         if (!ok) break;
         ptx::tc_fence_after_sync();
@@ -260,13 +291,9 @@ __global__ void __launch_bounds__(kStreamThreads) i8_stream_kernel(MmArgs a) {
   } else {
     ok = ptx::mbar_wait(sums, 0);
     ok = __all_sync(0xffffffffu, ok);
-    if (ok) {
-      ptx::tc_fence_after_sync();
-      const int quarter = warp & 3, channel = tile * kI8Tile + quarter * 32 + lane;
-      const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
-      const size_t scale_at = (size_t)tile * W * kI8Tile + quarter * 32 + lane;
-      const float ws = a.w_scale[scale_at], us = GATED ? a.w_scale[scale_at + kI8Tile] : 0.f;
-      const float bias = !GATED && a.bias && channel < a.n ? a.bias[channel] : 0.f;
+    ptx::tc_fence_after_sync();
+    if (ok && shares > 1) {
+      const int others = rows_here - (mine1 - mine0);
       for (int c0 = 0; c0 < rows_here; c0 += 16) {
         uint32_t v[16], u[16];
         ptx::tmem_ld16(acc + c0, v);
@@ -274,37 +301,108 @@ __global__ void __launch_bounds__(kStreamThreads) i8_stream_kernel(MmArgs a) {
         ptx::tmem_ld_wait();
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          if (c0 + j >= rows_here || channel >= a.n) continue;
-          const size_t row = t0 + c0 + j, at = row * a.y_stride + channel;
-          const float step = a.step[row];
-          float y = (float)(int)v[j] * ws * step + bias;
-          if constexpr (GATED) y = activated(a.act, y) * ((float)(int)u[j] * us * step);
-          if (GATED || a.y_f32) reinterpret_cast<float*>(a.y)[at] = y;
-          else reinterpret_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16(y);
+          const int row = c0 + j;
+          if (row >= rows_here || (row >= mine0 && row < mine1)) continue;
+          int* to = parts + (row < mine0 ? row : row - (mine1 - mine0)) * kI8Tile + quarter * 32 + lane;
+          to[0] = (int)v[j];
+          if constexpr (GATED) to[others * kI8Tile] = (int)u[j];
         }
       }
     }
   }
+  if (shares > 1) ptx::cluster_sync();  // all sums are there
+  if (warp >= 2 && ok) {
+    const size_t scale_at = (size_t)tile * W * kI8Tile + quarter * 32 + lane;
+    const float ws = a.w_scale[scale_at], us = GATED ? a.w_scale[scale_at + kI8Tile] : 0.f;
+    const float bias = !GATED && a.bias && channel < a.n ? a.bias[channel] : 0.f;
+    for (int c0 = mine0; c0 < mine1; c0 += 16) {
+      uint32_t v[16], u[16];
+      ptx::tmem_ld16(acc + c0, v);
+      if constexpr (GATED) ptx::tmem_ld16(acc + a.tn + c0, u);
+      ptx::tmem_ld_wait();
+      for (int q = 0; q < shares; ++q) {
+        if (q == rank) continue;
+        const int q0 = first_of(q), qn = first_of(q + 1) - q0, others = rows_here - qn;
+        const uint32_t from = ptx::smem_u32(parts + (c0 < q0 ? c0 : c0 - qn) * kI8Tile + quarter * 32 + lane);
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (c0 + j < mine1) {
+            v[j] += (uint32_t)load_of_rank(from + j * kI8Tile * 4, q);
+            if constexpr (GATED) u[j] += (uint32_t)load_of_rank(from + (others + j) * kI8Tile * 4, q);
+          }
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        if (c0 + j >= mine1 || channel >= a.n) continue;
+        const size_t row = t0 + c0 + j, at = row * a.y_stride + channel;
+        const float y = output_of<GATED>(a, (int)v[j], GATED ? (int)u[j] : 0, ws, us, a.step[row], bias);
+        if (GATED || a.y_f32) reinterpret_cast<float*>(a.y)[at] = y;
+        else reinterpret_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16(y);
+      }
+    }
+  }
   if (!ok) atomicExch(a.err, B200_ERR_DEVICE_FLAGGED);
+  __syncwarp();
   ptx::tc_fence_before_sync();
-  __syncthreads();
+  if (shares > 1) ptx::cluster_sync();  // nobody leaves while its sums may be read
+  else __syncthreads();
   if (warp == 1) ptx::tmem_dealloc(tmem, cols);
 }
 
+// A launch in clusters of `size` (1: none) whose start-up overlaps the end of the kernel ahead.
+template <class... P>
+void launch_clusters(void (*kernel)(P...), int size, dim3 grid, int threads, size_t smem, cudaStream_t s, P... args) {
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // (as launch_after)
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = size;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = size > 1 ? 2 : 1;
+  (void)cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 template <bool GATED>
-b200_status launch_product(MmArgs& a, cudaStream_t s) {
-  static bool configured = false;
-  constexpr int kShared = 112 * 1024, W = GATED ? 2 : 1;  // two CTAs on an SM
-  if (!configured) {
-    B200_CUDA_TRY(cudaFuncSetAttribute(i8_stream_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared));
-    configured = true;
+b200_status launch_stream(MmArgs& a, cudaStream_t s) {
+  constexpr int W = GATED ? 2 : 1;
+  static int at_once[kMostShares + 1] = {};  // CTAs that run at the same time, by the cluster's size
+  if (at_once[1] == 0) {
+    B200_CUDA_TRY(cudaFuncSetAttribute(i8_stream_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamShared));
+    for (int size = kMostShares; size > 0; --size) at_once[size] = ctas_in_clusters(i8_stream_kernel<GATED>, size, 2, b200_sm_count(), kStreamThreads, kStreamShared);
   }
   const int most = GATED ? 128 : 256;
   a.tn = 16;
   while (a.tn < most && a.tn < a.rows) a.tn *= 2;
-  const int stage = W * kI8Block + a.tn * kI8Chunk;
-  a.stages = std::min(a.chunks, (kShared - 2048) / stage);
-  launch_after(i8_stream_kernel<GATED>, dim3(a.tiles / W, (a.rows + a.tn - 1) / a.tn), kStreamThreads, (size_t)a.stages * stage + 2048, s, a);
+  const int tiles = a.tiles / W, row_tiles = (a.rows + a.tn - 1) / a.tn;
+  const int stage = W * kI8Block + a.tn * kI8Chunk, room = kStreamShared - 2048;
+  // Sums that go to the cluster's other CTAs, in bytes; they lie where the stages were.
+  auto parts = [&](int shares) {
+    size_t most = 0;
+    for (int rows_here : {std::min(a.rows, a.tn), a.rows - (row_tiles - 1) * a.tn}) {
+      const int per = rows_per_rank(a.tn, rows_here, shares);
+      for (int q = 0; q < shares; ++q) {
+        const int own = std::min(rows_here, (q + 1) * per) - std::min(rows_here, q * per);
+        most = std::max(most, (size_t)W * (rows_here - own) * kI8Tile * 4);
+      }
+    }
+    return most;
+  };
+  // As many shares of K as still run at once, each of two blocks or more.
+  a.shares = 1;
+  for (int n = 2; n <= kMostShares && a.chunks >= 2 * n; ++n) {
+    const int per = (a.chunks + n - 1) / n;
+    if ((long long)tiles * row_tiles * n <= at_once[n] && (n - 1) * per < a.chunks && (parts(n) + stage - 1) / stage * stage <= (size_t)room) a.shares = n;
+  }
+  const int per_share = (a.chunks + a.shares - 1) / a.shares;
+  a.stages = std::min(per_share, room / stage);
+  while (a.shares > 1 && (size_t)a.stages * stage < parts(a.shares)) ++a.stages;
+  launch_clusters(i8_stream_kernel<GATED>, a.shares, dim3(tiles * a.shares, row_tiles), kStreamThreads, (size_t)a.stages * stage + 2048, s, a);
   B200_LAUNCH_CHECK();
   return B200_OK;
 }
@@ -315,7 +413,7 @@ b200_status product(const b200_i8_weight* w, const I8RowsDev& x, int rows, const
   if (st != B200_OK) return st;
   a.w = w->q; a.w_scale = w->scale; a.q = x.q; a.step = x.scale; a.bias = bias; a.y = y; a.y_stride = y_stride; a.y_f32 = y_f32; a.act = act;
   a.rows = rows; a.n = w->n; a.chunks = w->chunks; a.tiles = w->tiles;
-  return w->gated ? launch_product<true>(a, s) : launch_product<false>(a, s);
+  return w->gated ? launch_stream<true>(a, s) : launch_stream<false>(a, s);
 }
 
 // ---- handles -------------------------------------------------------------------------------------------------------------------
