@@ -141,6 +141,7 @@ struct MmArgs {
   long long y_stride;
   int* err;
   int rows, n, chunks, tiles, tn, stages, shares;
+  int y_vec;       // rows of y start on 16 bytes
   int y_f32, act;  // (a feed-forward block's inner rows are f32)
 };
 
@@ -157,10 +158,10 @@ __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64
 __device__ __forceinline__ uint32_t idesc_i8(uint32_t m, uint32_t n) { return 2u << 4 | 1u << 7 | 1u << 10 | (n >> 3) << 17 | (m >> 4) << 24; }
 
 __device__ __forceinline__ float activated(int act, float g) {
-  if (act == B200_ACT_SILU) return g / (1.0f + __expf(-g));
+  if (act == B200_ACT_SILU) return __fdividef(g, 1.0f + __expf(-g));  // (a divisor past 2^126 makes 0, as it should)
   if (act == B200_ACT_GELU) return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
   // 0.5 g (1 + tanh z) = g / (1 + e^-2z)
-  return g / (1.0f + __expf(-1.5957691216057308f * (g + 0.044715f * g * g * g)));
+  return __fdividef(g, 1.0f + __expf(-1.5957691216057308f * (g + 0.044715f * g * g * g)));
 }
 
 // One output of a product; in a feed-forward block `u` is up's sum, and the gate's goes through the activation.
@@ -317,6 +318,7 @@ __global__ void __launch_bounds__(kStreamThreads) i8_stream_kernel(MmArgs a) {
     const float bias = !GATED && a.bias && channel < a.n ? a.bias[channel] : 0.f;
     for (int c0 = mine0; c0 < mine1; c0 += 16) {
       uint32_t v[16], u[16];
+      const float steps = c0 + (lane & 15) < mine1 ? a.step[t0 + c0 + (lane & 15)] : 0.f;  // (ahead of the stores, which loads do not pass)
       ptx::tmem_ld16(acc + c0, v);
       if constexpr (GATED) ptx::tmem_ld16(acc + a.tn + c0, u);
       ptx::tmem_ld_wait();
@@ -333,9 +335,10 @@ __global__ void __launch_bounds__(kStreamThreads) i8_stream_kernel(MmArgs a) {
       }
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
+        const float step = __shfl_sync(0xffffffffu, steps, j);
         if (c0 + j >= mine1 || channel >= a.n) continue;
-        const size_t row = t0 + c0 + j, at = row * a.y_stride + channel;
-        const float y = output_of<GATED>(a, (int)v[j], GATED ? (int)u[j] : 0, ws, us, a.step[row], bias);
+        const size_t at = (size_t)(t0 + c0 + j) * a.y_stride + channel;
+        const float y = output_of<GATED>(a, (int)v[j], GATED ? (int)u[j] : 0, ws, us, step, bias);
         if (GATED || a.y_f32) reinterpret_cast<float*>(a.y)[at] = y;
         else reinterpret_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16(y);
       }
@@ -347,6 +350,236 @@ __global__ void __launch_bounds__(kStreamThreads) i8_stream_kernel(MmArgs a) {
   if (shares > 1) ptx::cluster_sync();  // nobody leaves while its sums may be read
   else __syncthreads();
   if (warp == 1) ptx::tmem_dealloc(tmem, cols);
+}
+
+// ---- many rows: pairs of CTAs ----
+// Two CTAs (a cluster) share an MMA of 256 rows by 256 weight rows: each brings 128 of both and holds the sums of its 128 rows, so that an MMA reads 8 KiB of
+// each CTA's shared memory in the 128 cycles that it takes.  Persistent: a pair walks the items, a tile of rows by a pair of weight tiles (gated: the
+// gate's and up's of the same 128 channels), rows fastest within bands, so that both operands come from L2.  An item's sums are half of tensor
+// memory: eight warps drain one half while the MMAs fill the other.
+// Warps: 0 loads both operands of this CTA, 1 multiplies (in the first CTA), 2 tells the first CTA that this one's stage is complete, 4-11 bring the
+// sums to the output.
+constexpr int kPairThreads = 384, kPairStage = 2 * kI8Block, kPairStages = 6, kPairRows = 256, kPairBand = 16;
+constexpr int kPairPitch = 20;  // epilogue: words between rows in a warp's staging tile of 32 rows by 16 words
+constexpr int kPairShared = 1024 + kPairStages * kPairStage + 8 * 32 * kPairPitch * 4 + 8 * (3 * kPairStages + 5) + 16;
+
+__device__ __forceinline__ void umma2_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+template <bool GATED>
+__global__ void __launch_bounds__(kPairThreads, 1) i8_pair_kernel(MmArgs a) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  constexpr int S = kPairStages;
+  float* staging = reinterpret_cast<float*>(smem + (size_t)S * kPairStage);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + 8 * 32 * kPairPitch);
+  const uint32_t smem_u = ptx::smem_u32(smem), full = ptx::smem_u32(bars);  // [S] this CTA's half of the stage has landed
+  const uint32_t done = full + 8u * S;        // [S] the MMAs that read the stage are done
+  const uint32_t ready = done + 8u * S;       // [S] first CTA: both CTAs' halves have landed
+  const uint32_t acc_full = ready + 8u * S;   // [2] an item's sums are complete
+  const uint32_t acc_free = acc_full + 16u;   // [2] first CTA: both CTAs have read them
+  const uint32_t drain = acc_free + 16u;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * S + 5);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = ptx::cluster_rank();
+  const int row_tiles = (a.rows + kPairRows - 1) / kPairRows, pairs = (a.tiles + 1) / 2;
+  const long long items = (long long)row_tiles * pairs, step = gridDim.x / 2;
+  struct Item { int tile, row; };  // this CTA's weight tile and first row
+  auto item_of = [&](long long i) {
+    const long long band = (long long)kPairBand * pairs;
+    const int b = (int)(i / band), rest = (int)(i - b * band), high = min(kPairBand, row_tiles - b * kPairBand);
+    return Item{2 * (rest / high) + (int)rank, (b * kPairBand + rest % high) * kPairRows + (int)rank * kI8Tile};
+  };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      ptx::mbar_init(&bars[s], 1);
+      ptx::mbar_init(&bars[S + s], 1);
+      ptx::mbar_init(&bars[2 * S + s], 2);
+    }
+    for (int q = 0; q < 2; ++q) {
+      ptx::mbar_init(&bars[3 * S + q], 1);
+      ptx::mbar_init(&bars[3 * S + 2 + q], 16);
+    }
+    ptx::mbar_init(&bars[3 * S + 4], 1);
+    ptx::mbar_fence_init();
+  }
+  __syncthreads();
+  wait_previous();
+  ptx::cluster_sync();  // both CTAs' barriers are there
+  if (warp == 1) {
+    ptx::tmem_alloc2(tmem_slot, 512);
+    ptx::tmem_relinquish2();
+  }
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  ptx::tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  bool ok = true;
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t s = 0, ph = 1;
+      long long issued = 0;
+      for (long long i = blockIdx.x / 2; i < items && ok; i += step) {
+        const Item it = item_of(i);
+        // (what does not exist is not loaded: its products go nowhere)
+        const bool rows_there = it.row < a.rows, tile_there = it.tile < a.tiles;
+        const signed char* rows = a.q + (size_t)(it.row / kI8Tile) * a.chunks * kI8Block;
+        const signed char* weights = a.w + (size_t)it.tile * a.chunks * kI8Block;
+        for (int c = 0; c < a.chunks; ++c) {
+          ok = ptx::mbar_wait_addr(done + 8u * s, ph);
+          if (!ok) break;
+          const uint32_t at = smem_u + s * kPairStage, bar = full + 8u * s;
+          ptx::mbar_expect_tx_addr(bar, (rows_there ? kI8Block : 0) + (tile_there ? kI8Block : 0));
+          if (rows_there) ptx::bulk_g2s_addr(at, rows + (size_t)c * kI8Block, kI8Block, bar);
+          if (tile_there) ptx::bulk_g2s_addr(at + kI8Block, weights + (size_t)c * kI8Block, kI8Block, bar);
+          ++issued;
+          if (++s == (uint32_t)S) { s = 0; ph ^= 1u; }
+        }
+      }
+      let_next_start();
+      if (!ok)  // copies are on their way into this memory
+        for (long long i = issued > S ? issued - S : 0; i < issued; ++i) ptx::mbar_wait_addr(full + 8u * (uint32_t)(i % S), (uint32_t)(i / S) & 1u);
+    }
+  } else if (warp == 2) {
+    if (lane == 0) {
+      const uint32_t to = ptx::map_to_rank(ready, 0);
+      uint32_t s = 0, ph = 0;
+      for (long long i = blockIdx.x / 2; i < items && ok; i += step)
+        for (int c = 0; c < a.chunks; ++c) {
+          ok = ptx::mbar_wait_addr(full + 8u * s, ph);
+          if (!ok) break;
+          ptx::mbar_arrive_cluster(to + 8u * s);
+          if (++s == (uint32_t)S) { s = 0; ph ^= 1u; }
+        }
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && ptx::elect_one()) {
+      const uint32_t idesc = idesc_i8(2 * kI8Tile, 2 * kI8Tile);
+      uint32_t s = 0, ph = 0, n_item = 0;
+      for (long long i = blockIdx.x / 2; i < items && ok; i += step, ++n_item) {
+        const uint32_t set = n_item & 1u, acc = tmem + set * 256u;
+        if (n_item >= 2) ok = ptx::mbar_wait_cluster(acc_free + 8u * set, ((n_item >> 1) - 1u) & 1u);
+        if (!ok) break;
+        ptx::tc_fence_after_sync();
+        for (int c = 0; c < a.chunks; ++c) {
+          ok = ptx::mbar_wait_cluster(ready + 8u * s, ph);
+          if (!ok) break;
+          ptx::tc_fence_after_sync();
+          const uint64_t da = ptx::umma_desc_k_sw128(smem_u + s * kPairStage), db = ptx::umma_desc_k_sw128(smem_u + s * kPairStage + kI8Block);
+#pragma unroll
+          for (int k4 = 0; k4 < 4; ++k4) umma2_i8(acc, da + 2 * k4, db + 2 * k4, idesc, (c > 0 || k4 > 0) ? 1u : 0u);
+          ptx::umma2_commit(done + 8u * s);
+          if (++s == (uint32_t)S) { s = 0; ph ^= 1u; }
+        }
+        if (ok) ptx::umma2_commit(acc_full + 8u * set);
+      }
+      if (!ok) {  // the MMAs on the way read both CTAs' shared memory
+        ptx::umma2_commit(drain);
+        ptx::mbar_wait_addr(drain, 0);
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // A lane is a row; 32 columns at a time go through shared memory, so that a store is a row's 64 or 128 contiguous bytes.
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    float* mine = staging + (warp - 4) * 32 * kPairPitch;
+    const uint32_t to = ptx::map_to_rank(acc_free, 0);
+    uint32_t n_item = 0;
+    for (long long i = blockIdx.x / 2; i < items; i += step, ++n_item) {
+      const Item it = item_of(i);
+      const uint32_t set = n_item & 1u;
+      const int row0 = it.row + quarter * 32, first = it.tile - (int)rank;  // the item's first weight tile
+      const float row_step = row0 + lane < a.rows ? a.step[row0 + lane] : 0.f;
+      ok = ptx::mbar_wait_addr(acc_full + 8u * set, (n_item >> 1) & 1u);
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      ptx::tc_fence_after_sync();
+      const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + set * 256u;
+      const int rows_here = min(32, a.rows - row0);
+      const int c_end = GATED ? half * 64 + 64 : half * 128 + 128;
+      for (int c0 = GATED ? half * 64 : half * 128; c0 < c_end; c0 += 32) {
+        const int n0 = (GATED ? first / 2 : first) * kI8Tile + c0;
+        if (n0 >= a.n || rows_here <= 0) break;
+        uint32_t v[32], u[32];
+        ptx::tmem_ld32(acc + (uint32_t)c0, v);
+        if constexpr (GATED) ptx::tmem_ld32(acc + (uint32_t)(kI8Tile + c0), u);
+        ptx::tmem_ld_wait();
+        const float4* ws = reinterpret_cast<const float4*>(a.w_scale + (size_t)first * kI8Tile + c0);
+#pragma unroll
+        for (int j4 = 0; j4 < 8; ++j4) {
+          const float4 w4 = ws[j4], u4 = GATED ? ws[j4 + kI8Tile / 4] : make_float4(0.f, 0.f, 0.f, 0.f);
+          float b[4] = {0.f, 0.f, 0.f, 0.f};
+          if (!GATED && a.bias) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) b[e] = n0 + 4 * j4 + e < a.n ? a.bias[n0 + 4 * j4 + e] : 0.f;
+          }
+          const float w[4] = {w4.x, w4.y, w4.z, w4.w}, up[4] = {u4.x, u4.y, u4.z, u4.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            v[4 * j4 + e] = __float_as_uint(output_of<GATED>(a, (int)v[4 * j4 + e], GATED ? (int)u[4 * j4 + e] : 0, w[e], up[e], row_step, b[e]));
+        }
+        const int cols = min(32, a.n - n0);
+        if (GATED || a.y_f32) {
+#pragma unroll
+          for (int x = 0; x < 32; x += 16) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<uint4*>(mine + lane * kPairPitch + 4 * q) = make_uint4(v[x + 4 * q], v[x + 4 * q + 1], v[x + 4 * q + 2], v[x + 4 * q + 3]);
+            __syncwarp();
+            float* y = reinterpret_cast<float*>(a.y) + (size_t)row0 * a.y_stride + n0 + x;
+            if (a.y_vec && cols == 32) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const int r = q * 8 + (lane >> 2), c = (lane & 3) * 4;
+                if (r < rows_here) *reinterpret_cast<float4*>(y + (size_t)r * a.y_stride + c) = *reinterpret_cast<const float4*>(mine + r * kPairPitch + c);
+              }
+            } else if (x + (lane & 15) < cols) {
+              for (int r = lane >> 4; r < rows_here; r += 2) y[(size_t)r * a.y_stride + (lane & 15)] = mine[r * kPairPitch + (lane & 15)];
+            }
+            __syncwarp();
+          }
+        } else {
+          uint32_t* words = reinterpret_cast<uint32_t*>(mine);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t h[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(v[8 * q + 2 * e]), __uint_as_float(v[8 * q + 2 * e + 1]));
+              h[e] = *reinterpret_cast<const uint32_t*>(&b);
+            }
+            *reinterpret_cast<uint4*>(words + lane * kPairPitch + 4 * q) = make_uint4(h[0], h[1], h[2], h[3]);
+          }
+          __syncwarp();
+          __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(a.y) + (size_t)row0 * a.y_stride + n0;
+          if (a.y_vec && cols == 32) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int r = q * 8 + (lane >> 2), c = (lane & 3) * 4;
+              if (r < rows_here) *reinterpret_cast<uint4*>(y + (size_t)r * a.y_stride + 2 * c) = *reinterpret_cast<const uint4*>(words + r * kPairPitch + c);
+            }
+          } else if (lane < cols) {
+            for (int r = 0; r < rows_here; ++r) y[(size_t)r * a.y_stride + lane] = reinterpret_cast<const __nv_bfloat16*>(words + r * kPairPitch)[lane];
+          }
+        }
+        __syncwarp();
+      }
+      // all that this warp reads of the item's sums has been read
+      ptx::tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster_relaxed(to + 8u * set);
+    }
+  }
+  if (!ok) atomicExch(a.err, B200_ERR_DEVICE_FLAGGED);
+  __syncwarp();
+  ptx::tc_fence_before_sync();
+  ptx::cluster_sync();  // nobody leaves while its memory may be read or arrived on
+  if (warp == 1) ptx::tmem_dealloc2(tmem, 512);
 }
 
 // A launch in clusters of `size` (1: none) whose start-up overlaps the end of the kernel ahead.
@@ -407,12 +640,29 @@ b200_status launch_stream(MmArgs& a, cudaStream_t s) {
   return B200_OK;
 }
 
+template <bool GATED>
+b200_status launch_pair(MmArgs& a, cudaStream_t s) {
+  static int most_pairs = 0;
+  if (most_pairs == 0) {
+    B200_CUDA_TRY(cudaFuncSetAttribute(i8_pair_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairShared));
+    const int n = ctas_in_clusters(i8_pair_kernel<GATED>, 2, 1, b200_sm_count(), kPairThreads, kPairShared) / 2;
+    if (n < 1) { b200_set_error("i8: no pair of CTAs fits the device"); return B200_ERR_CAPACITY; }
+    most_pairs = n;
+  }
+  const long long items = (long long)((a.rows + kPairRows - 1) / kPairRows) * ((a.tiles + 1) / 2);
+  launch_clusters(i8_pair_kernel<GATED>, 2, dim3((unsigned)(2 * std::min<long long>(items, most_pairs))), kPairThreads, kPairShared, s, a);
+  B200_LAUNCH_CHECK();
+  return B200_OK;
+}
+
 b200_status product(const b200_i8_weight* w, const I8RowsDev& x, int rows, const float* bias, int act, void* y, long long y_stride, int y_f32, cudaStream_t s) {
   MmArgs a{};
   b200_status st = b200_qmm_ensure_err_word(&a.err);
   if (st != B200_OK) return st;
   a.w = w->q; a.w_scale = w->scale; a.q = x.q; a.step = x.scale; a.bias = bias; a.y = y; a.y_stride = y_stride; a.y_f32 = y_f32; a.act = act;
   a.rows = rows; a.n = w->n; a.chunks = w->chunks; a.tiles = w->tiles;
+  a.y_vec = ((uintptr_t)y & 15) == 0 && y_stride * (w->gated || y_f32 ? 4 : 2) % 16 == 0;
+  if (rows > 256) return w->gated ? launch_pair<true>(a, s) : launch_pair<false>(a, s);
   return w->gated ? launch_stream<true>(a, s) : launch_stream<false>(a, s);
 }
 
