@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import array
 import ctypes as C
+import functools
 import math
 import operator
 from typing import List, Optional, Sequence
@@ -338,19 +339,21 @@ class LayeredKVCache(PagedKVCache):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-def _rows(t: torch.Tensor, shape: tuple, device: int, dtype: torch.dtype = torch.bfloat16) -> int:
+_BF16, _F32 = torch.bfloat16, torch.float32
+
+
+def _rows(t: torch.Tensor, shape: tuple, device: int, dtype: torch.dtype = _BF16) -> int:
     """Checks rows of a type (bf16) on the device whose numbers lie one behind the other within a row; returns the elements between rows."""
     if t.dtype != dtype or t.shape != shape or t.get_device() != device:
         raise ValueError(f"expected {str(dtype)[6:]} rows of shape {shape} on the current device, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    inner = math.prod(shape[1:])
     if t.is_contiguous():
-        return inner
+        return shape[1] if len(shape) == 2 else math.prod(shape[1:])
     width = 1
     for n, stride in zip(reversed(shape[1:]), reversed(t.stride()[1:])):
         if n > 1 and stride != width:
             raise ValueError(f"the numbers of a row are not contiguous: strides {t.stride()}")
         width *= n
-    return t.stride(0) if shape[0] > 1 else inner
+    return t.stride(0) if shape[0] > 1 else width
 
 
 def _ints(t: torch.Tensor, n: int, device: int) -> int:
@@ -362,7 +365,7 @@ def _ints(t: torch.Tensor, n: int, device: int) -> int:
 def _weight(w: Optional[torch.Tensor], d: int, device: int) -> Optional[int]:
     if w is None:
         return None
-    if w.dtype != torch.bfloat16 or w.shape != (d,) or w.get_device() != device or not w.is_contiguous():
+    if w.dtype != _BF16 or w.shape != (d,) or w.get_device() != device or not w.is_contiguous():
         raise ValueError(f"expected {d} contiguous bf16 weights on the current device, got {w.dtype} {tuple(w.shape)} on {w.device}")
     return w.data_ptr()
 
@@ -555,11 +558,13 @@ class I8Rows:
         return x.data_ptr(), _rows(x, (t, k), device), t
 
 
-def _out_rows(out: Optional[torch.Tensor], t: int, n: int, dtype: torch.dtype, device: int):
-    """(out, stride): a new tensor, or the caller's (rows may be strided)."""
-    if out is None:
-        return torch.empty((t, n), dtype=dtype, device="cuda"), n
-    return out, _rows(out, (t, n), device, dtype)
+def _new_rows(t: int, n: int, dtype: torch.dtype, device: int) -> torch.Tensor:
+    return torch.empty((t, n), dtype=dtype, device=_device(device))
+
+
+@functools.lru_cache(maxsize=None)
+def _device(index: int) -> torch.device:
+    return torch.device("cuda", index)
 
 
 def i8_mm(w: I8Weight, rows: I8Rows, x: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
@@ -569,7 +574,11 @@ def i8_mm(w: I8Weight, rows: I8Rows, x: Optional[torch.Tensor] = None, bias: Opt
     at, stride, t = rows._take(x, w.k, device)
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (w.n,) or bias.get_device() != device or not bias.is_contiguous()):
         raise ValueError(f"expected a bias of {w.n} contiguous f32 on the current device, got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
-    out, out_stride = _out_rows(out, t, w.n, torch.float32 if f32 else torch.bfloat16, device)
+    dtype, out_stride = _F32 if f32 else _BF16, w.n
+    if out is None:
+        out = _new_rows(t, w.n, dtype, device)
+    else:
+        out_stride = _rows(out, (t, w.n), device, dtype)
     _lib.check(lib.b200_i8_mm(w._h, rows._h, at, stride, t, None if bias is None else bias.data_ptr(), out.data_ptr(), out_stride, f32, _raw_stream(device)))
     rows.rows, rows.k = t, w.k
     return out
@@ -583,7 +592,11 @@ def i8_ffn(gate_up: I8Weight, down: I8Weight, rows: I8Rows, x: Optional[torch.Te
     """b200_i8_ffn: down(act(gate x) * (up x)), the rows in 8 bits in front of each product.  x as in i8_mm."""
     device = torch.cuda.current_device()
     at, stride, t = rows._take(x, gate_up.k, device)
-    out, out_stride = _out_rows(out, t, down.n, torch.bfloat16, device)
+    out_stride = down.n
+    if out is None:
+        out = _new_rows(t, down.n, _BF16, device)
+    else:
+        out_stride = _rows(out, (t, down.n), device)
     _lib.check(lib.b200_i8_ffn(gate_up._h, down._h, rows._h, at, stride, t, ACTIVATIONS[activation], out.data_ptr(), out_stride, _raw_stream(device)))
     rows.rows, rows.k = t, gate_up.k
     return out
@@ -594,24 +607,38 @@ def residual_norm(h: torch.Tensor, y: torch.Tensor, norm_weight: Optional[torch.
                   x_out: Optional[torch.Tensor] = None, rows: Optional[I8Rows] = None):
     """b200_residual_norm: h + scale * gate * norm(y), and the norm of that for the next block.  h, y [T, n] bf16 or f32, gate bf16 [n] or [T, n] (rows may be
     strided), a weight that is None is no norm.  Returns (h, x): x bf16, or None where it goes into `rows` in 8 bits.  h_out may be h."""
-    device, shape = torch.cuda.current_device(), tuple(h.shape)
+    device, shape = torch.cuda.current_device(), h.shape
     t, n = shape
-    h_out = torch.empty(shape, dtype=h.dtype, device="cuda") if h_out is None else h_out
-    if rows is None and x_out is None:
-        x_out = torch.empty(shape, dtype=torch.bfloat16, device="cuda")
-    gate_stride = 0
+    h_type, y_type = _F32 if h.dtype == _F32 else _BF16, _F32 if y.dtype == _F32 else _BF16
+    h_stride, y_stride = _rows(h, shape, device, h_type), _rows(y, shape, device, y_type)
+    gate_at = x_at = None
+    gate_stride = h_out_stride = x_out_stride = n
     if gate is not None:
-        gate_stride = _rows(gate, shape, device) if gate.dim() == 2 else (_weight(gate, n, device), 0)[1]
-    f32 = torch.float32
-    as_c = _lib.ResidualNormShape(n, h.dtype == f32, y.dtype == f32, gate_sigmoid, scale, eps)
-    kind = lambda v: f32 if v.dtype == f32 else torch.bfloat16  # noqa: E731
-    _lib.check(lib.b200_residual_norm(C.byref(as_c), h.data_ptr(), _rows(h, shape, device, kind(h)), y.data_ptr(), _rows(y, shape, device, kind(y)),
-                                      None if gate is None else gate.data_ptr(), gate_stride, _weight(post_weight, n, device), _weight(norm_weight, n, device), t,
-                                      h_out.data_ptr(), _rows(h_out, shape, device, kind(h)), None if x_out is None else x_out.data_ptr(),
-                                      0 if x_out is None else _rows(x_out, shape, device), None if rows is None else rows._h, _raw_stream(device)))
+        if gate.dim() == 2:
+            gate_at, gate_stride = gate.data_ptr(), _rows(gate, shape, device)
+        else:
+            gate_at, gate_stride = _weight(gate, n, device), 0
+    if h_out is None:
+        h_out = torch.empty_like(h) if h.is_contiguous() else _new_rows(t, n, h_type, device)
+    else:
+        h_out_stride = _rows(h_out, shape, device, h_type)
+    if x_out is not None:
+        x_out_stride = _rows(x_out, shape, device)
+    elif rows is None:
+        x_out = torch.empty_like(h_out) if h_type is _BF16 and h_out.is_contiguous() else _new_rows(t, n, _BF16, device)
+    if x_out is not None:
+        x_at = x_out.data_ptr()
+    _lib.check(lib.b200_residual_norm(_norm_shape(n, h_type is _F32, y_type is _F32, gate_sigmoid, scale, eps), h.data_ptr(), h_stride, y.data_ptr(), y_stride,
+                                      gate_at, gate_stride, _weight(post_weight, n, device), _weight(norm_weight, n, device), t, h_out.data_ptr(), h_out_stride, x_at,
+                                      x_out_stride, None if rows is None else rows._h, _raw_stream(device)))
     if rows is not None:
         rows.rows, rows.k = t, n
     return h_out, x_out
+
+
+@functools.lru_cache(maxsize=256)
+def _norm_shape(n: int, h_f32: bool, y_f32: bool, gate_sigmoid: bool, scale: float, eps: float):
+    return C.byref(_lib.ResidualNormShape(n, h_f32, y_f32, gate_sigmoid, scale, eps))
 
 
 def set_attn_pages_per_chunk(n: int):
