@@ -141,6 +141,7 @@ struct MmArgs {
   long long y_stride;
   int* err;
   int rows, n, chunks, tiles, tn, stages, shares;
+  int over_stages, pushed_at, bars_at;  // places in shared memory (i8_stream_kernel)
   int y_vec;       // rows of y start on 16 bytes
   int y_f32, act;  // (a feed-forward block's inner rows are f32)
 };
@@ -176,45 +177,59 @@ __device__ __forceinline__ float output_of(const MmArgs& a, int sum, int up, flo
 // A weight tile (gated: the gate's and up's tile of the same channels) by up to tn rows and a share of K per CTA.  The weights are the MMA's M, the rows
 // its N, so that few rows waste nothing; a lane of tensor memory is a channel.  Warp 0 loads, warp 1 multiplies, four bring the sums to the output.
 // Bound by the weights, which come at the rate of memory only if every SM asks for them: a cluster of up to eight CTAs shares K (as many as still run at
-// the same time, two CTAs on an SM), and each CTA adds up, over the cluster's shared memory, a share of the rows.
+// the same time, two CTAs on an SM).  Each of them brings a share of the rows to the output and gets the others' sums of these pushed into its
+// shared memory, where the stages were unless there is room beside them, with a barrier that counts their bytes.
 constexpr int kStreamThreads = 192, kStreamShared = 112 * 1024, kMostShares = 8;
 
-__device__ __forceinline__ int load_of_rank(uint32_t addr, uint32_t rank) {
-  int v;
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(ptx::map_to_rank(addr, rank)) : "memory");
-  return v;
+// Four words to another CTA of the cluster, counted by a barrier there.
+__device__ __forceinline__ void push4(uint32_t mapped, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t mapped_bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(mapped), "r"(a), "r"(b), "r"(c), "r"(d),
+               "r"(mapped_bar) : "memory");
 }
+// The rows that a CTA of the cluster brings to the output: CTA q the q-th so many, a multiple of four.
+__host__ __device__ constexpr int rows_per_rank(int rows_here, int shares) { return ((rows_here + shares - 1) / shares + 3) / 4 * 4; }
+// What it gets pushed: [other CTA][gate, up][four rows][channel][row].
+__host__ __device__ constexpr int pushed_bytes(int rows_here, int shares, int parts) { return (shares - 1) * parts * rows_per_rank(rows_here, shares) * kI8Tile * 4; }
 
-// The rows that a CTA of the cluster brings to the output: CTA q the q-th so many.
-__host__ __device__ constexpr int rows_per_rank(int tn, int rows_here, int shares) {
-  return tn <= 32 ? (rows_here + shares - 1) / shares : ((rows_here + shares - 1) / shares + 15) / 16 * 16;
+// Tensor memory of a CTA.  Those of a cluster wait for one another while they hold theirs, so a CTA on the same SM may never have to wait for its own: a
+// launch asks for at least kSharedPerCol bytes of shared memory a column, of which an SM's 228 KB (a KB of them for itself in every CTA) are 512 columns' at most.
+__host__ __device__ constexpr uint32_t stream_cols(int tn, int parts) { return tn * parts < 32 ? 32u : (uint32_t)(tn * parts); }
+constexpr int kSharedPerCol = 440;
+
+// Sums of four rows from `col` on, of this warp's 32 channels.
+__device__ __forceinline__ void tmem_ld4(uint32_t taddr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(taddr) : "memory");
 }
 
 template <bool GATED>
-__global__ void __launch_bounds__(kStreamThreads) i8_stream_kernel(MmArgs a) {
+__global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   constexpr int W = GATED ? 2 : 1;
   const int S = a.stages, stage_bytes = W * kI8Block + a.tn * kI8Chunk;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)S * stage_bytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + a.bars_at);
   uint64_t* done = full + S;
   uint64_t* sums = done + S;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sums + 1);
+  uint64_t* pushed = sums + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pushed + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int shares = a.shares, rank = shares > 1 ? (int)ptx::cluster_rank() : 0;
   const int tile = blockIdx.x / shares, t0 = blockIdx.y * a.tn, rows_here = min(a.tn, a.rows - t0), n_here = (rows_here + 15) / 16 * 16;
   const int per_share = (a.chunks + shares - 1) / shares, chunk0 = rank * per_share, chunks = min(per_share, a.chunks - chunk0);  // (never none)
-  uint32_t cols = 32;  // (the sums' 16 columns from any row on are there; from 64 rows on shares begin at a multiple of 16)
-  while (cols < (uint32_t)(W * a.tn + (a.tn <= 32 ? 16 : 0))) cols *= 2;
+  const int per_rank = rows_per_rank(rows_here, shares), mine0 = min(rows_here, rank * per_rank), mine1 = min(rows_here, mine0 + per_rank);
+  const uint32_t cols = stream_cols(a.tn, W);
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       ptx::mbar_init(&full[s], 1);
       ptx::mbar_init(&done[s], 1);
     }
     ptx::mbar_init(sums, 1);
+    ptx::mbar_init(pushed, 1);
     ptx::mbar_fence_init();
+    ptx::mbar_expect_tx(pushed, (shares - 1) * W * ((mine1 - mine0 + 3) / 4) * kI8Tile * 16);
   }
   __syncthreads();
+  if (shares > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this CTA's barriers are there
   auto load_weights = [&](int i, int s) {
     ptx::mbar_expect_tx(&full[s], W * kI8Block + n_here * kI8Chunk);
     for (int h = 0; h < W; ++h)
@@ -240,12 +255,6 @@ __global__ void __launch_bounds__(kStreamThreads) i8_stream_kernel(MmArgs a) {
   ptx::tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
   bool ok = true;
-  const int quarter = warp & 3, channel = tile * kI8Tile + quarter * 32 + lane;
-  const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
-  const int per_rank = rows_per_rank(a.tn, rows_here, shares);
-  auto first_of = [&](int q) { return min(rows_here, q * per_rank); };
-  int* parts = reinterpret_cast<int*>(smem);  // [gate, up][row of another's][channel]: this CTA's sums for the others, where the stages were
-  const int mine0 = first_of(rank), mine1 = first_of(rank + 1);
   if (warp == 0) {
     if (lane == 0) {
       int s = 0, issued = 0;
@@ -289,49 +298,69 @@ __global__ void __launch_bounds__(kStreamThreads) i8_stream_kernel(MmArgs a) {
       if (!ok) ptx::mbar_wait(sums, 0);
     }
     __syncwarp();
-  } else {
+  }
+  const int quarter = warp & 3, channel = tile * kI8Tile + quarter * 32 + lane;
+  const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
+  float ws = 0.f, us = 0.f, bias = 0.f, steps = 0.f;
+  auto steps_of = [&](int c0) { return c0 + (lane & 15) < mine1 ? a.step[t0 + c0 + (lane & 15)] : 0.f; };  // sixteen rows' in the lanes
+  if (warp >= 2) {
+    const size_t scale_at = (size_t)tile * W * kI8Tile + quarter * 32 + lane;
+    ws = a.w_scale[scale_at];
+    if (GATED) us = a.w_scale[scale_at + kI8Tile];
+    if (!GATED && a.bias && channel < a.n) bias = a.bias[channel];
+    steps = steps_of(mine0);
     ok = ptx::mbar_wait(sums, 0);
     ok = __all_sync(0xffffffffu, ok);
     ptx::tc_fence_after_sync();
-    if (ok && shares > 1) {
-      const int others = rows_here - (mine1 - mine0);
+  }
+  if (shares > 1) {
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the others' barriers are there
+    if (a.over_stages) ptx::cluster_sync();                              // nobody's stages are in use
+    if (warp >= 2 && ok) {
+      int q = 0, next = per_rank;  // whose the rows are
       for (int c0 = 0; c0 < rows_here; c0 += 16) {
         uint32_t v[16], u[16];
         ptx::tmem_ld16(acc + c0, v);
         if constexpr (GATED) ptx::tmem_ld16(acc + a.tn + c0, u);
         ptx::tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int row = c0 + j;
-          if (row >= rows_here || (row >= mine0 && row < mine1)) continue;
-          int* to = parts + (row < mine0 ? row : row - (mine1 - mine0)) * kI8Tile + quarter * 32 + lane;
-          to[0] = (int)v[j];
-          if constexpr (GATED) to[others * kI8Tile] = (int)u[j];
+        for (int g = 0; g < 16; g += 4) {
+          const int row = c0 + g;
+          if (row >= next) { ++q; next += per_rank; }
+          if (row >= rows_here || q == rank) continue;
+          const int at = ((rank - (rank > q)) * W * (per_rank / 4) + (row + per_rank - next) / 4) * kI8Tile + quarter * 32 + lane;
+          const uint32_t to = ptx::map_to_rank(ptx::smem_u32(smem + a.pushed_at + at * 16), q), bar = ptx::map_to_rank(ptx::smem_u32(pushed), q);
+          push4(to, v[g], v[g + 1], v[g + 2], v[g + 3], bar);
+          if constexpr (GATED) push4(to + per_rank / 4 * kI8Tile * 16, u[g], u[g + 1], u[g + 2], u[g + 3], bar);
         }
       }
     }
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   }
-  if (shares > 1) ptx::cluster_sync();  // all sums are there
-  if (warp >= 2 && ok) {
-    const size_t scale_at = (size_t)tile * W * kI8Tile + quarter * 32 + lane;
-    const float ws = a.w_scale[scale_at], us = GATED ? a.w_scale[scale_at + kI8Tile] : 0.f;
-    const float bias = !GATED && a.bias && channel < a.n ? a.bias[channel] : 0.f;
-    for (int c0 = mine0; c0 < mine1; c0 += 16) {
+  if (warp >= 2 && ok && mine0 < mine1) {
+    if (shares > 1) ok = __all_sync(0xffffffffu, ptx::mbar_wait(pushed, 0));
+    for (int c0 = mine0; c0 < mine1 && ok; c0 += 16) {
       uint32_t v[16], u[16];
-      const float steps = c0 + (lane & 15) < mine1 ? a.step[t0 + c0 + (lane & 15)] : 0.f;  // (ahead of the stores, which loads do not pass)
-      ptx::tmem_ld16(acc + c0, v);
-      if constexpr (GATED) ptx::tmem_ld16(acc + a.tn + c0, u);
-      ptx::tmem_ld_wait();
-      for (int q = 0; q < shares; ++q) {
-        if (q == rank) continue;
-        const int q0 = first_of(q), qn = first_of(q + 1) - q0, others = rows_here - qn;
-        const uint32_t from = ptx::smem_u32(parts + (c0 < q0 ? c0 : c0 - qn) * kI8Tile + quarter * 32 + lane);
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (c0 + j < mine1) {
-            v[j] += (uint32_t)load_of_rank(from + j * kI8Tile * 4, q);
-            if constexpr (GATED) u[j] += (uint32_t)load_of_rank(from + (others + j) * kI8Tile * 4, q);
+      for (int g = 0; g < 16; g += 4)
+        if (c0 + g < mine1) {
+          tmem_ld4(acc + c0 + g, v[g], v[g + 1], v[g + 2], v[g + 3]);
+          if constexpr (GATED) tmem_ld4(acc + a.tn + c0 + g, u[g], u[g + 1], u[g + 2], u[g + 3]);
+        }
+      ptx::tmem_ld_wait();
+      const uint4* from = reinterpret_cast<const uint4*>(smem + a.pushed_at) + (c0 - mine0) / 4 * kI8Tile + quarter * 32 + lane;
+      for (int q = 0; q < shares - 1; ++q, from += W * (per_rank / 4) * kI8Tile) {
+#pragma unroll
+        for (int g = 0; g < 16; g += 4) {
+          if (c0 + g >= mine1) break;
+          const uint4 p = from[g / 4 * kI8Tile];
+          v[g] += p.x; v[g + 1] += p.y; v[g + 2] += p.z; v[g + 3] += p.w;
+          if constexpr (GATED) {
+            const uint4 p2 = from[(per_rank / 4 + g / 4) * kI8Tile];
+            u[g] += p2.x; u[g + 1] += p2.y; u[g + 2] += p2.z; u[g + 3] += p2.w;
           }
+        }
       }
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
@@ -342,13 +371,14 @@ __global__ void __launch_bounds__(kStreamThreads) i8_stream_kernel(MmArgs a) {
         if (GATED || a.y_f32) reinterpret_cast<float*>(a.y)[at] = y;
         else reinterpret_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16(y);
       }
+      steps = steps_of(c0 + 16);
     }
   }
   if (!ok) atomicExch(a.err, B200_ERR_DEVICE_FLAGGED);
   __syncwarp();
   ptx::tc_fence_before_sync();
-  if (shares > 1) ptx::cluster_sync();  // nobody leaves while its sums may be read
-  else __syncthreads();
+  if (shares > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // nobody leaves while something may be pushed to it
+  __syncthreads();
   if (warp == 1) ptx::tmem_dealloc(tmem, cols);
 }
 
@@ -607,35 +637,29 @@ b200_status launch_stream(MmArgs& a, cudaStream_t s) {
   static int at_once[kMostShares + 1] = {};  // CTAs that run at the same time, by the cluster's size
   if (at_once[1] == 0) {
     B200_CUDA_TRY(cudaFuncSetAttribute(i8_stream_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamShared));
-    for (int size = kMostShares; size > 0; --size) at_once[size] = ctas_in_clusters(i8_stream_kernel<GATED>, size, 2, b200_sm_count(), kStreamThreads, kStreamShared);
+    for (int size = kMostShares; size > 0; --size) {
+      // (the occupancy calculation counts one CTA of a kernel that allocates tensor memory to an SM; this one takes half of that memory at most)
+      at_once[size] = 2 * ctas_in_clusters(i8_stream_kernel<GATED>, size, 1, b200_sm_count(), kStreamThreads, kStreamShared);
+    }
   }
   const int most = GATED ? 128 : 256;
   a.tn = 16;
   while (a.tn < most && a.tn < a.rows) a.tn *= 2;
   const int tiles = a.tiles / W, row_tiles = (a.rows + a.tn - 1) / a.tn;
-  const int stage = W * kI8Block + a.tn * kI8Chunk, room = kStreamShared - 2048;
-  // Sums that go to the cluster's other CTAs, in bytes; they lie where the stages were.
-  auto parts = [&](int shares) {
-    size_t most = 0;
-    for (int rows_here : {std::min(a.rows, a.tn), a.rows - (row_tiles - 1) * a.tn}) {
-      const int per = rows_per_rank(a.tn, rows_here, shares);
-      for (int q = 0; q < shares; ++q) {
-        const int own = std::min(rows_here, (q + 1) * per) - std::min(rows_here, q * per);
-        most = std::max(most, (size_t)W * (rows_here - own) * kI8Tile * 4);
-      }
-    }
-    return most;
-  };
+  const int stage = W * kI8Block + a.tn * kI8Chunk, room = kStreamShared - 2048, rows_most = std::min(a.rows, a.tn);
   // As many shares of K as still run at once, each of two blocks or more.
   a.shares = 1;
   for (int n = 2; n <= kMostShares && a.chunks >= 2 * n; ++n) {
     const int per = (a.chunks + n - 1) / n;
-    if ((long long)tiles * row_tiles * n <= at_once[n] && (n - 1) * per < a.chunks && (parts(n) + stage - 1) / stage * stage <= (size_t)room) a.shares = n;
+    if ((long long)tiles * row_tiles * n <= at_once[n] && (n - 1) * per < a.chunks && pushed_bytes(rows_most, n, W) <= room) a.shares = n;
   }
-  const int per_share = (a.chunks + a.shares - 1) / a.shares;
-  a.stages = std::min(per_share, room / stage);
-  while (a.shares > 1 && (size_t)a.stages * stage < parts(a.shares)) ++a.stages;
-  launch_clusters(i8_stream_kernel<GATED>, a.shares, dim3(tiles * a.shares, row_tiles), kStreamThreads, (size_t)a.stages * stage + 2048, s, a);
+  const int per_share = (a.chunks + a.shares - 1) / a.shares, pushed = pushed_bytes(rows_most, a.shares, W);
+  // What is pushed has a place beside the stages where that is a quarter of the room at most.
+  a.over_stages = pushed > room / 4;
+  a.stages = std::min(per_share, (room - (a.over_stages ? 0 : pushed)) / stage);
+  a.pushed_at = a.over_stages ? 0 : a.stages * stage;
+  a.bars_at = std::max(a.stages * stage, a.pushed_at + pushed);
+  launch_clusters(i8_stream_kernel<GATED>, a.shares, dim3(tiles * a.shares, row_tiles), kStreamThreads, std::max<size_t>(a.bars_at + 2048, kSharedPerCol * stream_cols(a.tn, W)), s, a);
   B200_LAUNCH_CHECK();
   return B200_OK;
 }
