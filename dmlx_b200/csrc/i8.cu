@@ -383,15 +383,17 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
 }
 
 // ---- many rows: pairs of CTAs ----
-// Two CTAs (a cluster) share an MMA of 256 rows by 256 weight rows: each brings 128 of both and holds the sums of its 128 rows, so that an MMA reads 8 KiB of
-// each CTA's shared memory in the 128 cycles that it takes.  Persistent: a pair walks the items, a tile of rows by a pair of weight tiles (gated: the
-// gate's and up's of the same 128 channels), rows fastest within bands, so that both operands come from L2.  An item's sums are half of tensor
-// memory: eight warps drain one half while the MMAs fill the other.
-// Warps: 0 loads both operands of this CTA, 1 multiplies (in the first CTA), 2 tells the first CTA that this one's stage is complete, 4-11 bring the
+// Two CTAs share an MMA of 256 rows by 256 weight rows: each brings 128 of both and holds the sums of its 128 rows, so that an MMA reads 8 KiB of each CTA's
+// shared memory in the 128 cycles that it takes.  Persistent: a pair walks the items, a tile of rows by a pair of weight tiles (gated: the gate's and
+// up's of the same 128 channels), rows fastest within bands, so that both operands come from L2.  An item's sums are half of tensor memory: eight
+// warps drain one half while the MMAs fill the other.
+// Where there are fewer items than pairs, a cluster of up to four pairs shares an item's K, an item to a cluster: groups of 32 columns go to the pairs in
+// turn, and a CTA gets the others' sums of its groups pushed into its shared memory, where the stages were.
+// Warps: 0 loads both operands of this CTA, 1 multiplies (in a pair's first CTA), 2 tells the first CTA that this one's stage is complete, 4-11 bring the
 // sums to the output.
-constexpr int kPairThreads = 384, kPairStage = 2 * kI8Block, kPairStages = 6, kPairRows = 256, kPairBand = 16;
+constexpr int kPairThreads = 384, kPairStage = 2 * kI8Block, kPairStages = 6, kPairRows = 256, kPairBand = 16, kMostPairs = 4;
 constexpr int kPairPitch = 20;  // epilogue: words between rows in a warp's staging tile of 32 rows by 16 words
-constexpr int kPairShared = 1024 + kPairStages * kPairStage + 8 * 32 * kPairPitch * 4 + 8 * (3 * kPairStages + 5) + 16;
+constexpr int kPairShared = 1024 + kPairStages * kPairStage + 8 * 32 * kPairPitch * 4 + 8 * (3 * kPairStages + 6) + 16;
 
 __device__ __forceinline__ void umma2_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -401,12 +403,82 @@ __device__ __forceinline__ void umma2_i8(uint32_t tmem_d, uint64_t desc_a, uint6
       "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// ptx::umma2_commit in a cluster of several pairs.
+__device__ __forceinline__ void commit_pair(uint32_t bar, uint16_t ctas) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(ctas) : "memory");
+}
+
+// A warp's 32 rows by 32 columns from the item's column c0 on, whose sums are v (gated: with up's in u), to the output, through shared memory, so that a
+// store is 64 contiguous bytes of a row.
+template <bool GATED>
+__device__ __forceinline__ void store_sums(const MmArgs& a, uint32_t (&v)[32], const uint32_t (&u)[GATED ? 32 : 1], float* mine, int first_tile, int c0, int row0, float row_step) {
+  const int lane = threadIdx.x & 31, rows_here = min(32, a.rows - row0), n0 = (GATED ? first_tile / 2 : first_tile) * kI8Tile + c0, cols = min(32, a.n - n0);
+  if (cols <= 0 || rows_here <= 0) return;
+  const float4* ws = reinterpret_cast<const float4*>(a.w_scale + (size_t)first_tile * kI8Tile + c0);
+#pragma unroll
+  for (int j4 = 0; j4 < 8; ++j4) {
+    const float4 w4 = ws[j4], u4 = GATED ? ws[j4 + kI8Tile / 4] : make_float4(0.f, 0.f, 0.f, 0.f);
+    float b[4] = {0.f, 0.f, 0.f, 0.f};
+    if (!GATED && a.bias) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) b[e] = n0 + 4 * j4 + e < a.n ? a.bias[n0 + 4 * j4 + e] : 0.f;
+    }
+    const float w[4] = {w4.x, w4.y, w4.z, w4.w}, up[4] = {u4.x, u4.y, u4.z, u4.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      v[4 * j4 + e] = __float_as_uint(output_of<GATED>(a, (int)v[4 * j4 + e], GATED ? (int)u[4 * j4 + e] : 0, w[e], up[e], row_step, b[e]));
+  }
+  if (GATED || a.y_f32) {
+#pragma unroll
+    for (int x = 0; x < 32; x += 16) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<uint4*>(mine + lane * kPairPitch + 4 * q) = make_uint4(v[x + 4 * q], v[x + 4 * q + 1], v[x + 4 * q + 2], v[x + 4 * q + 3]);
+      __syncwarp();
+      float* y = reinterpret_cast<float*>(a.y) + (size_t)row0 * a.y_stride + n0 + x;
+      if (a.y_vec && cols == 32) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int r = q * 8 + (lane >> 2), c = (lane & 3) * 4;
+          if (r < rows_here) *reinterpret_cast<float4*>(y + (size_t)r * a.y_stride + c) = *reinterpret_cast<const float4*>(mine + r * kPairPitch + c);
+        }
+      } else if (x + (lane & 15) < cols) {
+        for (int r = lane >> 4; r < rows_here; r += 2) y[(size_t)r * a.y_stride + (lane & 15)] = mine[r * kPairPitch + (lane & 15)];
+      }
+      __syncwarp();
+    }
+  } else {
+    uint32_t* words = reinterpret_cast<uint32_t*>(mine);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t h[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(v[8 * q + 2 * e]), __uint_as_float(v[8 * q + 2 * e + 1]));
+        h[e] = *reinterpret_cast<const uint32_t*>(&b);
+      }
+      *reinterpret_cast<uint4*>(words + lane * kPairPitch + 4 * q) = make_uint4(h[0], h[1], h[2], h[3]);
+    }
+    __syncwarp();
+    __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(a.y) + (size_t)row0 * a.y_stride + n0;
+    if (a.y_vec && cols == 32) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int r = q * 8 + (lane >> 2), c = (lane & 3) * 4;
+        if (r < rows_here) *reinterpret_cast<uint4*>(y + (size_t)r * a.y_stride + 2 * c) = *reinterpret_cast<const uint4*>(words + r * kPairPitch + c);
+      }
+    } else if (lane < cols) {
+      for (int r = 0; r < rows_here; ++r) y[(size_t)r * a.y_stride + lane] = reinterpret_cast<const __nv_bfloat16*>(words + r * kPairPitch)[lane];
+    }
+    __syncwarp();
+  }
+}
 
 template <bool GATED>
 __global__ void __launch_bounds__(kPairThreads, 1) i8_pair_kernel(MmArgs a) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  constexpr int S = kPairStages;
+  constexpr int S = kPairStages, W = GATED ? 2 : 1, G = GATED ? 4 : 8;  // G: groups of 32 columns of an item
   float* staging = reinterpret_cast<float*>(smem + (size_t)S * kPairStage);
   uint64_t* bars = reinterpret_cast<uint64_t*>(staging + 8 * 32 * kPairPitch);
   const uint32_t smem_u = ptx::smem_u32(smem), full = ptx::smem_u32(bars);  // [S] this CTA's half of the stage has landed
@@ -415,17 +487,22 @@ __global__ void __launch_bounds__(kPairThreads, 1) i8_pair_kernel(MmArgs a) {
   const uint32_t acc_full = ready + 8u * S;   // [2] an item's sums are complete
   const uint32_t acc_free = acc_full + 16u;   // [2] first CTA: both CTAs have read them
   const uint32_t drain = acc_free + 16u;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * S + 5);
+  const uint32_t pushed = drain + 8u;         // the other pairs' sums are here
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * S + 6);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = ptx::cluster_rank();
+  const uint32_t in_cluster = ptx::cluster_rank(), rank = in_cluster & 1u, leader = in_cluster & ~1u;
+  const uint16_t both = (uint16_t)(3u << leader);
+  const int shares = a.shares, share = (int)in_cluster / 2;
+  const int per_share = (a.chunks + shares - 1) / shares, chunk0 = share * per_share, chunks = min(per_share, a.chunks - chunk0);  // (never none)
   const int row_tiles = (a.rows + kPairRows - 1) / kPairRows, pairs = (a.tiles + 1) / 2;
-  const long long items = (long long)row_tiles * pairs, step = gridDim.x / 2;
+  const long long items = (long long)row_tiles * pairs, first_item = blockIdx.x / (2 * shares), step = gridDim.x / (2 * shares);
   struct Item { int tile, row; };  // this CTA's weight tile and first row
   auto item_of = [&](long long i) {
     const long long band = (long long)kPairBand * pairs;
     const int b = (int)(i / band), rest = (int)(i - b * band), high = min(kPairBand, row_tiles - b * kPairBand);
     return Item{2 * (rest / high) + (int)rank, (b * kPairBand + rest % high) * kPairRows + (int)rank * kI8Tile};
   };
+  const int own_groups = (G - share + shares - 1) / shares, most_groups = (G + shares - 1) / shares;
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       ptx::mbar_init(&bars[s], 1);
@@ -437,11 +514,22 @@ __global__ void __launch_bounds__(kPairThreads, 1) i8_pair_kernel(MmArgs a) {
       ptx::mbar_init(&bars[3 * S + 2 + q], 16);
     }
     ptx::mbar_init(&bars[3 * S + 4], 1);
+    ptx::mbar_init(&bars[3 * S + 5], 1);
     ptx::mbar_fence_init();
+    ptx::mbar_expect_tx_addr(pushed, (uint32_t)((shares - 1) * own_groups * W) * kI8Block);
   }
   __syncthreads();
+  // (what does not exist is not loaded: its products go nowhere)
+  auto load_weights = [&](const Item& it, int c, uint32_t s) {
+    const bool rows_there = it.row < a.rows, tile_there = it.tile < a.tiles;
+    ptx::mbar_expect_tx_addr(full + 8u * s, (rows_there ? kI8Block : 0) + (tile_there ? kI8Block : 0));
+    if (tile_there) ptx::bulk_g2s_addr(smem_u + s * kPairStage + kI8Block, a.w + ((size_t)it.tile * a.chunks + chunk0 + c) * kI8Block, kI8Block, full + 8u * s);
+  };
+  const int ahead = min(S, chunks);  // weights asked for before the kernels ahead have ended
+  if (threadIdx.x == 0)
+    for (int c = 0; c < ahead; ++c) load_weights(item_of(first_item), c, (uint32_t)c);
   wait_previous();
-  ptx::cluster_sync();  // both CTAs' barriers are there
+  ptx::cluster_sync();  // all barriers are there
   if (warp == 1) {
     ptx::tmem_alloc2(tmem_slot, 512);
     ptx::tmem_relinquish2();
@@ -451,23 +539,24 @@ __global__ void __launch_bounds__(kPairThreads, 1) i8_pair_kernel(MmArgs a) {
   ptx::tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
   bool ok = true;
+  const int quarter = warp & 3, half = (warp - 4) >> 2;  // of the epilogue's warps
+  float* mine = staging + (warp - 4) * 32 * kPairPitch;
+  const uint32_t acc0 = tmem + ((uint32_t)(quarter * 32) << 16);
+  float row_step = 0.f;
   if (warp == 0) {
     if (lane == 0) {
       uint32_t s = 0, ph = 1;
       long long issued = 0;
-      for (long long i = blockIdx.x / 2; i < items && ok; i += step) {
+      for (long long i = first_item; i < items && ok; i += step) {
         const Item it = item_of(i);
-        // (what does not exist is not loaded: its products go nowhere)
-        const bool rows_there = it.row < a.rows, tile_there = it.tile < a.tiles;
-        const signed char* rows = a.q + (size_t)(it.row / kI8Tile) * a.chunks * kI8Block;
-        const signed char* weights = a.w + (size_t)it.tile * a.chunks * kI8Block;
-        for (int c = 0; c < a.chunks; ++c) {
-          ok = ptx::mbar_wait_addr(done + 8u * s, ph);
-          if (!ok) break;
-          const uint32_t at = smem_u + s * kPairStage, bar = full + 8u * s;
-          ptx::mbar_expect_tx_addr(bar, (rows_there ? kI8Block : 0) + (tile_there ? kI8Block : 0));
-          if (rows_there) ptx::bulk_g2s_addr(at, rows + (size_t)c * kI8Block, kI8Block, bar);
-          if (tile_there) ptx::bulk_g2s_addr(at + kI8Block, weights + (size_t)c * kI8Block, kI8Block, bar);
+        const signed char* rows = a.q + ((size_t)(it.row / kI8Tile) * a.chunks + chunk0) * kI8Block;
+        for (int c = 0; c < chunks; ++c) {
+          if (issued >= ahead) {
+            ok = ptx::mbar_wait_addr(done + 8u * s, ph);
+            if (!ok) break;
+            load_weights(it, c, s);
+          }
+          if (it.row < a.rows) ptx::bulk_g2s_addr(smem_u + s * kPairStage, rows + (size_t)c * kI8Block, kI8Block, full + 8u * s);
           ++issued;
           if (++s == (uint32_t)S) { s = 0; ph ^= 1u; }
         }
@@ -478,10 +567,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) i8_pair_kernel(MmArgs a) {
     }
   } else if (warp == 2) {
     if (lane == 0) {
-      const uint32_t to = ptx::map_to_rank(ready, 0);
+      const uint32_t to = ptx::map_to_rank(ready, leader);
       uint32_t s = 0, ph = 0;
-      for (long long i = blockIdx.x / 2; i < items && ok; i += step)
-        for (int c = 0; c < a.chunks; ++c) {
+      for (long long i = first_item; i < items && ok; i += step)
+        for (int c = 0; c < chunks; ++c) {
           ok = ptx::mbar_wait_addr(full + 8u * s, ph);
           if (!ok) break;
           ptx::mbar_arrive_cluster(to + 8u * s);
@@ -492,112 +581,48 @@ __global__ void __launch_bounds__(kPairThreads, 1) i8_pair_kernel(MmArgs a) {
     if (rank == 0 && ptx::elect_one()) {
       const uint32_t idesc = idesc_i8(2 * kI8Tile, 2 * kI8Tile);
       uint32_t s = 0, ph = 0, n_item = 0;
-      for (long long i = blockIdx.x / 2; i < items && ok; i += step, ++n_item) {
+      for (long long i = first_item; i < items && ok; i += step, ++n_item) {
         const uint32_t set = n_item & 1u, acc = tmem + set * 256u;
         if (n_item >= 2) ok = ptx::mbar_wait_cluster(acc_free + 8u * set, ((n_item >> 1) - 1u) & 1u);
         if (!ok) break;
         ptx::tc_fence_after_sync();
-        for (int c = 0; c < a.chunks; ++c) {
+        for (int c = 0; c < chunks; ++c) {
           ok = ptx::mbar_wait_cluster(ready + 8u * s, ph);
           if (!ok) break;
           ptx::tc_fence_after_sync();
           const uint64_t da = ptx::umma_desc_k_sw128(smem_u + s * kPairStage), db = ptx::umma_desc_k_sw128(smem_u + s * kPairStage + kI8Block);
 #pragma unroll
           for (int k4 = 0; k4 < 4; ++k4) umma2_i8(acc, da + 2 * k4, db + 2 * k4, idesc, (c > 0 || k4 > 0) ? 1u : 0u);
-          ptx::umma2_commit(done + 8u * s);
+          commit_pair(done + 8u * s, both);
           if (++s == (uint32_t)S) { s = 0; ph ^= 1u; }
         }
-        if (ok) ptx::umma2_commit(acc_full + 8u * set);
+        if (ok) commit_pair(acc_full + 8u * set, both);
       }
       if (!ok) {  // the MMAs on the way read both CTAs' shared memory
-        ptx::umma2_commit(drain);
+        commit_pair(drain, both);
         ptx::mbar_wait_addr(drain, 0);
       }
     }
     __syncwarp();
   } else if (warp >= 4) {
-    // A lane is a row; 32 columns at a time go through shared memory, so that a store is a row's 64 or 128 contiguous bytes.
-    const int quarter = warp & 3, half = (warp - 4) >> 2;
-    float* mine = staging + (warp - 4) * 32 * kPairPitch;
-    const uint32_t to = ptx::map_to_rank(acc_free, 0);
+    // A lane is a row.
+    const uint32_t to = ptx::map_to_rank(acc_free, leader);
     uint32_t n_item = 0;
-    for (long long i = blockIdx.x / 2; i < items; i += step, ++n_item) {
+    for (long long i = first_item; i < items; i += step, ++n_item) {
       const Item it = item_of(i);
       const uint32_t set = n_item & 1u;
-      const int row0 = it.row + quarter * 32, first = it.tile - (int)rank;  // the item's first weight tile
-      const float row_step = row0 + lane < a.rows ? a.step[row0 + lane] : 0.f;
+      const int row0 = it.row + quarter * 32;
+      row_step = row0 + lane < a.rows ? a.step[row0 + lane] : 0.f;
       ok = ptx::mbar_wait_addr(acc_full + 8u * set, (n_item >> 1) & 1u);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       ptx::tc_fence_after_sync();
-      const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + set * 256u;
-      const int rows_here = min(32, a.rows - row0);
-      const int c_end = GATED ? half * 64 + 64 : half * 128 + 128;
-      for (int c0 = GATED ? half * 64 : half * 128; c0 < c_end; c0 += 32) {
-        const int n0 = (GATED ? first / 2 : first) * kI8Tile + c0;
-        if (n0 >= a.n || rows_here <= 0) break;
-        uint32_t v[32], u[32];
-        ptx::tmem_ld32(acc + (uint32_t)c0, v);
-        if constexpr (GATED) ptx::tmem_ld32(acc + (uint32_t)(kI8Tile + c0), u);
+      if (shares > 1) break;
+      for (int g = half * (G / 2); g < half * (G / 2) + G / 2; ++g) {
+        uint32_t v[32], u[GATED ? 32 : 1];
+        ptx::tmem_ld32(acc0 + set * 256u + (uint32_t)(g * 32), v);
+        if constexpr (GATED) ptx::tmem_ld32(acc0 + set * 256u + (uint32_t)(kI8Tile + g * 32), u);
         ptx::tmem_ld_wait();
-        const float4* ws = reinterpret_cast<const float4*>(a.w_scale + (size_t)first * kI8Tile + c0);
-#pragma unroll
-        for (int j4 = 0; j4 < 8; ++j4) {
-          const float4 w4 = ws[j4], u4 = GATED ? ws[j4 + kI8Tile / 4] : make_float4(0.f, 0.f, 0.f, 0.f);
-          float b[4] = {0.f, 0.f, 0.f, 0.f};
-          if (!GATED && a.bias) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) b[e] = n0 + 4 * j4 + e < a.n ? a.bias[n0 + 4 * j4 + e] : 0.f;
-          }
-          const float w[4] = {w4.x, w4.y, w4.z, w4.w}, up[4] = {u4.x, u4.y, u4.z, u4.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            v[4 * j4 + e] = __float_as_uint(output_of<GATED>(a, (int)v[4 * j4 + e], GATED ? (int)u[4 * j4 + e] : 0, w[e], up[e], row_step, b[e]));
-        }
-        const int cols = min(32, a.n - n0);
-        if (GATED || a.y_f32) {
-#pragma unroll
-          for (int x = 0; x < 32; x += 16) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              *reinterpret_cast<uint4*>(mine + lane * kPairPitch + 4 * q) = make_uint4(v[x + 4 * q], v[x + 4 * q + 1], v[x + 4 * q + 2], v[x + 4 * q + 3]);
-            __syncwarp();
-            float* y = reinterpret_cast<float*>(a.y) + (size_t)row0 * a.y_stride + n0 + x;
-            if (a.y_vec && cols == 32) {
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const int r = q * 8 + (lane >> 2), c = (lane & 3) * 4;
-                if (r < rows_here) *reinterpret_cast<float4*>(y + (size_t)r * a.y_stride + c) = *reinterpret_cast<const float4*>(mine + r * kPairPitch + c);
-              }
-            } else if (x + (lane & 15) < cols) {
-              for (int r = lane >> 4; r < rows_here; r += 2) y[(size_t)r * a.y_stride + (lane & 15)] = mine[r * kPairPitch + (lane & 15)];
-            }
-            __syncwarp();
-          }
-        } else {
-          uint32_t* words = reinterpret_cast<uint32_t*>(mine);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t h[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(v[8 * q + 2 * e]), __uint_as_float(v[8 * q + 2 * e + 1]));
-              h[e] = *reinterpret_cast<const uint32_t*>(&b);
-            }
-            *reinterpret_cast<uint4*>(words + lane * kPairPitch + 4 * q) = make_uint4(h[0], h[1], h[2], h[3]);
-          }
-          __syncwarp();
-          __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(a.y) + (size_t)row0 * a.y_stride + n0;
-          if (a.y_vec && cols == 32) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int r = q * 8 + (lane >> 2), c = (lane & 3) * 4;
-              if (r < rows_here) *reinterpret_cast<uint4*>(y + (size_t)r * a.y_stride + 2 * c) = *reinterpret_cast<const uint4*>(words + r * kPairPitch + c);
-            }
-          } else if (lane < cols) {
-            for (int r = 0; r < rows_here; ++r) y[(size_t)r * a.y_stride + lane] = reinterpret_cast<const __nv_bfloat16*>(words + r * kPairPitch)[lane];
-          }
-        }
-        __syncwarp();
+        store_sums<GATED>(a, v, u, mine, it.tile - (int)rank, g * 32, row0, row_step);
       }
       // all that this warp reads of the item's sums has been read
       ptx::tc_fence_before_sync();
@@ -605,10 +630,53 @@ __global__ void __launch_bounds__(kPairThreads, 1) i8_pair_kernel(MmArgs a) {
       if (lane == 0) ptx::mbar_arrive_cluster_relaxed(to + 8u * set);
     }
   }
+  if (shares > 1) {
+    __syncwarp();
+    ptx::cluster_sync();  // nobody's stages are in use
+    if (warp >= 4 && ok) {
+      const Item it = item_of(first_item);
+      // [other pair][group][gate, up][four columns][row]
+      auto place = [&](int from, int group, int part, int j4) { return (((((from * most_groups + group) * W + part) * 8 + j4) * kI8Tile) + quarter * 32 + lane) * 16; };
+      for (int g = half; g < G; g += 2) {
+        const int owner = g % shares;
+        if (owner == share) continue;
+        const uint32_t cta = (uint32_t)owner * 2 + rank, to = ptx::map_to_rank(smem_u, cta), bar = ptx::map_to_rank(pushed, cta);
+        const int from = share - (share > owner);
+#pragma unroll
+        for (int part = 0; part < W; ++part) {
+          uint32_t v[32];
+          ptx::tmem_ld32(acc0 + (uint32_t)(part * kI8Tile + g * 32), v);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int j4 = 0; j4 < 8; ++j4) push4(to + place(from, g / shares, part, j4), v[4 * j4], v[4 * j4 + 1], v[4 * j4 + 2], v[4 * j4 + 3], bar);
+        }
+      }
+      ok = __all_sync(0xffffffffu, ptx::mbar_wait_addr(pushed, 0));
+      for (int i = half; i < own_groups && ok; i += 2) {
+        const int g = share + i * shares;
+        uint32_t v[32], u[GATED ? 32 : 1];
+        ptx::tmem_ld32(acc0 + (uint32_t)(g * 32), v);
+        if constexpr (GATED) ptx::tmem_ld32(acc0 + (uint32_t)(kI8Tile + g * 32), u);
+        ptx::tmem_ld_wait();
+        for (int from = 0; from < shares - 1; ++from) {
+#pragma unroll
+          for (int j4 = 0; j4 < 8; ++j4) {
+            const uint4 p = *reinterpret_cast<const uint4*>(smem + place(from, i, 0, j4));
+            v[4 * j4] += p.x; v[4 * j4 + 1] += p.y; v[4 * j4 + 2] += p.z; v[4 * j4 + 3] += p.w;
+            if constexpr (GATED) {
+              const uint4 q = *reinterpret_cast<const uint4*>(smem + place(from, i, 1, j4));
+              u[4 * j4] += q.x; u[4 * j4 + 1] += q.y; u[4 * j4 + 2] += q.z; u[4 * j4 + 3] += q.w;
+            }
+          }
+        }
+        store_sums<GATED>(a, v, u, mine, it.tile - (int)rank, g * 32, it.row + quarter * 32, row_step);
+      }
+    }
+  }
   if (!ok) atomicExch(a.err, B200_ERR_DEVICE_FLAGGED);
   __syncwarp();
   ptx::tc_fence_before_sync();
-  ptx::cluster_sync();  // nobody leaves while its memory may be read or arrived on
+  ptx::cluster_sync();  // nobody leaves while its memory may be read, written or arrived on
   if (warp == 1) ptx::tmem_dealloc2(tmem, 512);
 }
 
@@ -666,15 +734,17 @@ b200_status launch_stream(MmArgs& a, cudaStream_t s) {
 
 template <bool GATED>
 b200_status launch_pair(MmArgs& a, cudaStream_t s) {
-  static int most_pairs = 0;
-  if (most_pairs == 0) {
+  static int at_once[kMostPairs + 1] = {};  // clusters that run at the same time, by their pairs
+  if (at_once[1] == 0) {
     B200_CUDA_TRY(cudaFuncSetAttribute(i8_pair_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairShared));
-    const int n = ctas_in_clusters(i8_pair_kernel<GATED>, 2, 1, b200_sm_count(), kPairThreads, kPairShared) / 2;
-    if (n < 1) { b200_set_error("i8: no pair of CTAs fits the device"); return B200_ERR_CAPACITY; }
-    most_pairs = n;
+    for (int n = kMostPairs; n > 0; --n) at_once[n] = ctas_in_clusters(i8_pair_kernel<GATED>, 2 * n, 1, b200_sm_count(), kPairThreads, kPairShared) / (2 * n);
+    if (at_once[1] < 1) { b200_set_error("i8: no pair of CTAs fits the device"); return B200_ERR_CAPACITY; }
   }
   const long long items = (long long)((a.rows + kPairRows - 1) / kPairRows) * ((a.tiles + 1) / 2);
-  launch_clusters(i8_pair_kernel<GATED>, 2, dim3((unsigned)(2 * std::min<long long>(items, most_pairs))), kPairThreads, kPairShared, s, a);
+  a.shares = 1;
+  for (int n = 2; n <= kMostPairs && a.chunks >= 4 * n; ++n)
+    if (items <= at_once[n] && (n - 1) * ((a.chunks + n - 1) / n) < a.chunks) a.shares = n;
+  launch_clusters(i8_pair_kernel<GATED>, 2 * a.shares, dim3((unsigned)(2 * a.shares * std::min<long long>(items, at_once[a.shares]))), kPairThreads, kPairShared, s, a);
   B200_LAUNCH_CHECK();
   return B200_OK;
 }
