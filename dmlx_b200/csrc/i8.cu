@@ -313,25 +313,35 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
     ok = __all_sync(0xffffffffu, ok);
     ptx::tc_fence_after_sync();
   }
+  // Sixteen rows' sums, as far as they go.
+  auto load_sums = [&](int c0, int end, uint32_t (&v)[16], uint32_t (&u)[16]) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = u[j] = 0u;
+#pragma unroll
+    for (int g = 0; g < 16; g += 4)
+      if (c0 + g < end) {
+        tmem_ld4(acc + c0 + g, v[g], v[g + 1], v[g + 2], v[g + 3]);
+        if constexpr (GATED) tmem_ld4(acc + a.tn + c0 + g, u[g], u[g + 1], u[g + 2], u[g + 3]);
+      }
+    ptx::tmem_ld_wait();
+  };
   if (shares > 1) {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the others' barriers are there
     if (a.over_stages) ptx::cluster_sync();                              // nobody's stages are in use
     if (warp >= 2 && ok) {
-      int q = 0, next = per_rank;  // whose the rows are
-      for (int c0 = 0; c0 < rows_here; c0 += 16) {
-        uint32_t v[16], u[16];
-        ptx::tmem_ld16(acc + c0, v);
-        if constexpr (GATED) ptx::tmem_ld16(acc + a.tn + c0, u);
-        ptx::tmem_ld_wait();
+      for (int i = 1; i < shares; ++i) {
+        const int q = rank + i < shares ? rank + i : rank + i - shares, q0 = min(rows_here, q * per_rank), q1 = min(rows_here, q0 + per_rank);
+        const uint32_t bar = ptx::map_to_rank(ptx::smem_u32(pushed), q), part = per_rank / 4 * kI8Tile * 16;
+        uint32_t to = ptx::map_to_rank(ptx::smem_u32(smem + a.pushed_at), q) + (rank - (rank > q)) * W * part + (quarter * 32 + lane) * 16;
+        for (int c0 = q0; c0 < q1; c0 += 16, to += 4 * kI8Tile * 16) {
+          uint32_t v[16], u[16];
+          load_sums(c0, q1, v, u);
 #pragma unroll
-        for (int g = 0; g < 16; g += 4) {
-          const int row = c0 + g;
-          if (row >= next) { ++q; next += per_rank; }
-          if (row >= rows_here || q == rank) continue;
-          const int at = ((rank - (rank > q)) * W * (per_rank / 4) + (row + per_rank - next) / 4) * kI8Tile + quarter * 32 + lane;
-          const uint32_t to = ptx::map_to_rank(ptx::smem_u32(smem + a.pushed_at + at * 16), q), bar = ptx::map_to_rank(ptx::smem_u32(pushed), q);
-          push4(to, v[g], v[g + 1], v[g + 2], v[g + 3], bar);
-          if constexpr (GATED) push4(to + per_rank / 4 * kI8Tile * 16, u[g], u[g + 1], u[g + 2], u[g + 3], bar);
+          for (int g = 0; g < 16; g += 4)
+            if (c0 + g < q1) {
+              push4(to + g / 4 * kI8Tile * 16, v[g], v[g + 1], v[g + 2], v[g + 3], bar);
+              if constexpr (GATED) push4(to + part + g / 4 * kI8Tile * 16, u[g], u[g + 1], u[g + 2], u[g + 3], bar);
+            }
         }
       }
     }
@@ -342,34 +352,36 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
     if (shares > 1) ok = __all_sync(0xffffffffu, ptx::mbar_wait(pushed, 0));
     for (int c0 = mine0; c0 < mine1 && ok; c0 += 16) {
       uint32_t v[16], u[16];
-#pragma unroll
-      for (int g = 0; g < 16; g += 4)
-        if (c0 + g < mine1) {
-          tmem_ld4(acc + c0 + g, v[g], v[g + 1], v[g + 2], v[g + 3]);
-          if constexpr (GATED) tmem_ld4(acc + a.tn + c0 + g, u[g], u[g + 1], u[g + 2], u[g + 3]);
-        }
-      ptx::tmem_ld_wait();
+      load_sums(c0, mine1, v, u);
       const uint4* from = reinterpret_cast<const uint4*>(smem + a.pushed_at) + (c0 - mine0) / 4 * kI8Tile + quarter * 32 + lane;
       for (int q = 0; q < shares - 1; ++q, from += W * (per_rank / 4) * kI8Tile) {
 #pragma unroll
-        for (int g = 0; g < 16; g += 4) {
-          if (c0 + g >= mine1) break;
-          const uint4 p = from[g / 4 * kI8Tile];
-          v[g] += p.x; v[g + 1] += p.y; v[g + 2] += p.z; v[g + 3] += p.w;
-          if constexpr (GATED) {
-            const uint4 p2 = from[(per_rank / 4 + g / 4) * kI8Tile];
-            u[g] += p2.x; u[g + 1] += p2.y; u[g + 2] += p2.z; u[g + 3] += p2.w;
+        for (int g = 0; g < 16; g += 4)
+          if (c0 + g < mine1) {
+            const uint4 p = from[g / 4 * kI8Tile];
+            v[g] += p.x; v[g + 1] += p.y; v[g + 2] += p.z; v[g + 3] += p.w;
+            if constexpr (GATED) {
+              const uint4 p2 = from[(per_rank / 4 + g / 4) * kI8Tile];
+              u[g] += p2.x; u[g + 1] += p2.y; u[g + 2] += p2.z; u[g + 3] += p2.w;
+            }
           }
-        }
       }
+      // All sixteen are worked out before the first is stored: one after the other each took 100 cycles of latencies.
+      float y[16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float step = __shfl_sync(0xffffffffu, steps, j);
-        if (c0 + j >= mine1 || channel >= a.n) continue;
-        const size_t at = (size_t)(t0 + c0 + j) * a.y_stride + channel;
-        const float y = output_of<GATED>(a, (int)v[j], GATED ? (int)u[j] : 0, ws, us, step, bias);
-        if (GATED || a.y_f32) reinterpret_cast<float*>(a.y)[at] = y;
-        else reinterpret_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16(y);
+      for (int j = 0; j < 16; ++j) y[j] = output_of<GATED>(a, (int)v[j], GATED ? (int)u[j] : 0, ws, us, __shfl_sync(0xffffffffu, steps, j), bias);
+      const size_t at = (size_t)(t0 + c0) * a.y_stride + channel;
+      const int rows_left = channel < a.n ? mine1 - c0 : 0;
+      if (GATED || a.y_f32) {
+        float* to = reinterpret_cast<float*>(a.y) + at;
+#pragma unroll
+        for (int j = 0; j < 16; ++j, to += a.y_stride)
+          if (j < rows_left) *to = y[j];
+      } else {
+        __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(a.y) + at;
+#pragma unroll
+        for (int j = 0; j < 16; ++j, to += a.y_stride)
+          if (j < rows_left) *to = __float2bfloat16(y[j]);
       }
       steps = steps_of(c0 + 16);
     }
