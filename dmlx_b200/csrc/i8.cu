@@ -177,9 +177,9 @@ __device__ __forceinline__ float output_of(const MmArgs& a, int sum, int up, flo
 // A weight tile (gated: the gate's and up's tile of the same channels) by up to tn rows and a share of K per CTA.  The weights are the MMA's M, the rows
 // its N, so that few rows waste nothing; a lane of tensor memory is a channel.  Warp 0 loads, warp 1 multiplies, four bring the sums to the output.
 // Bound by the weights, which come at the rate of memory only if every SM asks for them: a cluster of up to eight CTAs shares K (as many as still run at
-// the same time, two CTAs on an SM).  Each of them brings a share of the rows to the output and gets the others' sums of these pushed into its
+// the same time).  Each of them brings a share of the rows to the output and gets the others' sums of these pushed into its
 // shared memory, where the stages were unless there is room beside them, with a barrier that counts their bytes.
-constexpr int kStreamThreads = 192, kStreamShared = 112 * 1024, kMostShares = 8;
+constexpr int kStreamThreads = 192, kStreamShared = 112 * 1024, kStreamAlone = 226 * 1024, kMostShares = 8;  // (shared memory of two CTAs on an SM, of one)
 
 // Four words to another CTA of the cluster, counted by a barrier there.
 __device__ __forceinline__ void push4(uint32_t mapped, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t mapped_bar) {
@@ -246,6 +246,8 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
   if (threadIdx.x == 0)
     for (int i = 0; i < ahead; ++i) load_weights(i, i);
   wait_previous();
+  if (threadIdx.x == 0)
+    for (int i = 0; i < ahead; ++i) load_rows(i, i);
   if (warp == 1) {
     ptx::tmem_alloc(tmem_slot, cols);
     ptx::tmem_relinquish();
@@ -257,14 +259,12 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
   bool ok = true;
   if (warp == 0) {
     if (lane == 0) {
-      int s = 0, issued = 0;
-      uint32_t ph = 1;
-      for (int i = 0; i < chunks; ++i) {
-        if (i >= ahead) {
-          ok = ptx::mbar_wait(&done[s], ph);
-          if (!ok) break;
-          load_weights(i, s);
-        }
+      int s = ahead == S ? 0 : ahead, issued = ahead;
+      uint32_t ph = 0;
+      for (int i = ahead; i < chunks; ++i) {
+        ok = ptx::mbar_wait(&done[s], ph);
+        if (!ok) break;
+        load_weights(i, s);
         load_rows(i, s);
         ++issued;
         if (++s == S) { s = 0; ph ^= 1u; }
@@ -329,10 +329,12 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the others' barriers are there
     if (a.over_stages) ptx::cluster_sync();                              // nobody's stages are in use
     if (warp >= 2 && ok) {
+#pragma unroll 1
       for (int i = 1; i < shares; ++i) {
         const int q = rank + i < shares ? rank + i : rank + i - shares, q0 = min(rows_here, q * per_rank), q1 = min(rows_here, q0 + per_rank);
         const uint32_t bar = ptx::map_to_rank(ptx::smem_u32(pushed), q), part = per_rank / 4 * kI8Tile * 16;
         uint32_t to = ptx::map_to_rank(ptx::smem_u32(smem + a.pushed_at), q) + (rank - (rank > q)) * W * part + (quarter * 32 + lane) * 16;
+#pragma unroll 1
         for (int c0 = q0; c0 < q1; c0 += 16, to += 4 * kI8Tile * 16) {
           uint32_t v[16], u[16];
           load_sums(c0, q1, v, u);
@@ -350,10 +352,12 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
   }
   if (warp >= 2 && ok && mine0 < mine1) {
     if (shares > 1) ok = __all_sync(0xffffffffu, ptx::mbar_wait(pushed, 0));
+#pragma unroll 1
     for (int c0 = mine0; c0 < mine1 && ok; c0 += 16) {
       uint32_t v[16], u[16];
       load_sums(c0, mine1, v, u);
       const uint4* from = reinterpret_cast<const uint4*>(smem + a.pushed_at) + (c0 - mine0) / 4 * kI8Tile + quarter * 32 + lane;
+#pragma unroll 1
       for (int q = 0; q < shares - 1; ++q, from += W * (per_rank / 4) * kI8Tile) {
 #pragma unroll
         for (int g = 0; g < 16; g += 4)
@@ -405,7 +409,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
 // sums to the output.
 constexpr int kPairThreads = 384, kPairStage = 2 * kI8Block, kPairStages = 6, kPairRows = 256, kPairBand = 16, kMostPairs = 4;
 constexpr int kPairPitch = 20;  // epilogue: words between rows in a warp's staging tile of 32 rows by 16 words
-constexpr int kPairShared = 1024 + kPairStages * kPairStage + 8 * 32 * kPairPitch * 4 + 8 * (3 * kPairStages + 6) + 16;
+constexpr int kPairShared = 1024 + kPairStages * kPairStage + 8 * 32 * kPairPitch * 4 + 8 * 2 * kI8Tile * 4 + 8 * (3 * kPairStages + 6) + 16;
 
 __device__ __forceinline__ void umma2_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -421,24 +425,18 @@ __device__ __forceinline__ void commit_pair(uint32_t bar, uint16_t ctas) {
 }
 
 // A warp's 32 rows by 32 columns from the item's column c0 on, whose sums are v (gated: with up's in u), to the output, through shared memory, so that a
-// store is 64 contiguous bytes of a row.
+// store is 64 contiguous bytes of a row.  scales: these columns' factors, and 128 floats behind them up's, or the bias.
 template <bool GATED>
-__device__ __forceinline__ void store_sums(const MmArgs& a, uint32_t (&v)[32], const uint32_t (&u)[GATED ? 32 : 1], float* mine, int first_tile, int c0, int row0, float row_step) {
+__device__ __forceinline__ void store_sums(const MmArgs& a, uint32_t (&v)[32], const uint32_t (&u)[GATED ? 32 : 1], float* mine, const float* scales, int first_tile, int c0, int row0, float row_step) {
   const int lane = threadIdx.x & 31, rows_here = min(32, a.rows - row0), n0 = (GATED ? first_tile / 2 : first_tile) * kI8Tile + c0, cols = min(32, a.n - n0);
   if (cols <= 0 || rows_here <= 0) return;
-  const float4* ws = reinterpret_cast<const float4*>(a.w_scale + (size_t)first_tile * kI8Tile + c0);
 #pragma unroll
   for (int j4 = 0; j4 < 8; ++j4) {
-    const float4 w4 = ws[j4], u4 = GATED ? ws[j4 + kI8Tile / 4] : make_float4(0.f, 0.f, 0.f, 0.f);
-    float b[4] = {0.f, 0.f, 0.f, 0.f};
-    if (!GATED && a.bias) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) b[e] = n0 + 4 * j4 + e < a.n ? a.bias[n0 + 4 * j4 + e] : 0.f;
-    }
-    const float w[4] = {w4.x, w4.y, w4.z, w4.w}, up[4] = {u4.x, u4.y, u4.z, u4.w};
+    const float4 w4 = *reinterpret_cast<const float4*>(scales + 4 * j4), o4 = *reinterpret_cast<const float4*>(scales + kI8Tile + 4 * j4);
+    const float w[4] = {w4.x, w4.y, w4.z, w4.w}, o[4] = {o4.x, o4.y, o4.z, o4.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      v[4 * j4 + e] = __float_as_uint(output_of<GATED>(a, (int)v[4 * j4 + e], GATED ? (int)u[4 * j4 + e] : 0, w[e], up[e], row_step, b[e]));
+      v[4 * j4 + e] = __float_as_uint(output_of<GATED>(a, (int)v[4 * j4 + e], GATED ? (int)u[4 * j4 + e] : 0, w[e], GATED ? o[e] : 0.f, row_step, GATED ? 0.f : o[e]));
   }
   if (GATED || a.y_f32) {
 #pragma unroll
@@ -492,7 +490,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) i8_pair_kernel(MmArgs a) {
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   constexpr int S = kPairStages, W = GATED ? 2 : 1, G = GATED ? 4 : 8;  // G: groups of 32 columns of an item
   float* staging = reinterpret_cast<float*>(smem + (size_t)S * kPairStage);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + 8 * 32 * kPairPitch);
+  float* scale_rows = staging + 8 * 32 * kPairPitch;  // [epilogue warp][factors of 128 columns, up's or the bias]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(scale_rows + 8 * 2 * kI8Tile);
   const uint32_t smem_u = ptx::smem_u32(smem), full = ptx::smem_u32(bars);  // [S] this CTA's half of the stage has landed
   const uint32_t done = full + 8u * S;        // [S] the MMAs that read the stage are done
   const uint32_t ready = done + 8u * S;       // [S] first CTA: both CTAs' halves have landed
@@ -507,11 +506,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) i8_pair_kernel(MmArgs a) {
   const int shares = a.shares, share = (int)in_cluster / 2;
   const int per_share = (a.chunks + shares - 1) / shares, chunk0 = share * per_share, chunks = min(per_share, a.chunks - chunk0);  // (never none)
   const int row_tiles = (a.rows + kPairRows - 1) / kPairRows, pairs = (a.tiles + 1) / 2;
-  const long long items = (long long)row_tiles * pairs, first_item = blockIdx.x / (2 * shares), step = gridDim.x / (2 * shares);
+  const int items = row_tiles * pairs, first_item = blockIdx.x / (2 * shares), step = gridDim.x / (2 * shares);
   struct Item { int tile, row; };  // this CTA's weight tile and first row
-  auto item_of = [&](long long i) {
-    const long long band = (long long)kPairBand * pairs;
-    const int b = (int)(i / band), rest = (int)(i - b * band), high = min(kPairBand, row_tiles - b * kPairBand);
+  auto item_of = [&](int i) {
+    const int band = kPairBand * pairs, b = i / band, rest = i - b * band, high = min(kPairBand, row_tiles - b * kPairBand);
     return Item{2 * (rest / high) + (int)rank, (b * kPairBand + rest % high) * kPairRows + (int)rank * kI8Tile};
   };
   const int own_groups = (G - share + shares - 1) / shares, most_groups = (G + shares - 1) / shares;
@@ -531,17 +529,24 @@ __global__ void __launch_bounds__(kPairThreads, 1) i8_pair_kernel(MmArgs a) {
     ptx::mbar_expect_tx_addr(pushed, (uint32_t)((shares - 1) * own_groups * W) * kI8Block);
   }
   __syncthreads();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this CTA's barriers are there
   // (what does not exist is not loaded: its products go nowhere)
   auto load_weights = [&](const Item& it, int c, uint32_t s) {
     const bool rows_there = it.row < a.rows, tile_there = it.tile < a.tiles;
     ptx::mbar_expect_tx_addr(full + 8u * s, (rows_there ? kI8Block : 0) + (tile_there ? kI8Block : 0));
     if (tile_there) ptx::bulk_g2s_addr(smem_u + s * kPairStage + kI8Block, a.w + ((size_t)it.tile * a.chunks + chunk0 + c) * kI8Block, kI8Block, full + 8u * s);
   };
+  auto load_rows = [&](const Item& it, int c, uint32_t s) {
+    if (it.row < a.rows) ptx::bulk_g2s_addr(smem_u + s * kPairStage, a.q + ((size_t)(it.row / kI8Tile) * a.chunks + chunk0 + c) * kI8Block, kI8Block, full + 8u * s);
+  };
   const int ahead = min(S, chunks);  // weights asked for before the kernels ahead have ended
+  const Item first = item_of(first_item);
   if (threadIdx.x == 0)
-    for (int c = 0; c < ahead; ++c) load_weights(item_of(first_item), c, (uint32_t)c);
+    for (int c = 0; c < ahead; ++c) load_weights(first, c, (uint32_t)c);
   wait_previous();
-  ptx::cluster_sync();  // all barriers are there
+  if (threadIdx.x == 0)
+    for (int c = 0; c < ahead; ++c) load_rows(first, c, (uint32_t)c);
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the others' are
   if (warp == 1) {
     ptx::tmem_alloc2(tmem_slot, 512);
     ptx::tmem_relinquish2();
@@ -552,23 +557,39 @@ __global__ void __launch_bounds__(kPairThreads, 1) i8_pair_kernel(MmArgs a) {
   const uint32_t tmem = *tmem_slot;
   bool ok = true;
   const int quarter = warp & 3, half = (warp - 4) >> 2;  // of the epilogue's warps
-  float* mine = staging + (warp - 4) * 32 * kPairPitch;
+  float *mine = staging + (warp - 4) * 32 * kPairPitch, *scales = scale_rows + (warp - 4) * 2 * kI8Tile;
+  // The factors of the four groups of columns that this warp brings to the output, asked for before their sums are there.
+  const int my_group = shares > 1 ? share + (half + 2 * (lane / 8)) * shares : GATED ? lane / 8 : half * 4 + lane / 8;
+  auto fetch_scales = [&](int first_tile) {
+    const int c = my_group * 32 + lane % 8 * 4, n = first_tile * kI8Tile + c;
+    const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+    const bool there = my_group < G && first_tile + c / kI8Tile < a.tiles;
+    float4 w = there ? *reinterpret_cast<const float4*>(a.w_scale + n) : none, o = none;
+    if (GATED) {
+      if (there) o = *reinterpret_cast<const float4*>(a.w_scale + n + kI8Tile);
+    } else if (a.bias && there) {
+      o = make_float4(n < a.n ? a.bias[n] : 0.f, n + 1 < a.n ? a.bias[n + 1] : 0.f, n + 2 < a.n ? a.bias[n + 2] : 0.f, n + 3 < a.n ? a.bias[n + 3] : 0.f);
+    }
+    __syncwarp();
+    *reinterpret_cast<float4*>(scales + lane * 4) = w;
+    *reinterpret_cast<float4*>(scales + kI8Tile + lane * 4) = o;
+    __syncwarp();
+  };
   const uint32_t acc0 = tmem + ((uint32_t)(quarter * 32) << 16);
   float row_step = 0.f;
   if (warp == 0) {
     if (lane == 0) {
       uint32_t s = 0, ph = 1;
       long long issued = 0;
-      for (long long i = first_item; i < items && ok; i += step) {
+      for (int i = first_item; i < items && ok; i += step) {
         const Item it = item_of(i);
-        const signed char* rows = a.q + ((size_t)(it.row / kI8Tile) * a.chunks + chunk0) * kI8Block;
         for (int c = 0; c < chunks; ++c) {
           if (issued >= ahead) {
             ok = ptx::mbar_wait_addr(done + 8u * s, ph);
             if (!ok) break;
             load_weights(it, c, s);
+            load_rows(it, c, s);
           }
-          if (it.row < a.rows) ptx::bulk_g2s_addr(smem_u + s * kPairStage, rows + (size_t)c * kI8Block, kI8Block, full + 8u * s);
           ++issued;
           if (++s == (uint32_t)S) { s = 0; ph ^= 1u; }
         }
@@ -581,7 +602,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) i8_pair_kernel(MmArgs a) {
     if (lane == 0) {
       const uint32_t to = ptx::map_to_rank(ready, leader);
       uint32_t s = 0, ph = 0;
-      for (long long i = first_item; i < items && ok; i += step)
+      for (int i = first_item; i < items && ok; i += step)
         for (int c = 0; c < chunks; ++c) {
           ok = ptx::mbar_wait_addr(full + 8u * s, ph);
           if (!ok) break;
@@ -593,7 +614,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) i8_pair_kernel(MmArgs a) {
     if (rank == 0 && ptx::elect_one()) {
       const uint32_t idesc = idesc_i8(2 * kI8Tile, 2 * kI8Tile);
       uint32_t s = 0, ph = 0, n_item = 0;
-      for (long long i = first_item; i < items && ok; i += step, ++n_item) {
+      for (int i = first_item; i < items && ok; i += step, ++n_item) {
         const uint32_t set = n_item & 1u, acc = tmem + set * 256u;
         if (n_item >= 2) ok = ptx::mbar_wait_cluster(acc_free + 8u * set, ((n_item >> 1) - 1u) & 1u);
         if (!ok) break;
@@ -620,21 +641,23 @@ __global__ void __launch_bounds__(kPairThreads, 1) i8_pair_kernel(MmArgs a) {
     // A lane is a row.
     const uint32_t to = ptx::map_to_rank(acc_free, leader);
     uint32_t n_item = 0;
-    for (long long i = first_item; i < items; i += step, ++n_item) {
+    for (int i = first_item; i < items; i += step, ++n_item) {
       const Item it = item_of(i);
       const uint32_t set = n_item & 1u;
       const int row0 = it.row + quarter * 32;
       row_step = row0 + lane < a.rows ? a.step[row0 + lane] : 0.f;
+      fetch_scales(it.tile - (int)rank);
       ok = ptx::mbar_wait_addr(acc_full + 8u * set, (n_item >> 1) & 1u);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       ptx::tc_fence_after_sync();
       if (shares > 1) break;
+#pragma unroll 1  // (an epilogue that runs once per CTA waits for its instructions)
       for (int g = half * (G / 2); g < half * (G / 2) + G / 2; ++g) {
         uint32_t v[32], u[GATED ? 32 : 1];
         ptx::tmem_ld32(acc0 + set * 256u + (uint32_t)(g * 32), v);
         if constexpr (GATED) ptx::tmem_ld32(acc0 + set * 256u + (uint32_t)(kI8Tile + g * 32), u);
         ptx::tmem_ld_wait();
-        store_sums<GATED>(a, v, u, mine, it.tile - (int)rank, g * 32, row0, row_step);
+        store_sums<GATED>(a, v, u, mine, scales + (GATED ? g : g % 4) * 32, it.tile - (int)rank, g * 32, row0, row_step);
       }
       // all that this warp reads of the item's sums has been read
       ptx::tc_fence_before_sync();
@@ -649,6 +672,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) i8_pair_kernel(MmArgs a) {
       const Item it = item_of(first_item);
       // [other pair][group][gate, up][four columns][row]
       auto place = [&](int from, int group, int part, int j4) { return (((((from * most_groups + group) * W + part) * 8 + j4) * kI8Tile) + quarter * 32 + lane) * 16; };
+#pragma unroll 1
       for (int g = half; g < G; g += 2) {
         const int owner = g % shares;
         if (owner == share) continue;
@@ -664,12 +688,14 @@ __global__ void __launch_bounds__(kPairThreads, 1) i8_pair_kernel(MmArgs a) {
         }
       }
       ok = __all_sync(0xffffffffu, ptx::mbar_wait_addr(pushed, 0));
+#pragma unroll 1
       for (int i = half; i < own_groups && ok; i += 2) {
         const int g = share + i * shares;
         uint32_t v[32], u[GATED ? 32 : 1];
         ptx::tmem_ld32(acc0 + (uint32_t)(g * 32), v);
         if constexpr (GATED) ptx::tmem_ld32(acc0 + (uint32_t)(kI8Tile + g * 32), u);
         ptx::tmem_ld_wait();
+#pragma unroll 1
         for (int from = 0; from < shares - 1; ++from) {
 #pragma unroll
           for (int j4 = 0; j4 < 8; ++j4) {
@@ -681,7 +707,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) i8_pair_kernel(MmArgs a) {
             }
           }
         }
-        store_sums<GATED>(a, v, u, mine, it.tile - (int)rank, g * 32, it.row + quarter * 32, row_step);
+        store_sums<GATED>(a, v, u, mine, scales + (i >> 1) * 32, it.tile - (int)rank, g * 32, it.row + quarter * 32, row_step);
       }
     }
   }
@@ -714,25 +740,24 @@ void launch_clusters(void (*kernel)(P...), int size, dim3 grid, int threads, siz
 template <bool GATED>
 b200_status launch_stream(MmArgs& a, cudaStream_t s) {
   constexpr int W = GATED ? 2 : 1;
-  static int at_once[kMostShares + 1] = {};  // CTAs that run at the same time, by the cluster's size
+  static int at_once[kMostShares + 1] = {};  // CTAs that run at the same time on an SM each, by the cluster's size
   if (at_once[1] == 0) {
-    B200_CUDA_TRY(cudaFuncSetAttribute(i8_stream_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamShared));
-    for (int size = kMostShares; size > 0; --size) {
-      // (the occupancy calculation counts one CTA of a kernel that allocates tensor memory to an SM; this one takes half of that memory at most)
-      at_once[size] = 2 * ctas_in_clusters(i8_stream_kernel<GATED>, size, 1, b200_sm_count(), kStreamThreads, kStreamShared);
-    }
+    B200_CUDA_TRY(cudaFuncSetAttribute(i8_stream_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamAlone));
+    for (int size = kMostShares; size > 0; --size) at_once[size] = ctas_in_clusters(i8_stream_kernel<GATED>, size, 1, b200_sm_count(), kStreamThreads, kStreamAlone);
+    if (at_once[1] < 1) { b200_set_error("i8: no CTA fits the device"); return B200_ERR_CAPACITY; }
   }
   const int most = GATED ? 128 : 256;
   a.tn = 16;
   while (a.tn < most && a.tn < a.rows) a.tn *= 2;
   const int tiles = a.tiles / W, row_tiles = (a.rows + a.tn - 1) / a.tn;
-  const int stage = W * kI8Block + a.tn * kI8Chunk, room = kStreamShared - 2048, rows_most = std::min(a.rows, a.tn);
-  // As many shares of K as still run at once, each of two blocks or more.
+  const int stage = W * kI8Block + a.tn * kI8Chunk, rows_most = std::min(a.rows, a.tn);
+  // As many shares of K as still run at once, an SM to each, and are two blocks or more: more of them push more sums than they save of the stream.
   a.shares = 1;
   for (int n = 2; n <= kMostShares && a.chunks >= 2 * n; ++n) {
     const int per = (a.chunks + n - 1) / n;
-    if ((long long)tiles * row_tiles * n <= at_once[n] && (n - 1) * per < a.chunks && pushed_bytes(rows_most, n, W) <= room) a.shares = n;
+    if ((long long)tiles * row_tiles * n <= at_once[n] && (n - 1) * per < a.chunks && pushed_bytes(rows_most, n, W) <= kStreamAlone - 2048) a.shares = n;
   }
+  const int room = ((long long)tiles * row_tiles * a.shares <= at_once[a.shares] ? kStreamAlone : kStreamShared) - 2048;
   const int per_share = (a.chunks + a.shares - 1) / a.shares, pushed = pushed_bytes(rows_most, a.shares, W);
   // What is pushed has a place beside the stages where that is a quarter of the room at most.
   a.over_stages = pushed > room / 4;
@@ -753,6 +778,7 @@ b200_status launch_pair(MmArgs& a, cudaStream_t s) {
     if (at_once[1] < 1) { b200_set_error("i8: no pair of CTAs fits the device"); return B200_ERR_CAPACITY; }
   }
   const long long items = (long long)((a.rows + kPairRows - 1) / kPairRows) * ((a.tiles + 1) / 2);
+  if (items > 0x3fffffff) { b200_set_error("i8: %d rows of %d channels in one call", a.rows, a.n); return B200_ERR_CAPACITY; }
   a.shares = 1;
   for (int n = 2; n <= kMostPairs && a.chunks >= 4 * n; ++n)
     if (items <= at_once[n] && (n - 1) * ((a.chunks + n - 1) / n) < a.chunks) a.shares = n;
