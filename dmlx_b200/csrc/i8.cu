@@ -737,52 +737,83 @@ void launch_clusters(void (*kernel)(P...), int size, dim3 grid, int threads, siz
   (void)cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// What a product is expected to take with one kernel or the other.  Microseconds of launches one behind the other in a graph, fitted to 2048 x 2048 to 4096 x 14336
+// and 28672 x 4096 at 32 to 1024 rows: a block of weights reaches an SM in 0.27 us however few rows go with it, a row that a CTA brings to the output costs
+// 0.029 us, one whose sums it pushes 0.025, and sharing K 1.2.  4096 x 4096: 256 rows as 64 tiles of 128 in two shares 9.4 us (model 9.6), as 32 of 256
+// in four 11.2 (11.1), as pairs in two shares 11.5 (12.7); 512 rows as pairs 12.9, as tiles of 256 13.3; 1024 rows as pairs 15.8, as tiles 18.6.
+struct Plan {
+  float us = 1e30f;
+  bool pair = false;
+  int tn = 0, shares = 1;
+};
+
 template <bool GATED>
-b200_status launch_stream(MmArgs& a, cudaStream_t s) {
+Plan plan_of(const MmArgs& a, const int* stream_at_once, const int* pairs_at_once) {
   constexpr int W = GATED ? 2 : 1;
-  static int at_once[kMostShares + 1] = {};  // CTAs that run at the same time on an SM each, by the cluster's size
-  if (at_once[1] == 0) {
-    B200_CUDA_TRY(cudaFuncSetAttribute(i8_stream_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamAlone));
-    for (int size = kMostShares; size > 0; --size) at_once[size] = ctas_in_clusters(i8_stream_kernel<GATED>, size, 1, b200_sm_count(), kStreamThreads, kStreamAlone);
-    if (at_once[1] < 1) { b200_set_error("i8: no CTA fits the device"); return B200_ERR_CAPACITY; }
+  Plan best;
+  const auto split = [&](int n, int least) { return n == 1 || (a.chunks >= least * n && (n - 1) * ((a.chunks + n - 1) / n) < a.chunks); };  // into n shares, none of them empty
+  const int tiles = a.tiles / W, sms = b200_sm_count();
+  for (int tn = 16; W * tn <= 256; tn *= 2) {
+    const long long row_tiles = (a.rows + tn - 1) / tn;
+    const int rows_here = std::min(a.rows, tn);
+    if (row_tiles > 4096) continue;
+    for (int n = 1; n <= kMostShares; ++n) {
+      const long long ctas = tiles * row_tiles * n;
+      if (!split(n, 2) || pushed_bytes(rows_here, n, W) > kStreamAlone - 2048 || (n > 1 && ctas > stream_at_once[n])) continue;
+      const int own = std::min(rows_here, rows_per_rank(rows_here, n));
+      float us = 0.6f + 0.029f * W * own + (float)((a.chunks + n - 1) / n) * W * std::max(0.27f, 0.0014f * tn);
+      if (n > 1) us += 1.2f + 0.025f * W * (rows_here - own);
+      if (ctas > sms) us *= 1.18f * ctas / sms;
+      if (us < best.us) best = {us, false, tn, n};
+    }
+    if (tn >= a.rows) break;
   }
-  const int most = GATED ? 128 : 256;
-  a.tn = 16;
-  while (a.tn < most && a.tn < a.rows) a.tn *= 2;
-  const int tiles = a.tiles / W, row_tiles = (a.rows + a.tn - 1) / a.tn;
-  const int stage = W * kI8Block + a.tn * kI8Chunk, rows_most = std::min(a.rows, a.tn);
-  // As many shares of K as still run at once, an SM to each, and are two blocks or more: more of them push more sums than they save of the stream.
-  a.shares = 1;
-  for (int n = 2; n <= kMostShares && a.chunks >= 2 * n; ++n) {
-    const int per = (a.chunks + n - 1) / n;
-    if ((long long)tiles * row_tiles * n <= at_once[n] && (n - 1) * per < a.chunks && pushed_bytes(rows_most, n, W) <= kStreamAlone - 2048) a.shares = n;
+  const long long items = (long long)((a.rows + kPairRows - 1) / kPairRows) * ((a.tiles + 1) / 2);
+  for (int n = 1; n <= kMostPairs; ++n) {
+    if (!split(n, 4) || pairs_at_once[n] < 1 || (n > 1 && items > pairs_at_once[n])) continue;
+    const float waves = (float)((items + pairs_at_once[n] - 1) / pairs_at_once[n]);
+    const float us = (n == 1 ? 6.4f : 7.6f) + waves * (0.8f + 0.27f * ((a.chunks + n - 1) / n));
+    if (us < best.us) best = {us, true, 0, n};
   }
-  const int room = ((long long)tiles * row_tiles * a.shares <= at_once[a.shares] ? kStreamAlone : kStreamShared) - 2048;
-  const int per_share = (a.chunks + a.shares - 1) / a.shares, pushed = pushed_bytes(rows_most, a.shares, W);
-  // What is pushed has a place beside the stages where that is a quarter of the room at most.
-  a.over_stages = pushed > room / 4;
-  a.stages = std::min(per_share, (room - (a.over_stages ? 0 : pushed)) / stage);
-  a.pushed_at = a.over_stages ? 0 : a.stages * stage;
-  a.bars_at = std::max(a.stages * stage, a.pushed_at + pushed);
-  launch_clusters(i8_stream_kernel<GATED>, a.shares, dim3(tiles * a.shares, row_tiles), kStreamThreads, std::max<size_t>(a.bars_at + 2048, kSharedPerCol * stream_cols(a.tn, W)), s, a);
-  B200_LAUNCH_CHECK();
-  return B200_OK;
+  return best;
 }
 
 template <bool GATED>
-b200_status launch_pair(MmArgs& a, cudaStream_t s) {
-  static int at_once[kMostPairs + 1] = {};  // clusters that run at the same time, by their pairs
+b200_status launch_product(MmArgs& a, cudaStream_t s) {
+  constexpr int W = GATED ? 2 : 1;
+  // What runs at the same time with an SM for each CTA, by the cluster's size: CTAs of the one kernel, clusters of the other.  (The occupancy calculation counts
+  // one CTA of a kernel that allocates tensor memory to an SM; of i8_stream_kernel's two share that memory.)
+  static int at_once[kMostShares + 1] = {}, pairs_at_once[kMostPairs + 1] = {};
   if (at_once[1] == 0) {
+    B200_CUDA_TRY(cudaFuncSetAttribute(i8_stream_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamAlone));
     B200_CUDA_TRY(cudaFuncSetAttribute(i8_pair_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairShared));
-    for (int n = kMostPairs; n > 0; --n) at_once[n] = ctas_in_clusters(i8_pair_kernel<GATED>, 2 * n, 1, b200_sm_count(), kPairThreads, kPairShared) / (2 * n);
-    if (at_once[1] < 1) { b200_set_error("i8: no pair of CTAs fits the device"); return B200_ERR_CAPACITY; }
+    for (int n = kMostPairs; n > 0; --n) pairs_at_once[n] = ctas_in_clusters(i8_pair_kernel<GATED>, 2 * n, 1, b200_sm_count(), kPairThreads, kPairShared) / (2 * n);
+    for (int n = kMostShares; n > 0; --n) at_once[n] = ctas_in_clusters(i8_stream_kernel<GATED>, n, 1, b200_sm_count(), kStreamThreads, kStreamAlone);
+    if (at_once[1] < 1 || pairs_at_once[1] < 1) {
+      at_once[1] = 0;
+      b200_set_error("i8: the kernels do not fit the device");
+      return B200_ERR_CAPACITY;
+    }
   }
-  const long long items = (long long)((a.rows + kPairRows - 1) / kPairRows) * ((a.tiles + 1) / 2);
-  if (items > 0x3fffffff) { b200_set_error("i8: %d rows of %d channels in one call", a.rows, a.n); return B200_ERR_CAPACITY; }
-  a.shares = 1;
-  for (int n = 2; n <= kMostPairs && a.chunks >= 4 * n; ++n)
-    if (items <= at_once[n] && (n - 1) * ((a.chunks + n - 1) / n) < a.chunks) a.shares = n;
-  launch_clusters(i8_pair_kernel<GATED>, 2 * a.shares, dim3((unsigned)(2 * a.shares * std::min<long long>(items, at_once[a.shares]))), kPairThreads, kPairShared, s, a);
+  const Plan plan = plan_of<GATED>(a, at_once, pairs_at_once);
+  a.shares = plan.shares;
+  if (plan.pair) {
+    const long long items = (long long)((a.rows + kPairRows - 1) / kPairRows) * ((a.tiles + 1) / 2);
+    if (items > 0x3fffffff) { b200_set_error("i8: %d rows of %d channels in one call", a.rows, a.n); return B200_ERR_CAPACITY; }
+    launch_clusters(i8_pair_kernel<GATED>, 2 * a.shares, dim3((unsigned)(2 * a.shares * std::min<long long>(items, pairs_at_once[a.shares]))), kPairThreads, kPairShared, s, a);
+  } else {
+    a.tn = plan.tn;
+    const int tiles = a.tiles / W, row_tiles = (a.rows + a.tn - 1) / a.tn, stage = W * kI8Block + a.tn * kI8Chunk;
+    const int room = ((long long)tiles * row_tiles * a.shares <= at_once[a.shares] ? kStreamAlone : kStreamShared) - 2048;
+    const int per_share = (a.chunks + a.shares - 1) / a.shares, pushed = pushed_bytes(std::min(a.rows, a.tn), a.shares, W);
+    // What is pushed has a place beside the stages where that is a quarter of the room at most.
+    a.over_stages = pushed > room / 4;
+    a.stages = std::min(per_share, (room - (a.over_stages ? 0 : pushed)) / stage);
+    a.pushed_at = a.over_stages ? 0 : a.stages * stage;
+    a.bars_at = std::max(a.stages * stage, a.pushed_at + pushed);
+    launch_clusters(i8_stream_kernel<GATED>, a.shares, dim3(tiles * a.shares, row_tiles), kStreamThreads,
+                    std::max<size_t>(a.bars_at + 2048, kSharedPerCol * stream_cols(a.tn, W)), s, a);
+  }
   B200_LAUNCH_CHECK();
   return B200_OK;
 }
@@ -794,8 +825,7 @@ b200_status product(const b200_i8_weight* w, const I8RowsDev& x, int rows, const
   a.w = w->q; a.w_scale = w->scale; a.q = x.q; a.step = x.scale; a.bias = bias; a.y = y; a.y_stride = y_stride; a.y_f32 = y_f32; a.act = act;
   a.rows = rows; a.n = w->n; a.chunks = w->chunks; a.tiles = w->tiles;
   a.y_vec = ((uintptr_t)y & 15) == 0 && y_stride * (w->gated || y_f32 ? 4 : 2) % 16 == 0;
-  if (rows > 256) return w->gated ? launch_pair<true>(a, s) : launch_pair<false>(a, s);
-  return w->gated ? launch_stream<true>(a, s) : launch_stream<false>(a, s);
+  return w->gated ? launch_product<true>(a, s) : launch_product<false>(a, s);
 }
 
 // ---- handles -------------------------------------------------------------------------------------------------------------------
