@@ -69,18 +69,41 @@ struct I8Scale {
 template <typename T>
 struct Eight { uint4 r[sizeof(T) / 2]; };
 
+// From column c of a row of n on; fit: rows start on 16 bytes.  Elsewhere the 16-byte pieces that hold the numbers are fetched and shifted into place
+// (rows of 5003 bf16 and f32 one number at a time took three times as long); at a row's ends, where a piece would reach beyond it, one by one.
 template <typename T>
 __device__ __forceinline__ Eight<T> load_eight(const T* p, int c, int n, bool fit) {
+  constexpr int R = sizeof(T) / 2, kWords = 4 * R;
   Eight<T> e;
+  const uint32_t off = fit ? 0u : (uint32_t)(reinterpret_cast<uintptr_t>(p + c) & 15);
+  const int before = (int)(off / sizeof(T));  // numbers of the first piece that come ahead
   if (fit && c + 8 <= n) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) e.r[i] = reinterpret_cast<const uint4*>(p + c)[i];
+    for (int i = 0; i < R; ++i) e.r[i] = reinterpret_cast<const uint4*>(p + c)[i];
+  } else if (!fit && c >= before && c - before + 8 + 16 / (int)sizeof(T) <= n) {
+    const uint4* at = reinterpret_cast<const uint4*>(p + c - before);
+    uint32_t w[kWords + 4];
+#pragma unroll
+    for (int i = 0; i <= R; ++i) {
+      const uint4 q = at[i];
+      w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
+    }
+#pragma unroll
+    for (int i = 0; i < kWords + 2; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < kWords + 1; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (off & 2) * 8);
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) e.r[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
   } else {
     T v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = c + i < n ? p[c + i] : T(0.f);
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+    for (int i = 0; i < R; ++i) {
       uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {

@@ -28,33 +28,60 @@ struct ResidualNormArgs {
   int fit;  // bits: which rows may be read and written in vectors of eight
   float scale, eps;
 };
-enum { kFitH = 1, kFitY = 2, kFitGate = 4, kFitPost = 8, kFitNorm = 16, kFitHOut = 32, kFitXOut = 64 };
+enum { kFitH = 1, kFitY = 2, kFitGate = 4, kFitPost = 8, kFitNorm = 16, kFitHOut = 32, kFitXOut = 64, kFitAll = 127 };
 
+// The lanes' numbers, eight for each, neighbouring lanes' next to one another, to a row of n from column c of each lane on.  Where rows do not start on 16
+// bytes a lane's numbers behind the first boundary and the next lane's ahead of it are a piece; a warp's ends go one by one.  (All lanes of the warp.)
 template <typename T>
 __device__ __forceinline__ void store_eight(T* p, int c, int n, bool fit, const float (&v)[8]) {
-  if (fit && c + 8 <= n) {
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(p + c) = make_float4(v[0], v[1], v[2], v[3]);
-      *reinterpret_cast<float4*>(p + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      uint32_t w[4];
+  constexpr int kWords = 2 * (int)sizeof(T);
+  uint32_t w[kWords + 4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&b);
-      }
-      *reinterpret_cast<uint4*>(p + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  for (int i = 0; i < kWords; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      w[i] = __float_as_uint(v[i]);
+    } else {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&b);
     }
-  } else {
+  }
+  if (fit) {
+    if (c + 8 <= n) {
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i) reinterpret_cast<uint4*>(p + c)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (c + i < n) st(p + c + i, v[i]);
+    return;
   }
+  const uint32_t off = (16u - (uint32_t)(reinterpret_cast<uintptr_t>(p + c) & 15)) & 15;  // bytes up to the first boundary
+  const int head = (int)(off / sizeof(T)), lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[kWords + i] = __shfl_down_sync(0xffffffffu, w[i], 1);
+#pragma unroll
+  for (int i = 0; i < kWords + 2; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < kWords + 1; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (off & 2) * 8);
+  }
+  const bool pieces = (lane < 31 || head == 0) && c + head + 8 <= n;
+  if (pieces) {
+#pragma unroll
+    for (int i = 0; i < kWords / 4; ++i) reinterpret_cast<uint4*>(p + c + head)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  }
+  const bool before = lane == 0 || c + head > n;  // the lane ahead has not taken this one's first
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (c + i < n && (i < head ? before : !pieces)) st(p + c + i, v[i]);
 }
 
-// NV vectors of eight columns for each thread.  WARP: a warp for a row.  (1024 threads with 32 numbers each have 64 registers: half of a row's y is
+// NV vectors of eight columns for each thread.  WARP: a warp for a row.  FIT: all rows start on 16 bytes and are whole vectors.  (1024 threads with 32 numbers each have 64 registers: half of a row's y is
 // still in its 16 bits while h comes.)
-template <typename H, typename Y, int NV, bool WARP>
+template <typename H, typename Y, int NV, bool WARP, bool FIT>
 __global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const __grid_constant__ ResidualNormArgs a) {
   after_previous();
   __shared__ float part[3][32];
@@ -76,9 +103,20 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const 
   Eight<Y> yr[NV];
   Eight<H> hr[NV];
 #pragma unroll
-  for (int u = 0; u < NV; ++u) yr[u] = load_eight(y, column(u), a.n, a.fit & kFitY);
+  for (int u = 0; u < NV; ++u) yr[u] = load_eight(y, column(u), a.n, FIT || (a.fit & kFitY));
 #pragma unroll
-  for (int u = 0; u < NV; ++u) hr[u] = load_eight(h, column(u), a.n, a.fit & kFitH);
+  for (int u = 0; u < NV; ++u) hr[u] = load_eight(h, column(u), a.n, FIT || (a.fit & kFitH));
+  Eight<__nv_bfloat16> gr[NV <= 2 ? NV : 1];
+  if (NV <= 2 && a.gate) {
+#pragma unroll
+    for (int u = 0; u < NV; ++u) gr[u] = load_eight(a.gate + (size_t)row * a.gate_stride, column(u), a.n, FIT || (a.fit & kFitGate));
+  }
+  Eight<__nv_bfloat16> pr[NV <= 2 ? NV : 1], nr[NV == 1 ? NV : 1];
+  if (NV <= 2 && a.post_w) {
+#pragma unroll
+    for (int u = 0; u < NV; ++u) pr[u] = load_eight(a.post_w, column(u), a.n, FIT || (a.fit & kFitPost));
+  }
+  if (NV == 1 && a.norm_w) nr[0] = load_eight(a.norm_w, column(0), a.n, FIT || (a.fit & kFitNorm));
   float ry = 1.f;
   if (a.post_w) {
     float ss = 0.f;
@@ -100,12 +138,12 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const 
     float p[8], w[8];
     widen(yr[u], p);
     if (a.post_w) {
-      widen(load_eight(a.post_w, c, a.n, a.fit & kFitPost), w);
+      widen(NV <= 2 ? pr[NV <= 2 ? u : 0] : load_eight(a.post_w, c, a.n, FIT || (a.fit & kFitPost)), w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) p[e] = p[e] * ry * w[e];
     }
     if (a.gate) {
-      widen(load_eight(a.gate + (size_t)row * a.gate_stride, c, a.n, a.fit & kFitGate), w);
+      widen(NV <= 2 ? gr[NV <= 2 ? u : 0] : load_eight(a.gate + (size_t)row * a.gate_stride, c, a.n, FIT || (a.fit & kFitGate)), w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) p[e] *= a.sigmoid ? __fdividef(1.0f, 1.0f + __expf(-w[e])) : w[e];
     }
@@ -115,9 +153,9 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const 
       x[u][e] = fmaf(a.scale, p[e], w[e]);
       ss = fmaf(x[u][e], x[u][e], ss);  // (behind the last column all is zero)
     }
-    if (c < a.n) store_eight((H*)a.h_out + (size_t)row * a.h_out_stride, c, a.n, a.fit & kFitHOut, x[u]);
+    store_eight((H*)a.h_out + (size_t)row * a.h_out_stride, c, a.n, FIT || (a.fit & kFitHOut), x[u]);
     if (a.norm_w) {
-      widen(load_eight(a.norm_w, c, a.n, a.fit & kFitNorm), w);
+      widen(NV == 1 ? nr[0] : load_eight(a.norm_w, c, a.n, FIT || (a.fit & kFitNorm)), w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[u][e] *= w[e];
     }
@@ -136,7 +174,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const 
   for (int u = 0; u < NV; ++u) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[u][e] *= r;
-    if (a.x_out && column(u) < a.n) store_eight(a.x_out + (size_t)row * a.x_out_stride, column(u), a.n, a.fit & kFitXOut, x[u]);
+    if (a.x_out) store_eight(a.x_out + (size_t)row * a.x_out_stride, column(u), a.n, FIT || (a.fit & kFitXOut), x[u]);
   }
   if (!a.q.q) return;
   if constexpr (!WARP) most = __reduce_max_sync(0xffffffffu, (t & 31) < (threads >> 5) ? __float_as_uint(part[2][t & 31]) : 0u);
@@ -147,25 +185,30 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const 
     if (column(u) < a.chunks * kI8Chunk) i8_store8(a.q.q, row, column(u), a.chunks, s, x[u]);
 }
 
-template <typename H, typename Y>
+template <typename H, typename Y, bool FIT>
 b200_status launch(const ResidualNormArgs& a, cudaStream_t s) {
   const int vectors = a.chunks * (kI8Chunk / 8);
   if (vectors <= 32 * 2) {
     const int warps = a.rows >= 8 * b200_sm_count() ? 8 : 1;
     const unsigned grid = (unsigned)((a.rows + warps - 1) / warps);
-    if (vectors <= 32) launch_after(residual_norm_kernel<H, Y, 1, true>, grid, warps * 32, 0, s, a);
-    else launch_after(residual_norm_kernel<H, Y, 2, true>, grid, warps * 32, 0, s, a);
+    if (vectors <= 32) launch_after(residual_norm_kernel<H, Y, 1, true, FIT>, grid, warps * 32, 0, s, a);
+    else launch_after(residual_norm_kernel<H, Y, 2, true, FIT>, grid, warps * 32, 0, s, a);
   } else {
     // few rows: more threads, each with fewer loads to wait for
     const bool few = a.rows <= 2 * b200_sm_count();
     const int nv = vectors <= 1024 && few ? 1 : vectors <= 2048 ? 2 : 4;
     const int threads = (vectors + 32 * nv - 1) / (32 * nv) * 32;
-    if (nv == 1) launch_after(residual_norm_kernel<H, Y, 1, false>, a.rows, threads, 0, s, a);
-    else if (nv == 2) launch_after(residual_norm_kernel<H, Y, 2, false>, a.rows, threads, 0, s, a);
-    else launch_after(residual_norm_kernel<H, Y, 4, false>, a.rows, threads, 0, s, a);
+    if (nv == 1) launch_after(residual_norm_kernel<H, Y, 1, false, FIT>, a.rows, threads, 0, s, a);
+    else if (nv == 2) launch_after(residual_norm_kernel<H, Y, 2, false, FIT>, a.rows, threads, 0, s, a);
+    else launch_after(residual_norm_kernel<H, Y, 4, false, FIT>, a.rows, threads, 0, s, a);
   }
   B200_LAUNCH_CHECK();
   return B200_OK;
+}
+
+template <typename H, typename Y>
+b200_status launch_any(const ResidualNormArgs& a, cudaStream_t s) {
+  return a.n % 8 == 0 && a.fit == kFitAll ? launch<H, Y, true>(a, s) : launch<H, Y, false>(a, s);
 }
 
 constexpr int kMostColumns = 32768;  // 1024 threads of four vectors
@@ -205,6 +248,6 @@ extern "C" b200_status b200_residual_norm(const b200_residual_norm_shape* shape,
   a.fit = fits(d_h, h_stride, h_size, kFitH) | fits(d_y, y_stride, y_size, kFitY) | fits(d_gate, gate_stride, 2, kFitGate) | fits(d_post_weight, 0, 2, kFitPost) |
           fits(d_norm_weight, 0, 2, kFitNorm) | fits(d_h_out, h_out_stride, h_size, kFitHOut) | fits(d_x_out, x_out_stride, 2, kFitXOut);
   cudaStream_t s = (cudaStream_t)stream;
-  if (shape->h_f32) return shape->y_f32 ? launch<float, float>(a, s) : launch<float, __nv_bfloat16>(a, s);
-  return shape->y_f32 ? launch<__nv_bfloat16, float>(a, s) : launch<__nv_bfloat16, __nv_bfloat16>(a, s);
+  if (shape->h_f32) return shape->y_f32 ? launch_any<float, float>(a, s) : launch_any<float, __nv_bfloat16>(a, s);
+  return shape->y_f32 ? launch_any<__nv_bfloat16, float>(a, s) : launch_any<__nv_bfloat16, __nv_bfloat16>(a, s);
 }
