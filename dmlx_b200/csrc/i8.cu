@@ -18,39 +18,35 @@
 namespace {
 
 // ---- rows into 8 bits ----------------------------------------------------------------------------------------------------
-// A block per row, or a warp for rows of up to 32 * 8 * NV columns; the row waits in registers while its largest is looked for.  Bound by
-// what it reads and writes.
-template <typename T>
+// A row waits in registers while its largest is looked for: a block for each, or a warp where a row is short.  Bound by what it reads and writes.
 struct QuantizeArgs {
-  const T* x;
+  const __nv_bfloat16* x;
   long long x_stride;
   signed char* q;
   float* scale;
   int rows, k, chunks, aligned;
 };
 
-// NV: vectors of eight columns of a thread; 0: any number, the row is read twice.  WARP: a warp for a row.
-template <typename T, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) i8_quantize_kernel(QuantizeArgs<T> a) {
+// NV: vectors of eight columns of a thread; 0: any number, the row is read twice.  WARP: a warp for a row.  FIT: rows start on 16 bytes and are whole vectors.
+template <int NV, bool WARP, bool FIT>
+__global__ void __launch_bounds__(WARP ? 256 : 1024) i8_quantize_kernel(QuantizeArgs a) {
   after_previous();
   __shared__ uint32_t part[32];
   const int threads = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
   const int row = WARP ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
   if (row >= a.rows) return;
-  const T* x = a.x + (size_t)row * a.x_stride;
+  const __nv_bfloat16* x = a.x + (size_t)row * a.x_stride;
   const int vectors = a.chunks * (kI8Chunk / 8);
-  Eight<T> keep[NV > 0 ? NV : 1];
+  auto load = [&](int v) { return load_eight(x, v * 8, a.k, FIT || a.aligned); };
+  Eight<__nv_bfloat16> keep[NV > 0 ? NV : 1];
   uint32_t most = 0u;
   if constexpr (NV > 0) {
 #pragma unroll
-    for (int u = 0; u < NV; ++u) keep[u] = load_eight(x, (t + u * threads) * 8, a.k, a.aligned);
+    for (int u = 0; u < NV; ++u) keep[u] = load(t + u * threads);
 #pragma unroll
     for (int u = 0; u < NV; ++u) most = most_of(most, keep[u]);
   } else {
-    for (int v = t; v < vectors; v += threads) {
-      keep[0] = load_eight(x, v * 8, a.k, a.aligned);
-      most = most_of(most, keep[0]);
-    }
+    for (int v = t; v < vectors; v += threads) most = most_of(most, load(v));
   }
   most = __reduce_max_sync(0xffffffffu, most);
   if constexpr (!WARP) {
@@ -60,45 +56,89 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) i8_quantize_kernel(Quantize
   }
   const I8Scale s = I8Scale::of(__uint_as_float(most));
   if (t == 0) a.scale[row] = s.step();
-  auto put = [&](int v, const Eight<T>& raw) {
+  // (a round further on is threads / 16 blocks further on, at the same place)
+  signed char* to = a.q + i8_at(row, t * 8, a.chunks);
+  auto put = [&](const Eight<__nv_bfloat16>& raw, int round) {
     float f[8];
     widen(raw, f);
-    i8_store8(a.q, row, v * 8, a.chunks, s, f);
+    *reinterpret_cast<uint2*>(to + (size_t)round * (threads / 16) * kI8Block) = s.quantize(f);
   };
   if constexpr (NV > 0) {
 #pragma unroll
     for (int u = 0; u < NV; ++u)
-      if (t + u * threads < vectors) put(t + u * threads, keep[u]);
+      if (t + u * threads < vectors) put(keep[u], u);
   } else {
-    for (int v = t; v < vectors; v += threads) {
-      keep[0] = load_eight(x, v * 8, a.k, a.aligned);
-      put(v, keep[0]);
+    for (int v = t, u = 0; v < vectors; v += threads, ++u) put(load(v), u);
+  }
+}
+
+template <bool FIT>
+void launch_quantize(const QuantizeArgs& a, cudaStream_t s) {
+  const int vectors = a.chunks * (kI8Chunk / 8), rows = a.rows;
+  if (vectors <= 32 * 2) {
+    const int warps = rows >= 8 * b200_sm_count() ? 8 : 1;
+    const unsigned grid = (unsigned)((rows + warps - 1) / warps);
+    if (vectors <= 32) launch_after(i8_quantize_kernel<1, true, FIT>, grid, warps * 32, 0, s, a);
+    else launch_after(i8_quantize_kernel<2, true, FIT>, grid, warps * 32, 0, s, a);
+  } else if (vectors <= 4 * 1024) {
+    const int nv = vectors <= 1024 ? 4 : vectors <= 2048 ? 2 : 4, threads = (vectors + 32 * nv - 1) / (32 * nv) * 32;
+    if (nv == 1) launch_after(i8_quantize_kernel<1, false, FIT>, rows, threads, 0, s, a);
+    else if (nv == 2) launch_after(i8_quantize_kernel<2, false, FIT>, rows, threads, 0, s, a);
+    else launch_after(i8_quantize_kernel<4, false, FIT>, rows, threads, 0, s, a);
+  } else {
+    launch_after(i8_quantize_kernel<0, false, FIT>, rows, 1024, 0, s, a);
+  }
+}
+
+b200_status quantize(const __nv_bfloat16* x, long long x_stride, int rows, int k, const I8RowsDev& to, cudaStream_t s) {
+  QuantizeArgs a;
+  a.x = x; a.x_stride = x_stride; a.q = to.q; a.scale = to.scale; a.rows = rows; a.k = k; a.chunks = i8_chunks(k);
+  a.aligned = ((uintptr_t)x & 15) == 0 && x_stride % 8 == 0;
+  if (a.aligned && k % 8 == 0) launch_quantize<true>(a, s);
+  else launch_quantize<false>(a, s);
+  B200_LAUNCH_CHECK();
+  return B200_OK;
+}
+
+// The feed-forward block's inner rows, of which the product that made them has left the largest of every 32 channels, so that nothing waits for a row to be
+// read and a row may be many blocks'.  A block's warps take eight neighbouring rows, whose bytes lie together.
+constexpr int kInnerThreads = 256, kInnerAhead = 4;  // (loads of 256 columns that a warp has in flight)
+
+__global__ void __launch_bounds__(kInnerThreads, 3) i8_quantize_inner_kernel(const float* h, long long h_stride, const float* most, int groups, signed char* __restrict__ q,
+                                                                             float* __restrict__ steps, int rows, int k, int chunks, int per_block) {
+  after_previous();
+  const int lane = threadIdx.x & 31, row = blockIdx.x * (kInnerThreads / 32) + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int first = blockIdx.y * per_block, last = min(first + per_block, chunks * kI8Chunk);
+  const float* from = h + (size_t)row * h_stride;
+  Eight<float> keep[kInnerAhead];
+  auto load = [&](int c0) {
+#pragma unroll
+    for (int u = 0; u < kInnerAhead; ++u) keep[u] = load_eight(from, c0 + u * 256 + lane * 8, k, true);
+  };
+  load(first);
+  uint32_t m = 0u;
+  for (int g = lane; g < groups; g += 32) m = max(m, __float_as_uint(most[(size_t)row * groups + g]));
+  const I8Scale s = I8Scale::of(__uint_as_float(__reduce_max_sync(0xffffffffu, m)));
+  if (blockIdx.y == 0 && lane == 0) steps[row] = s.step();
+  signed char* to = q + i8_at(row, first + lane * 8, chunks);
+  for (int c0 = first; c0 < last; c0 += kInnerAhead * 256, to += kInnerAhead * 2 * kI8Block) {
+    if (c0 > first) load(c0);
+#pragma unroll
+    for (int u = 0; u < kInnerAhead; ++u) {
+      float f[8];
+      widen(keep[u], f);
+      if (c0 + u * 256 + lane * 8 < last) *reinterpret_cast<uint2*>(to + u * 2 * kI8Block) = s.quantize(f);
     }
   }
 }
 
-template <typename T>
-b200_status quantize(const T* x, long long x_stride, int rows, int k, const I8RowsDev& to, cudaStream_t s) {
-  QuantizeArgs<T> a;
-  a.x = x; a.x_stride = x_stride; a.q = to.q; a.scale = to.scale; a.rows = rows; a.k = k; a.chunks = i8_chunks(k);
-  a.aligned = ((uintptr_t)x & 15) == 0 && x_stride * sizeof(T) % 16 == 0;
-  const int vectors = a.chunks * (kI8Chunk / 8);
-  if (vectors <= 32 * 4) {
-    const int warps = rows >= 8 * b200_sm_count() ? 8 : 1;
-    const unsigned grid = (unsigned)((rows + warps - 1) / warps);
-    if (vectors <= 32 * 1) launch_after(i8_quantize_kernel<T, 1, true>, grid, warps * 32, 0, s, a);
-    else if (vectors <= 32 * 2) launch_after(i8_quantize_kernel<T, 2, true>, grid, warps * 32, 0, s, a);
-    else launch_after(i8_quantize_kernel<T, 4, true>, grid, warps * 32, 0, s, a);
-  } else if (vectors <= 4 * 1024) {
-    // few rows: more threads, each with fewer loads to wait for
-    const int nv = vectors <= 1024 && rows <= 2 * b200_sm_count() ? 1 : vectors <= 2048 && rows <= 2 * b200_sm_count() ? 2 : 4;
-    const int threads = (vectors + 32 * nv - 1) / (32 * nv) * 32;
-    if (nv == 1) launch_after(i8_quantize_kernel<T, 1, false>, rows, threads, 0, s, a);
-    else if (nv == 2) launch_after(i8_quantize_kernel<T, 2, false>, rows, threads, 0, s, a);
-    else launch_after(i8_quantize_kernel<T, 4, false>, rows, threads, 0, s, a);
-  } else {
-    launch_after(i8_quantize_kernel<T, 0, false>, rows, 1024, 0, s, a);
-  }
+b200_status quantize_inner(const b200_i8_rows* r, int rows, int k, cudaStream_t s) {
+  const int chunks = i8_chunks(k), eights = (rows + 7) / 8;
+  int per_block = kInnerAhead * 256;  // columns: fewer blocks where there are enough of them
+  while (per_block < 4096 && (long long)eights * ((chunks * kI8Chunk + per_block - 1) / per_block) >= 8 * b200_sm_count()) per_block *= 2;
+  launch_after(i8_quantize_inner_kernel, dim3(eights, (chunks * kI8Chunk + per_block - 1) / per_block), kInnerThreads, 0, s, r->h, (long long)r->h_stride, r->most, chunks * 4,
+               r->hidden.q, r->hidden.scale, rows, k, chunks, per_block);
   B200_LAUNCH_CHECK();
   return B200_OK;
 }
@@ -139,6 +179,7 @@ struct MmArgs {
   const float* bias;
   void* y;
   long long y_stride;
+  float* most;  // a feed-forward block's inner rows: [row][tiles * 2] the largest magnitude of 32 channels
   int* err;
   int rows, n, chunks, tiles, tn, stages, shares;
   int over_stages, pushed_at, bars_at;  // places in shared memory (i8_stream_kernel)
@@ -374,6 +415,15 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
       float y[16];
 #pragma unroll
       for (int j = 0; j < 16; ++j) y[j] = output_of<GATED>(a, (int)v[j], GATED ? (int)u[j] : 0, ws, us, __shfl_sync(0xffffffffu, steps, j), bias);
+      if constexpr (GATED) {  // lane j keeps row j's
+        uint32_t most = 0u;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(y[j]) & 0x7fffffffu);
+          if (lane == j) most = m;
+        }
+        if (c0 + lane < mine1 && lane < 16) a.most[(size_t)(t0 + c0 + lane) * (a.tiles * 2) + tile * 4 + quarter] = __uint_as_float(most);
+      }
       const size_t at = (size_t)(t0 + c0) * a.y_stride + channel;
       const int rows_left = channel < a.n ? mine1 - c0 : 0;
       if (GATED || a.y_f32) {
@@ -429,7 +479,11 @@ __device__ __forceinline__ void commit_pair(uint32_t bar, uint16_t ctas) {
 template <bool GATED>
 __device__ __forceinline__ void store_sums(const MmArgs& a, uint32_t (&v)[32], const uint32_t (&u)[GATED ? 32 : 1], float* mine, const float* scales, int first_tile, int c0, int row0, float row_step) {
   const int lane = threadIdx.x & 31, rows_here = min(32, a.rows - row0), n0 = (GATED ? first_tile / 2 : first_tile) * kI8Tile + c0, cols = min(32, a.n - n0);
-  if (cols <= 0 || rows_here <= 0) return;
+  if (rows_here <= 0) return;
+  if (cols <= 0) {  // (nothing is the largest there)
+    if (GATED && lane < rows_here) a.most[(size_t)(row0 + lane) * (a.tiles * 2) + n0 / 32] = 0.f;
+    return;
+  }
 #pragma unroll
   for (int j4 = 0; j4 < 8; ++j4) {
     const float4 w4 = *reinterpret_cast<const float4*>(scales + 4 * j4), o4 = *reinterpret_cast<const float4*>(scales + kI8Tile + 4 * j4);
@@ -437,6 +491,12 @@ __device__ __forceinline__ void store_sums(const MmArgs& a, uint32_t (&v)[32], c
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       v[4 * j4 + e] = __float_as_uint(output_of<GATED>(a, (int)v[4 * j4 + e], GATED ? (int)u[4 * j4 + e] : 0, w[e], GATED ? o[e] : 0.f, row_step, GATED ? 0.f : o[e]));
+  }
+  if constexpr (GATED) {
+    uint32_t most = 0u;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) most = max(most, v[j] & 0x7fffffffu);
+    if (lane < rows_here) a.most[(size_t)(row0 + lane) * (a.tiles * 2) + n0 / 32] = __uint_as_float(most);
   }
   if (GATED || a.y_f32) {
 #pragma unroll
@@ -772,7 +832,7 @@ Plan plan_of(const MmArgs& a, const int* stream_at_once, const int* pairs_at_onc
   for (int n = 1; n <= kMostPairs; ++n) {
     if (!split(n, 4) || pairs_at_once[n] < 1 || (n > 1 && items > pairs_at_once[n])) continue;
     const float waves = (float)((items + pairs_at_once[n] - 1) / pairs_at_once[n]);
-    const float us = (n == 1 ? 6.4f : 7.6f) + waves * (0.8f + 0.27f * ((a.chunks + n - 1) / n));
+    const float us = (n == 1 ? 6.4f : 7.6f) + waves * ((GATED ? 2.5f : 0.8f) + 0.27f * ((a.chunks + n - 1) / n));
     if (us < best.us) best = {us, true, 0, n};
   }
   return best;
@@ -818,11 +878,11 @@ b200_status launch_product(MmArgs& a, cudaStream_t s) {
   return B200_OK;
 }
 
-b200_status product(const b200_i8_weight* w, const I8RowsDev& x, int rows, const float* bias, int act, void* y, long long y_stride, int y_f32, cudaStream_t s) {
+b200_status product(const b200_i8_weight* w, const I8RowsDev& x, int rows, const float* bias, int act, void* y, long long y_stride, int y_f32, float* most, cudaStream_t s) {
   MmArgs a{};
   b200_status st = b200_qmm_ensure_err_word(&a.err);
   if (st != B200_OK) return st;
-  a.w = w->q; a.w_scale = w->scale; a.q = x.q; a.step = x.scale; a.bias = bias; a.y = y; a.y_stride = y_stride; a.y_f32 = y_f32; a.act = act;
+  a.w = w->q; a.w_scale = w->scale; a.q = x.q; a.step = x.scale; a.bias = bias; a.y = y; a.y_stride = y_stride; a.y_f32 = y_f32; a.act = act; a.most = most;
   a.rows = rows; a.n = w->n; a.chunks = w->chunks; a.tiles = w->tiles;
   a.y_vec = ((uintptr_t)y & 15) == 0 && y_stride * (w->gated || y_f32 ? 4 : 2) % 16 == 0;
   return w->gated ? launch_product<true>(a, s) : launch_product<false>(a, s);
@@ -956,6 +1016,7 @@ extern "C" b200_status b200_i8_rows_create(int32_t max_rows, int32_t max_k, int3
   if (max_hidden > 0) {
     make(r->hidden, max_hidden);
     if (e == cudaSuccess) e = cudaMalloc((void**)&r->h, sizeof(float) * (size_t)max_rows * r->h_stride);
+    if (e == cudaSuccess) e = cudaMalloc((void**)&r->most, sizeof(float) * (size_t)max_rows * i8_chunks(max_hidden) * 4);
   }
   if (e == cudaSuccess) e = cudaDeviceSynchronize();
   if (e != cudaSuccess) {
@@ -970,7 +1031,7 @@ extern "C" b200_status b200_i8_rows_create(int32_t max_rows, int32_t max_k, int3
 
 extern "C" void b200_i8_rows_destroy(b200_i8_rows* r) {
   if (!r) return;
-  for (void* p : {(void*)r->x.q, (void*)r->x.scale, (void*)r->hidden.q, (void*)r->hidden.scale, (void*)r->h}) if (p) cudaFree(p);
+  for (void* p : {(void*)r->x.q, (void*)r->x.scale, (void*)r->hidden.q, (void*)r->hidden.scale, (void*)r->h, (void*)r->most}) if (p) cudaFree(p);
   delete r;
 }
 
@@ -1000,7 +1061,7 @@ extern "C" b200_status b200_i8_mm(const b200_i8_weight* w, b200_i8_rows* r, cons
   if (st == B200_OK) st = b200_require_device();
   if (st == B200_OK) st = take_rows("i8 mm", r, d_x, x_stride, rows, w->k, (cudaStream_t)stream);
   if (st != B200_OK || rows == 0) return st;
-  return product(w, r->x, rows, d_bias, 0, d_y, y_stride, y_f32 != 0, (cudaStream_t)stream);
+  return product(w, r->x, rows, d_bias, 0, d_y, y_stride, y_f32 != 0, nullptr, (cudaStream_t)stream);
 }
 
 extern "C" b200_status b200_i8_ffn(const b200_i8_weight* gate_up, const b200_i8_weight* down, b200_i8_rows* r, const void* d_x, int64_t x_stride, int32_t rows,
@@ -1017,8 +1078,8 @@ extern "C" b200_status b200_i8_ffn(const b200_i8_weight* gate_up, const b200_i8_
   if (st == B200_OK) st = take_rows("i8 ffn", r, d_x, x_stride, rows, gate_up->k, (cudaStream_t)stream);
   if (st != B200_OK || rows == 0) return st;
   cudaStream_t s = (cudaStream_t)stream;
-  st = product(gate_up, r->x, rows, nullptr, activation, r->h, r->h_stride, 0, s);
-  if (st == B200_OK) st = quantize(r->h, r->h_stride, rows, down->k, r->hidden, s);
-  if (st == B200_OK) st = product(down, r->hidden, rows, nullptr, 0, d_y, y_stride, 0, s);
+  st = product(gate_up, r->x, rows, nullptr, activation, r->h, r->h_stride, 0, r->most, s);
+  if (st == B200_OK) st = quantize_inner(r, rows, down->k, s);
+  if (st == B200_OK) st = product(down, r->hidden, rows, nullptr, 0, d_y, y_stride, 0, nullptr, s);
   return st;
 }

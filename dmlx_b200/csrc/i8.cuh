@@ -29,6 +29,7 @@ struct b200_i8_rows {
   // rounded twice goes to another of 255 numbers one time in twenty, and a rounded largest moves a row's every step).
   float* h = nullptr;
   int h_stride = 0;
+  float* most = nullptr;                // [max_rows][their groups of 32 channels]: the largest magnitude in each
 };
 
 struct b200_i8_weight {
@@ -48,23 +49,37 @@ __device__ __forceinline__ size_t i8_at(int row, int c, int chunks) {
 }
 
 // A row's numbers as multiples of most / 127, most = its largest magnitude.  The quotient 127 x / most is rounded to the nearest, halves to the even, as if
-// it were exact: the product with the rounded 127 / most is at most 2^-15 off, and where that could decide, the division is made.  (For x of bf16 127 x is
-// exact, and the division rounds correctly: halves are numbers of f32, so it can reach one but not cross it, and nothing is left to chance.)
+// it were exact: its product with the rounded 127 / most is at most 127 * 2^-24 off, and where that could decide, the division is made.  (For x of bf16
+// 127 x is exact, and the division rounds correctly: halves are numbers of f32, so it can reach one but not cross it, and nothing is left to chance.)
 struct I8Scale {
   float most, inv;
-  static __device__ __forceinline__ I8Scale of(float m) { return I8Scale{m, __fdiv_rn(127.0f, m)}; }
+  bool plain;  // else all zeros: a row of nothing, or one without numbers
+  static __device__ __forceinline__ I8Scale of(float m) { return I8Scale{m, __fdiv_rn(127.0f, m), m > 0.f && m < __int_as_float(0x7f800000)}; }
   __device__ __forceinline__ float step() const { return __fdiv_rn(most, 127.0f); }
-  __device__ __forceinline__ bool plain() const { return most > 0.f && most < __int_as_float(0x7f800000); }  // else all zeros: a row of nothing, or one without numbers
-  __device__ __forceinline__ int quantize(float x) const {
-    const float t = x * inv;
-    float r = rintf(t);
-    if (!(fabsf(t - r) < 0.4999f)) {
-      const float down = most > 1e30f ? 0.00390625f : 1.0f;  // (127 times the largest numbers is none of f32)
-      r = rintf(__fdiv_rn(127.0f * (x * down), most * down));
+  // The eight numbers in eight bytes.  (1.5 * 2^23 added leaves the nearest whole number in the low bits.)
+  __device__ __forceinline__ uint2 quantize(const float (&v)[8]) const {
+    if (!plain) return make_uint2(0u, 0u);
+    constexpr float kWhole = 12582912.0f, kNearHalf = 0.49999f;
+    uint32_t q[8];
+    float d[8], off = 0.f;  // distances to the whole numbers, the largest
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float r = fmaf(v[e], inv, kWhole);
+      d[e] = fmaf(v[e], inv, kWhole - r);
+      off = fmaxf(off, fabsf(d[e]));
+      q[e] = __float_as_uint(r);
     }
-    return (int)r;
+    if (!(off < kNearHalf) || !(inv < 1e38f)) {  // (or 127 / most is no f32)
+      const float down = most > 1e30f ? 0.00390625f : 1.0f;  // (127 times the largest numbers is none either)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (!(fabsf(d[e]) < kNearHalf) || !(inv < 1e38f)) q[e] = (uint32_t)(int)rintf(__fdiv_rn(127.0f * (v[e] * down), most * down));
+    }
+    return make_uint2(__byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410));
   }
 };
+
 // Eight neighbouring numbers of a row as they lie in memory, those behind the last as zeros.
 template <typename T>
 struct Eight { uint4 r[sizeof(T) / 2]; };
@@ -144,11 +159,6 @@ __device__ __forceinline__ uint32_t most_of(uint32_t m, const Eight<float>& e) {
 
 // Eight neighbouring columns, the first a multiple of eight.
 __device__ __forceinline__ void i8_store8(signed char* q, int row, int c, int chunks, const I8Scale& s, const float (&v)[8]) {
-  uint32_t w[2] = {0u, 0u};
-  if (s.plain()) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w[e / 4] |= ((uint32_t)s.quantize(v[e]) & 0xffu) << (8 * (e % 4));
-  }
-  *reinterpret_cast<uint2*>(q + i8_at(row, c, chunks)) = make_uint2(w[0], w[1]);
+  *reinterpret_cast<uint2*>(q + i8_at(row, c, chunks)) = s.quantize(v);
 }
 #endif
