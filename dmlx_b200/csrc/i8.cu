@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <new>
+#include <type_traits>
 
 #include "common.h"
 #include "i8.cuh"
@@ -41,8 +42,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) i8_quantize_kernel(Quantize
   Eight<__nv_bfloat16> keep[NV > 0 ? NV : 1];
   uint32_t most = 0u;
   if constexpr (NV > 0) {
-#pragma unroll
-    for (int u = 0; u < NV; ++u) keep[u] = load(t + u * threads);
+    load_eights(keep, x, a.k, FIT || a.aligned, [&](int u) { return (t + u * threads) * 8; });
 #pragma unroll
     for (int u = 0; u < NV; ++u) most = most_of(most, keep[u]);
   } else {
@@ -81,7 +81,8 @@ void launch_quantize(const QuantizeArgs& a, cudaStream_t s) {
     if (vectors <= 32) launch_after(i8_quantize_kernel<1, true, FIT>, grid, warps * 32, 0, s, a);
     else launch_after(i8_quantize_kernel<2, true, FIT>, grid, warps * 32, 0, s, a);
   } else if (vectors <= 4 * 1024) {
-    const int nv = vectors <= 1024 ? 4 : vectors <= 2048 ? 2 : 4, threads = (vectors + 32 * nv - 1) / (32 * nv) * 32;
+    // few rows: more threads, each with fewer loads to wait for (96 rows of 4096 2.7 us with one, 4.6 with four; 8192 33 and 24)
+    const int nv = rows > 4 * b200_sm_count() || vectors > 2048 ? 4 : vectors > 1024 ? 2 : 1, threads = (vectors + 32 * nv - 1) / (32 * nv) * 32;
     if (nv == 1) launch_after(i8_quantize_kernel<1, false, FIT>, rows, threads, 0, s, a);
     else if (nv == 2) launch_after(i8_quantize_kernel<2, false, FIT>, rows, threads, 0, s, a);
     else launch_after(i8_quantize_kernel<4, false, FIT>, rows, threads, 0, s, a);
@@ -104,7 +105,7 @@ b200_status quantize(const __nv_bfloat16* x, long long x_stride, int rows, int k
 // read and a row may be many blocks'.  A block's warps take eight neighbouring rows, whose bytes lie together.
 constexpr int kInnerThreads = 256, kInnerAhead = 4;  // (loads of 256 columns that a warp has in flight)
 
-__global__ void __launch_bounds__(kInnerThreads, 3) i8_quantize_inner_kernel(const float* h, long long h_stride, const float* most, int groups, signed char* __restrict__ q,
+__global__ void __launch_bounds__(kInnerThreads, 2) i8_quantize_inner_kernel(const float* h, long long h_stride, const float* most, int groups, signed char* __restrict__ q,
                                                                              float* __restrict__ steps, int rows, int k, int chunks, int per_block) {
   after_previous();
   const int lane = threadIdx.x & 31, row = blockIdx.x * (kInnerThreads / 32) + (threadIdx.x >> 5);
@@ -113,8 +114,7 @@ __global__ void __launch_bounds__(kInnerThreads, 3) i8_quantize_inner_kernel(con
   const float* from = h + (size_t)row * h_stride;
   Eight<float> keep[kInnerAhead];
   auto load = [&](int c0) {
-#pragma unroll
-    for (int u = 0; u < kInnerAhead; ++u) keep[u] = load_eight(from, c0 + u * 256 + lane * 8, k, true);
+    load_eights(keep, from, k, true, [&](int u) { return c0 + u * 256 + lane * 8; });
   };
   load(first);
   uint32_t m = 0u;
@@ -182,7 +182,14 @@ struct MmArgs {
   float* most;  // a feed-forward block's inner rows: [row][tiles * 2] the largest magnitude of 32 channels
   int* err;
   int rows, n, chunks, tiles, tn, stages, shares;
-  int over_stages, pushed_at, bars_at;  // places in shared memory (i8_stream_kernel)
+  int over_stages, pushed_at, raw_at, bars_at;  // places in shared memory (i8_stream_kernel)
+  // Rows that the kernel brings into 8 bits itself
+  const void* raw;
+  long long raw_stride;
+  int raw_inner, raw_fit, k;  // f32, with the largest of every 32 channels in raw_most; or bf16, which go into q_out and step_out as well
+  const float* raw_most;
+  signed char* q_out;
+  float* step_out;
   int y_vec;       // rows of y start on 16 bytes
   int y_f32, act;  // (a feed-forward block's inner rows are f32)
 };
@@ -199,19 +206,23 @@ __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64
 // Instruction descriptor: signed 8-bit A and B (both K-major), 32-bit sums, tile m x n.
 __device__ __forceinline__ uint32_t idesc_i8(uint32_t m, uint32_t n) { return 2u << 4 | 1u << 7 | 1u << 10 | (n >> 3) << 17 | (m >> 4) << 24; }
 
-__device__ __forceinline__ float activated(int act, float g) {
-  if (act == B200_ACT_SILU) return __fdividef(g, 1.0f + __expf(-g));  // (a divisor past 2^126 makes 0, as it should)
-  if (act == B200_ACT_GELU) return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
+template <int ACT>
+__device__ __forceinline__ float activated(float g) {
+  if constexpr (ACT == B200_ACT_SILU) return __fdividef(g, 1.0f + __expf(-g));  // (a divisor past 2^126 makes 0, as it should)
+  if constexpr (ACT == B200_ACT_GELU) return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
   // 0.5 g (1 + tanh z) = g / (1 + e^-2z)
   return __fdividef(g, 1.0f + __expf(-1.5957691216057308f * (g + 0.044715f * g * g * g)));
 }
-
-// One output of a product; in a feed-forward block `u` is up's sum, and the gate's goes through the activation.
-template <bool GATED>
-__device__ __forceinline__ float output_of(const MmArgs& a, int sum, int up, float ws, float us, float step, float bias) {
-  const float y = (float)sum * ws * step + bias;
-  if constexpr (GATED) return activated(a.act, y) * ((float)up * us * step);
-  else return y;
+// y[j] = act(y[j]) * up[j]; the activation is chosen once.
+template <int N>
+__device__ __forceinline__ void gate_with(int act, float (&y)[N], const float (&up)[N]) {
+  auto each = [&](auto which) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) y[j] = activated<decltype(which)::value>(y[j]) * up[j];
+  };
+  if (act == B200_ACT_SILU) each(std::integral_constant<int, B200_ACT_SILU>{});
+  else if (act == B200_ACT_GELU) each(std::integral_constant<int, B200_ACT_GELU>{});
+  else each(std::integral_constant<int, B200_ACT_GELU_TANH>{});
 }
 
 // ---- up to a few hundred rows: streams of weights ----
@@ -222,6 +233,17 @@ __device__ __forceinline__ float output_of(const MmArgs& a, int sum, int up, flo
 // shared memory, where the stages were unless there is room beside them, with a barrier that counts their bytes.
 constexpr int kStreamThreads = 192, kStreamShared = 112 * 1024, kStreamAlone = 226 * 1024, kMostShares = 8;  // (shared memory of two CTAs on an SM, of one)
 
+// Weights that go through L2 once: they leave it ahead of what else is there.  (Among it are the instructions, which a kernel fetches anew: behind 117 MB of
+// weights the last ones came from memory, 4 to 8 us for the output of one row.)
+__device__ __forceinline__ uint64_t passing_through() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ void bulk_g2s_with(void* dst_smem, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(ptx::smem_u32(dst_smem)), "l"(src), "r"(bytes),
+               "r"(ptx::smem_u32(bar)), "l"(policy) : "memory");
+}
 // Four words to another CTA of the cluster, counted by a barrier there.
 __device__ __forceinline__ void push4(uint32_t mapped, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t mapped_bar) {
   asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(mapped), "r"(a), "r"(b), "r"(c), "r"(d),
@@ -242,17 +264,78 @@ __device__ __forceinline__ void tmem_ld4(uint32_t taddr, uint32_t& a, uint32_t& 
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(taddr) : "memory");
 }
 
-template <bool GATED>
+constexpr int kRawRows = 4, kRawNumbers = 16384, kRawChunks = 32;  // rows of RAW; their numbers at most; blocks of K in a share at most
+
+// Warps 2 to 5: rows into 8 bits, as i8_quantize_kernel and i8_quantize_inner_kernel do, blocks chunk0 and on as an operand of 16 rows each at `to` (the rows that
+// are not there hold anything), steps into `steps`; `out` and `first`: into the handle too, and the steps.
+template <typename T>
+__device__ __forceinline__ void raw_rows(const MmArgs& a, const T* x, bool fit, unsigned char* to, int chunk0, int chunks, bool out, bool first, uint64_t* ready, float* steps,
+                                         uint32_t* part) {
+  constexpr bool kInner = sizeof(T) == 4;
+  constexpr int kAhead = 4;
+  const int t = threadIdx.x - 64, lane = t & 31, warp = t >> 5;
+#pragma unroll 1
+  for (int r = 0; r < a.rows; ++r) {
+    uint32_t m = 0u;
+    if constexpr (kInner) {
+      for (int g = t; g < a.chunks * 4; g += 128) m = max(m, __float_as_uint(a.raw_most[(size_t)r * (a.chunks * 4) + g]));
+    } else {
+#pragma unroll 1
+      for (int v = t; v * 8 < a.k; v += kAhead * 128) {
+        Eight<T> e[kAhead];
+        load_eights(e, x + (size_t)r * a.raw_stride, a.k, fit, [&](int u) { return (v + u * 128) * 8; });
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) m = most_of(m, e[u]);
+      }
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0) part[warp * kRawRows + r] = m;
+  }
+  asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll 1
+  for (int r = 0; r < a.rows; ++r) {
+    const I8Scale s = I8Scale::of(__uint_as_float(max(max(part[r], part[kRawRows + r]), max(part[2 * kRawRows + r], part[3 * kRawRows + r]))));
+    if (t == 0) {
+      steps[r] = s.step();
+      if (out && first && !kInner) a.step_out[r] = s.step();
+    }
+#pragma unroll 1
+    for (int v = t; v < chunks * 16; v += kAhead * 128) {
+      Eight<T> e[kAhead];
+      load_eights(e, x + (size_t)r * a.raw_stride, a.k, fit, [&](int u) { return chunk0 * kI8Chunk + (v + u * 128) * 8; });
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int at = v + u * 128, piece = at & 15;
+        if (at >= chunks * 16) break;
+        float f[8];
+        widen(e[u], f);
+        const uint2 q = s.quantize(f);
+        *reinterpret_cast<uint2*>(to + (at >> 4) * 16 * kI8Chunk + r * kI8Chunk + (((piece >> 1) ^ r) << 4) + (piece & 1) * 8) = q;
+        if (out && !kInner) *reinterpret_cast<uint2*>(a.q_out + i8_at(r, chunk0 * kI8Chunk + at * 8, a.chunks)) = q;
+      }
+    }
+  }
+  ptx::fence_proxy_async_smem();
+  asm volatile("bar.sync 1, 128;" ::: "memory");  // the steps are there
+  if (lane == 0) ptx::mbar_arrive(ready);
+}
+
+// RAW: up to kRawRows rows that are not 8 bits yet: every CTA looks for their largest numbers itself and keeps its share of K in shared memory, while the first
+// weights come.  (A kernel of its own for one row costs 2.5 us, and as much of the host's time.)
+template <bool GATED, bool RAW>
 __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   constexpr int W = GATED ? 2 : 1;
-  const int S = a.stages, stage_bytes = W * kI8Block + a.tn * kI8Chunk;
+  const int S = a.stages, stage_bytes = W * kI8Block + (RAW ? 0 : a.tn * kI8Chunk);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + a.bars_at);
   uint64_t* done = full + S;
   uint64_t* sums = done + S;
   uint64_t* pushed = sums + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pushed + 1);
+  uint64_t* rows_ready = pushed + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rows_ready + 1);
+  float* raw_steps = reinterpret_cast<float*>(tmem_slot + 1);                    // [kRawRows]
+  uint32_t* raw_part = reinterpret_cast<uint32_t*>(raw_steps + kRawRows);        // [warp][kRawRows]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int shares = a.shares, rank = shares > 1 ? (int)ptx::cluster_rank() : 0;
   const int tile = blockIdx.x / shares, t0 = blockIdx.y * a.tn, rows_here = min(a.tn, a.rows - t0), n_here = (rows_here + 15) / 16 * 16;
@@ -266,18 +349,20 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
     }
     ptx::mbar_init(sums, 1);
     ptx::mbar_init(pushed, 1);
+    ptx::mbar_init(rows_ready, 4);
     ptx::mbar_fence_init();
     ptx::mbar_expect_tx(pushed, (shares - 1) * W * ((mine1 - mine0 + 3) / 4) * kI8Tile * 16);
   }
   __syncthreads();
   if (shares > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this CTA's barriers are there
+  const uint64_t policy = passing_through();
   auto load_weights = [&](int i, int s) {
-    ptx::mbar_expect_tx(&full[s], W * kI8Block + n_here * kI8Chunk);
+    ptx::mbar_expect_tx(&full[s], W * kI8Block + (RAW ? 0 : n_here * kI8Chunk));
     for (int h = 0; h < W; ++h)
-      ptx::bulk_g2s(smem + (size_t)s * stage_bytes + h * kI8Block, a.w + ((size_t)(tile * W + h) * a.chunks + chunk0 + i) * kI8Block, kI8Block, &full[s]);
+      bulk_g2s_with(smem + (size_t)s * stage_bytes + h * kI8Block, a.w + ((size_t)(tile * W + h) * a.chunks + chunk0 + i) * kI8Block, kI8Block, &full[s], policy);
   };
   auto load_rows = [&](int i, int s) {  // (a tile of 256 rows is two of the layout's)
-    for (int r = 0; r < n_here; r += kI8Tile) {
+    for (int r = 0; r < n_here && !RAW; r += kI8Tile) {
       const int row = t0 + r;
       ptx::bulk_g2s(smem + (size_t)s * stage_bytes + W * kI8Block + r * kI8Chunk,
                     a.q + ((size_t)(row / kI8Tile) * a.chunks + chunk0 + i) * kI8Block + row % kI8Tile * kI8Chunk, min(kI8Tile, n_here - r) * kI8Chunk, &full[s]);
@@ -320,12 +405,14 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
       const uint32_t idesc = idesc_i8(kI8Tile, n_here);
       int s = 0;
       uint32_t ph = 0;
-      for (int i = 0; i < chunks; ++i) {
+      if constexpr (RAW) ok = ptx::mbar_wait(rows_ready, 0);
+      const int todo = ok ? chunks : 0;
+      for (int i = 0; i < todo; ++i) {
         ok = ptx::mbar_wait(&full[s], ph);
         if (!ok) break;
         ptx::tc_fence_after_sync();
         const uint32_t at = ptx::smem_u32(smem + (size_t)s * stage_bytes);
-        const uint64_t db = ptx::umma_desc_k_sw128(at + W * kI8Block);
+        const uint64_t db = ptx::umma_desc_k_sw128(RAW ? ptx::smem_u32(smem + a.raw_at) + i * 16 * kI8Chunk : at + W * kI8Block);
 #pragma unroll
         for (int h = 0; h < W; ++h) {
           const uint64_t da = ptx::umma_desc_k_sw128(at + h * kI8Block);
@@ -343,7 +430,16 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
   const int quarter = warp & 3, channel = tile * kI8Tile + quarter * 32 + lane;
   const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
   float ws = 0.f, us = 0.f, bias = 0.f, steps = 0.f;
-  auto steps_of = [&](int c0) { return c0 + (lane & 15) < mine1 ? a.step[t0 + c0 + (lane & 15)] : 0.f; };  // sixteen rows' in the lanes
+  auto steps_of = [&](int c0) { return c0 + (lane & 15) < mine1 ? (RAW ? raw_steps[(c0 + lane) & 3] : a.step[t0 + c0 + (lane & 15)]) : 0.f; };  // sixteen rows' in the lanes
+  if constexpr (RAW) {
+    if (warp >= 2) {
+      const bool out = blockIdx.x < shares;
+      unsigned char* to = smem + a.raw_at;
+      if (!GATED && a.raw_inner) raw_rows(a, (const float*)a.raw, true, to, chunk0, chunks, false, false, rows_ready, raw_steps, raw_part);
+      else if (a.raw_fit) raw_rows(a, (const __nv_bfloat16*)a.raw, true, to, chunk0, chunks, out, rank == 0, rows_ready, raw_steps, raw_part);
+      else raw_rows(a, (const __nv_bfloat16*)a.raw, false, to, chunk0, chunks, out, rank == 0, rows_ready, raw_steps, raw_part);
+    }
+  }
   if (warp >= 2) {
     const size_t scale_at = (size_t)tile * W * kI8Tile + quarter * 32 + lane;
     ws = a.w_scale[scale_at];
@@ -412,9 +508,14 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
           }
       }
       // All sixteen are worked out before the first is stored: one after the other each took 100 cycles of latencies.
-      float y[16];
+      float y[16], up[16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) y[j] = output_of<GATED>(a, (int)v[j], GATED ? (int)u[j] : 0, ws, us, __shfl_sync(0xffffffffu, steps, j), bias);
+      for (int j = 0; j < 16; ++j) {
+        const float step = __shfl_sync(0xffffffffu, steps, j);
+        y[j] = (float)(int)v[j] * ws * step + bias;
+        if constexpr (GATED) up[j] = (float)(int)u[j] * us * step;
+      }
+      if constexpr (GATED) gate_with(a.act, y, up);
       if constexpr (GATED) {  // lane j keeps row j's
         uint32_t most = 0u;
 #pragma unroll
@@ -484,14 +585,21 @@ __device__ __forceinline__ void store_sums(const MmArgs& a, uint32_t (&v)[32], c
     if (GATED && lane < rows_here) a.most[(size_t)(row0 + lane) * (a.tiles * 2) + n0 / 32] = 0.f;
     return;
   }
+  float y[32], up[GATED ? 32 : 1];
 #pragma unroll
   for (int j4 = 0; j4 < 8; ++j4) {
     const float4 w4 = *reinterpret_cast<const float4*>(scales + 4 * j4), o4 = *reinterpret_cast<const float4*>(scales + kI8Tile + 4 * j4);
     const float w[4] = {w4.x, w4.y, w4.z, w4.w}, o[4] = {o4.x, o4.y, o4.z, o4.w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      v[4 * j4 + e] = __float_as_uint(output_of<GATED>(a, (int)v[4 * j4 + e], GATED ? (int)u[4 * j4 + e] : 0, w[e], GATED ? o[e] : 0.f, row_step, GATED ? 0.f : o[e]));
+    for (int e = 0; e < 4; ++e) {
+      const int j = 4 * j4 + e;
+      y[j] = (float)(int)v[j] * w[e] * row_step + (GATED ? 0.f : o[e]);
+      if constexpr (GATED) up[j] = (float)(int)u[j] * o[e] * row_step;
+    }
   }
+  if constexpr (GATED) gate_with(a.act, y, up);
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(y[j]);
   if constexpr (GATED) {
     uint32_t most = 0u;
 #pragma unroll
@@ -505,15 +613,15 @@ __device__ __forceinline__ void store_sums(const MmArgs& a, uint32_t (&v)[32], c
       for (int q = 0; q < 4; ++q)
         *reinterpret_cast<uint4*>(mine + lane * kPairPitch + 4 * q) = make_uint4(v[x + 4 * q], v[x + 4 * q + 1], v[x + 4 * q + 2], v[x + 4 * q + 3]);
       __syncwarp();
-      float* y = reinterpret_cast<float*>(a.y) + (size_t)row0 * a.y_stride + n0 + x;
+      float* out = reinterpret_cast<float*>(a.y) + (size_t)row0 * a.y_stride + n0 + x;
       if (a.y_vec && cols == 32) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int r = q * 8 + (lane >> 2), c = (lane & 3) * 4;
-          if (r < rows_here) *reinterpret_cast<float4*>(y + (size_t)r * a.y_stride + c) = *reinterpret_cast<const float4*>(mine + r * kPairPitch + c);
+          if (r < rows_here) *reinterpret_cast<float4*>(out + (size_t)r * a.y_stride + c) = *reinterpret_cast<const float4*>(mine + r * kPairPitch + c);
         }
       } else if (x + (lane & 15) < cols) {
-        for (int r = lane >> 4; r < rows_here; r += 2) y[(size_t)r * a.y_stride + (lane & 15)] = mine[r * kPairPitch + (lane & 15)];
+        for (int r = lane >> 4; r < rows_here; r += 2) out[(size_t)r * a.y_stride + (lane & 15)] = mine[r * kPairPitch + (lane & 15)];
       }
       __syncwarp();
     }
@@ -530,15 +638,15 @@ __device__ __forceinline__ void store_sums(const MmArgs& a, uint32_t (&v)[32], c
       *reinterpret_cast<uint4*>(words + lane * kPairPitch + 4 * q) = make_uint4(h[0], h[1], h[2], h[3]);
     }
     __syncwarp();
-    __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(a.y) + (size_t)row0 * a.y_stride + n0;
+    __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.y) + (size_t)row0 * a.y_stride + n0;
     if (a.y_vec && cols == 32) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int r = q * 8 + (lane >> 2), c = (lane & 3) * 4;
-        if (r < rows_here) *reinterpret_cast<uint4*>(y + (size_t)r * a.y_stride + 2 * c) = *reinterpret_cast<const uint4*>(words + r * kPairPitch + c);
+        if (r < rows_here) *reinterpret_cast<uint4*>(out + (size_t)r * a.y_stride + 2 * c) = *reinterpret_cast<const uint4*>(words + r * kPairPitch + c);
       }
     } else if (lane < cols) {
-      for (int r = 0; r < rows_here; ++r) y[(size_t)r * a.y_stride + lane] = reinterpret_cast<const __nv_bfloat16*>(words + r * kPairPitch)[lane];
+      for (int r = 0; r < rows_here; ++r) out[(size_t)r * a.y_stride + lane] = reinterpret_cast<const __nv_bfloat16*>(words + r * kPairPitch)[lane];
     }
     __syncwarp();
   }
@@ -838,17 +946,25 @@ Plan plan_of(const MmArgs& a, const int* stream_at_once, const int* pairs_at_onc
   return best;
 }
 
+// Rows that are not 8 bits yet: bf16, or the inner rows of a feed-forward block.
+struct RawRows {
+  const void* x = nullptr;
+  long long stride = 0;
+  const b200_i8_rows* inner = nullptr;
+};
+
 template <bool GATED>
-b200_status launch_product(MmArgs& a, cudaStream_t s) {
+b200_status launch_product(MmArgs& a, const I8RowsDev& to, const RawRows& raw, cudaStream_t s) {
   constexpr int W = GATED ? 2 : 1;
   // What runs at the same time with an SM for each CTA, by the cluster's size: CTAs of the one kernel, clusters of the other.  (The occupancy calculation counts
   // one CTA of a kernel that allocates tensor memory to an SM; of i8_stream_kernel's two share that memory.)
   static int at_once[kMostShares + 1] = {}, pairs_at_once[kMostPairs + 1] = {};
   if (at_once[1] == 0) {
-    B200_CUDA_TRY(cudaFuncSetAttribute(i8_stream_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamAlone));
+    B200_CUDA_TRY(cudaFuncSetAttribute(i8_stream_kernel<GATED, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamAlone));
+    B200_CUDA_TRY(cudaFuncSetAttribute(i8_stream_kernel<GATED, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamAlone));
     B200_CUDA_TRY(cudaFuncSetAttribute(i8_pair_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairShared));
     for (int n = kMostPairs; n > 0; --n) pairs_at_once[n] = ctas_in_clusters(i8_pair_kernel<GATED>, 2 * n, 1, b200_sm_count(), kPairThreads, kPairShared) / (2 * n);
-    for (int n = kMostShares; n > 0; --n) at_once[n] = ctas_in_clusters(i8_stream_kernel<GATED>, n, 1, b200_sm_count(), kStreamThreads, kStreamAlone);
+    for (int n = kMostShares; n > 0; --n) at_once[n] = ctas_in_clusters(i8_stream_kernel<GATED, false>, n, 1, b200_sm_count(), kStreamThreads, kStreamAlone);
     if (at_once[1] < 1 || pairs_at_once[1] < 1) {
       at_once[1] = 0;
       b200_set_error("i8: the kernels do not fit the device");
@@ -857,35 +973,49 @@ b200_status launch_product(MmArgs& a, cudaStream_t s) {
   }
   const Plan plan = plan_of<GATED>(a, at_once, pairs_at_once);
   a.shares = plan.shares;
+  const int per_share = (a.chunks + a.shares - 1) / a.shares;
+  const bool in_kernel = raw.x && !plan.pair && a.rows <= kRawRows && per_share <= kRawChunks && (raw.inner || a.rows * a.k <= kRawNumbers);
+  if (raw.x && !in_kernel) {
+    const b200_status st = raw.inner ? quantize_inner(raw.inner, a.rows, a.k, s) : quantize((const __nv_bfloat16*)raw.x, raw.stride, a.rows, a.k, to, s);
+    if (st != B200_OK) return st;
+  }
   if (plan.pair) {
     const long long items = (long long)((a.rows + kPairRows - 1) / kPairRows) * ((a.tiles + 1) / 2);
     if (items > 0x3fffffff) { b200_set_error("i8: %d rows of %d channels in one call", a.rows, a.n); return B200_ERR_CAPACITY; }
     launch_clusters(i8_pair_kernel<GATED>, 2 * a.shares, dim3((unsigned)(2 * a.shares * std::min<long long>(items, pairs_at_once[a.shares]))), kPairThreads, kPairShared, s, a);
   } else {
     a.tn = plan.tn;
-    const int tiles = a.tiles / W, row_tiles = (a.rows + a.tn - 1) / a.tn, stage = W * kI8Block + a.tn * kI8Chunk;
+    const int tiles = a.tiles / W, row_tiles = (a.rows + a.tn - 1) / a.tn, stage = W * kI8Block + (in_kernel ? 0 : a.tn * kI8Chunk);
     const int room = ((long long)tiles * row_tiles * a.shares <= at_once[a.shares] ? kStreamAlone : kStreamShared) - 2048;
-    const int per_share = (a.chunks + a.shares - 1) / a.shares, pushed = pushed_bytes(std::min(a.rows, a.tn), a.shares, W);
+    const int pushed = pushed_bytes(std::min(a.rows, a.tn), a.shares, W), raw_bytes = in_kernel ? per_share * 16 * kI8Chunk : 0;
     // What is pushed has a place beside the stages where that is a quarter of the room at most.
     a.over_stages = pushed > room / 4;
-    a.stages = std::min(per_share, (room - (a.over_stages ? 0 : pushed)) / stage);
-    a.pushed_at = a.over_stages ? 0 : a.stages * stage;
-    a.bars_at = std::max(a.stages * stage, a.pushed_at + pushed);
-    launch_clusters(i8_stream_kernel<GATED>, a.shares, dim3(tiles * a.shares, row_tiles), kStreamThreads,
-                    std::max<size_t>(a.bars_at + 2048, kSharedPerCol * stream_cols(a.tn, W)), s, a);
+    a.stages = std::min(per_share, (room - raw_bytes - (a.over_stages ? 0 : pushed)) / stage);
+    a.raw_at = a.stages * stage;
+    a.pushed_at = a.over_stages ? 0 : a.stages * stage + raw_bytes;
+    a.bars_at = std::max(a.stages * stage + raw_bytes, a.pushed_at + pushed);
+    const size_t shared = std::max<size_t>(a.bars_at + 2048, kSharedPerCol * stream_cols(a.tn, W));
+    if (in_kernel) {
+      a.raw = raw.x; a.raw_stride = raw.stride; a.raw_inner = raw.inner != nullptr; a.q_out = to.q; a.step_out = to.scale;
+      a.raw_fit = ((uintptr_t)raw.x & 15) == 0 && raw.stride % 8 == 0;
+      if (raw.inner) a.raw_most = raw.inner->most;
+      launch_clusters(i8_stream_kernel<GATED, true>, a.shares, dim3(tiles * a.shares, row_tiles), kStreamThreads, shared, s, a);
+    } else {
+      launch_clusters(i8_stream_kernel<GATED, false>, a.shares, dim3(tiles * a.shares, row_tiles), kStreamThreads, shared, s, a);
+    }
   }
   B200_LAUNCH_CHECK();
   return B200_OK;
 }
 
-b200_status product(const b200_i8_weight* w, const I8RowsDev& x, int rows, const float* bias, int act, void* y, long long y_stride, int y_f32, float* most, cudaStream_t s) {
+b200_status product(const b200_i8_weight* w, const I8RowsDev& x, const RawRows& raw, int rows, const float* bias, int act, void* y, long long y_stride, int y_f32, float* most, cudaStream_t s) {
   MmArgs a{};
   b200_status st = b200_qmm_ensure_err_word(&a.err);
   if (st != B200_OK) return st;
   a.w = w->q; a.w_scale = w->scale; a.q = x.q; a.step = x.scale; a.bias = bias; a.y = y; a.y_stride = y_stride; a.y_f32 = y_f32; a.act = act; a.most = most;
-  a.rows = rows; a.n = w->n; a.chunks = w->chunks; a.tiles = w->tiles;
+  a.rows = rows; a.n = w->n; a.chunks = w->chunks; a.tiles = w->tiles; a.k = w->k;
   a.y_vec = ((uintptr_t)y & 15) == 0 && y_stride * (w->gated || y_f32 ? 4 : 2) % 16 == 0;
-  return w->gated ? launch_product<true>(a, s) : launch_product<false>(a, s);
+  return w->gated ? launch_product<true>(a, x, raw, s) : launch_product<false>(a, x, raw, s);
 }
 
 // ---- handles -------------------------------------------------------------------------------------------------------------------
@@ -942,7 +1072,7 @@ b200_status create_weight(int n, int k, bool gated, const int8_t* const* q, cons
 }
 
 // The checks of x and the rows that a product reads.
-b200_status take_rows(const char* who, b200_i8_rows* r, const void* d_x, int64_t x_stride, int32_t rows, int32_t k, cudaStream_t s) {
+b200_status take_rows(const char* who, b200_i8_rows* r, const void* d_x, int64_t x_stride, int32_t rows, int32_t k) {
   if (rows < 0 || rows > r->max_rows) { b200_set_error("%s: %d rows, the handle is for %d", who, rows, r->max_rows); return rows < 0 ? B200_ERR_INVALID_ARGUMENT : B200_ERR_CAPACITY; }
   if (k > r->max_k) { b200_set_error("%s: rows of %d columns, the handle is for %d", who, k, r->max_k); return B200_ERR_CAPACITY; }
   if (rows == 0) {  // (whether x is there or not)
@@ -959,7 +1089,11 @@ b200_status take_rows(const char* who, b200_i8_rows* r, const void* d_x, int64_t
   }
   if (rows > 1 && x_stride < k) { b200_set_error("%s: rows of %d columns %lld apart", who, k, (long long)x_stride); return B200_ERR_INVALID_ARGUMENT; }
   if (((uintptr_t)d_x & 1) != 0) { b200_set_error("%s: x is not on a number's boundary", who); return B200_ERR_INVALID_ARGUMENT; }
-  b200_status st = quantize((const __nv_bfloat16*)d_x, x_stride, rows, k, r->x, s);
+  r->rows = -1;  // (until the rows are on their way)
+  return B200_OK;
+}
+
+b200_status taken(b200_i8_rows* r, int32_t rows, int32_t k, b200_status st) {
   if (st == B200_OK) { r->rows = rows; r->k = k; }
   return st;
 }
@@ -1039,7 +1173,9 @@ extern "C" b200_status b200_i8_quantize(b200_i8_rows* r, const void* d_x, int64_
   if (!r || k <= 0 || (rows > 0 && !d_x)) { b200_set_error("i8 quantize: no handle, or no rows"); return B200_ERR_INVALID_ARGUMENT; }
   b200_status st = b200_require_device();
   if (st != B200_OK) return st;
-  return take_rows("i8 quantize", r, d_x, x_stride, rows, k, (cudaStream_t)stream);
+  st = take_rows("i8 quantize", r, d_x, x_stride, rows, k);
+  if (st != B200_OK || rows == 0) return st;
+  return taken(r, rows, k, quantize((const __nv_bfloat16*)d_x, x_stride, rows, k, r->x, (cudaStream_t)stream));
 }
 
 extern "C" b200_status b200_i8_rows_get(const b200_i8_rows* r, void* d_q, float* d_steps, void* stream) {
@@ -1059,9 +1195,9 @@ extern "C" b200_status b200_i8_mm(const b200_i8_weight* w, b200_i8_rows* r, cons
   if (w->gated) { b200_set_error("i8 mm: the weight is a feed-forward block's gate and up"); return B200_ERR_INVALID_ARGUMENT; }
   b200_status st = check_out("i8 mm", d_y, y_stride, rows, w->n, y_f32 ? 4 : 2);
   if (st == B200_OK) st = b200_require_device();
-  if (st == B200_OK) st = take_rows("i8 mm", r, d_x, x_stride, rows, w->k, (cudaStream_t)stream);
+  if (st == B200_OK) st = take_rows("i8 mm", r, d_x, x_stride, rows, w->k);
   if (st != B200_OK || rows == 0) return st;
-  return product(w, r->x, rows, d_bias, 0, d_y, y_stride, y_f32 != 0, nullptr, (cudaStream_t)stream);
+  return taken(r, rows, w->k, product(w, r->x, RawRows{d_x, x_stride, nullptr}, rows, d_bias, 0, d_y, y_stride, y_f32 != 0, nullptr, (cudaStream_t)stream));
 }
 
 extern "C" b200_status b200_i8_ffn(const b200_i8_weight* gate_up, const b200_i8_weight* down, b200_i8_rows* r, const void* d_x, int64_t x_stride, int32_t rows,
@@ -1075,11 +1211,10 @@ extern "C" b200_status b200_i8_ffn(const b200_i8_weight* gate_up, const b200_i8_
   if (down->k > r->max_hidden) { b200_set_error("i8 ffn: %d channels inside the block, the handle is for %d", down->k, r->max_hidden); return B200_ERR_CAPACITY; }
   b200_status st = check_out("i8 ffn", d_y, y_stride, rows, down->n, 2);
   if (st == B200_OK) st = b200_require_device();
-  if (st == B200_OK) st = take_rows("i8 ffn", r, d_x, x_stride, rows, gate_up->k, (cudaStream_t)stream);
+  if (st == B200_OK) st = take_rows("i8 ffn", r, d_x, x_stride, rows, gate_up->k);
   if (st != B200_OK || rows == 0) return st;
   cudaStream_t s = (cudaStream_t)stream;
-  st = product(gate_up, r->x, rows, nullptr, activation, r->h, r->h_stride, 0, r->most, s);
-  if (st == B200_OK) st = quantize_inner(r, rows, down->k, s);
-  if (st == B200_OK) st = product(down, r->hidden, rows, nullptr, 0, d_y, y_stride, 0, nullptr, s);
+  st = taken(r, rows, gate_up->k, product(gate_up, r->x, RawRows{d_x, x_stride, nullptr}, rows, nullptr, activation, r->h, r->h_stride, 0, r->most, s));
+  if (st == B200_OK) st = product(down, r->hidden, RawRows{r->h, r->h_stride, r}, rows, nullptr, 0, d_y, y_stride, 0, nullptr, s);
   return st;
 }

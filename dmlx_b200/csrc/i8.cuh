@@ -84,36 +84,55 @@ struct I8Scale {
 template <typename T>
 struct Eight { uint4 r[sizeof(T) / 2]; };
 
-// From column c of a row of n on; fit: rows start on 16 bytes.  Elsewhere the 16-byte pieces that hold the numbers are fetched and shifted into place
-// (rows of 5003 bf16 and f32 one number at a time took three times as long); at a row's ends, where a piece would reach beyond it, one by one.
-template <typename T>
-__device__ __forceinline__ Eight<T> load_eight(const T* p, int c, int n, bool fit) {
+// N times eight numbers of a row of n, at columns at(0), at(1), ..., multiples of eight; fit: the row starts on 16 bytes.  Elsewhere the 16-byte pieces that
+// hold the numbers are fetched and shifted into place (rows of 5003 bf16 and f32 one number at a time took three times as long).  All loads are on
+// their way before the first is looked at; what lies at a row's ends, where a piece would reach beyond it, is fetched number by number behind them.
+template <typename T, int N, class At>
+__device__ __forceinline__ void load_eights(Eight<T> (&e)[N], const T* p, int n, bool fit, At at) {
   constexpr int R = sizeof(T) / 2, kWords = 4 * R;
-  Eight<T> e;
-  const uint32_t off = fit ? 0u : (uint32_t)(reinterpret_cast<uintptr_t>(p + c) & 15);
+  const uint32_t off = fit ? 0u : (uint32_t)(reinterpret_cast<uintptr_t>(p) & 15);
   const int before = (int)(off / sizeof(T));  // numbers of the first piece that come ahead
-  if (fit && c + 8 <= n) {
+  const uint4* pieces = reinterpret_cast<const uint4*>(p - before);
+  uint4 last[N];
+  auto whole = [&](int c) { return fit ? c + 8 <= n : c >= before && c - before + 8 + 16 / (int)sizeof(T) <= n; };
 #pragma unroll
-    for (int i = 0; i < R; ++i) e.r[i] = reinterpret_cast<const uint4*>(p + c)[i];
-  } else if (!fit && c >= before && c - before + 8 + 16 / (int)sizeof(T) <= n) {
-    const uint4* at = reinterpret_cast<const uint4*>(p + c - before);
-    uint32_t w[kWords + 4];
+  for (int k = 0; k < N; ++k) {
+    const int c = at(k);
+    const bool here = whole(c);
+    const uint4* from = pieces + (size_t)(c / 8) * R;
 #pragma unroll
-    for (int i = 0; i <= R; ++i) {
-      const uint4 q = at[i];
-      w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
+    for (int i = 0; i < R; ++i) {
+      e[k].r[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (here) e[k].r[i] = from[i];
     }
+    last[k] = make_uint4(0u, 0u, 0u, 0u);
+    if (!fit && here) last[k] = from[R];
+  }
+  if (!fit) {
 #pragma unroll
-    for (int i = 0; i < kWords + 2; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+    for (int k = 0; k < N; ++k) {
+      uint32_t w[kWords + 4];
 #pragma unroll
-    for (int i = 0; i < kWords + 1; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
-    if constexpr (sizeof(T) == 2) {
+      for (int i = 0; i <= R; ++i) {
+        const uint4 q = i < R ? e[k].r[i < R ? i : 0] : last[k];
+        w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
+      }
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (off & 2) * 8);
+      for (int i = 0; i < kWords + 2; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+#pragma unroll
+      for (int i = 0; i < kWords + 1; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
+      if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (off & 2) * 8);
+      }
+#pragma unroll
+      for (int i = 0; i < R; ++i) e[k].r[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
     }
+  }
 #pragma unroll
-    for (int i = 0; i < R; ++i) e.r[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-  } else {
+  for (int k = 0; k < N; ++k) {
+    const int c = at(k);
+    if (whole(c) || c >= n) continue;
     T v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = c + i < n ? p[c + i] : T(0.f);
@@ -125,10 +144,15 @@ __device__ __forceinline__ Eight<T> load_eight(const T* p, int c, int n, bool fi
         if constexpr (sizeof(T) == 4) w[j] = __float_as_uint(v[4 * i + j]);
         else w[j] = (uint32_t)__bfloat16_as_ushort(v[2 * j]) | (uint32_t)__bfloat16_as_ushort(v[2 * j + 1]) << 16;
       }
-      e.r[i] = make_uint4(w[0], w[1], w[2], w[3]);
+      e[k].r[i] = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
-  return e;
+}
+template <typename T>
+__device__ __forceinline__ Eight<T> load_eight(const T* p, int c, int n, bool fit) {
+  Eight<T> e[1];
+  load_eights(e, p, n, fit, [&](int) { return c; });
+  return e[0];
 }
 __device__ __forceinline__ void widen(const Eight<__nv_bfloat16>& e, float (&v)[8]) {
   const uint32_t w[4] = {e.r[0].x, e.r[0].y, e.r[0].z, e.r[0].w};

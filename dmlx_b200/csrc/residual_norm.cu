@@ -102,19 +102,15 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const 
   const Y* y = (const Y*)a.y + (size_t)row * a.y_stride;
   Eight<Y> yr[NV];
   Eight<H> hr[NV];
-#pragma unroll
-  for (int u = 0; u < NV; ++u) yr[u] = load_eight(y, column(u), a.n, FIT || (a.fit & kFitY));
-#pragma unroll
-  for (int u = 0; u < NV; ++u) hr[u] = load_eight(h, column(u), a.n, FIT || (a.fit & kFitH));
+  load_eights(yr, y, a.n, FIT || (a.fit & kFitY), column);
+  load_eights(hr, h, a.n, FIT || (a.fit & kFitH), column);
   Eight<__nv_bfloat16> gr[NV <= 2 ? NV : 1];
-  if (NV <= 2 && a.gate) {
-#pragma unroll
-    for (int u = 0; u < NV; ++u) gr[u] = load_eight(a.gate + (size_t)row * a.gate_stride, column(u), a.n, FIT || (a.fit & kFitGate));
+  if constexpr (NV <= 2) {
+    if (a.gate) load_eights(gr, a.gate + (size_t)row * a.gate_stride, a.n, FIT || (a.fit & kFitGate), column);
   }
   Eight<__nv_bfloat16> pr[NV <= 2 ? NV : 1], nr[NV == 1 ? NV : 1];
-  if (NV <= 2 && a.post_w) {
-#pragma unroll
-    for (int u = 0; u < NV; ++u) pr[u] = load_eight(a.post_w, column(u), a.n, FIT || (a.fit & kFitPost));
+  if constexpr (NV <= 2) {
+    if (a.post_w) load_eights(pr, a.post_w, a.n, FIT || (a.fit & kFitPost), column);
   }
   if (NV == 1 && a.norm_w) nr[0] = load_eight(a.norm_w, column(0), a.n, FIT || (a.fit & kFitNorm));
   float ry = 1.f;
