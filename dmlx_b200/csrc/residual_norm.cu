@@ -222,8 +222,8 @@ extern "C" b200_status b200_residual_norm(const b200_residual_norm_shape* shape,
   auto holds = [&](const void* p, int64_t stride, int size) { return p && ((uintptr_t)p & (size - 1)) == 0 && (rows <= 1 || stride >= n); };
   if (rows > 0 && (!holds(d_h, h_stride, h_size) || !holds(d_y, y_stride, y_size) || !holds(d_h_out, h_out_stride, h_size) || (d_x_out && !holds(d_x_out, x_out_stride, 2)) ||
                    (d_gate && gate_stride != 0 && !holds(d_gate, gate_stride, 2)) || (((uintptr_t)d_gate | (uintptr_t)d_post_weight | (uintptr_t)d_norm_weight) & 1) != 0 ||
-                   (d_h_out == d_h && rows > 1 && h_out_stride != h_stride))) {
-    b200_set_error("residual norm: rows of %d columns, each on a number's boundary, strides that hold a row; h_out is h itself or apart from it", n);
+                   (d_h_out == d_h && rows > 1 && h_out_stride != h_stride) || d_h_out == d_y || (d_x_out && (d_x_out == d_h || d_x_out == d_y || d_x_out == d_h_out || d_x_out == d_gate)))) {
+    b200_set_error("residual norm: rows of %d columns, each on a number's boundary, strides that hold a row; h_out is h itself, all else apart", n);
     return B200_ERR_INVALID_ARGUMENT;
   }
   if (q_out && (rows > q_out->max_rows || n > q_out->max_k)) {

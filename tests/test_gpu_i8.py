@@ -114,8 +114,46 @@ def test_rows_of_the_smallest_and_largest_numbers():
     assert bool((got[1] == 0).all())
 
 
+LARGER = [  # rows, k, n: shares of K of a few rows, tiles of rows, pairs that share K, pairs that walk many items, a weight of more tiles than there are SMs
+    (1, 14336, 4096), (4, 4096, 6144), (33, 2048, 2048), (130, 4096, 1024), (200, 4096, 4096), (300, 2048, 1024), (300, 14336, 256), (512, 4096, 4096), (700, 1000, 9000),
+    (1100, 4096, 6144), (2500, 520, 3000), (20, 300, 30001), (260, 200, 20000),
+]
+
+
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows", [5, 300])
+@pytest.mark.parametrize("rows,k,n", LARGER)
+@pytest.mark.parametrize("f32", [False, True])
+def test_product_larger(rows, k, n, f32):
+    from dmlx_b200 import device as dev
+
+    w, scales = (t.cuda() for t in _weight(n, k, 15))
+    x, bias = _x(rows, k, 16).cuda(), torch.randn(n, generator=torch.Generator().manual_seed(17)).cuda()
+    got = dev.i8_mm(dev.I8Weight(w, scales), dev.I8Rows(rows, k), x, bias=bias, f32=f32)
+    want = _product(*_quantized(x), w, scales)
+    tol = 5 * 2.0 ** -24 * (want.abs() + bias.double().abs())
+    want = want + bias.double()
+    _off(got, want, tol if f32 else tol + 2.0 ** -8 * want.abs())
+    assert dev.qmm_error_word() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,f", [(1, 4096, 14336), (3, 5000, 1000), (96, 4096, 8192), (128, 1024, 14336), (333, 2222, 5777), (600, 512, 9000), (1500, 300, 3000)])
+def test_feed_forward_larger(rows, k, f):
+    from dmlx_b200 import device as dev
+
+    def scaled(n, k, seed):
+        q, s = _weight(n, k, seed)
+        return q.cuda(), (s * 0.7 * k ** -0.5).cuda()
+
+    gate, up, down = scaled(f, k, 4), scaled(f, k, 5), scaled(k, f, 6)
+    x = _x(rows, k, 7).cuda()
+    got = dev.i8_ffn(dev.I8Weight.gated(*gate, *up), dev.I8Weight(*down), dev.I8Rows(rows, k, f), x)
+    _check_ffn(got, x, gate, up, down, "silu")
+    assert dev.qmm_error_word() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [4, 5, 300])
 def test_rows_that_hold_no_number(rows):
     """Such a row is NaN in every column; the others keep their bits."""
     from dmlx_b200 import device as dev
@@ -130,7 +168,7 @@ def test_rows_that_hold_no_number(rows):
     bad[0, 3] = float("nan")
     bad[2, 699] = float("inf")
     bad[3, 0], bad[3, 1] = -float("inf"), float("nan")
-    rest = [r for r in range(rows) if r not in (0, 2, 3)]
+    rest = [r for r in range(rows) if r not in (0, 2, 3)]  # (of four, one)
     for got, want in zip((dev.i8_mm(w, held, bad.cuda()), dev.i8_ffn(gate_up, down, held, bad.cuda())), good):
         assert bool(got[[0, 2, 3]].isnan().all())
         assert torch.equal(got[rest], want[rest])
@@ -175,7 +213,7 @@ def _check_ffn(got, x, gate, up, down, act):
     w = down[0].double().abs() * down[1].double()[:, None]
     want = _product(q, s, *down)
     tol = s * (open_ @ w.T) + loose * s * (q.abs() @ w.T)
-    _off(got.double().cpu(), want, tol + (2.0 ** -8 + 2.0 ** -21) * want.abs())
+    _off(got.double().to(want.device), want, tol + (2.0 ** -8 + 2.0 ** -21) * want.abs())
     return want
 
 
@@ -212,7 +250,7 @@ def test_a_row_s_bits_do_not_depend_on_its_batch():
     gate_up, down = dev.I8Weight.gated(*_weight(f, k, 22), *_weight(f, k, 23)), dev.I8Weight(*_weight(n, f, 24))
     held = dev.I8Rows(1200, k, f)
     whole = dev.i8_mm(w, held, x, f32=True), dev.i8_ffn(gate_up, down, held, x)
-    for first, rows in ((0, 1), (3, 2), (100, 16), (7, 31), (500, 64), (250, 128), (40, 200), (11, 300), (600, 513)):
+    for first, rows in ((0, 1), (3, 2), (9, 4), (20, 5), (100, 16), (7, 31), (500, 64), (250, 128), (40, 200), (11, 300), (600, 513)):
         part = x[first:first + rows]
         assert torch.equal(dev.i8_mm(w, held, part, f32=True), whole[0][first:first + rows]), rows
         assert torch.equal(dev.i8_ffn(gate_up, down, held, part), whole[1][first:first + rows]), rows
@@ -275,6 +313,20 @@ def test_no_rows():
     assert dev.i8_mm(w, held, none).shape == (0, 32) and dev.i8_mm(w, held).shape == (0, 32)
     assert dev.i8_ffn(gate_up, w, held, none).shape == (0, 32)
     assert held.get()[0].shape == (0, 64)
+
+
+@pytest.mark.gpu
+def test_a_handle_through_calls_of_many_and_few_rows():
+    """Blocks of other widths and batches of other sizes one after the other: nothing of an earlier call is seen by a later one."""
+    from dmlx_b200 import device as dev
+
+    blocks = [(dev.I8Weight.gated(*_weight(f, k, f), *_weight(f, k, f + 1)), dev.I8Weight(*_weight(k, f, f + 2)), k) for k, f in ((256, 1500), (512, 130), (384, 700))]
+    held = dev.I8Rows(400, 512, 1500)
+    for seed, (rows, which) in enumerate(((400, 0), (3, 1), (17, 2), (400, 1), (1, 0), (260, 2), (4, 0), (90, 1))):
+        gate_up, down, k = blocks[which]
+        x = _x(rows, k, 200 + seed).cuda()
+        assert torch.equal(dev.i8_ffn(gate_up, down, held, x), dev.i8_ffn(gate_up, down, dev.I8Rows(rows, k, 1500), x)), (rows, which)
+        assert torch.equal(held.get()[0].cpu().double(), _quantized(x.cpu())[0])
 
 
 @pytest.mark.gpu

@@ -221,6 +221,10 @@ def test_refusals():
     assert e.value.status == _lib.ERR_CAPACITY
     with pytest.raises(_lib.B200Error):
         dev.residual_norm(h, y, norm, eps=-1.0)
+    for call in (lambda: dev.residual_norm(h, y, norm, h_out=y), lambda: dev.residual_norm(h, y, norm, x_out=h), lambda: dev.residual_norm(h, y, norm, x_out=y)):
+        with pytest.raises(_lib.B200Error) as e:
+            call()
+        assert e.value.status == _lib.ERR_INVALID_ARGUMENT
     wide = torch.zeros((1, 32769), dtype=torch.bfloat16, device="cuda")
     with pytest.raises(_lib.B200Error) as e:
         dev.residual_norm(wide, wide)
