@@ -227,11 +227,11 @@ __device__ __forceinline__ void gate_with(int act, float (&y)[N], const float (&
 
 // ---- up to a few hundred rows: streams of weights ----
 // A weight tile (gated: the gate's and up's tile of the same channels) by up to tn rows and a share of K per CTA.  The weights are the MMA's M, the rows
-// its N, so that few rows waste nothing; a lane of tensor memory is a channel.  Warp 0 loads, warp 1 multiplies, four bring the sums to the output.
+// its N, so that few rows waste nothing; a lane of tensor memory is a channel.  Warp 0 loads, warp 1 multiplies, eight bring the sums to the output, every other sixteen rows of 32 channels each.
 // Bound by the weights, which come at the rate of memory only if every SM asks for them: a cluster of up to eight CTAs shares K (as many as still run at
 // the same time).  Each of them brings a share of the rows to the output and gets the others' sums of these pushed into its
 // shared memory, where the stages were unless there is room beside them, with a barrier that counts their bytes.
-constexpr int kStreamThreads = 192, kStreamShared = 112 * 1024, kStreamAlone = 226 * 1024, kMostShares = 8;  // (shared memory of two CTAs on an SM, of one)
+constexpr int kStreamThreads = 320, kStreamShared = 112 * 1024, kStreamAlone = 226 * 1024, kMostShares = 8;  // (shared memory of two CTAs on an SM, of one)
 
 // Weights that go through L2 once: they leave it ahead of what else is there.  (Among it are the instructions, which a kernel fetches anew: behind 117 MB of
 // weights the last ones came from memory, 4 to 8 us for the output of one row.)
@@ -266,24 +266,24 @@ __device__ __forceinline__ void tmem_ld4(uint32_t taddr, uint32_t& a, uint32_t& 
 
 constexpr int kRawRows = 4, kRawNumbers = 16384, kRawChunks = 32;  // rows of RAW; their numbers at most; blocks of K in a share at most
 
-// Warps 2 to 5: rows into 8 bits, as i8_quantize_kernel and i8_quantize_inner_kernel do, blocks chunk0 and on as an operand of 16 rows each at `to` (the rows that
+// Warps 2 to 9: rows into 8 bits, as i8_quantize_kernel and i8_quantize_inner_kernel do, blocks chunk0 and on as an operand of 16 rows each at `to` (the rows that
 // are not there hold anything), steps into `steps`; `out` and `first`: into the handle too, and the steps.
 template <typename T>
 __device__ __forceinline__ void raw_rows(const MmArgs& a, const T* x, bool fit, unsigned char* to, int chunk0, int chunks, bool out, bool first, uint64_t* ready, float* steps,
                                          uint32_t* part) {
   constexpr bool kInner = sizeof(T) == 4;
-  constexpr int kAhead = 4;
+  constexpr int kAhead = 2, kThreads = kStreamThreads - 64;
   const int t = threadIdx.x - 64, lane = t & 31, warp = t >> 5;
 #pragma unroll 1
   for (int r = 0; r < a.rows; ++r) {
     uint32_t m = 0u;
     if constexpr (kInner) {
-      for (int g = t; g < a.chunks * 4; g += 128) m = max(m, __float_as_uint(a.raw_most[(size_t)r * (a.chunks * 4) + g]));
+      for (int g = t; g < a.chunks * 4; g += kThreads) m = max(m, __float_as_uint(a.raw_most[(size_t)r * (a.chunks * 4) + g]));
     } else {
 #pragma unroll 1
-      for (int v = t; v * 8 < a.k; v += kAhead * 128) {
+      for (int v = t; v * 8 < a.k; v += kAhead * kThreads) {
         Eight<T> e[kAhead];
-        load_eights(e, x + (size_t)r * a.raw_stride, a.k, fit, [&](int u) { return (v + u * 128) * 8; });
+        load_eights(e, x + (size_t)r * a.raw_stride, a.k, fit, [&](int u) { return (v + u * kThreads) * 8; });
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) m = most_of(m, e[u]);
       }
@@ -291,21 +291,21 @@ __device__ __forceinline__ void raw_rows(const MmArgs& a, const T* x, bool fit, 
     m = __reduce_max_sync(0xffffffffu, m);
     if (lane == 0) part[warp * kRawRows + r] = m;
   }
-  asm volatile("bar.sync 1, 128;" ::: "memory");
+  asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
 #pragma unroll 1
   for (int r = 0; r < a.rows; ++r) {
-    const I8Scale s = I8Scale::of(__uint_as_float(max(max(part[r], part[kRawRows + r]), max(part[2 * kRawRows + r], part[3 * kRawRows + r]))));
+    const I8Scale s = I8Scale::of(__uint_as_float(__reduce_max_sync(0xffffffffu, part[lane % (kThreads / 32) * kRawRows + r])));
     if (t == 0) {
       steps[r] = s.step();
       if (out && first && !kInner) a.step_out[r] = s.step();
     }
 #pragma unroll 1
-    for (int v = t; v < chunks * 16; v += kAhead * 128) {
+    for (int v = t; v < chunks * 16; v += kAhead * kThreads) {
       Eight<T> e[kAhead];
-      load_eights(e, x + (size_t)r * a.raw_stride, a.k, fit, [&](int u) { return chunk0 * kI8Chunk + (v + u * 128) * 8; });
+      load_eights(e, x + (size_t)r * a.raw_stride, a.k, fit, [&](int u) { return chunk0 * kI8Chunk + (v + u * kThreads) * 8; });
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        const int at = v + u * 128, piece = at & 15;
+        const int at = v + u * kThreads, piece = at & 15;
         if (at >= chunks * 16) break;
         float f[8];
         widen(e[u], f);
@@ -316,7 +316,7 @@ __device__ __forceinline__ void raw_rows(const MmArgs& a, const T* x, bool fit, 
     }
   }
   ptx::fence_proxy_async_smem();
-  asm volatile("bar.sync 1, 128;" ::: "memory");  // the steps are there
+  asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");  // the steps are there
   if (lane == 0) ptx::mbar_arrive(ready);
 }
 
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
     }
     ptx::mbar_init(sums, 1);
     ptx::mbar_init(pushed, 1);
-    ptx::mbar_init(rows_ready, 4);
+    ptx::mbar_init(rows_ready, 8);
     ptx::mbar_fence_init();
     ptx::mbar_expect_tx(pushed, (shares - 1) * W * ((mine1 - mine0 + 3) / 4) * kI8Tile * 16);
   }
@@ -427,9 +427,9 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
     }
     __syncwarp();
   }
-  const int quarter = warp & 3, channel = tile * kI8Tile + quarter * 32 + lane;
+  const int quarter = warp & 3, half = (warp - 2) >> 2, channel = tile * kI8Tile + quarter * 32 + lane;
   const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
-  float ws = 0.f, us = 0.f, bias = 0.f, steps = 0.f;
+  float ws = 0.f, us = 0.f, bias = 0.f;
   auto steps_of = [&](int c0) { return c0 + (lane & 15) < mine1 ? (RAW ? raw_steps[(c0 + lane) & 3] : a.step[t0 + c0 + (lane & 15)]) : 0.f; };  // sixteen rows' in the lanes
   if constexpr (RAW) {
     if (warp >= 2) {
@@ -439,16 +439,6 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
       else if (a.raw_fit) raw_rows(a, (const __nv_bfloat16*)a.raw, true, to, chunk0, chunks, out, rank == 0, rows_ready, raw_steps, raw_part);
       else raw_rows(a, (const __nv_bfloat16*)a.raw, false, to, chunk0, chunks, out, rank == 0, rows_ready, raw_steps, raw_part);
     }
-  }
-  if (warp >= 2) {
-    const size_t scale_at = (size_t)tile * W * kI8Tile + quarter * 32 + lane;
-    ws = a.w_scale[scale_at];
-    if (GATED) us = a.w_scale[scale_at + kI8Tile];
-    if (!GATED && a.bias && channel < a.n) bias = a.bias[channel];
-    steps = steps_of(mine0);
-    ok = ptx::mbar_wait(sums, 0);
-    ok = __all_sync(0xffffffffu, ok);
-    ptx::tc_fence_after_sync();
   }
   // Sixteen rows' sums, as far as they go.
   auto load_sums = [&](int c0, int end, uint32_t (&v)[16], uint32_t (&u)[16]) {
@@ -462,84 +452,104 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
       }
     ptx::tmem_ld_wait();
   };
-  if (shares > 1) {
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the others' barriers are there
-    if (a.over_stages) ptx::cluster_sync();                              // nobody's stages are in use
-    if (warp >= 2 && ok) {
+  if (warp >= 2) {
+    const size_t scale_at = (size_t)tile * W * kI8Tile + quarter * 32 + lane;
+    ws = a.w_scale[scale_at];
+    if (GATED) us = a.w_scale[scale_at + kI8Tile];
+    if (!GATED && a.bias && channel < a.n) bias = a.bias[channel];
+    // Once without sums, while these are made: the instructions are then there when they are needed.
 #pragma unroll 1
-      for (int i = 1; i < shares; ++i) {
-        const int q = rank + i < shares ? rank + i : rank + i - shares, q0 = min(rows_here, q * per_rank), q1 = min(rows_here, q0 + per_rank);
-        const uint32_t bar = ptx::map_to_rank(ptx::smem_u32(pushed), q), part = per_rank / 4 * kI8Tile * 16;
-        uint32_t to = ptx::map_to_rank(ptx::smem_u32(smem + a.pushed_at), q) + (rank - (rank > q)) * W * part + (quarter * 32 + lane) * 16;
+    for (int live = 0; live < 2; ++live) {
+      int end = live ? mine1 : mine0 + half * 16 + 1;  // (one round)
+      if (live) {
+        ok = ptx::mbar_wait(sums, 0);
+        ok = __all_sync(0xffffffffu, ok);
+        ptx::tc_fence_after_sync();
+        if (shares > 1) {
+          asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the others' barriers are there
+          if (a.over_stages) ptx::cluster_sync();                              // nobody's stages are in use
+          if (ok) {
 #pragma unroll 1
-        for (int c0 = q0; c0 < q1; c0 += 16, to += 4 * kI8Tile * 16) {
-          uint32_t v[16], u[16];
-          load_sums(c0, q1, v, u);
+            for (int i = 1; i < shares; ++i) {
+              const int q = rank + i < shares ? rank + i : rank + i - shares, q0 = min(rows_here, q * per_rank), q1 = min(rows_here, q0 + per_rank);
+              const uint32_t bar = ptx::map_to_rank(ptx::smem_u32(pushed), q), part = per_rank / 4 * kI8Tile * 16;
+              uint32_t to = ptx::map_to_rank(ptx::smem_u32(smem + a.pushed_at), q) + (rank - (rank > q)) * W * part + (half * 4 * kI8Tile + quarter * 32 + lane) * 16;
+#pragma unroll 1
+              for (int c0 = q0 + half * 16; c0 < q1; c0 += 32, to += 8 * kI8Tile * 16) {
+                uint32_t v[16], u[16];
+                load_sums(c0, q1, v, u);
 #pragma unroll
-          for (int g = 0; g < 16; g += 4)
-            if (c0 + g < q1) {
-              push4(to + g / 4 * kI8Tile * 16, v[g], v[g + 1], v[g + 2], v[g + 3], bar);
-              if constexpr (GATED) push4(to + part + g / 4 * kI8Tile * 16, u[g], u[g + 1], u[g + 2], u[g + 3], bar);
-            }
-        }
-      }
-    }
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  }
-  if (warp >= 2 && ok && mine0 < mine1) {
-    if (shares > 1) ok = __all_sync(0xffffffffu, ptx::mbar_wait(pushed, 0));
-#pragma unroll 1
-    for (int c0 = mine0; c0 < mine1 && ok; c0 += 16) {
-      uint32_t v[16], u[16];
-      load_sums(c0, mine1, v, u);
-      const uint4* from = reinterpret_cast<const uint4*>(smem + a.pushed_at) + (c0 - mine0) / 4 * kI8Tile + quarter * 32 + lane;
-#pragma unroll 1
-      for (int q = 0; q < shares - 1; ++q, from += W * (per_rank / 4) * kI8Tile) {
-#pragma unroll
-        for (int g = 0; g < 16; g += 4)
-          if (c0 + g < mine1) {
-            const uint4 p = from[g / 4 * kI8Tile];
-            v[g] += p.x; v[g + 1] += p.y; v[g + 2] += p.z; v[g + 3] += p.w;
-            if constexpr (GATED) {
-              const uint4 p2 = from[(per_rank / 4 + g / 4) * kI8Tile];
-              u[g] += p2.x; u[g + 1] += p2.y; u[g + 2] += p2.z; u[g + 3] += p2.w;
+                for (int g = 0; g < 16; g += 4)
+                  if (c0 + g < q1) {
+                    push4(to + g / 4 * kI8Tile * 16, v[g], v[g + 1], v[g + 2], v[g + 3], bar);
+                    if constexpr (GATED) push4(to + part + g / 4 * kI8Tile * 16, u[g], u[g + 1], u[g + 2], u[g + 3], bar);
+                  }
+              }
             }
           }
+          __syncwarp();
+          asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+          if (ok && mine0 < mine1) ok = __all_sync(0xffffffffu, ptx::mbar_wait(pushed, 0));
+        }
+        if (!ok) end = 0;
       }
-      // All sixteen are worked out before the first is stored: one after the other each took 100 cycles of latencies.
-      float y[16], up[16];
+#pragma unroll 1
+      for (int c0 = mine0 + half * 16; c0 < end; c0 += 32) {
+        uint32_t v[16], u[16];
+        const float steps = steps_of(c0);  // (ahead of the stores, which loads do not pass)
+        load_sums(c0, live ? mine1 : 0, v, u);
+        const uint4* from = reinterpret_cast<const uint4*>(smem + a.pushed_at) + (c0 - mine0) / 4 * kI8Tile + quarter * 32 + lane;
+#pragma unroll 1
+        for (int q = 0; q < shares - 1; ++q, from += W * (per_rank / 4) * kI8Tile) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float step = __shfl_sync(0xffffffffu, steps, j);
-        y[j] = (float)(int)v[j] * ws * step + bias;
-        if constexpr (GATED) up[j] = (float)(int)u[j] * us * step;
-      }
-      if constexpr (GATED) gate_with(a.act, y, up);
-      if constexpr (GATED) {  // lane j keeps row j's
-        uint32_t most = 0u;
+          for (int g = 0; g < 16; g += 4)
+            if (live && c0 + g < mine1) {
+              const uint4 p = from[g / 4 * kI8Tile];
+              v[g] += p.x; v[g + 1] += p.y; v[g + 2] += p.z; v[g + 3] += p.w;
+              if constexpr (GATED) {
+                const uint4 p2 = from[(per_rank / 4 + g / 4) * kI8Tile];
+                u[g] += p2.x; u[g + 1] += p2.y; u[g + 2] += p2.z; u[g + 3] += p2.w;
+              }
+            }
+        }
+        // All sixteen are worked out before the first is stored: one after the other each took 100 cycles of latencies.
+        float y[16], up[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(y[j]) & 0x7fffffffu);
-          if (lane == j) most = m;
+          const float step = __shfl_sync(0xffffffffu, steps, j);
+          y[j] = (float)(int)v[j] * ws * step + bias;
+          if constexpr (GATED) up[j] = (float)(int)u[j] * us * step;
         }
-        if (c0 + lane < mine1 && lane < 16) a.most[(size_t)(t0 + c0 + lane) * (a.tiles * 2) + tile * 4 + quarter] = __uint_as_float(most);
-      }
-      const size_t at = (size_t)(t0 + c0) * a.y_stride + channel;
-      const int rows_left = channel < a.n ? mine1 - c0 : 0;
-      if (GATED || a.y_f32) {
-        float* to = reinterpret_cast<float*>(a.y) + at;
+        if constexpr (GATED) {
+          gate_with(a.act, y, up);
+          uint32_t most = 0u;  // lane j keeps row j's
 #pragma unroll
-        for (int j = 0; j < 16; ++j, to += a.y_stride)
-          if (j < rows_left) *to = y[j];
-      } else {
-        __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(a.y) + at;
+          for (int j = 0; j < 16; ++j) {
+            const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(y[j]) & 0x7fffffffu);
+            if (lane == j) most = m;
+          }
+          if (live && c0 + lane < mine1 && lane < 16) a.most[(size_t)(t0 + c0 + lane) * (a.tiles * 2) + tile * 4 + quarter] = __uint_as_float(most);
+        }
+        const size_t at = (size_t)(t0 + c0) * a.y_stride + channel;
+        const int rows_left = live && channel < a.n ? mine1 - c0 : 0;
+        if (GATED || a.y_f32) {
+          float* to = reinterpret_cast<float*>(a.y) + at;
 #pragma unroll
-        for (int j = 0; j < 16; ++j, to += a.y_stride)
-          if (j < rows_left) *to = __float2bfloat16(y[j]);
+          for (int j = 0; j < 16; ++j, to += a.y_stride)
+            if (j < rows_left) *to = y[j];
+        } else {
+          __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(a.y) + at;
+#pragma unroll
+          for (int j = 0; j < 16; ++j, to += a.y_stride)
+            if (j < rows_left) *to = __float2bfloat16(y[j]);
+        }
       }
-      steps = steps_of(c0 + 16);
     }
+  } else if (shares > 1) {
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (a.over_stages) ptx::cluster_sync();
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   }
   if (!ok) atomicExch(a.err, B200_ERR_DEVICE_FLAGGED);
   __syncwarp();
@@ -906,9 +916,10 @@ void launch_clusters(void (*kernel)(P...), int size, dim3 grid, int threads, siz
 }
 
 // What a product is expected to take with one kernel or the other.  Microseconds of launches one behind the other in a graph, fitted to 2048 x 2048 to 4096 x 14336
-// and 28672 x 4096 at 32 to 1024 rows: a block of weights reaches an SM in 0.27 us however few rows go with it, a row that a CTA brings to the output costs
-// 0.029 us, one whose sums it pushes 0.025, and sharing K 1.2.  4096 x 4096: 256 rows as 64 tiles of 128 in two shares 9.4 us (model 9.6), as 32 of 256
-// in four 11.2 (11.1), as pairs in two shares 11.5 (12.7); 512 rows as pairs 12.9, as tiles of 256 13.3; 1024 rows as pairs 15.8, as tiles 18.6.
+// and 28672 x 4096 at 1 to 1024 rows: a block of weights reaches an SM in 0.27 us however few rows go with it, a row that a CTA brings to the output costs
+// 0.02 us, one whose sums it pushes as much, and a cluster 0.55 for each of its CTAs.  4096 x 4096: 256 rows as 64 tiles of 128 in two shares 9.0 us (model 8.6), as
+// 32 of 256 in four 10.7 (10.8), as pairs in two shares 11.6 (12.1); 512 rows as 128 tiles of 128 12.2 (11.8), as pairs 13.0 (12.1); 1024 rows as pairs 15.8 (15.8),
+// as tiles 18.6 (16.1 at least).
 struct Plan {
   float us = 1e30f;
   bool pair = false;
@@ -929,8 +940,8 @@ Plan plan_of(const MmArgs& a, const int* stream_at_once, const int* pairs_at_onc
       const long long ctas = tiles * row_tiles * n;
       if (!split(n, 2) || pushed_bytes(rows_here, n, W) > kStreamAlone - 2048 || (n > 1 && ctas > stream_at_once[n])) continue;
       const int own = std::min(rows_here, rows_per_rank(rows_here, n));
-      float us = 0.6f + 0.029f * W * own + (float)((a.chunks + n - 1) / n) * W * std::max(0.27f, 0.0014f * tn);
-      if (n > 1) us += 1.2f + 0.025f * W * (rows_here - own);
+      float us = 0.6f + 0.02f * W * own + (float)((a.chunks + n - 1) / n) * W * std::max(0.27f, 0.0014f * tn);
+      if (n > 1) us += 0.55f * n + 0.02f * W * (rows_here - own);
       if (ctas > sms) us *= 1.18f * ctas / sms;
       if (us < best.us) best = {us, false, tn, n};
     }
@@ -940,7 +951,7 @@ Plan plan_of(const MmArgs& a, const int* stream_at_once, const int* pairs_at_onc
   for (int n = 1; n <= kMostPairs; ++n) {
     if (!split(n, 4) || pairs_at_once[n] < 1 || (n > 1 && items > pairs_at_once[n])) continue;
     const float waves = (float)((items + pairs_at_once[n] - 1) / pairs_at_once[n]);
-    const float us = (n == 1 ? 6.4f : 7.6f) + waves * ((GATED ? 2.5f : 0.8f) + 0.27f * ((a.chunks + n - 1) / n));
+    const float us = (n == 1 ? 6.4f : 7.0f) + waves * ((GATED ? 2.5f : 0.8f) + 0.27f * ((a.chunks + n - 1) / n));
     if (us < best.us) best = {us, true, 0, n};
   }
   return best;

@@ -576,7 +576,7 @@ def i8_mm(w: I8Weight, rows: I8Rows, x: Optional[torch.Tensor] = None, bias: Opt
         raise ValueError(f"expected a bias of {w.n} contiguous f32 on the current device, got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
     dtype, out_stride = _F32 if f32 else _BF16, w.n
     if out is None:
-        out = _new_rows(t, w.n, dtype, device)
+        out = _new_rows(t, w.n, dtype, device) if x is None or f32 else x.new_empty((t, w.n))
     else:
         out_stride = _rows(out, (t, w.n), device, dtype)
     _lib.check(lib.b200_i8_mm(w._h, rows._h, at, stride, t, None if bias is None else bias.data_ptr(), out.data_ptr(), out_stride, f32, _raw_stream(device)))
@@ -594,7 +594,7 @@ def i8_ffn(gate_up: I8Weight, down: I8Weight, rows: I8Rows, x: Optional[torch.Te
     at, stride, t = rows._take(x, gate_up.k, device)
     out_stride = down.n
     if out is None:
-        out = _new_rows(t, down.n, _BF16, device)
+        out = _new_rows(t, down.n, _BF16, device) if x is None else x.new_empty((t, down.n))
     else:
         out_stride = _rows(out, (t, down.n), device)
     _lib.check(lib.b200_i8_ffn(gate_up._h, down._h, rows._h, at, stride, t, ACTIVATIONS[activation], out.data_ptr(), out_stride, _raw_stream(device)))

@@ -577,11 +577,13 @@ b200_status b200_lora_apply(const b200_lora* l, b200_lora_batch* b, const void* 
  * the sum is exact (32 bits), the rest f32, one rounding.  A row of zeros has the product 0; a row that holds an infinity or no number gives NaN in all its
  * columns and changes no other row.  Same bits for a row whatever shares its batch.
  * A b200_i8_rows holds the rows of a step in 8 bits and is the workspace of the products that read them: steps that may run at the same time (two
- * captured graphs on two streams) have one each.  All calls but those that create are asynchronous on the stream and may be captured.  A wait inside the
- * kernels that runs out is reported through b200_qmm_error_word. */
+ * captured graphs on two streams) have one each.  A captured product without its rows' making works on what the handle holds when it runs.  All calls but
+ * those that create are asynchronous on the stream and may be captured.  Rows, strides and widths may be any.  A wait inside the kernels that runs out is
+ * reported through b200_qmm_error_word. */
 typedef struct b200_i8_weight b200_i8_weight;
 typedef struct b200_i8_rows b200_i8_rows;
-/* q int8 [n, k], scales f32 [n], in host or device memory; n up to 2^24, k up to 131072.  Synchronous. */
+/* q int8 [n, k], scales f32 [n], in host or device memory; n up to 2^24, k up to 131072.  Synchronous: the numbers are copied into an order of the
+ * library's own. */
 b200_status b200_i8_weight_create(int32_t n, int32_t k, const int8_t* q, const float* scales, b200_i8_weight** out);
 /* The gate and the up projection of a gated feed-forward block side by side, each int8 [n, k] with f32 [n]. */
 b200_status b200_i8_weight_create_gated(int32_t n, int32_t k, const int8_t* gate_q, const float* gate_scales, const int8_t* up_q, const float* up_scales,
@@ -590,12 +592,12 @@ void b200_i8_weight_destroy(b200_i8_weight* w);
 /* Up to max_rows rows of up to max_k columns; max_hidden: the widest feed-forward block that reads them (0: none). */
 b200_status b200_i8_rows_create(int32_t max_rows, int32_t max_k, int32_t max_hidden, b200_i8_rows** out);
 void b200_i8_rows_destroy(b200_i8_rows* r);
-/* rows <- x [rows, k] bf16, stride in elements (any; rows on 16 bytes with strides of a multiple of 8 are read fastest). */
+/* rows <- x [rows, k] bf16, stride in elements. */
 b200_status b200_i8_quantize(b200_i8_rows* r, const void* d_x, int64_t x_stride, int32_t rows, int32_t k, void* stream);
 /* What the handle holds: q int8 [rows, k] and the steps m / 127 f32 [rows], either may be null. */
 b200_status b200_i8_rows_get(const b200_i8_rows* r, void* d_q, float* d_steps, void* stream);
 /* y [rows, n] bf16 (y_f32: f32), stride in elements; bias f32 [n] or null.  With d_x (bf16 [rows, k]) the rows are made from it first, as b200_i8_quantize
- * does; d_x null takes the `rows` rows that the handle holds.  y may not overlap what the handle or x hold. */
+ * does; d_x null takes the `rows` rows that the handle holds.  y does not overlap x.  A refused call changes nothing. */
 b200_status b200_i8_mm(const b200_i8_weight* w, b200_i8_rows* r, const void* d_x, int64_t x_stride, int32_t rows, const float* d_bias, void* d_y,
                        int64_t y_stride, int32_t y_f32, void* stream);
 /* y = W_down q(act(W_gate x) * (W_up x)) bf16 [rows, n of down]: both projections, the activation and the product in one kernel, whose result stays
@@ -608,8 +610,8 @@ b200_status b200_i8_ffn(const b200_i8_weight* gate_up, const b200_i8_weight* dow
  *   p = y, or y / sqrt(mean(y^2) + eps) * post_weight; p = p * gate, or p * sigmoid(gate); h_out = h + scale * p;
  *   x = h_out, or h_out / sqrt(mean(h_out^2) + eps) * norm_weight (h_out before its rounding).
  * f32 in between, one rounding each.  y and h are rows of n numbers (bf16, or f32 with y_f32, h_f32; h_out is like h and may be h), weights bf16 [n], null =
- * no norm; gate bf16, null = none, gate_stride 0: one for all rows.  x goes to x_out (bf16) and, in 8 bits, into q_out, either null.  n up to 32768;
- * strides in elements, any. */
+ * no norm; gate bf16, null = none, gate_stride 0: one for all rows.  x goes to x_out (bf16) and, in 8 bits, into q_out, either null.  Nothing but h_out and
+ * h overlaps.  n up to 32768; strides in elements, any. */
 typedef struct b200_residual_norm_shape {
   int32_t n;
   int32_t h_f32, y_f32;
