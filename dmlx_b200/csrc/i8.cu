@@ -105,16 +105,23 @@ b200_status quantize(const __nv_bfloat16* x, long long x_stride, int rows, int k
 // read and a row may be many blocks'.  A block's warps take eight neighbouring rows, whose bytes lie together.
 constexpr int kInnerThreads = 256, kInnerAhead = 4;  // (loads of 256 columns that a warp has in flight)
 
-__global__ void __launch_bounds__(kInnerThreads, 2) i8_quantize_inner_kernel(const float* h, long long h_stride, const float* most, int groups, signed char* __restrict__ q,
+__global__ void __launch_bounds__(kInnerThreads, 3) i8_quantize_inner_kernel(const float* h, long long h_stride, const float* most, int groups, signed char* __restrict__ q,
                                                                              float* __restrict__ steps, int rows, int k, int chunks, int per_block) {
   after_previous();
   const int lane = threadIdx.x & 31, row = blockIdx.x * (kInnerThreads / 32) + (threadIdx.x >> 5);
   if (row >= rows) return;
   const int first = blockIdx.y * per_block, last = min(first + per_block, chunks * kI8Chunk);
-  const float* from = h + (size_t)row * h_stride;
-  Eight<float> keep[kInnerAhead];
-  auto load = [&](int c0) {
-    load_eights(keep, from, k, true, [&](int u) { return c0 + u * 256 + lane * 8; });
+  const float* from = h + (size_t)row * h_stride + lane * 8;
+  float4 keep[kInnerAhead][2];
+  auto load = [&](int c0) {  // (rows are whole vectors, what lies behind the last column of the last one is not looked at)
+#pragma unroll
+    for (int u = 0; u < kInnerAhead; ++u) {
+      keep[u][0] = keep[u][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (c0 + u * 256 + lane * 8 < k) {
+        keep[u][0] = *reinterpret_cast<const float4*>(from + c0 + u * 256);
+        keep[u][1] = *reinterpret_cast<const float4*>(from + c0 + u * 256 + 4);
+      }
+    }
   };
   load(first);
   uint32_t m = 0u;
@@ -126,8 +133,13 @@ __global__ void __launch_bounds__(kInnerThreads, 2) i8_quantize_inner_kernel(con
     if (c0 > first) load(c0);
 #pragma unroll
     for (int u = 0; u < kInnerAhead; ++u) {
-      float f[8];
-      widen(keep[u], f);
+      float f[8] = {keep[u][0].x, keep[u][0].y, keep[u][0].z, keep[u][0].w, keep[u][1].x, keep[u][1].y, keep[u][1].z, keep[u][1].w};
+      const int left = k - (c0 + u * 256 + lane * 8);
+      if (left < 8) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e >= left) f[e] = 0.f;
+      }
       if (c0 + u * 256 + lane * 8 < last) *reinterpret_cast<uint2*>(to + u * 2 * kI8Block) = s.quantize(f);
     }
   }
@@ -264,7 +276,9 @@ __device__ __forceinline__ void tmem_ld4(uint32_t taddr, uint32_t& a, uint32_t& 
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(taddr) : "memory");
 }
 
-constexpr int kRawRows = 4, kRawNumbers = 16384, kRawChunks = 32;  // rows of RAW; their numbers at most; blocks of K in a share at most
+// RAW's rows; their numbers at most; blocks of K in a share at most, and times the rows (four rows through a block of 14336: 35.1 us with kernels of their own for
+// the rows, 37.6 without; two 34.8 and 33.8; four through one of 8192 17.8 and 16.7).
+constexpr int kRawRows = 4, kRawNumbers = 16384, kRawChunks = 32, kRawWork = 64;
 
 // Warps 2 to 9: rows into 8 bits, as i8_quantize_kernel and i8_quantize_inner_kernel do, blocks chunk0 and on as an operand of 16 rows each at `to` (the rows that
 // are not there hold anything), steps into `steps`; `out` and `first`: into the handle too, and the steps.
@@ -272,40 +286,40 @@ template <typename T>
 __device__ __forceinline__ void raw_rows(const MmArgs& a, const T* x, bool fit, unsigned char* to, int chunk0, int chunks, bool out, bool first, uint64_t* ready, float* steps,
                                          uint32_t* part) {
   constexpr bool kInner = sizeof(T) == 4;
-  constexpr int kAhead = 2, kThreads = kStreamThreads - 64;
-  const int t = threadIdx.x - 64, lane = t & 31, warp = t >> 5;
+  constexpr int kAhead = 4, kWarps = kStreamThreads / 32 - 2;
+  // The rows at the same time, each by as many warps.
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - 2, warps = a.rows == 1 ? kWarps : a.rows == 2 ? kWarps / 2 : kWarps / 4, threads = warps * 32;
+  const int r = warp / warps, t = (warp - r * warps) * 32 + lane;
+  const bool there = r < a.rows;
+  const T* row = x + (size_t)(there ? r : 0) * a.raw_stride;
+  uint32_t m = 0u;
+  if constexpr (kInner) {
+    for (int g = t; g < a.chunks * 4; g += threads) m = max(m, __float_as_uint(a.raw_most[(size_t)(there ? r : 0) * (a.chunks * 4) + g]));
+  } else {
 #pragma unroll 1
-  for (int r = 0; r < a.rows; ++r) {
-    uint32_t m = 0u;
-    if constexpr (kInner) {
-      for (int g = t; g < a.chunks * 4; g += kThreads) m = max(m, __float_as_uint(a.raw_most[(size_t)r * (a.chunks * 4) + g]));
-    } else {
-#pragma unroll 1
-      for (int v = t; v * 8 < a.k; v += kAhead * kThreads) {
-        Eight<T> e[kAhead];
-        load_eights(e, x + (size_t)r * a.raw_stride, a.k, fit, [&](int u) { return (v + u * kThreads) * 8; });
+    for (int v = t; v * 8 < a.k; v += kAhead * threads) {
+      Eight<T> e[kAhead];
+      load_eights(e, row, a.k, fit, [&](int u) { return (v + u * threads) * 8; });
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) m = most_of(m, e[u]);
-      }
+      for (int u = 0; u < kAhead; ++u) m = most_of(m, e[u]);
     }
-    m = __reduce_max_sync(0xffffffffu, m);
-    if (lane == 0) part[warp * kRawRows + r] = m;
   }
-  asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
-#pragma unroll 1
-  for (int r = 0; r < a.rows; ++r) {
-    const I8Scale s = I8Scale::of(__uint_as_float(__reduce_max_sync(0xffffffffu, part[lane % (kThreads / 32) * kRawRows + r])));
+  m = __reduce_max_sync(0xffffffffu, m);
+  if (lane == 0) part[warp] = m;
+  asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
+  if (there) {
+    const I8Scale s = I8Scale::of(__uint_as_float(__reduce_max_sync(0xffffffffu, part[r * warps + lane % warps])));
     if (t == 0) {
       steps[r] = s.step();
       if (out && first && !kInner) a.step_out[r] = s.step();
     }
 #pragma unroll 1
-    for (int v = t; v < chunks * 16; v += kAhead * kThreads) {
+    for (int v = t; v < chunks * 16; v += kAhead * threads) {
       Eight<T> e[kAhead];
-      load_eights(e, x + (size_t)r * a.raw_stride, a.k, fit, [&](int u) { return chunk0 * kI8Chunk + (v + u * kThreads) * 8; });
+      load_eights(e, row, a.k, fit, [&](int u) { return chunk0 * kI8Chunk + (v + u * threads) * 8; });
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        const int at = v + u * kThreads, piece = at & 15;
+        const int at = v + u * threads, piece = at & 15;
         if (at >= chunks * 16) break;
         float f[8];
         widen(e[u], f);
@@ -316,7 +330,7 @@ __device__ __forceinline__ void raw_rows(const MmArgs& a, const T* x, bool fit, 
     }
   }
   ptx::fence_proxy_async_smem();
-  asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");  // the steps are there
+  asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");  // the steps are there
   if (lane == 0) ptx::mbar_arrive(ready);
 }
 
@@ -335,7 +349,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
   uint64_t* rows_ready = pushed + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rows_ready + 1);
   float* raw_steps = reinterpret_cast<float*>(tmem_slot + 1);                    // [kRawRows]
-  uint32_t* raw_part = reinterpret_cast<uint32_t*>(raw_steps + kRawRows);        // [warp][kRawRows]
+  uint32_t* raw_part = reinterpret_cast<uint32_t*>(raw_steps + kRawRows);        // [warp]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int shares = a.shares, rank = shares > 1 ? (int)ptx::cluster_rank() : 0;
   const int tile = blockIdx.x / shares, t0 = blockIdx.y * a.tn, rows_here = min(a.tn, a.rows - t0), n_here = (rows_here + 15) / 16 * 16;
@@ -430,7 +444,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
   const int quarter = warp & 3, half = (warp - 2) >> 2, channel = tile * kI8Tile + quarter * 32 + lane;
   const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
   float ws = 0.f, us = 0.f, bias = 0.f;
-  auto steps_of = [&](int c0) { return c0 + (lane & 15) < mine1 ? (RAW ? raw_steps[(c0 + lane) & 3] : a.step[t0 + c0 + (lane & 15)]) : 0.f; };  // sixteen rows' in the lanes
+  auto steps_of = [&](int c0) { return c0 + (lane & 15) < mine1 ? (RAW ? raw_steps[(c0 + lane) % kRawRows] : a.step[t0 + c0 + (lane & 15)]) : 0.f; };  // sixteen rows' in the lanes
   if constexpr (RAW) {
     if (warp >= 2) {
       const bool out = blockIdx.x < shares;
@@ -985,7 +999,7 @@ b200_status launch_product(MmArgs& a, const I8RowsDev& to, const RawRows& raw, c
   const Plan plan = plan_of<GATED>(a, at_once, pairs_at_once);
   a.shares = plan.shares;
   const int per_share = (a.chunks + a.shares - 1) / a.shares;
-  const bool in_kernel = raw.x && !plan.pair && a.rows <= kRawRows && per_share <= kRawChunks && (raw.inner || a.rows * a.k <= kRawNumbers);
+  const bool in_kernel = raw.x && !plan.pair && a.rows <= kRawRows && per_share <= kRawChunks && a.rows * per_share <= kRawWork && (raw.inner || a.rows * a.k <= kRawNumbers);
   if (raw.x && !in_kernel) {
     const b200_status st = raw.inner ? quantize_inner(raw.inner, a.rows, a.k, s) : quantize((const __nv_bfloat16*)raw.x, raw.stride, a.rows, a.k, to, s);
     if (st != B200_OK) return st;
