@@ -585,6 +585,9 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
 constexpr int kPairThreads = 384, kPairStage = 2 * kI8Block, kPairStages = 6, kPairRows = 256, kPairBand = 16, kMostPairs = 4;
 constexpr int kPairPitch = 20;  // epilogue: words between rows in a warp's staging tile of 32 rows by 16 words
 constexpr int kPairShared = 1024 + kPairStages * kPairStage + 8 * 32 * kPairPitch * 4 + 8 * 2 * kI8Tile * 4 + 8 * (3 * kPairStages + 6) + 16;
+// (A pair's CTAs hold all tensor memory of their SMs while they wait for one another, so none may lie beside another kernel's that holds some: what is left has no room
+// for a CTA of i8_stream_kernel, whose one block of weights and rows is 18 KB.)
+static_assert(kPairShared > (228 - 20) * 1024, "a pair's CTA has its SM for itself");
 
 __device__ __forceinline__ void umma2_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
