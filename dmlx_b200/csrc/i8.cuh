@@ -87,14 +87,15 @@ struct Eight { uint4 r[sizeof(T) / 2]; };
 // N times eight numbers of a row of n, at columns at(0), at(1), ..., multiples of eight; fit: the row starts on 16 bytes.  Elsewhere the 16-byte pieces that
 // hold the numbers are fetched and shifted into place (rows of 5003 bf16 and f32 one number at a time took three times as long).  All loads are on
 // their way before the first is looked at; what lies at a row's ends, where a piece would reach beyond it, is fetched number by number behind them.
+// The row may begin at column lo.
 template <typename T, int N, class At>
-__device__ __forceinline__ void load_eights(Eight<T> (&e)[N], const T* p, int n, bool fit, At at) {
+__device__ __forceinline__ void load_eights(Eight<T> (&e)[N], const T* p, int n, bool fit, At at, int lo = 0) {
   constexpr int R = sizeof(T) / 2, kWords = 4 * R;
   const uint32_t off = fit ? 0u : (uint32_t)(reinterpret_cast<uintptr_t>(p) & 15);
   const int before = (int)(off / sizeof(T));  // numbers of the first piece that come ahead
   const uint4* pieces = reinterpret_cast<const uint4*>(p - before);
   uint4 last[N];
-  auto whole = [&](int c) { return fit ? c + 8 <= n : c >= before && c - before + 8 + 16 / (int)sizeof(T) <= n; };
+  auto whole = [&](int c) { return c - before >= lo && (fit ? c + 8 <= n : c - before + 8 + 16 / (int)sizeof(T) <= n); };
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     const int c = at(k);
@@ -135,7 +136,7 @@ __device__ __forceinline__ void load_eights(Eight<T> (&e)[N], const T* p, int n,
     if (whole(c) || c >= n) continue;
     T v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < n ? p[c + i] : T(0.f);
+    for (int i = 0; i < 8; ++i) v[i] = c + i >= lo && c + i < n ? p[c + i] : T(0.f);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       uint32_t w[4];
@@ -149,9 +150,9 @@ __device__ __forceinline__ void load_eights(Eight<T> (&e)[N], const T* p, int n,
   }
 }
 template <typename T>
-__device__ __forceinline__ Eight<T> load_eight(const T* p, int c, int n, bool fit) {
+__device__ __forceinline__ Eight<T> load_eight(const T* p, int c, int n, bool fit, int lo = 0) {
   Eight<T> e[1];
-  load_eights(e, p, n, fit, [&](int) { return c; });
+  load_eights(e, p, n, fit, [&](int) { return c; }, lo);
   return e[0];
 }
 __device__ __forceinline__ void widen(const Eight<__nv_bfloat16>& e, float (&v)[8]) {

@@ -25,15 +25,14 @@ struct ResidualNormArgs {
   I8RowsDev q;
   long long h_stride, y_stride, gate_stride, h_out_stride, x_out_stride;
   int rows, n, chunks, sigmoid;
-  int fit;  // bits: which rows may be read and written in vectors of eight
+  int shift;  // columns may be dealt out from ahead of the first: no 8-bit rows, which want them from the first, and room for a vector more
   float scale, eps;
 };
-enum { kFitH = 1, kFitY = 2, kFitGate = 4, kFitPost = 8, kFitNorm = 16, kFitHOut = 32, kFitXOut = 64, kFitAll = 127 };
 
 // The lanes' numbers, eight for each, neighbouring lanes' next to one another, to a row of n from column c of each lane on.  Where rows do not start on 16
 // bytes a lane's numbers behind the first boundary and the next lane's ahead of it are a piece; a warp's ends go one by one.  (All lanes of the warp.)
 template <typename T>
-__device__ __forceinline__ void store_eight(T* p, int c, int n, bool fit, const float (&v)[8]) {
+__device__ __forceinline__ void store_eight(T* p, int c, int n, bool fit, const float (&v)[8], int lo = 0) {
   constexpr int kWords = 2 * (int)sizeof(T);
   uint32_t w[kWords + 4];
 #pragma unroll
@@ -46,14 +45,14 @@ __device__ __forceinline__ void store_eight(T* p, int c, int n, bool fit, const 
     }
   }
   if (fit) {
-    if (c + 8 <= n) {
+    if (c >= lo && c + 8 <= n) {
 #pragma unroll
       for (int i = 0; i < kWords / 4; ++i) reinterpret_cast<uint4*>(p + c)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
       return;
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (c + i < n) st(p + c + i, v[i]);
+      if (c + i >= lo && c + i < n) st(p + c + i, v[i]);
     return;
   }
   const uint32_t off = (16u - (uint32_t)(reinterpret_cast<uintptr_t>(p + c) & 15)) & 15;  // bytes up to the first boundary
@@ -68,15 +67,15 @@ __device__ __forceinline__ void store_eight(T* p, int c, int n, bool fit, const 
 #pragma unroll
     for (int i = 0; i < kWords; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (off & 2) * 8);
   }
-  const bool pieces = (lane < 31 || head == 0) && c + head + 8 <= n;
+  const bool pieces = (lane < 31 || head == 0) && c + head >= lo && c + head + 8 <= n;
   if (pieces) {
 #pragma unroll
     for (int i = 0; i < kWords / 4; ++i) reinterpret_cast<uint4*>(p + c + head)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
   }
-  const bool before = lane == 0 || c + head > n;  // the lane ahead has not taken this one's first
+  const bool before = lane == 0 || c + head > n || c - 8 + head < lo;  // the lane ahead has not taken this one's first
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    if (c + i < n && (i < head ? before : !pieces)) st(p + c + i, v[i]);
+    if (c + i >= lo && c + i < n && (i < head ? before : !pieces)) st(p + c + i, v[i]);
 }
 
 // NV vectors of eight columns for each thread.  WARP: a warp for a row.  FIT: all rows start on 16 bytes and are whole vectors.  (1024 threads with 32 numbers each have 64 registers: half of a row's y is
@@ -98,21 +97,31 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const 
     }
     return v;
   };
-  const H* h = (const H*)a.h + (size_t)row * a.h_stride;
-  const Y* y = (const Y*)a.y + (size_t)row * a.y_stride;
+  // Where rows do not start on 16 bytes, the columns are dealt out from a boundary of h_out ahead of its row (`lo` columns that are not there), and so are on
+  // boundaries of all that lies like it.
+  const int lo = FIT || !a.shift ? 0 : (int)((reinterpret_cast<uintptr_t>((H*)a.h_out + (size_t)row * a.h_out_stride) / sizeof(H)) % 8);
+  const int n = a.n + lo;
+  const H* h = (const H*)a.h + (size_t)row * a.h_stride - lo;
+  const Y* y = (const Y*)a.y + (size_t)row * a.y_stride - lo;
+  const __nv_bfloat16 *gate = a.gate ? a.gate + (size_t)row * a.gate_stride - lo : nullptr, *post_w = a.post_w ? a.post_w - lo : nullptr, *norm_w = a.norm_w ? a.norm_w - lo : nullptr;
+  H* h_out = (H*)a.h_out + (size_t)row * a.h_out_stride - lo;
+  __nv_bfloat16* x_out = a.x_out ? a.x_out + (size_t)row * a.x_out_stride - lo : nullptr;
+  auto fits = [](const void* p) { return FIT || (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   Eight<Y> yr[NV];
   Eight<H> hr[NV];
-  load_eights(yr, y, a.n, FIT || (a.fit & kFitY), column);
-  load_eights(hr, h, a.n, FIT || (a.fit & kFitH), column);
+  load_eights(yr, y, n, fits(y), column, lo);
+  load_eights(hr, h, n, fits(h), column, lo);
   Eight<__nv_bfloat16> gr[NV <= 2 ? NV : 1];
   if constexpr (NV <= 2) {
-    if (a.gate) load_eights(gr, a.gate + (size_t)row * a.gate_stride, a.n, FIT || (a.fit & kFitGate), column);
+    if (gate) load_eights(gr, gate, n, fits(gate), column, lo);
   }
   Eight<__nv_bfloat16> pr[NV <= 2 ? NV : 1], nr[NV == 1 ? NV : 1];
   if constexpr (NV <= 2) {
-    if (a.post_w) load_eights(pr, a.post_w, a.n, FIT || (a.fit & kFitPost), column);
+    if (post_w) load_eights(pr, post_w, n, fits(post_w), column, lo);
   }
-  if (NV == 1 && a.norm_w) nr[0] = load_eight(a.norm_w, column(0), a.n, FIT || (a.fit & kFitNorm));
+  if constexpr (NV == 1) {
+    if (norm_w) load_eights(nr, norm_w, n, fits(norm_w), column, lo);
+  }
   float ry = 1.f;
   if (a.post_w) {
     float ss = 0.f;
@@ -134,12 +143,12 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const 
     float p[8], w[8];
     widen(yr[u], p);
     if (a.post_w) {
-      widen(NV <= 2 ? pr[NV <= 2 ? u : 0] : load_eight(a.post_w, c, a.n, FIT || (a.fit & kFitPost)), w);
+      widen(NV <= 2 ? pr[NV <= 2 ? u : 0] : load_eight(post_w, c, n, fits(post_w), lo), w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) p[e] = p[e] * ry * w[e];
     }
     if (a.gate) {
-      widen(NV <= 2 ? gr[NV <= 2 ? u : 0] : load_eight(a.gate + (size_t)row * a.gate_stride, c, a.n, FIT || (a.fit & kFitGate)), w);
+      widen(NV <= 2 ? gr[NV <= 2 ? u : 0] : load_eight(gate, c, n, fits(gate), lo), w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) p[e] *= a.sigmoid ? __fdividef(1.0f, 1.0f + __expf(-w[e])) : w[e];
     }
@@ -149,9 +158,9 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const 
       x[u][e] = fmaf(a.scale, p[e], w[e]);
       ss = fmaf(x[u][e], x[u][e], ss);  // (behind the last column all is zero)
     }
-    store_eight((H*)a.h_out + (size_t)row * a.h_out_stride, c, a.n, FIT || (a.fit & kFitHOut), x[u]);
+    store_eight(h_out, c, n, fits(h_out), x[u], lo);
     if (a.norm_w) {
-      widen(NV == 1 ? nr[0] : load_eight(a.norm_w, c, a.n, FIT || (a.fit & kFitNorm)), w);
+      widen(NV == 1 ? nr[0] : load_eight(norm_w, c, n, fits(norm_w), lo), w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[u][e] *= w[e];
     }
@@ -170,7 +179,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const 
   for (int u = 0; u < NV; ++u) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[u][e] *= r;
-    if (a.x_out) store_eight(a.x_out + (size_t)row * a.x_out_stride, column(u), a.n, FIT || (a.fit & kFitXOut), x[u]);
+    if (x_out) store_eight(x_out, column(u), n, fits(x_out), x[u], lo);
   }
   if (!a.q.q) return;
   if constexpr (!WARP) most = __reduce_max_sync(0xffffffffu, (t & 31) < (threads >> 5) ? __float_as_uint(part[2][t & 31]) : 0u);
@@ -183,16 +192,16 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const 
 
 template <typename H, typename Y, bool FIT>
 b200_status launch(const ResidualNormArgs& a, cudaStream_t s) {
-  const int vectors = a.chunks * (kI8Chunk / 8);
+  const int vectors = std::max(a.chunks * (kI8Chunk / 8), a.shift ? (a.n + 14) / 8 : 0);  // (up to seven columns ahead of the first)
   if (vectors <= 32 * 2) {
     const int warps = a.rows >= 8 * b200_sm_count() ? 8 : 1;
     const unsigned grid = (unsigned)((a.rows + warps - 1) / warps);
     if (vectors <= 32) launch_after(residual_norm_kernel<H, Y, 1, true, FIT>, grid, warps * 32, 0, s, a);
     else launch_after(residual_norm_kernel<H, Y, 2, true, FIT>, grid, warps * 32, 0, s, a);
   } else {
-    // few rows: more threads, each with fewer loads to wait for
-    const bool few = a.rows <= 2 * b200_sm_count();
-    const int nv = vectors <= 1024 && few ? 1 : vectors <= 2048 ? 2 : 4;
+    // Few rows: more threads, each with fewer loads to wait for, while all of them run at once (200 rows of 4096 3.2 us with one vector a thread, 3.4 with two; 600
+    // 6.8 and 5.7; 64 of 8192 3.2 and 3.5, 200 5.9 and 4.6).
+    const int nv = vectors <= 1024 && (long long)a.rows * vectors <= 864ll * b200_sm_count() ? 1 : vectors <= 2048 ? 2 : 4;
     const int threads = (vectors + 32 * nv - 1) / (32 * nv) * 32;
     if (nv == 1) launch_after(residual_norm_kernel<H, Y, 1, false, FIT>, a.rows, threads, 0, s, a);
     else if (nv == 2) launch_after(residual_norm_kernel<H, Y, 2, false, FIT>, a.rows, threads, 0, s, a);
@@ -203,8 +212,8 @@ b200_status launch(const ResidualNormArgs& a, cudaStream_t s) {
 }
 
 template <typename H, typename Y>
-b200_status launch_any(const ResidualNormArgs& a, cudaStream_t s) {
-  return a.n % 8 == 0 && a.fit == kFitAll ? launch<H, Y, true>(a, s) : launch<H, Y, false>(a, s);
+b200_status launch_any(const ResidualNormArgs& a, bool fit, cudaStream_t s) {
+  return fit ? launch<H, Y, true>(a, s) : launch<H, Y, false>(a, s);
 }
 
 constexpr int kMostColumns = 32768;  // 1024 threads of four vectors
@@ -240,10 +249,11 @@ extern "C" b200_status b200_residual_norm(const b200_residual_norm_shape* shape,
   if (q_out) a.q = q_out->x;
   a.h_stride = h_stride; a.y_stride = y_stride; a.gate_stride = gate_stride; a.h_out_stride = h_out_stride; a.x_out_stride = x_out_stride;
   a.rows = rows; a.n = n; a.chunks = i8_chunks(n); a.sigmoid = shape->gate_sigmoid != 0; a.scale = shape->scale; a.eps = shape->eps;
-  auto fits = [&](const void* p, int64_t stride, int size, int bit) { return ((uintptr_t)p & 15) == 0 && (rows <= 1 || stride * size % 16 == 0) ? bit : 0; };
-  a.fit = fits(d_h, h_stride, h_size, kFitH) | fits(d_y, y_stride, y_size, kFitY) | fits(d_gate, gate_stride, 2, kFitGate) | fits(d_post_weight, 0, 2, kFitPost) |
-          fits(d_norm_weight, 0, 2, kFitNorm) | fits(d_h_out, h_out_stride, h_size, kFitHOut) | fits(d_x_out, x_out_stride, 2, kFitXOut);
+  auto fits = [&](const void* p, int64_t stride, int size) { return ((uintptr_t)p & 15) == 0 && (rows <= 1 || stride * size % 16 == 0); };
+  const bool fit = n % 8 == 0 && fits(d_h, h_stride, h_size) && fits(d_y, y_stride, y_size) && fits(d_gate, gate_stride, 2) && fits(d_post_weight, 0, 2) &&
+                   fits(d_norm_weight, 0, 2) && fits(d_h_out, h_out_stride, h_size) && fits(d_x_out, x_out_stride, 2);
+  a.shift = !fit && !q_out && (n + 14) / 8 <= kMostColumns / 8;
   cudaStream_t s = (cudaStream_t)stream;
-  if (shape->h_f32) return shape->y_f32 ? launch_any<float, float>(a, s) : launch_any<float, __nv_bfloat16>(a, s);
-  return shape->y_f32 ? launch_any<__nv_bfloat16, float>(a, s) : launch_any<__nv_bfloat16, __nv_bfloat16>(a, s);
+  if (shape->h_f32) return shape->y_f32 ? launch_any<float, float>(a, fit, s) : launch_any<float, __nv_bfloat16>(a, fit, s);
+  return shape->y_f32 ? launch_any<__nv_bfloat16, float>(a, fit, s) : launch_any<__nv_bfloat16, __nv_bfloat16>(a, fit, s);
 }

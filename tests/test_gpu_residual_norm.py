@@ -47,7 +47,7 @@ def _cuda(t):
 
 
 SHAPES = [(1, 1), (1, 4096), (2, 7), (3, 128), (5, 129), (64, 256), (33, 512), (1300, 512), (40, 513), (400, 1000), (7, 2880), (300, 4096), (320, 5003), (2, 8192), (310, 8200),
-          (3, 16384), (300, 16384), (2, 16392), (5, 20001), (2, 32768)]
+          (3, 16384), (300, 16384), (2, 16392), (5, 20001), (2, 32768), (3, 32767), (3, 32761), (5, 1023), (300, 255), (1300, 129), (4, 511), (230, 8191)]
 
 
 @pytest.mark.gpu
