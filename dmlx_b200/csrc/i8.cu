@@ -2,6 +2,10 @@
 //   y[t][n] = (sum_k q[t][k] w[n][k]) scale[n] step[t] + bias[n],   q[t][k] = round(127 x[t][k] / max_k |x[t][k]|),  step[t] = max_k |x[t][k]| / 127.
 //
 // The sums are exact (int32 on tcgen05.mma kind::i8), so neither the order of K nor what shares a tile changes a bit of a row.
+//
+// Few rows are bound by the weights: one row of 4096 to 6144 7.3 us in a graph, one through a block of 14336 33 (176 MB, 5.4 TB/s), 96 through it 43.  Many are bound by
+// the tensor cores under the power cap: 8192 rows of 4096 to 6144 127 to 132 us beside 20 to 30 for the rows themselves, 3.2 PFLOP/s, through a block of 14336
+// 1130 to 1200, 600 to 630 of them the first product, 270 to 280 the second, 115 to 140 the inner rows into 8 bits.
 #include <cuda_bf16.h>
 #include <math.h>
 
@@ -19,7 +23,8 @@
 namespace {
 
 // ---- rows into 8 bits ----------------------------------------------------------------------------------------------------
-// A row waits in registers while its largest is looked for: a block for each, or a warp where a row is short.  Bound by what it reads and writes.
+// A row waits in registers while its largest is looked for: a block for each, or a warp where a row is short.  Bound by what it reads and writes, and by its
+// arithmetic in turn: 8192 rows of 4096 20 to 24 us (4.2 TB/s), 96 2.3.  (A warp for each of eight neighbouring rows, whose bytes lie together: 38.)
 struct QuantizeArgs {
   const __nv_bfloat16* x;
   long long x_stride;
@@ -102,7 +107,8 @@ b200_status quantize(const __nv_bfloat16* x, long long x_stride, int rows, int k
 }
 
 // The feed-forward block's inner rows, of which the product that made them has left the largest of every 32 channels, so that nothing waits for a row to be
-// read and a row may be many blocks'.  A block's warps take eight neighbouring rows, whose bytes lie together.
+// read and a row may be many blocks'.  A block's warps take eight neighbouring rows, whose bytes lie together.  Bound by what it reads and writes: 8192 rows of 14336
+// 118 us, 5 TB/s (141 as a block for each row); behind a short product, whose results are still on their way to memory, 130.
 constexpr int kInnerThreads = 256, kInnerAhead = 4;  // (loads of 256 columns that a warp has in flight)
 
 __global__ void __launch_bounds__(kInnerThreads, 3) i8_quantize_inner_kernel(const float* h, long long h_stride, const float* most, int groups, signed char* __restrict__ q,
@@ -239,10 +245,11 @@ __device__ __forceinline__ void gate_with(int act, float (&y)[N], const float (&
 
 // ---- up to a few hundred rows: streams of weights ----
 // A weight tile (gated: the gate's and up's tile of the same channels) by up to tn rows and a share of K per CTA.  The weights are the MMA's M, the rows
-// its N, so that few rows waste nothing; a lane of tensor memory is a channel.  Warp 0 loads, warp 1 multiplies, eight bring the sums to the output, every other sixteen rows of 32 channels each.
-// Bound by the weights, which come at the rate of memory only if every SM asks for them: a cluster of up to eight CTAs shares K (as many as still run at
-// the same time).  Each of them brings a share of the rows to the output and gets the others' sums of these pushed into its
-// shared memory, where the stages were unless there is room beside them, with a barrier that counts their bytes.
+// its N, so that few rows waste nothing; a lane of tensor memory is a channel.  Warp 0 loads, warp 1 multiplies, eight bring the sums to the output, each every
+// other sixteen rows of 32 channels.
+// Bound by the weights, which come at the rate of memory only if every SM asks for them (an SM gets 16 KB of them in 0.27 us, however many are on their way): a
+// cluster of up to eight CTAs shares K, an SM for each.  A CTA brings a share of the rows to the output and gets the others' sums of these
+// pushed into its shared memory, where the stages were unless there is room beside them, with a barrier that counts their bytes.
 constexpr int kStreamThreads = 320, kStreamShared = 112 * 1024, kStreamAlone = 226 * 1024, kMostShares = 8;  // (shared memory of two CTAs on an SM, of one)
 
 // Weights that go through L2 once: they leave it ahead of what else is there.  (Among it are the instructions, which a kernel fetches anew: behind 117 MB of

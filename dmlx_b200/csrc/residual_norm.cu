@@ -1,9 +1,12 @@
 // The norms behind and before a block with its gate and its factor on the residual, in one pass over the rows:
 //   p = y r(y) w_post (or y), times the gate or its sigmoid;  h' = h + scale p;  x = h' r(h') w_norm (or h'),  r(v) = 1 / sqrt(mean(v^2) + eps).
 //
-// A row waits in registers, a block of threads for it (a warp where it is short, eight rows to a block), and two rounds of sums: |y|^2, then |h'|^2
-// together with the largest |h' w_norm|, from which the 8-bit form's step follows without a third (r > 0, and rounding keeps the order).  x is made of h'
-// before its rounding.  f32 in between, one rounding for each result.  Bound by what it reads and writes.
+// A row waits in registers, a block of threads for it (a warp where it is short), and two rounds of sums: |y|^2, then |h'|^2 together with the
+// largest |h' w_norm|, from which the 8-bit form's step follows without a third (r > 0, and rounding keeps the order).  x is made of h' before its rounding.
+// f32 in between, one rounding for each result.  Everything a row needs is asked for before its first sum.
+//
+// Bound by what it reads and writes: 8192 rows of 4096 bf16 with a gate for each take 58 to 61 us, 5.6 TB/s (the gate behind the first sum 64, weights too 75); one row 2.4 us,
+// a launch's latency; 333 rows of 5003, f32 beside bf16, 7.1 (number by number 18).
 #include <cuda_bf16.h>
 
 #include <algorithm>

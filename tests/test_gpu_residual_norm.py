@@ -248,3 +248,22 @@ def test_refusals_without_a_device():
     assert run(_lib.ResidualNormShape(8, 0, 0, 0, 1.0, 1e-5), p=None) == bad
     assert run(_lib.ResidualNormShape(8, 1, 0, 0, 1.0, 1e-5), p=66) == bad
     assert run(_lib.ResidualNormShape(8, 0, 0, 0, 1.0, 1e-5), rows=2, stride=7) == bad
+
+
+def test_the_shape_has_the_header_s_layout(tmp_path):
+    import ctypes as C
+    import os
+    import shutil
+    import subprocess
+
+    from dmlx_b200 import _lib
+
+    if shutil.which("gcc") is None:
+        return
+    shape = _lib.ResidualNormShape
+    lines = "".join(f'printf("%zu ", offsetof(b200_residual_norm_shape, {name}));' for name, _ in shape._fields_)
+    (tmp_path / "l.c").write_text('#include <stdio.h>\n#include <stddef.h>\n#include "dmlx_b200.h"\nint main(void) {' + lines + 'printf("%zu", sizeof(b200_residual_norm_shape)); return 0; }')
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    subprocess.run(["gcc", "-std=c99", "-I", include, str(tmp_path / "l.c"), "-o", str(tmp_path / "l")], check=True)
+    got = [int(v) for v in subprocess.run([str(tmp_path / "l")], check=True, capture_output=True, text=True).stdout.split()]
+    assert got == [getattr(shape, name).offset for name, _ in shape._fields_] + [C.sizeof(shape)]
