@@ -1059,7 +1059,7 @@ b200_status create_weight(int n, int k, bool gated, const int8_t* const* q, cons
   *out = nullptr;
   const int parts = gated ? 2 : 1;
   for (int p = 0; p < parts; ++p)
-    if (!q[p] || !scales[p]) { b200_set_error("i8 weight: no numbers, or no scales"); return B200_ERR_INVALID_ARGUMENT; }
+    if (!q[p] || !scales[p] || ((uintptr_t)scales[p] & 3) != 0) { b200_set_error("i8 weight: no numbers, or no scales"); return B200_ERR_INVALID_ARGUMENT; }
   if (n <= 0 || k <= 0 || n > 1 << 24 || k > kI8MaxK) { b200_set_error("i8 weight: %d x %d (at most %d x %d)", n, k, 1 << 24, kI8MaxK); return B200_ERR_INVALID_ARGUMENT; }
   b200_status st = b200_require_device();
   if (st != B200_OK) return st;
@@ -1214,7 +1214,7 @@ extern "C" b200_status b200_i8_quantize(b200_i8_rows* r, const void* d_x, int64_
 }
 
 extern "C" b200_status b200_i8_rows_get(const b200_i8_rows* r, void* d_q, float* d_steps, void* stream) {
-  if (!r || r->rows < 0) { b200_set_error("i8 rows: nothing there"); return B200_ERR_INVALID_ARGUMENT; }
+  if (!r || r->rows < 0 || ((uintptr_t)d_steps & 3) != 0) { b200_set_error("i8 rows: nothing there, or no place for it"); return B200_ERR_INVALID_ARGUMENT; }
   b200_status st = b200_require_device();
   if (st != B200_OK) return st;
   if (r->rows == 0 || (!d_q && !d_steps)) return B200_OK;
@@ -1228,6 +1228,7 @@ extern "C" b200_status b200_i8_mm(const b200_i8_weight* w, b200_i8_rows* r, cons
                                   int64_t y_stride, int32_t y_f32, void* stream) {
   if (!w || !r) { b200_set_error("i8 mm: no weight, or no rows"); return B200_ERR_INVALID_ARGUMENT; }
   if (w->gated) { b200_set_error("i8 mm: the weight is a feed-forward block's gate and up"); return B200_ERR_INVALID_ARGUMENT; }
+  if (((uintptr_t)d_bias & 3) != 0) { b200_set_error("i8 mm: the bias is not on a number's boundary"); return B200_ERR_INVALID_ARGUMENT; }
   b200_status st = check_out("i8 mm", d_y, y_stride, rows, w->n, y_f32 ? 4 : 2);
   if (st == B200_OK) st = b200_require_device();
   if (st == B200_OK) st = take_rows("i8 mm", r, d_x, x_stride, rows, w->k);

@@ -366,6 +366,37 @@ def test_two_graphs_at_a_time_with_a_handle_each(rows):
 
 
 @pytest.mark.gpu
+def test_the_first_calls_of_a_process_may_be_captured():
+    """Nothing is allocated, and nothing waited for, once the handles are there."""
+    import os
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from dmlx_b200 import device as dev
+g = torch.Generator().manual_seed(1)
+w = lambda n, k: (torch.randint(-128, 128, (n, k), generator=g, dtype=torch.int16).to(torch.int8), torch.rand(n, generator=g) * 0.001)
+gate_up, down = dev.I8Weight.gated(*w(700, 300), *w(700, 300)), dev.I8Weight(*w(300, 700))
+graphs = []
+for rows in (2, 40, 900):
+    held, x = dev.I8Rows(rows, 300, 700), torch.randn((rows, 300), generator=g).bfloat16().cuda()
+    norm = torch.ones(300, dtype=torch.bfloat16, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        h, _ = dev.residual_norm(x, x, norm, rows=held)
+        y = dev.i8_ffn(gate_up, down, held)
+    graph.replay()
+    torch.cuda.synchronize()
+    h2, _ = dev.residual_norm(x, x, norm, rows=held)
+    assert torch.equal(y, dev.i8_ffn(gate_up, down, held)) and torch.equal(h, h2)
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.gpu
 def test_a_handle_s_rows_in_a_graph_without_what_made_them():
     """A product in a graph takes what the handle holds when it runs."""
     from dmlx_b200 import device as dev
@@ -426,6 +457,8 @@ def test_refusals():
     assert lib.b200_i8_mm(w._h, held._h, x.data_ptr(), 64, 4, None, None, 32, 0, stream) == _lib.ERR_INVALID_ARGUMENT
     assert lib.b200_i8_mm(w._h, held._h, x.data_ptr(), 64, -1, None, out.data_ptr(), 32, 0, stream) == _lib.ERR_INVALID_ARGUMENT
     assert lib.b200_i8_ffn(gate_up._h, down._h, held._h, x.data_ptr(), 64, 4, 3, out.data_ptr(), 64, stream) == _lib.ERR_INVALID_ARGUMENT
+    assert lib.b200_i8_mm(w._h, held._h, x.data_ptr(), 64, 4, x.data_ptr() + 2, out.data_ptr(), 32, 0, stream) == _lib.ERR_INVALID_ARGUMENT
+    assert lib.b200_i8_rows_get(held._h, None, out.data_ptr() + 2, stream) == _lib.ERR_INVALID_ARGUMENT
     # what was refused changed nothing
     q, _ = held.get()
     assert torch.equal(q.cpu().double(), _quantized(x.cpu())[0])
@@ -442,6 +475,7 @@ def test_refusals_without_handles():
         assert lib.b200_i8_weight_create(n, k, C.addressof(q), C.addressof(s), C.byref(h)) == bad and not h.value
     assert lib.b200_i8_weight_create(2, 2, None, C.addressof(s), C.byref(h)) == bad
     assert lib.b200_i8_weight_create(2, 2, C.addressof(q), None, C.byref(h)) == bad
+    assert lib.b200_i8_weight_create(1, 2, C.addressof(q), C.addressof(s) + 2, C.byref(h)) == bad
     assert lib.b200_i8_weight_create_gated(2, 2, C.addressof(q), C.addressof(s), None, C.addressof(s), C.byref(h)) == bad
     for rows, k, hidden in ((0, 8, 0), (8, 0, 0), (8, 8, -1), (2 ** 24 + 1, 8, 0), (8, 131073, 0), (8, 8, 131073)):
         assert lib.b200_i8_rows_create(rows, k, hidden, C.byref(h)) == bad and not h.value
