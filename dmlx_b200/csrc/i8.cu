@@ -1230,6 +1230,13 @@ extern "C" b200_status b200_i8_mm(const b200_i8_weight* w, b200_i8_rows* r, cons
   if (w->gated) { b200_set_error("i8 mm: the weight is a feed-forward block's gate and up"); return B200_ERR_INVALID_ARGUMENT; }
   if (((uintptr_t)d_bias & 3) != 0) { b200_set_error("i8 mm: the bias is not on a number's boundary"); return B200_ERR_INVALID_ARGUMENT; }
   b200_status st = check_out("i8 mm", d_y, y_stride, rows, w->n, y_f32 ? 4 : 2);
+  // (rows become 8 bits in the same kernel where they are few, while others' columns are stored already)
+  const int size = y_f32 ? 4 : 2;
+  const RowsAt y{d_y, rows, y_stride * size, (long long)w->n * size};
+  if (st == B200_OK && (rows_overlap(y, {d_x, rows, x_stride * 2, (long long)w->k * 2}) || rows_overlap(y, {d_bias, 1, 0, (long long)w->n * 4}))) {
+    b200_set_error("i8 mm: y lies over x or the bias");
+    return B200_ERR_INVALID_ARGUMENT;
+  }
   if (st == B200_OK) st = b200_require_device();
   if (st == B200_OK) st = take_rows("i8 mm", r, d_x, x_stride, rows, w->k);
   if (st != B200_OK || rows == 0) return st;

@@ -39,6 +39,23 @@ struct b200_i8_weight {
   float* scale = nullptr;               // [tiles * 128]
 };
 
+// Rows in memory, as one call gives them: `bytes` of each, `stride` bytes apart.
+struct RowsAt {
+  const void* p;
+  long long rows, stride, bytes;
+};
+// Whether two of them share a byte.  Rows of one buffer side by side (the same stride, other columns) do not.
+inline bool rows_overlap(const RowsAt& a, const RowsAt& b) {
+  if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0) return false;
+  const long long d = (long long)((uintptr_t)b.p - (uintptr_t)a.p), end_a = (a.rows - 1) * a.stride + a.bytes, end_b = (b.rows - 1) * b.stride + b.bytes;
+  if (d >= end_a || -d >= end_b) return false;
+  if (a.rows == 1 && b.rows == 1) return true;
+  const long long stride = a.rows > 1 ? a.stride : b.stride;
+  if (stride <= 0 || (a.rows > 1 && b.rows > 1 && a.stride != b.stride)) return true;  // (may be: no layout that a tensor's columns have)
+  const long long off = (d % stride + stride) % stride;
+  return off < a.bytes || off + b.bytes > stride;
+}
+
 inline int i8_chunks(int k) { return (k + kI8Chunk - 1) / kI8Chunk; }
 
 #ifdef __CUDACC__

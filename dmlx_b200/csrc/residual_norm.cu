@@ -233,9 +233,18 @@ extern "C" b200_status b200_residual_norm(const b200_residual_norm_shape* shape,
   const int h_size = shape->h_f32 ? 4 : 2, y_size = shape->y_f32 ? 4 : 2;
   auto holds = [&](const void* p, int64_t stride, int size) { return p && ((uintptr_t)p & (size - 1)) == 0 && (rows <= 1 || stride >= n); };
   if (rows > 0 && (!holds(d_h, h_stride, h_size) || !holds(d_y, y_stride, y_size) || !holds(d_h_out, h_out_stride, h_size) || (d_x_out && !holds(d_x_out, x_out_stride, 2)) ||
-                   (d_gate && gate_stride != 0 && !holds(d_gate, gate_stride, 2)) || (((uintptr_t)d_gate | (uintptr_t)d_post_weight | (uintptr_t)d_norm_weight) & 1) != 0 ||
-                   (d_h_out == d_h && rows > 1 && h_out_stride != h_stride) || d_h_out == d_y || (d_x_out && (d_x_out == d_h || d_x_out == d_y || d_x_out == d_h_out || d_x_out == d_gate)))) {
-    b200_set_error("residual norm: rows of %d columns, each on a number's boundary, strides that hold a row; h_out is h itself, all else apart", n);
+                   (d_gate && gate_stride != 0 && !holds(d_gate, gate_stride, 2)) || (((uintptr_t)d_gate | (uintptr_t)d_post_weight | (uintptr_t)d_norm_weight) & 1) != 0)) {
+    b200_set_error("residual norm: rows of %d columns, each on a number's boundary, strides that hold a row", n);
+    return B200_ERR_INVALID_ARGUMENT;
+  }
+  auto at = [&](const void* p, int64_t stride, int size) { return RowsAt{p, stride ? rows : 1, stride * size, (long long)n * size}; };
+  const RowsAt h_out = at(d_h_out, h_out_stride, h_size), x_out = at(d_x_out, x_out_stride, 2);
+  bool over = rows_overlap(h_out, x_out) || (rows_overlap(h_out, at(d_h, h_stride, h_size)) && (d_h_out != d_h || (rows > 1 && h_out_stride != h_stride))) ||
+              rows_overlap(x_out, at(d_h, h_stride, h_size));
+  for (const RowsAt& in : {at(d_y, y_stride, y_size), at(d_gate, gate_stride, 2), at(d_post_weight, 0, 2), at(d_norm_weight, 0, 2)})
+    over = over || rows_overlap(h_out, in) || rows_overlap(x_out, in);
+  if (rows > 0 && over) {
+    b200_set_error("residual norm: h_out is h itself or lies apart from all else, and so does x");
     return B200_ERR_INVALID_ARGUMENT;
   }
   if (q_out && (rows > q_out->max_rows || n > q_out->max_k)) {

@@ -505,6 +505,9 @@ class I8Weight:
             if q.dtype != torch.int8 or scales.dtype != torch.float32 or tuple(q.shape) != (n, k) or tuple(scales.shape) != (n,):
                 raise ValueError(f"expected int8 [{n}, {k}] and f32 [{n}], got {q.dtype} {tuple(q.shape)} and {scales.dtype} {tuple(scales.shape)}")
             kept += [q.detach().contiguous(), scales.detach().contiguous()]
+        for t in kept:
+            if t.is_cuda:
+                torch.cuda.current_stream(t.device).synchronize()  # (of any device)
         h = C.c_void_p()
         _lib.check(create(n, k, *(t.data_ptr() for t in kept), C.byref(h)))
         self._h, self.n, self.k, self.is_gated = h.value, n, k, is_gated
@@ -628,7 +631,7 @@ def residual_norm(h: torch.Tensor, y: torch.Tensor, norm_weight: Optional[torch.
         x_out = torch.empty_like(h) if h_type is _BF16 and h_stride == n else torch.empty_like(y) if y_type is _BF16 and y_stride == n else _new_rows(t, n, _BF16, device)
     if x_out is not None:
         x_at = x_out.data_ptr()
-    _lib.check(lib.b200_residual_norm(_norm_shape(n, h_type is _F32, y_type is _F32, gate_sigmoid, scale, eps), h.data_ptr(), h_stride, y.data_ptr(), y_stride,
+    _lib.check(lib.b200_residual_norm(_norm_shape(n, h_type is _F32, y_type is _F32, bool(gate_sigmoid), float(scale), float(eps)), h.data_ptr(), h_stride, y.data_ptr(), y_stride,
                                       gate_at, gate_stride, _weight(post_weight, n, device), _weight(norm_weight, n, device), t, h_out.data_ptr(), h_out_stride, x_at,
                                       x_out_stride, None if rows is None else rows._h, _raw_stream(device)))
     if rows is not None:

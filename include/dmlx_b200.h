@@ -597,7 +597,7 @@ b200_status b200_i8_quantize(b200_i8_rows* r, const void* d_x, int64_t x_stride,
 /* What the handle holds: q int8 [rows, k] and the steps m / 127 f32 [rows], either may be null. */
 b200_status b200_i8_rows_get(const b200_i8_rows* r, void* d_q, float* d_steps, void* stream);
 /* y [rows, n] bf16 (y_f32: f32), stride in elements; bias f32 [n] or null.  With d_x (bf16 [rows, k]) the rows are made from it first, as b200_i8_quantize
- * does; d_x null takes the `rows` rows that the handle holds.  y does not overlap x.  A refused call changes nothing. */
+ * does; d_x null takes the `rows` rows that the handle holds.  y overlaps neither x nor the bias (refused).  A refused call changes nothing. */
 b200_status b200_i8_mm(const b200_i8_weight* w, b200_i8_rows* r, const void* d_x, int64_t x_stride, int32_t rows, const float* d_bias, void* d_y,
                        int64_t y_stride, int32_t y_f32, void* stream);
 /* y = W_down q(act(W_gate x) * (W_up x)) bf16 [rows, n of down]: both projections, the activation and the product in one kernel, whose result stays
@@ -611,7 +611,7 @@ b200_status b200_i8_ffn(const b200_i8_weight* gate_up, const b200_i8_weight* dow
  *   x = h_out, or h_out / sqrt(mean(h_out^2) + eps) * norm_weight (h_out before its rounding).
  * f32 in between, one rounding each.  y and h are rows of n numbers (bf16, or f32 with y_f32, h_f32; h_out is like h and may be h), weights bf16 [n], null =
  * no norm; gate bf16, null = none, gate_stride 0: one for all rows.  x goes to x_out (bf16) and, in 8 bits, into q_out, either null.  Nothing but h_out and
- * h overlaps.  n up to 32768; strides in elements, any. */
+ * h overlaps (refused).  n up to 32768; strides in elements, any. */
 typedef struct b200_residual_norm_shape {
   int32_t n;
   int32_t h_f32, y_f32;

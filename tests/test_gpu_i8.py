@@ -458,6 +458,9 @@ def test_refusals():
     assert lib.b200_i8_mm(w._h, held._h, x.data_ptr(), 64, -1, None, out.data_ptr(), 32, 0, stream) == _lib.ERR_INVALID_ARGUMENT
     assert lib.b200_i8_ffn(gate_up._h, down._h, held._h, x.data_ptr(), 64, 4, 3, out.data_ptr(), 64, stream) == _lib.ERR_INVALID_ARGUMENT
     assert lib.b200_i8_mm(w._h, held._h, x.data_ptr(), 64, 4, x.data_ptr() + 2, out.data_ptr(), 32, 0, stream) == _lib.ERR_INVALID_ARGUMENT
+    square = dev.I8Weight(*_weight(64, 64, 6))
+    for over in (lambda: dev.i8_mm(square, held, x, out=x), lambda: dev.i8_mm(square, held, x[:3], out=x[1:]), lambda: dev.i8_mm(square, held, x[:1], out=x.view(torch.float32)[:2].view(1, 64), f32=True)):
+        refused(_lib.ERR_INVALID_ARGUMENT, over)
     assert lib.b200_i8_rows_get(held._h, None, out.data_ptr() + 2, stream) == _lib.ERR_INVALID_ARGUMENT
     # what was refused changed nothing
     q, _ = held.get()

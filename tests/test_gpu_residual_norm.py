@@ -225,12 +225,61 @@ def test_refusals():
         with pytest.raises(_lib.B200Error) as e:
             call()
         assert e.value.status == _lib.ERR_INVALID_ARGUMENT
+    both = torch.zeros((5, 128), dtype=torch.bfloat16, device="cuda")
+    side = both[:4, :64].copy_(h), both[:4, 64:]
+    for call in (lambda: dev.residual_norm(h, y, norm, gate=c["gate_row"], h_out=c["gate_row"]), lambda: dev.residual_norm(h, y, norm, x_out=c["gate_row"], gate=c["gate_row"]),
+                 lambda: dev.residual_norm(side[0], y, norm, h_out=both[1:, :64]), lambda: dev.residual_norm(side[0], y, norm, x_out=both[1:, 32:96]),
+                 lambda: dev.residual_norm(h[:1], y[:1], norm, x_out=norm[None]), lambda: dev.residual_norm(h[:1], y[:1], post_weight=norm, h_out=norm[None])):
+        with pytest.raises(_lib.B200Error) as e:
+            call()
+        assert e.value.status == _lib.ERR_INVALID_ARGUMENT
+    # columns side by side are apart
+    want = dev.residual_norm(h, y, norm, scale=0.5)
+    got = dev.residual_norm(side[0], y, norm, scale=0.5, h_out=side[0], x_out=side[1])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
     wide = torch.zeros((1, 32769), dtype=torch.bfloat16, device="cuda")
     with pytest.raises(_lib.B200Error) as e:
         dev.residual_norm(wide, wide)
     assert e.value.status == _lib.ERR_UNSUPPORTED
     none = torch.empty((0, 64), dtype=torch.bfloat16, device="cuda")
     assert dev.residual_norm(none, none, norm)[0].shape == (0, 64)
+
+
+@pytest.mark.gpu
+def test_a_factor_that_is_a_tensor_is_read_at_each_call():
+    from dmlx_b200 import device as dev
+
+    c = {k: v.cuda() for k, v in _make(2, 64, 11).items()}
+    factor = torch.tensor(0.25)
+    for value in (0.25, -3.0):
+        factor.fill_(value)
+        got, want = dev.residual_norm(c["h"], c["y"], c["norm"], scale=factor), dev.residual_norm(c["h"], c["y"], c["norm"], scale=value)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_outputs_over_inputs_are_refused_without_a_device():
+    import ctypes as C
+
+    from dmlx_b200 import _lib
+
+    shape = _lib.ResidualNormShape(8, 0, 0, 0, 1.0, 1e-5)
+    at = dict(h=0x10000, h_stride=32, y=0x20000, y_stride=32, gate=0x30000, gate_stride=32, post=0x40000, norm=0x50000, rows=3, out=0x60000, out_stride=32, x=0x70000, x_stride=32)
+
+    def run(**other):
+        a = dict(at, **other)
+        return _lib.lib.b200_residual_norm(C.byref(shape), a["h"], a["h_stride"], a["y"], a["y_stride"], a["gate"], a["gate_stride"], a["post"], a["norm"], a["rows"], a["out"],
+                                           a["out_stride"], a["x"], a["x_stride"], None, None)
+
+    # a row is 16 bytes, rows are 64 apart
+    over = [dict(out=at["y"]), dict(out=at["y"] + 14), dict(out=at["y"] + 2 * 64 + 14), dict(x=at["y"] - 2 * 64 - 14), dict(x=at["h"]), dict(out=at["h"] + 64), dict(out=at["h"], out_stride=40),
+            dict(out=at["gate"]), dict(x=at["gate"] + 8), dict(gate_stride=0, out=at["gate"] - 2 * 64), dict(out=at["post"] + 14), dict(x=at["norm"] - 64 - 14), dict(x=at["out"] + 2),
+            dict(x=at["out"] + 16, x_stride=40), dict(rows=1, out=at["y"] + 14)]
+    for other in over:
+        assert run(**other) == _lib.ERR_INVALID_ARGUMENT, other
+    if not torch.cuda.is_available():  # these are not run: the addresses are made up
+        for other in (dict(), dict(out=at["h"]), dict(out=at["y"] + 16), dict(out=at["y"] + 48), dict(x=at["out"] + 16), dict(x=at["y"] - 2 * 64 - 16), dict(rows=1, out=at["y"] + 16),
+                      dict(gate=None, out=at["gate"]), dict(gate_stride=0, out=at["gate"] + 16), dict(x=None)):
+            assert run(**other) not in (_lib.OK, _lib.ERR_INVALID_ARGUMENT), other
 
 
 def test_refusals_without_a_device():
