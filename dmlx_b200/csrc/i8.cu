@@ -268,6 +268,23 @@ __device__ __forceinline__ void push4(uint32_t mapped, uint32_t a, uint32_t b, u
   asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(mapped), "r"(a), "r"(b), "r"(c), "r"(d),
                "r"(mapped_bar) : "memory");
 }
+// Waits for what the other CTAs push.  It comes from outside this CTA, so the wait acquires in the cluster's scope: by an ordinary one, of this CTA's, the sums would not be
+// ordered ahead of the loads behind it.
+__device__ __forceinline__ bool wait_pushed(uint32_t bar) {
+  for (uint32_t i = 0; i < ptx::kSpinLimit; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], 0;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar)
+        : "memory");
+    if (ok) return true;
+    if (i > 64) __nanosleep(64);
+  }
+  return false;
+}
 // The rows that a CTA of the cluster brings to the output: CTA q the q-th so many, a multiple of four.
 __host__ __device__ constexpr int rows_per_rank(int rows_here, int shares) { return ((rows_here + shares - 1) / shares + 3) / 4 * 4; }
 // What it gets pushed: [other CTA][gate, up][four rows][channel][row].
@@ -510,7 +527,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
           }
           __syncwarp();
           asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-          if (ok && mine0 < mine1) ok = __all_sync(0xffffffffu, ptx::mbar_wait(pushed, 0));
+          if (ok && mine0 < mine1) ok = __all_sync(0xffffffffu, wait_pushed(ptx::smem_u32(pushed)));
         }
         if (!ok) end = 0;
       }
@@ -889,7 +906,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) i8_pair_kernel(MmArgs a) {
           for (int j4 = 0; j4 < 8; ++j4) push4(to + place(from, g / shares, part, j4), v[4 * j4], v[4 * j4 + 1], v[4 * j4 + 2], v[4 * j4 + 3], bar);
         }
       }
-      ok = __all_sync(0xffffffffu, ptx::mbar_wait_addr(pushed, 0));
+      ok = __all_sync(0xffffffffu, wait_pushed(pushed));
 #pragma unroll 1
       for (int i = half; i < own_groups && ok; i += 2) {
         const int g = share + i * shares;

@@ -257,6 +257,24 @@ def test_a_row_s_bits_do_not_depend_on_its_batch():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("k,n,sizes", [(14336, 512, (1, 2, 4, 5, 40, 130)), (4096, 1024, (1, 3, 33, 130, 250)), (14336, 256, (300, 500)), (2048, 2048, (1, 64, 96))])
+def test_sums_that_a_cluster_shares_out_meet_every_time(k, n, sizes):
+    """Few tiles of a long K: shares of it in every cluster, one call behind the other, against the calls of many rows."""
+    from dmlx_b200 import device as dev
+
+    rows = 4000
+    w, x = dev.I8Weight(*_weight(n, k, 35)), _x(rows, k, 36).cuda()
+    want, held = dev.i8_mm(w, dev.I8Rows(rows, k), x, f32=True), dev.I8Rows(rows, k)
+    for size in sizes:
+        got = torch.empty_like(want)
+        count = min(rows, 300 * size) // size * size
+        for first in range(0, count, size):
+            dev.i8_mm(w, held, x[first:first + size], out=got[first:first + size], f32=True)
+        assert torch.equal(got[:count], want[:count]), size
+    assert dev.qmm_error_word() == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [3, 70, 400])
 @pytest.mark.parametrize("at,x_more,y_at,y_more", [(8, 24, 16, 40), (1, 4, 3, 6), (5, 8, 0, 1)])
 def test_strided_rows_and_what_lies_around_them(rows, at, x_more, y_at, y_more):
