@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
           }
           __syncwarp();
           asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-          if (ok && mine0 < mine1) ok = __all_sync(0xffffffffu, wait_pushed(ptx::smem_u32(pushed)));
+          if (mine0 < mine1) ok &= (bool)__all_sync(0xffffffffu, wait_pushed(ptx::smem_u32(pushed)));  // (where a wait here ran out, too: the others push all the same)
         }
         if (!ok) end = 0;
       }
@@ -887,12 +887,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) i8_pair_kernel(MmArgs a) {
   if (shares > 1) {
     __syncwarp();
     ptx::cluster_sync();  // nobody's stages are in use
-    if (warp >= 4 && ok) {
+    if (warp >= 4) {
       const Item it = item_of(first_item);
       // [other pair][group][gate, up][four columns][row]
       auto place = [&](int from, int group, int part, int j4) { return (((((from * most_groups + group) * W + part) * 8 + j4) * kI8Tile) + quarter * 32 + lane) * 16; };
 #pragma unroll 1
-      for (int g = half; g < G; g += 2) {
+      for (int g = half; g < G && ok; g += 2) {
         const int owner = g % shares;
         if (owner == share) continue;
         const uint32_t cta = (uint32_t)owner * 2 + rank, to = ptx::map_to_rank(smem_u, cta), bar = ptx::map_to_rank(pushed, cta);
@@ -906,7 +906,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) i8_pair_kernel(MmArgs a) {
           for (int j4 = 0; j4 < 8; ++j4) push4(to + place(from, g / shares, part, j4), v[4 * j4], v[4 * j4 + 1], v[4 * j4 + 2], v[4 * j4 + 3], bar);
         }
       }
-      ok = __all_sync(0xffffffffu, wait_pushed(pushed));
+      ok &= (bool)__all_sync(0xffffffffu, wait_pushed(pushed));  // (where a wait here ran out, too: the others push all the same)
 #pragma unroll 1
       for (int i = half; i < own_groups && ok; i += 2) {
         const int g = share + i * shares;
