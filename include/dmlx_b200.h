@@ -575,7 +575,7 @@ b200_status b200_lora_apply(const b200_lora* l, b200_lora_batch* b, const void* 
  * even, m = max |x[k]|, a weight comes with a scale for each of its n channels, and
  *   y[r][n] = (sum_k q[r][k] w[n][k]) * scale[n] * (m_r / 127) + bias[n];
  * the sum is exact (32 bits), the rest f32, one rounding.  A row of zeros has the product 0; a row that holds an infinity or no number gives NaN in all its
- * columns and changes no other row.  Same bits for a row whatever shares its batch.
+ * columns and changes no other row.  The products give a row the same bits whatever shares its batch.
  * A b200_i8_rows holds the rows of a step in 8 bits and is the workspace of the products that read them: steps that may run at the same time (two
  * captured graphs on two streams) have one each.  A captured product without its rows' making works on what the handle holds when it runs.  All calls but
  * those that create are asynchronous on the stream and may be captured.  Rows, strides and widths may be any.  A wait inside the kernels that runs out is
@@ -609,7 +609,8 @@ b200_status b200_i8_ffn(const b200_i8_weight* gate_up, const b200_i8_weight* dow
 /* The norms behind and before a block with its gate and its factor on the residual:
  *   p = y, or y / sqrt(mean(y^2) + eps) * post_weight; p = p * gate, or p * sigmoid(gate); h_out = h + scale * p;
  *   x = h_out, or h_out / sqrt(mean(h_out^2) + eps) * norm_weight (h_out before its rounding).
- * f32 in between, one rounding each.  y and h are rows of n numbers (bf16, or f32 with y_f32, h_f32; h_out is like h and may be h), weights bf16 [n], null =
+ * f32 in between, one rounding each; the same bits for a row whatever shares its batch where n is a multiple of eight and the rows of all operands start on 16 bytes
+ * (elsewhere the order of a row's sums of squares, and with it their last bit, goes by where the row lies and by how many there are).  y and h are rows of n numbers (bf16, or f32 with y_f32, h_f32; h_out is like h and may be h), weights bf16 [n], null =
  * no norm; gate bf16, null = none, gate_stride 0: one for all rows.  x goes to x_out (bf16) and, in 8 bits, into q_out, either null.  Nothing but h_out and
  * h overlaps (refused).  n up to 32768; strides in elements, any. */
 typedef struct b200_residual_norm_shape {

@@ -205,6 +205,58 @@ def test_the_half_of_a_layer_in_a_graph(rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [136, 504, 1000, 2056, 4096, 8192, 8200, 16384, 20008, 32768])
+@pytest.mark.parametrize("h_f32,y_f32", [(False, False), (True, False), (True, True)])
+def test_a_row_s_bits_do_not_depend_on_its_batch(n, h_f32, y_f32):
+    """Its sums of squares are made in an order that its columns alone set, where rows are whole 16-byte pieces.  (An f32 h' shows the first sum's last bit, x and 8-bit
+    rows the second's.)"""
+    from dmlx_b200 import device as dev
+
+    rows = 1300 if n < 600 else 700 if n < 9000 else 200
+    c = _make(rows, n, n, h_f32, y_f32)
+    post, norm, gate = c["post"].cuda(), c["norm"].cuda(), c["gate"].cuda()
+
+    def run(h, y, h_out=None, x_out=None):
+        held = dev.I8Rows(len(h), n)
+        alone = dev.residual_norm(h, y, norm, post_weight=post, gate=gate, scale=0.37, h_out=h_out, x_out=x_out)
+        both = dev.residual_norm(h, y, norm, post_weight=post, gate=gate, scale=0.37, x_out=torch.empty((len(h), n), dtype=torch.bfloat16, device="cuda"), rows=held)
+        assert all(torch.equal(a, b) for a, b in zip(alone, both))
+        return *both, *held.get()
+
+    h, y = c["h"].cuda(), c["y"].cuda()
+    whole = run(h, y)
+    for first, count in ((0, 1), (1, 1), (5, 2), (6, 3), (11, 7), (40, 64), (37, 150)):
+        for got, want in zip(run(h[first:first + count], y[first:first + count]), whole):
+            assert torch.equal(got, want[first:first + count]), (first, count)
+    for at in (0, 8, 24):  # anywhere in wider rows
+        cut = [torch.zeros((20, n + 24), dtype=t, device="cuda")[:, at:at + n] for t in (h.dtype, y.dtype, h.dtype, torch.bfloat16)]
+        cut[0].copy_(h[:20])
+        cut[1].copy_(y[:20])
+        for got, want in zip(run(*cut), whole):
+            assert torch.equal(got, want[:20]), at
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n", [(5, 5003), (600, 1030), (3, 8195), (1300, 300)])
+@pytest.mark.parametrize("at", [0, 1, 3])
+@pytest.mark.parametrize("h_f32", [False, True])
+def test_into_h_itself_without_a_norm_behind_the_block(rows, n, at, h_f32):
+    """No sum stands between the loads and the stores then: rows of several warps, on no 16-byte boundary."""
+    from dmlx_b200 import device as dev
+
+    c = _make(rows, n + 5, 12, h_f32)
+    cut = lambda t: t[..., at:at + n]  # noqa: E731
+    h, y, norm = c["h"].cuda(), cut(c["y"].cuda()), cut(c["norm"].cuda())
+    for post in (False, True):
+        weight = cut(c["post"].cuda()) if post else None
+        want = dev.residual_norm(cut(h), y, norm, post_weight=weight, scale=0.7, h_out=cut(torch.empty_like(h)))
+        mine = h.clone()
+        got = dev.residual_norm(cut(mine), y, norm, post_weight=weight, scale=0.7, h_out=cut(mine))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert torch.equal(mine[:, :at], h[:, :at]) and torch.equal(mine[:, at + n:], h[:, at + n:])
+
+
+@pytest.mark.gpu
 def test_refusals():
     from dmlx_b200 import _lib
     from dmlx_b200 import device as dev
