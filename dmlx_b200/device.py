@@ -610,6 +610,8 @@ def residual_norm(h: torch.Tensor, y: torch.Tensor, norm_weight: Optional[torch.
                   x_out: Optional[torch.Tensor] = None, rows: Optional[I8Rows] = None):
     """b200_residual_norm: h + scale * gate * norm(y), and the norm of that for the next block.  h, y [T, n] bf16 or f32, gate bf16 [n] or [T, n] (rows may be
     strided), a weight that is None is no norm.  Returns (h, x): x bf16, or None where it goes into `rows` in 8 bits.  h_out may be h."""
+    if rows is not None and rows._h is None:  # (the call would take it for no rows)
+        raise ValueError("the 8-bit rows are closed")
     device, shape = torch.cuda.current_device(), h.shape
     t, n = shape
     h_type, y_type = _F32 if h.dtype == _F32 else _BF16, _F32 if y.dtype == _F32 else _BF16

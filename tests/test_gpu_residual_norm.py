@@ -257,6 +257,19 @@ def test_into_h_itself_without_a_norm_behind_the_block(rows, n, at, h_f32):
 
 
 @pytest.mark.gpu
+def test_8_bit_rows_that_are_closed_are_refused():
+    from dmlx_b200 import device as dev
+
+    c = {k: v.cuda() for k, v in _make(4, 64, 13).items()}
+    held = dev.I8Rows(4, 64)
+    held.close()
+    h = c["h"].clone()
+    with pytest.raises(ValueError, match="closed"):
+        dev.residual_norm(c["h"], c["y"], c["norm"], h_out=c["h"], rows=held)
+    assert torch.equal(h, c["h"])
+
+
+@pytest.mark.gpu
 def test_refusals():
     from dmlx_b200 import _lib
     from dmlx_b200 import device as dev
