@@ -593,6 +593,8 @@ ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 def i8_ffn(gate_up: I8Weight, down: I8Weight, rows: I8Rows, x: Optional[torch.Tensor] = None, activation: str = "silu",
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """b200_i8_ffn: down(act(gate x) * (up x)), the rows in 8 bits in front of each product.  x as in i8_mm."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation {activation!r}, there are {', '.join(ACTIVATIONS)}")
     device = torch.cuda.current_device()
     at, stride, t = rows._take(x, gate_up.k, device)
     out_stride = down.n

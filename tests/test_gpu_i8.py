@@ -275,6 +275,20 @@ def test_sums_that_a_cluster_shares_out_meet_every_time(k, n, sizes):
 
 
 @pytest.mark.gpu
+def test_an_activation_that_is_none_is_refused():
+    from dmlx_b200 import device as dev
+
+    gate_up, down = dev.I8Weight.gated(*_weight(48, 64, 2), *_weight(48, 64, 3)), dev.I8Weight(*_weight(64, 48, 4))
+    held = dev.I8Rows(4, 64, 48)
+    held.quantize(_x(3, 64, 6).cuda())
+    want = held.get()
+    for name in ("relu", "SiLU", None):
+        with pytest.raises(ValueError, match="activation"):
+            dev.i8_ffn(gate_up, down, held, _x(4, 64, 5).cuda(), activation=name)
+    assert held.rows == 3 and all(torch.equal(a, b) for a, b in zip(held.get(), want))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [3, 70, 400])
 @pytest.mark.parametrize("at,x_more,y_at,y_more", [(8, 24, 16, 40), (1, 4, 3, 6), (5, 8, 0, 1)])
 def test_strided_rows_and_what_lies_around_them(rows, at, x_more, y_at, y_more):
