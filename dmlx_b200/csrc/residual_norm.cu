@@ -81,56 +81,41 @@ __device__ __forceinline__ void store_eight(T* p, int c, int n, bool fit, const 
     if (c + i >= lo && c + i < n && (i < head ? before : !pieces)) st(p + c + i, v[i]);
 }
 
-// Where all rows start on 16 bytes and are whole vectors (FIT), a row's sum of squares is made in an order that its columns alone set, so that neither the threads that it is
-// given nor what shares its batch changes a bit of it: eight columns one after the other; 32 such vectors as a tree over lanes; these groups as a tree too, lane l those of
-// l, l + 32 and so on.  Elsewhere a thread's are one sum.  (There a vector may go on in the next lane, and in the next warp: 333 rows of 5003 8.4 us in place of 7.0, 3000 of
-// 16383 181 in place of 153.)
-
-// The sums of a lane's NV vectors as trees, each over the warp's 32 lanes, as warp_sum's, all at a time: lane l leaves with that of vector tree_of(l).
-template <int NV>
-__device__ __forceinline__ float trees(const float (&v)[NV]) {
-  const int lane = threadIdx.x & 31;
-  auto merge = [&](float a, float b, int o) { return (lane & o ? b : a) + __shfl_xor_sync(0xffffffffu, lane & o ? a : b, o); };
-  if constexpr (NV == 1) {
-    return warp_sum(v[0]);
-  } else {
-    float s;
-    if constexpr (NV == 2) {
-      s = merge(v[0], v[1], 16);
-      s += __shfl_xor_sync(0xffffffffu, s, 8);
-    } else {
-      static_assert(NV == 4);
-      s = merge(merge(v[0], v[1], 16), merge(v[2], v[3], 16), 8);
-    }
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    return s;
-  }
-}
-template <int NV>
-__device__ __forceinline__ int tree_of(int lane) { return NV == 1 ? 0 : NV == 2 ? lane >> 4 : (lane >> 4) + 2 * (lane >> 3 & 1); }
+// Where all rows start on 16 bytes and are whole vectors (FIT), a row's sum of squares is made in an order that its columns alone set, so that what shares its batch changes
+// no bit of it, though a thread has two vectors in place of one where the batch is larger: eight columns one after the other; 32 such vectors as a tree over lanes; these
+// groups as a tree too, lane l those of l and l + 32.  (With more vectors every batch has as many to a thread, and its sum comes first.)  Elsewhere bits go by where the row
+// lies: a vector may go on in the next lane, and in the next warp (an order by columns took 8.4 us in place of 7.0 for 333 rows of 5003, 181 in place of 153 for 3000 of 16383).
 
 // Eight more columns' squares.
-__device__ __forceinline__ float add_squares(float sum, const float (&v)[8]) {
+__device__ __forceinline__ float squares(float sum, const float (&v)[8]) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) sum = fmaf(v[e], v[e], sum);
   return sum;
 }
-// The row's sum, q what the t-th of its threads has of it, part a number for every warp of NV.  All its threads; a block's meet here.
-template <int NV, bool WARP>
-__device__ __forceinline__ float sum_of(float* part, const float (&q)[NV], int t, int threads) {
-  const int lane = threadIdx.x & 31, warps = threads >> 5;
-  const float tree = trees<NV>(q);
-  if constexpr (WARP) return NV == 1 ? tree : __shfl_sync(0xffffffffu, tree, 0) + __shfl_sync(0xffffffffu, tree, 16);
-  if ((lane & (32 / NV - 1)) == 0) part[(t >> 5) + tree_of<NV>(lane) * warps] = tree;
-  __syncthreads();
-  float row = 0.f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (i > 0 && i * 32 >= NV * warps) break;
-    if (i * 32 + lane < NV * warps) row += part[i * 32 + lane];
+// The row's sum of what each of its threads, a block's (or a warp's) all, has.
+template <bool WARP>
+__device__ __forceinline__ float sum_of(float* part, float v) {
+  v = warp_sum(v);
+  if constexpr (!WARP) {
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = warp_sum(lane < (blockDim.x >> 5) ? part[lane] : 0.f);
   }
-  return warp_sum(row);
+  return v;
+}
+// The same of two vectors a thread, each a tree of its own (both at a time: half of the lanes go on with one, half with the other).
+__device__ __forceinline__ float sum_of_two(float* part, float a, float b) {
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const bool second = lane >= 16;
+  float v = (second ? b : a) + __shfl_xor_sync(0xffffffffu, second ? a : b, 16);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((lane & 15) == 0) part[(threadIdx.x >> 5) + (second ? warps : 0)] = v;
+  __syncthreads();
+  v = lane < 2 * warps ? part[lane] : 0.f;
+  if (warps > 16 && lane + 32 < 2 * warps) v += part[lane + 32];
+  return warp_sum(v);
 }
 
 // NV vectors of eight columns for each thread.  WARP: a warp for a row.  FIT: all rows start on 16 bytes and are whole vectors.  (1024 threads with 32 numbers each have 64
@@ -138,9 +123,10 @@ __device__ __forceinline__ float sum_of(float* part, const float (&q)[NV], int t
 template <typename H, typename Y, int NV, bool WARP, bool FIT>
 __global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const __grid_constant__ ResidualNormArgs a) {
   after_previous();
-  constexpr int kSums = FIT ? NV : 1;  // of a thread
-  __shared__ float part[2][WARP ? 1 : kSums * 32];
-  __shared__ uint32_t largest[32];
+  // A row's vectors one after the other, or behind all stores: 8192 rows of 4096 bf16 57.8 and 54.8 us, 3000 f32 rows of 16384 119 and 127.
+  constexpr bool kTwo = FIT && NV == 2 && !WARP, kBehind = kTwo && sizeof(H) + sizeof(Y) == 4;
+  constexpr int kSums = kTwo ? 2 : 1;
+  __shared__ float part[3][kTwo ? 64 : 32];
   const int threads = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
   const int row = WARP ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
   if (row >= a.rows) return;
@@ -163,7 +149,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const 
   if constexpr (NV <= 2) {
     if (gate) load_eights(gr, gate, n, fits(gate), column, lo);
   }
-  Eight<__nv_bfloat16> pr[NV <= 2 ? NV : 1], nr[1] = {};
+  Eight<__nv_bfloat16> pr[NV <= 2 ? NV : 1], nr[NV == 1 ? NV : 1] = {};
   if constexpr (NV <= 2) {
     if (post_w) load_eights(pr, post_w, n, fits(post_w), column, lo);
   }
@@ -172,25 +158,29 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const 
   }
   float ry = 1.f;
   if (a.post_w) {
-    float v[NV][8], q[kSums] = {};
+    if constexpr (kBehind) {
+      float v[NV][8];
 #pragma unroll
-    for (int u = 0; u < NV; ++u) {
-      widen(yr[u], v[u]);
-      if constexpr (!FIT) q[u % kSums] = add_squares(q[u % kSums], v[u]);
+      for (int u = 0; u < NV; ++u) widen(yr[u], v[u]);
+      ry = sum_of_two(part[0], squares(0.f, v[0]), squares(0.f, v[NV - 1]));
+    } else {
+      float ss[kSums] = {};
+#pragma unroll
+      for (int u = 0; u < NV; ++u) {
+        float v[8];
+        widen(yr[u], v);
+        ss[u % kSums] = squares(ss[u % kSums], v);
+      }
+      if constexpr (kTwo) ry = sum_of_two(part[0], ss[0], ss[kSums - 1]);
+      else ry = sum_of<WARP>(part[0], ss[0]);
     }
-#pragma unroll
-    for (int u = 0; u < NV && FIT; ++u) q[u % kSums] = add_squares(q[u % kSums], v[u]);
-    ry = rsqrtf(sum_of<kSums, WARP>(part[0], q, t, threads) / (float)a.n + a.eps);
+    ry = rsqrtf(ry / (float)a.n + a.eps);
   }
-  float x[NV][8], q[kSums] = {};
+  float x[NV][8], ss[kSums] = {};
   uint32_t most = 0u;
-  // A vector's squares and its product with the weights; behind all stores where rows fit and a thread has several (8192 rows of 4096 55 us, right behind each vector's
-  // store 58), elsewhere not (333 rows of 5003 7.4 and 7.1).
-  constexpr bool kBehind = FIT && NV > 1;
   auto weigh = [&](int u) {
+    float w[8];
     if (a.norm_w) {
-      q[u % kSums] = add_squares(q[u % kSums], x[u]);
-      float w[8];
       widen(NV == 1 ? nr[0] : load_eight(norm_w, column(u), n, fits(norm_w), lo), w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[u][e] *= w[e];
@@ -215,22 +205,29 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const 
     }
     widen(hr[u], w);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[u][e] = fmaf(a.scale, p[e], w[e]);  // (behind the last column all is zero)
+    for (int e = 0; e < 8; ++e) {
+      x[u][e] = fmaf(a.scale, p[e], w[e]);
+      if constexpr (!kBehind) ss[u % kSums] = fmaf(x[u][e], x[u][e], ss[u % kSums]);  // (behind the last column all is zero)
+    }
     store_eight(h_out, c, n, fits(h_out), x[u], lo);
     if constexpr (!kBehind) weigh(u);
   }
   if (!a.x_out && !a.q.q) return;
   if constexpr (kBehind) {
 #pragma unroll
-    for (int u = 0; u < NV; ++u) weigh(u);
+    for (int u = 0; u < NV; ++u) {
+      ss[u] = squares(0.f, x[u]);
+      weigh(u);
+    }
   }
   float r = 1.f;
   most = __reduce_max_sync(0xffffffffu, most);
   if constexpr (!WARP) {
-    if ((t & 31) == 0) largest[t >> 5] = most;
+    if ((t & 31) == 0) part[2][t >> 5] = __uint_as_float(most);
   }
-  if (a.norm_w) r = rsqrtf(sum_of<kSums, WARP>(part[1], q, t, threads) / (float)a.n + a.eps);
-  else if constexpr (!WARP) __syncthreads();
+  if constexpr (kTwo) r = sum_of_two(part[1], ss[0], ss[kSums - 1]);
+  else if (a.norm_w || !WARP) r = sum_of<WARP>(part[1], ss[0]);
+  r = a.norm_w ? rsqrtf(r / (float)a.n + a.eps) : 1.f;
 #pragma unroll
   for (int u = 0; u < NV; ++u) {
 #pragma unroll
@@ -238,7 +235,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const 
     if (x_out) store_eight(x_out, column(u), n, fits(x_out), x[u], lo);
   }
   if (!a.q.q) return;
-  if constexpr (!WARP) most = __reduce_max_sync(0xffffffffu, (t & 31) < (threads >> 5) ? largest[t & 31] : 0u);
+  if constexpr (!WARP) most = __reduce_max_sync(0xffffffffu, (t & 31) < (threads >> 5) ? __float_as_uint(part[2][t & 31]) : 0u);
   const I8Scale s = I8Scale::of(__uint_as_float(most) * r);
   if (t == 0) a.q.scale[row] = s.step();
 #pragma unroll
