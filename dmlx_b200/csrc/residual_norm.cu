@@ -118,6 +118,19 @@ __device__ __forceinline__ float sum_of_two(float* part, float a, float b) {
   return warp_sum(v);
 }
 
+// The sigmoid of a gate of bf16, for an h' of type H.  In f32 2^t, t = z log2(e), takes log2(e) in two parts, the first of 16 bits, so that its product with z is exact, the
+// rest's a factor 1 + d: t's rounding alone would be 2^-19 of the result at |z| of 30.  (8192 rows of 4096, f32, 70.7 us as without that, 78.4 with expf and a division; 3000
+// of 16384 133, 126 and 142.)
+template <typename H>
+__device__ __forceinline__ float gate_sigmoid(float z) {
+  if constexpr (sizeof(H) == 2) return sigmoid_for<H>(z);
+  constexpr float kHigh = 47274.0f / 32768.0f, kLow = 4.8884952e-6f;  // log2(e) = kHigh + kLow / ln(2)
+  const float d = fmaxf(-kLow * z, -1.0f);  // (z = inf: p = 0)
+  float p;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(-kHigh * z));
+  return __fdividef(1.0f, 1.0f + fmaf(p, d, p));
+}
+
 // NV vectors of eight columns for each thread.  WARP: a warp for a row.  FIT: all rows start on 16 bytes and are whole vectors.  (1024 threads with 32 numbers each have 64
 // registers: half of a row's y is still in its 16 bits while h comes.)
 template <typename H, typename Y, int NV, bool WARP, bool FIT>
@@ -201,7 +214,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const 
     if (a.gate) {
       widen(NV <= 2 ? gr[NV <= 2 ? u : 0] : load_eight(gate, c, n, fits(gate), lo), w);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) p[e] *= a.sigmoid ? __fdividef(1.0f, 1.0f + __expf(-w[e])) : w[e];
+      for (int e = 0; e < 8; ++e) p[e] *= a.sigmoid ? gate_sigmoid<H>(w[e]) : w[e];
     }
     widen(hr[u], w);
 #pragma unroll

@@ -257,6 +257,23 @@ def test_into_h_itself_without_a_norm_behind_the_block(rows, n, at, h_f32):
 
 
 @pytest.mark.gpu
+def test_a_gate_s_sigmoid_in_f32():
+    """2^t with t exact is off by two of its last places, 4 u, its factor's second order by 88^2 (4.9e-6)^2 / 2 = 1.6 u at the most, the reciprocal by 2 u; that factor, the sum,
+    the products with y and with the scale and the sum with h by u each: 2^-20 in all.  Behind a divisor past 2^126 the quotient is
+    nothing, where the sigmoid is under 2^-126."""
+    from dmlx_b200 import device as dev
+
+    gate = torch.cat([torch.linspace(-60, 60, 2000), torch.tensor([-87.0, -87.5, -88.5, -89.0, -1e4, -3e38, 0.0, 89.0, 1e4, 3e38, -float("inf"), float("inf")])]).bfloat16()
+    n = len(gate)
+    y = torch.randn((3, n), generator=torch.Generator().manual_seed(2))
+    h, none = dev.residual_norm(torch.zeros((3, n), device="cuda"), y.cuda(), gate=gate.cuda(), gate_sigmoid=True, scale=1000.0, x_out=torch.empty((3, n), dtype=torch.bfloat16, device="cuda"))
+    want = 1000 * y.double() * torch.sigmoid(gate.double())
+    off = (h.cpu().double() - want).abs()
+    tol = 2.0 ** -20 * want.abs() + 1000 * y.double().abs() * 2.0 ** -126 + 2.0 ** -149
+    assert bool((off <= tol).all()), float((off / want.abs().clamp(min=1e-30)).max())
+
+
+@pytest.mark.gpu
 def test_8_bit_rows_that_are_closed_are_refused():
     from dmlx_b200 import device as dev
 
