@@ -224,19 +224,25 @@ __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64
 // Instruction descriptor: signed 8-bit A and B (both K-major), 32-bit sums, tile m x n.
 __device__ __forceinline__ uint32_t idesc_i8(uint32_t m, uint32_t n) { return 2u << 4 | 1u << 7 | 1u << 10 | (n >> 3) << 17 | (m >> 4) << 24; }
 
+// What follows is the same for every kernel, so the compiler is told which products and sums to fuse: a row's bits must not depend on the kernel that has it.
+// A sum as a number of the product.
+__device__ __forceinline__ float scaled(uint32_t sum, float w, float step, float bias) { return __fmaf_rn(__fmul_rn((float)(int)sum, w), step, bias); }
+__device__ __forceinline__ float scaled(uint32_t sum, float w, float step) { return __fmul_rn(__fmul_rn((float)(int)sum, w), step); }
+// The exponentials are the hardware's, off by 2 + 1.16 |z| of their last place: 2^-20 of a number at |z| of 9, whose own size is 1e-3 then, beside a step of 1/127 of the row's
+// largest in which the result is held.
 template <int ACT>
 __device__ __forceinline__ float activated(float g) {
-  if constexpr (ACT == B200_ACT_SILU) return __fdividef(g, 1.0f + __expf(-g));  // (a divisor past 2^126 makes 0, as it should)
-  if constexpr (ACT == B200_ACT_GELU) return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
+  if constexpr (ACT == B200_ACT_SILU) return __fdividef(g, __fadd_rn(1.0f, __expf(-g)));  // (a divisor past 2^126 makes 0, as it should)
+  if constexpr (ACT == B200_ACT_GELU) return __fmul_rn(__fmul_rn(0.5f, g), __fadd_rn(1.0f, erff(__fmul_rn(g, 0.70710678118654752f))));
   // 0.5 g (1 + tanh z) = g / (1 + e^-2z)
-  return __fdividef(g, 1.0f + __expf(-1.5957691216057308f * (g + 0.044715f * g * g * g)));
+  return __fdividef(g, __fadd_rn(1.0f, __expf(__fmul_rn(-1.5957691216057308f, __fmaf_rn(__fmul_rn(__fmul_rn(0.044715f, g), g), g, g)))));
 }
 // y[j] = act(y[j]) * up[j]; the activation is chosen once.
 template <int N>
 __device__ __forceinline__ void gate_with(int act, float (&y)[N], const float (&up)[N]) {
   auto each = [&](auto which) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) y[j] = activated<decltype(which)::value>(y[j]) * up[j];
+    for (int j = 0; j < N; ++j) y[j] = __fmul_rn(activated<decltype(which)::value>(y[j]), up[j]);
   };
   if (act == B200_ACT_SILU) each(std::integral_constant<int, B200_ACT_SILU>{});
   else if (act == B200_ACT_GELU) each(std::integral_constant<int, B200_ACT_GELU>{});
@@ -555,8 +561,8 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const float step = __shfl_sync(0xffffffffu, steps, j);
-          y[j] = (float)(int)v[j] * ws * step + bias;
-          if constexpr (GATED) up[j] = (float)(int)u[j] * us * step;
+          y[j] = scaled(v[j], ws, step, bias);
+          if constexpr (GATED) up[j] = scaled(u[j], us, step);
         }
         if constexpr (GATED) {
           gate_with(a.act, y, up);
@@ -644,8 +650,8 @@ __device__ __forceinline__ void store_sums(const MmArgs& a, uint32_t (&v)[32], c
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int j = 4 * j4 + e;
-      y[j] = (float)(int)v[j] * w[e] * row_step + (GATED ? 0.f : o[e]);
-      if constexpr (GATED) up[j] = (float)(int)u[j] * o[e] * row_step;
+      y[j] = scaled(v[j], w[e], row_step, GATED ? 0.f : o[e]);
+      if constexpr (GATED) up[j] = scaled(u[j], o[e], row_step);
     }
   }
   if constexpr (GATED) gate_with(a.act, y, up);

@@ -275,6 +275,30 @@ def test_sums_that_a_cluster_shares_out_meet_every_time(k, n, sizes):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+def test_a_row_s_bits_do_not_depend_on_its_batch_with_a_bias_and_any_activation(act):
+    """Each kernel brings its sums to the output by itself."""
+    from dmlx_b200 import device as dev
+
+    k, f, n = 1400, 1300, 650
+    x = _x(1200, k, 25).cuda()
+    w, bias = dev.I8Weight(*_weight(n, k, 26)), torch.randn(n, generator=torch.Generator().manual_seed(27)).cuda() * 30
+
+    def scaled(n, k, seed, by):
+        q, s = _weight(n, k, seed)
+        return q, s * by * k ** -0.5
+
+    gate_up, down = dev.I8Weight.gated(*scaled(f, k, 28, 0.7), *scaled(f, k, 29, 0.7)), dev.I8Weight(*scaled(n, f, 30, 0.7))
+    held = dev.I8Rows(1200, k, f)
+    whole = dev.i8_mm(w, held, x, bias=bias, f32=True), dev.i8_mm(w, held, x, bias=bias), dev.i8_ffn(gate_up, down, held, x, activation=act)
+    for first, rows in ((0, 1), (3, 2), (9, 4), (20, 5), (100, 16), (7, 31), (500, 64), (250, 128), (40, 200), (11, 300), (600, 513)):
+        part = x[first:first + rows]
+        got = dev.i8_mm(w, held, part, bias=bias, f32=True), dev.i8_mm(w, held, part, bias=bias), dev.i8_ffn(gate_up, down, held, part, activation=act)
+        for a, b in zip(got, whole):
+            assert torch.equal(a, b[first:first + rows]), rows
+
+
+@pytest.mark.gpu
 def test_an_activation_that_is_none_is_refused():
     from dmlx_b200 import device as dev
 
