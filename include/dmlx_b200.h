@@ -602,7 +602,7 @@ b200_status b200_i8_mm(const b200_i8_weight* w, b200_i8_rows* r, const void* d_x
                        int64_t y_stride, int32_t y_f32, void* stream);
 /* y = W_down q(act(W_gate x) * (W_up x)) bf16 [rows, n of down]: both projections, the activation and the product in one kernel, whose result stays
  * f32 until a row's largest is known.  gate_up from b200_i8_weight_create_gated; down's k is its n.  d_x as in b200_i8_mm; the rows that the
- * handle holds stay. */
+ * handle holds stay.  y may lie over x. */
 enum { B200_ACT_SILU = 0, B200_ACT_GELU = 1 /* erf */, B200_ACT_GELU_TANH = 2 };
 b200_status b200_i8_ffn(const b200_i8_weight* gate_up, const b200_i8_weight* down, b200_i8_rows* r, const void* d_x, int64_t x_stride, int32_t rows,
                         int32_t activation, void* d_y, int64_t y_stride, void* stream);

@@ -299,6 +299,39 @@ def test_a_row_s_bits_do_not_depend_on_its_batch_with_a_bias_and_any_activation(
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("rows", [10, 300])
+def test_activations_far_out(act, rows):
+    """Rows of gates around 1e-6, 1, 5 and 12 (where a GELU cancels), 90 (where an exponential is no f32), 1e4 and 1e13 (where a cube is none)."""
+    from dmlx_b200 import device as dev
+
+    k, f, n = 256, 640, 130
+
+    def scaled(n, k, seed):
+        q, s = _weight(n, k, seed)
+        return q, torch.full((n,), (3 * 74 * k ** 0.5) ** -1.0)
+
+    gate, up, down = scaled(f, k, 1), scaled(f, k, 2), scaled(n, f, 3)
+    x = (_x(rows, k, 4).float() * torch.tensor([1e-6, 1.0, 5.0, 12.0, 90.0, 1e4, 1e13]).repeat(rows)[:rows, None]).bfloat16()
+    got = dev.i8_ffn(dev.I8Weight.gated(*gate, *up), dev.I8Weight(*down), dev.I8Rows(rows, k, f), x.cuda(), activation=act)
+    assert bool(got.isfinite().all())
+    _check_ffn(got, x, gate, up, down, act)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 4, 5, 70, 600])
+def test_a_block_s_result_over_its_rows(rows):
+    """They are in 8 bits before the first number of it is there."""
+    from dmlx_b200 import device as dev
+
+    k, f = 520, 700
+    gate_up, down = dev.I8Weight.gated(*_weight(f, k, 31), *_weight(f, k, 32)), dev.I8Weight(*_weight(k, f, 33))
+    x, held = _x(rows, k, 34).cuda(), dev.I8Rows(rows, k, f)
+    want = dev.i8_ffn(gate_up, down, held, x)
+    assert torch.equal(dev.i8_ffn(gate_up, down, held, x, out=x), want) and torch.equal(x, want)
+
+
+@pytest.mark.gpu
 def test_an_activation_that_is_none_is_refused():
     from dmlx_b200 import device as dev
 
