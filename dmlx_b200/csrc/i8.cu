@@ -258,11 +258,12 @@ __device__ __forceinline__ void gate_with(int act, float (&y)[N], const float (&
 // pushed into its shared memory, where the stages were unless there is room beside them, with a barrier that counts their bytes.
 constexpr int kStreamThreads = 320, kStreamShared = 112 * 1024, kStreamAlone = 226 * 1024, kMostShares = 8;  // (shared memory of two CTAs on an SM, of one)
 
-// Weights that go through L2 once: they leave it ahead of what else is there.  (Among it are the instructions, which a kernel fetches anew: behind 117 MB of
-// weights the last ones came from memory, 4 to 8 us for the output of one row.)
-__device__ __forceinline__ uint64_t passing_through() {
+// Weights that go through L2 once, where all rows are one tile's, leave it ahead of what else is there.  (Among it are the instructions, which a kernel fetches anew: behind
+// 117 MB of weights the last ones came from memory, 4 to 8 us for the output of one row.)  With more tiles of rows they are read again, and stay as anything else does.
+__device__ __forceinline__ uint64_t weights_in_l2(bool once) {
   uint64_t p;
-  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  if (once) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  else asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
   return p;
 }
 __device__ __forceinline__ void bulk_g2s_with(void* dst_smem, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
@@ -399,7 +400,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
   }
   __syncthreads();
   if (shares > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this CTA's barriers are there
-  const uint64_t policy = passing_through();
+  const uint64_t policy = weights_in_l2(gridDim.y == 1);
   auto load_weights = [&](int i, int s) {
     ptx::mbar_expect_tx(&full[s], W * kI8Block + (RAW ? 0 : n_here * kI8Chunk));
     for (int h = 0; h < W; ++h)
