@@ -24,7 +24,7 @@ namespace {
 
 // ---- rows into 8 bits ----------------------------------------------------------------------------------------------------
 // A row waits in registers while its largest is looked for: a block for each, or a warp where a row is short.  Bound by what it reads and writes, and by its
-// arithmetic in turn: 8192 rows of 4096 20 to 24 us (4.2 TB/s), 96 2.3.  (A warp for each of eight neighbouring rows, whose bytes lie together: 38.)
+// arithmetic in turn: 8192 rows of 4096 22.6 us (4.4 TB/s), 96 1.9.  (A warp for each of eight neighbouring rows, whose bytes lie together: 38.)
 struct QuantizeArgs {
   const __nv_bfloat16* x;
   long long x_stride;
@@ -86,7 +86,7 @@ void launch_quantize(const QuantizeArgs& a, cudaStream_t s) {
     if (vectors <= 32) launch_after(i8_quantize_kernel<1, true, FIT>, grid, warps * 32, 0, s, a);
     else launch_after(i8_quantize_kernel<2, true, FIT>, grid, warps * 32, 0, s, a);
   } else if (vectors <= 4 * 1024) {
-    // few rows: more threads, each with fewer loads to wait for (96 rows of 4096 2.7 us with one, 4.6 with four; 8192 33 and 24)
+    // few rows: more threads, each with fewer loads to wait for (96 rows of 4096 1.9 us with one, 2.8 with four; 8192 46 and 22.6)
     const int nv = rows > 4 * b200_sm_count() || vectors > 2048 ? 4 : vectors > 1024 ? 2 : 1, threads = (vectors + 32 * nv - 1) / (32 * nv) * 32;
     if (nv == 1) launch_after(i8_quantize_kernel<1, false, FIT>, rows, threads, 0, s, a);
     else if (nv == 2) launch_after(i8_quantize_kernel<2, false, FIT>, rows, threads, 0, s, a);
@@ -153,7 +153,8 @@ __global__ void __launch_bounds__(kInnerThreads, 3) i8_quantize_inner_kernel(con
 
 b200_status quantize_inner(const b200_i8_rows* r, int rows, int k, cudaStream_t s) {
   const int chunks = i8_chunks(k), eights = (rows + 7) / 8;
-  int per_block = kInnerAhead * 256;  // columns: fewer blocks where there are enough of them
+  // Columns: fewer blocks where there are enough of them (8192 rows through a block of 14336 1018 us, 1044 with 1024 columns a block; no more than 4096: 1015).
+  int per_block = kInnerAhead * 256;
   while (per_block < 4096 && (long long)eights * ((chunks * kI8Chunk + per_block - 1) / per_block) >= 8 * b200_sm_count()) per_block *= 2;
   launch_after(i8_quantize_inner_kernel, dim3(eights, (chunks * kI8Chunk + per_block - 1) / per_block), kInnerThreads, 0, s, r->h, (long long)r->h_stride, r->most, chunks * 4,
                r->hidden.q, r->hidden.scale, rows, k, chunks, per_block);
@@ -607,7 +608,8 @@ __global__ void __launch_bounds__(kStreamThreads, 2) i8_stream_kernel(MmArgs a) 
 // ---- many rows: pairs of CTAs ----
 // Two CTAs share an MMA of 256 rows by 256 weight rows: each brings 128 of both and holds the sums of its 128 rows, so that an MMA reads 8 KiB of each CTA's
 // shared memory in the 128 cycles that it takes.  Persistent: a pair walks the items, a tile of rows by a pair of weight tiles (gated: the gate's and
-// up's of the same 128 channels), rows fastest within bands, so that both operands come from L2.  An item's sums are half of tensor memory: eight
+// up's of the same 128 channels), rows fastest within bands of kPairBand tiles, so that both
+// operands come from L2 (8192 rows through a block of 14336 1017 us in a graph, bands of 4, 8 and 32 tiles 1057, 1031 and 1023).  An item's sums are half of tensor memory: eight
 // warps drain one half while the MMAs fill the other.
 // Where there are fewer items than pairs, a cluster of up to four pairs shares an item's K, an item to a cluster: groups of 32 columns go to the pairs in
 // turn, and a CTA gets the others' sums of its groups pushed into its shared memory, where the stages were.
@@ -1047,7 +1049,8 @@ b200_status launch_product(MmArgs& a, const I8RowsDev& to, const RawRows& raw, c
     const int tiles = a.tiles / W, row_tiles = (a.rows + a.tn - 1) / a.tn, stage = W * kI8Block + (in_kernel ? 0 : a.tn * kI8Chunk);
     const int room = ((long long)tiles * row_tiles * a.shares <= at_once[a.shares] ? kStreamAlone : kStreamShared) - 2048;
     const int pushed = pushed_bytes(std::min(a.rows, a.tn), a.shares, W), raw_bytes = in_kernel ? per_share * 16 * kI8Chunk : 0;
-    // What is pushed has a place beside the stages where that is a quarter of the room at most.
+    // What is pushed has a place beside the stages where that is a quarter of the room at most (an eighth: 200 rows of 4096 to 4096 9.1 us in place of 8.8; half: 256 through a
+    // block of 14336 66 in place of 61).
     a.over_stages = pushed > room / 4;
     a.stages = std::min(per_share, (room - raw_bytes - (a.over_stages ? 0 : pushed)) / stage);
     a.raw_at = a.stages * stage;
