@@ -313,7 +313,7 @@ _sig("b200_lora_apply", i32, vp, vp, vp, i32, vp, i32, vp, i32, vp)
 
 
 class ResidualNormShape(C.Structure):
-    _fields_ = [(n, i32) for n in ("n", "h_f32", "y_f32", "gate_sigmoid")] + [("scale", f32), ("eps", f32)]
+    _fields_ = [(n, i32) for n in ("n", "h_f32", "y_f32", "gate_sigmoid")] + [("scale", f32), ("eps", f32)] + [("h_out", i32)]
 
 
 _sig("b200_i8_weight_create", i32, i32, i32, vp, vp, P(vp))
@@ -325,6 +325,7 @@ _sig("b200_i8_quantize", i32, vp, vp, i64, i32, i32, vp)
 _sig("b200_i8_rows_get", i32, vp, vp, vp, vp)
 _sig("b200_i8_mm", i32, vp, vp, vp, i64, i32, vp, vp, i64, i32, vp)
 _sig("b200_i8_ffn", i32, vp, vp, vp, vp, i64, i32, i32, vp, i64, vp)
+_sig("b200_i8_ffn_f32", i32, vp, vp, vp, vp, i64, i32, i32, vp, i64, vp)
 _sig("b200_residual_norm", i32, P(ResidualNormShape), vp, i64, vp, i64, vp, i64, vp, vp, i32, vp, i64, vp, i64, vp, vp)
 _sig("b200_kv_create_layers", i32, P(KvConfig), P(KvLayer), P(vp))
 _sig("b200_argmax_f32", i32, vp, i32, i32, vp, vp)

@@ -1168,6 +1168,25 @@ b200_status check_out(const char* who, const void* d_y, int64_t y_stride, int32_
   return B200_OK;
 }
 
+b200_status feed_forward(const b200_i8_weight* gate_up, const b200_i8_weight* down, b200_i8_rows* r, const void* d_x, int64_t x_stride, int32_t rows, int32_t activation,
+                         void* d_y, int64_t y_stride, bool y_f32, void* stream) {
+  if (!gate_up || !down || !r) { b200_set_error("i8 ffn: no weights, or no rows"); return B200_ERR_INVALID_ARGUMENT; }
+  if (!gate_up->gated || down->gated || down->k != gate_up->n) {
+    b200_set_error("i8 ffn: %s weight of %d channels in front of %s of %d columns", gate_up->gated ? "a gated" : "a plain", gate_up->n, down->gated ? "a gated one" : "one", down->k);
+    return B200_ERR_INVALID_ARGUMENT;
+  }
+  if (activation < B200_ACT_SILU || activation > B200_ACT_GELU_TANH) { b200_set_error("i8 ffn: activation %d", activation); return B200_ERR_INVALID_ARGUMENT; }
+  if (down->k > r->max_hidden) { b200_set_error("i8 ffn: %d channels inside the block, the handle is for %d", down->k, r->max_hidden); return B200_ERR_CAPACITY; }
+  b200_status st = check_out("i8 ffn", d_y, y_stride, rows, down->n, y_f32 ? 4 : 2);
+  if (st == B200_OK) st = b200_require_device();
+  if (st == B200_OK) st = take_rows("i8 ffn", r, d_x, x_stride, rows, gate_up->k);
+  if (st != B200_OK || rows == 0) return st;
+  cudaStream_t s = (cudaStream_t)stream;
+  st = taken(r, rows, gate_up->k, product(gate_up, r->x, RawRows{d_x, x_stride, nullptr}, rows, nullptr, activation, r->h, r->h_stride, 0, r->most, s));
+  if (st == B200_OK) st = product(down, r->hidden, RawRows{r->h, r->h_stride, r}, rows, nullptr, 0, d_y, y_stride, y_f32, nullptr, s);
+  return st;
+}
+
 }  // namespace
 
 extern "C" b200_status b200_i8_weight_create(int32_t n, int32_t k, const int8_t* q, const float* scales, b200_i8_weight** out) {
@@ -1272,19 +1291,10 @@ extern "C" b200_status b200_i8_mm(const b200_i8_weight* w, b200_i8_rows* r, cons
 
 extern "C" b200_status b200_i8_ffn(const b200_i8_weight* gate_up, const b200_i8_weight* down, b200_i8_rows* r, const void* d_x, int64_t x_stride, int32_t rows,
                                    int32_t activation, void* d_y, int64_t y_stride, void* stream) {
-  if (!gate_up || !down || !r) { b200_set_error("i8 ffn: no weights, or no rows"); return B200_ERR_INVALID_ARGUMENT; }
-  if (!gate_up->gated || down->gated || down->k != gate_up->n) {
-    b200_set_error("i8 ffn: %s weight of %d channels in front of %s of %d columns", gate_up->gated ? "a gated" : "a plain", gate_up->n, down->gated ? "a gated one" : "one", down->k);
-    return B200_ERR_INVALID_ARGUMENT;
-  }
-  if (activation < B200_ACT_SILU || activation > B200_ACT_GELU_TANH) { b200_set_error("i8 ffn: activation %d", activation); return B200_ERR_INVALID_ARGUMENT; }
-  if (down->k > r->max_hidden) { b200_set_error("i8 ffn: %d channels inside the block, the handle is for %d", down->k, r->max_hidden); return B200_ERR_CAPACITY; }
-  b200_status st = check_out("i8 ffn", d_y, y_stride, rows, down->n, 2);
-  if (st == B200_OK) st = b200_require_device();
-  if (st == B200_OK) st = take_rows("i8 ffn", r, d_x, x_stride, rows, gate_up->k);
-  if (st != B200_OK || rows == 0) return st;
-  cudaStream_t s = (cudaStream_t)stream;
-  st = taken(r, rows, gate_up->k, product(gate_up, r->x, RawRows{d_x, x_stride, nullptr}, rows, nullptr, activation, r->h, r->h_stride, 0, r->most, s));
-  if (st == B200_OK) st = product(down, r->hidden, RawRows{r->h, r->h_stride, r}, rows, nullptr, 0, d_y, y_stride, 0, nullptr, s);
-  return st;
+  return feed_forward(gate_up, down, r, d_x, x_stride, rows, activation, d_y, y_stride, false, stream);
+}
+
+extern "C" b200_status b200_i8_ffn_f32(const b200_i8_weight* gate_up, const b200_i8_weight* down, b200_i8_rows* r, const void* d_x, int64_t x_stride, int32_t rows,
+                                       int32_t activation, float* d_y, int64_t y_stride, void* stream) {
+  return feed_forward(gate_up, down, r, d_x, x_stride, rows, activation, d_y, y_stride, true, stream);
 }

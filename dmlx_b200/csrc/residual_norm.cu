@@ -118,12 +118,12 @@ __device__ __forceinline__ float sum_of_two(float* part, float a, float b) {
   return warp_sum(v);
 }
 
-// The sigmoid of a gate of bf16, for an h' of type H.  In f32 2^t, t = z log2(e), takes log2(e) in two parts, the first of 16 bits, so that its product with z is exact, the
+// The sigmoid of a gate of bf16, for an h' of type T.  In f32 2^t, t = z log2(e), takes log2(e) in two parts, the first of 16 bits, so that its product with z is exact, the
 // rest's a factor 1 + d: t's rounding alone would be 2^-19 of the result at |z| of 30.  (8192 rows of 4096, f32, 70.7 us as without that, 78.4 with expf and a division; 3000
 // of 16384 133, 126 and 142.)
-template <typename H>
+template <typename T>
 __device__ __forceinline__ float gate_sigmoid(float z) {
-  if constexpr (sizeof(H) == 2) return sigmoid_for<H>(z);
+  if constexpr (sizeof(T) == 2) return sigmoid_for<T>(z);
   constexpr float kHigh = 47274.0f / 32768.0f, kLow = 4.8884952e-6f;  // log2(e) = kHigh + kLow / ln(2)
   const float d = fmaxf(-kLow * z, -1.0f);  // (z = inf: p = 0)
   float p;
@@ -133,7 +133,7 @@ __device__ __forceinline__ float gate_sigmoid(float z) {
 
 // NV vectors of eight columns for each thread.  WARP: a warp for a row.  FIT: all rows start on 16 bytes and are whole vectors.  (1024 threads with 32 numbers each have 64
 // registers: half of a row's y is still in its 16 bits while h comes.)
-template <typename H, typename Y, int NV, bool WARP, bool FIT>
+template <typename H, typename Y, typename O, int NV, bool WARP, bool FIT>
 __global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const __grid_constant__ ResidualNormArgs a) {
   after_previous();
   // A row's vectors one after the other, or behind all stores: 8192 rows of 4096 bf16 57.8 and 54.8 us, 3000 f32 rows of 16384 119 and 127.
@@ -146,12 +146,12 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const 
   auto column = [&](int u) { return (t + u * threads) * 8; };
   // Where rows do not start on 16 bytes, the columns are dealt out from a boundary of h_out ahead of its row (`lo` columns that are not there), and so are on
   // boundaries of all that lies like it.
-  const int lo = FIT || !a.shift ? 0 : (int)((reinterpret_cast<uintptr_t>((H*)a.h_out + (size_t)row * a.h_out_stride) / sizeof(H)) % 8);
+  const int lo = FIT || !a.shift ? 0 : (int)((reinterpret_cast<uintptr_t>((O*)a.h_out + (size_t)row * a.h_out_stride) / sizeof(O)) % 8);
   const int n = a.n + lo;
   const H* h = (const H*)a.h + (size_t)row * a.h_stride - lo;
   const Y* y = (const Y*)a.y + (size_t)row * a.y_stride - lo;
   const __nv_bfloat16 *gate = a.gate ? a.gate + (size_t)row * a.gate_stride - lo : nullptr, *post_w = a.post_w ? a.post_w - lo : nullptr, *norm_w = a.norm_w ? a.norm_w - lo : nullptr;
-  H* h_out = (H*)a.h_out + (size_t)row * a.h_out_stride - lo;
+  O* h_out = (O*)a.h_out + (size_t)row * a.h_out_stride - lo;
   __nv_bfloat16* x_out = a.x_out ? a.x_out + (size_t)row * a.x_out_stride - lo : nullptr;
   auto fits = [](const void* p) { return FIT || (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   Eight<Y> yr[NV];
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const 
     if (a.gate) {
       widen(NV <= 2 ? gr[NV <= 2 ? u : 0] : load_eight(gate, c, n, fits(gate), lo), w);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) p[e] *= a.sigmoid ? gate_sigmoid<H>(w[e]) : w[e];
+      for (int e = 0; e < 8; ++e) p[e] *= a.sigmoid ? gate_sigmoid<O>(w[e]) : w[e];
     }
     widen(hr[u], w);
 #pragma unroll
@@ -256,30 +256,31 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) residual_norm_kernel(const 
     if (column(u) < a.chunks * kI8Chunk) i8_store8(a.q.q, row, column(u), a.chunks, s, x[u]);
 }
 
-template <typename H, typename Y, bool FIT>
+template <typename H, typename Y, typename O, bool FIT>
 b200_status launch(const ResidualNormArgs& a, cudaStream_t s) {
   const int vectors = std::max(a.chunks * (kI8Chunk / 8), a.shift ? (a.n + 14) / 8 : 0);  // (up to seven columns ahead of the first)
   if (vectors <= 32 * 2) {
     const int warps = a.rows >= 8 * b200_sm_count() ? 8 : 1;
     const unsigned grid = (unsigned)((a.rows + warps - 1) / warps);
-    if (vectors <= 32) launch_after(residual_norm_kernel<H, Y, 1, true, FIT>, grid, warps * 32, 0, s, a);
-    else launch_after(residual_norm_kernel<H, Y, 2, true, FIT>, grid, warps * 32, 0, s, a);
+    if (vectors <= 32) launch_after(residual_norm_kernel<H, Y, O, 1, true, FIT>, grid, warps * 32, 0, s, a);
+    else launch_after(residual_norm_kernel<H, Y, O, 2, true, FIT>, grid, warps * 32, 0, s, a);
   } else {
     // Few rows: more threads, each with fewer loads to wait for, while all of them run at once (200 rows of 4096 3.2 us with one vector a thread, 3.4 with two; 600
     // 6.8 and 5.7; 64 of 8192 3.2 and 3.5, 200 5.9 and 4.6).
     const int nv = vectors <= 1024 && (long long)a.rows * vectors <= 864ll * b200_sm_count() ? 1 : vectors <= 2048 ? 2 : 4;
     const int threads = (vectors + 32 * nv - 1) / (32 * nv) * 32;
-    if (nv == 1) launch_after(residual_norm_kernel<H, Y, 1, false, FIT>, a.rows, threads, 0, s, a);
-    else if (nv == 2) launch_after(residual_norm_kernel<H, Y, 2, false, FIT>, a.rows, threads, 0, s, a);
-    else launch_after(residual_norm_kernel<H, Y, 4, false, FIT>, a.rows, threads, 0, s, a);
+    if (nv == 1) launch_after(residual_norm_kernel<H, Y, O, 1, false, FIT>, a.rows, threads, 0, s, a);
+    else if (nv == 2) launch_after(residual_norm_kernel<H, Y, O, 2, false, FIT>, a.rows, threads, 0, s, a);
+    else launch_after(residual_norm_kernel<H, Y, O, 4, false, FIT>, a.rows, threads, 0, s, a);
   }
   B200_LAUNCH_CHECK();
   return B200_OK;
 }
 
 template <typename H, typename Y>
-b200_status launch_any(const ResidualNormArgs& a, bool fit, cudaStream_t s) {
-  return fit ? launch<H, Y, true>(a, s) : launch<H, Y, false>(a, s);
+b200_status launch_any(const ResidualNormArgs& a, bool out_f32, bool fit, cudaStream_t s) {
+  if (out_f32) return fit ? launch<H, Y, float, true>(a, s) : launch<H, Y, float, false>(a, s);
+  return fit ? launch<H, Y, __nv_bfloat16, true>(a, s) : launch<H, Y, __nv_bfloat16, false>(a, s);
 }
 
 constexpr int kMostColumns = 32768;  // 1024 threads of four vectors
@@ -293,16 +294,18 @@ extern "C" b200_status b200_residual_norm(const b200_residual_norm_shape* shape,
   const int n = shape->n;
   if (n <= 0 || n > kMostColumns) { b200_set_error("residual norm: rows of %d columns (at most %d)", n, kMostColumns); return B200_ERR_UNSUPPORTED; }
   if (!(shape->eps >= 0.f)) { b200_set_error("residual norm: eps %g", (double)shape->eps); return B200_ERR_INVALID_ARGUMENT; }
-  const int h_size = shape->h_f32 ? 4 : 2, y_size = shape->y_f32 ? 4 : 2;
+  if (shape->h_out < B200_H_OUT_AS_H || shape->h_out > B200_H_OUT_F32) { b200_set_error("residual norm: h_out of type %d", shape->h_out); return B200_ERR_INVALID_ARGUMENT; }
+  const bool out_f32 = shape->h_out == B200_H_OUT_AS_H ? shape->h_f32 != 0 : shape->h_out == B200_H_OUT_F32;
+  const int h_size = shape->h_f32 ? 4 : 2, y_size = shape->y_f32 ? 4 : 2, out_size = out_f32 ? 4 : 2;
   auto holds = [&](const void* p, int64_t stride, int size) { return p && ((uintptr_t)p & (size - 1)) == 0 && (rows <= 1 || stride >= n); };
-  if (rows > 0 && (!holds(d_h, h_stride, h_size) || !holds(d_y, y_stride, y_size) || !holds(d_h_out, h_out_stride, h_size) || (d_x_out && !holds(d_x_out, x_out_stride, 2)) ||
+  if (rows > 0 && (!holds(d_h, h_stride, h_size) || !holds(d_y, y_stride, y_size) || !holds(d_h_out, h_out_stride, out_size) || (d_x_out && !holds(d_x_out, x_out_stride, 2)) ||
                    (d_gate && gate_stride != 0 && !holds(d_gate, gate_stride, 2)) || (((uintptr_t)d_gate | (uintptr_t)d_post_weight | (uintptr_t)d_norm_weight) & 1) != 0)) {
     b200_set_error("residual norm: rows of %d columns, each on a number's boundary, strides that hold a row", n);
     return B200_ERR_INVALID_ARGUMENT;
   }
   auto at = [&](const void* p, int64_t stride, int size) { return RowsAt{p, stride ? rows : 1, stride * size, (long long)n * size}; };
-  const RowsAt h_out = at(d_h_out, h_out_stride, h_size), x_out = at(d_x_out, x_out_stride, 2);
-  bool over = rows_overlap(h_out, x_out) || (rows_overlap(h_out, at(d_h, h_stride, h_size)) && (d_h_out != d_h || (rows > 1 && h_out_stride != h_stride))) ||
+  const RowsAt h_out = at(d_h_out, h_out_stride, out_size), x_out = at(d_x_out, x_out_stride, 2);
+  bool over = rows_overlap(h_out, x_out) || (rows_overlap(h_out, at(d_h, h_stride, h_size)) && (d_h_out != d_h || out_size != h_size || (rows > 1 && h_out_stride != h_stride))) ||
               rows_overlap(x_out, at(d_h, h_stride, h_size));
   for (const RowsAt& in : {at(d_y, y_stride, y_size), at(d_gate, gate_stride, 2), at(d_post_weight, 0, 2), at(d_norm_weight, 0, 2)})
     over = over || rows_overlap(h_out, in) || rows_overlap(x_out, in);
@@ -326,9 +329,9 @@ extern "C" b200_status b200_residual_norm(const b200_residual_norm_shape* shape,
   a.rows = rows; a.n = n; a.chunks = i8_chunks(n); a.sigmoid = shape->gate_sigmoid != 0; a.scale = shape->scale; a.eps = shape->eps;
   auto fits = [&](const void* p, int64_t stride, int size) { return ((uintptr_t)p & 15) == 0 && (rows <= 1 || stride * size % 16 == 0); };
   const bool fit = n % 8 == 0 && fits(d_h, h_stride, h_size) && fits(d_y, y_stride, y_size) && fits(d_gate, gate_stride, 2) && fits(d_post_weight, 0, 2) &&
-                   fits(d_norm_weight, 0, 2) && fits(d_h_out, h_out_stride, h_size) && fits(d_x_out, x_out_stride, 2);
+                   fits(d_norm_weight, 0, 2) && fits(d_h_out, h_out_stride, out_size) && fits(d_x_out, x_out_stride, 2);
   a.shift = !fit && !q_out && (n + 14) / 8 <= kMostColumns / 8;
   cudaStream_t s = (cudaStream_t)stream;
-  if (shape->h_f32) return shape->y_f32 ? launch_any<float, float>(a, fit, s) : launch_any<float, __nv_bfloat16>(a, fit, s);
-  return shape->y_f32 ? launch_any<__nv_bfloat16, float>(a, fit, s) : launch_any<__nv_bfloat16, __nv_bfloat16>(a, fit, s);
+  if (shape->h_f32) return shape->y_f32 ? launch_any<float, float>(a, out_f32, fit, s) : launch_any<float, __nv_bfloat16>(a, out_f32, fit, s);
+  return shape->y_f32 ? launch_any<__nv_bfloat16, float>(a, out_f32, fit, s) : launch_any<__nv_bfloat16, __nv_bfloat16>(a, out_f32, fit, s);
 }

@@ -591,32 +591,37 @@ ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 
 
 def i8_ffn(gate_up: I8Weight, down: I8Weight, rows: I8Rows, x: Optional[torch.Tensor] = None, activation: str = "silu",
-           out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """b200_i8_ffn: down(act(gate x) * (up x)), the rows in 8 bits in front of each product.  x as in i8_mm."""
+           out: Optional[torch.Tensor] = None, f32: bool = False) -> torch.Tensor:
+    """b200_i8_ffn (b200_i8_ffn_f32): down(act(gate x) * (up x)), the rows in 8 bits in front of each product; bf16, or f32.  x as in i8_mm."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation {activation!r}, there are {', '.join(ACTIVATIONS)}")
     device = torch.cuda.current_device()
     at, stride, t = rows._take(x, gate_up.k, device)
-    out_stride = down.n
+    dtype, out_stride = _F32 if f32 else _BF16, down.n
     if out is None:
-        out = _new_rows(t, down.n, _BF16, device) if x is None else x.new_empty((t, down.n))
+        out = _new_rows(t, down.n, dtype, device) if x is None or f32 else x.new_empty((t, down.n))
     else:
-        out_stride = _rows(out, (t, down.n), device)
-    _lib.check(lib.b200_i8_ffn(gate_up._h, down._h, rows._h, at, stride, t, ACTIVATIONS[activation], out.data_ptr(), out_stride, _raw_stream(device)))
+        out_stride = _rows(out, (t, down.n), device, dtype)
+    call = lib.b200_i8_ffn_f32 if f32 else lib.b200_i8_ffn
+    _lib.check(call(gate_up._h, down._h, rows._h, at, stride, t, ACTIVATIONS[activation], out.data_ptr(), out_stride, _raw_stream(device)))
     rows.rows, rows.k = t, gate_up.k
     return out
 
 
 def residual_norm(h: torch.Tensor, y: torch.Tensor, norm_weight: Optional[torch.Tensor] = None, post_weight: Optional[torch.Tensor] = None,
                   gate: Optional[torch.Tensor] = None, gate_sigmoid: bool = False, scale: float = 1.0, eps: float = 1e-5, h_out: Optional[torch.Tensor] = None,
-                  x_out: Optional[torch.Tensor] = None, rows: Optional[I8Rows] = None):
+                  x_out: Optional[torch.Tensor] = None, rows: Optional[I8Rows] = None, h_dtype: Optional[torch.dtype] = None):
     """b200_residual_norm: h + scale * gate * norm(y), and the norm of that for the next block.  h, y [T, n] bf16 or f32, gate bf16 [n] or [T, n] (rows may be
-    strided), a weight that is None is no norm.  Returns (h, x): x bf16, or None where it goes into `rows` in 8 bits.  h_out may be h."""
+    strided), a weight that is None is no norm.  Returns (h, x): x bf16, or None where it goes into `rows` in 8 bits.  h_out may be h.  h_dtype:
+    the type of the h that leaves, bf16 or f32 (that of h)."""
     if rows is not None and rows._h is None:  # (the call would take it for no rows)
         raise ValueError("the 8-bit rows are closed")
     device, shape = torch.cuda.current_device(), h.shape
     t, n = shape
     h_type, y_type = _F32 if h.dtype == _F32 else _BF16, _F32 if y.dtype == _F32 else _BF16
+    o_type = h_type if h_dtype is None else h_dtype
+    if o_type is not _BF16 and o_type is not _F32:
+        raise ValueError(f"h of {o_type}: bf16 or f32")
     h_stride, y_stride = _rows(h, shape, device, h_type), _rows(y, shape, device, y_type)
     gate_at = x_at = None
     gate_stride = h_out_stride = x_out_stride = n
@@ -626,16 +631,16 @@ def residual_norm(h: torch.Tensor, y: torch.Tensor, norm_weight: Optional[torch.
         else:
             gate_at, gate_stride = _weight(gate, n, device), 0
     if h_out is None:
-        h_out = torch.empty_like(h) if h_stride == n else _new_rows(t, n, h_type, device)  # (1.3 us of the host's time for 2.5)
+        h_out = torch.empty_like(h) if h_stride == n and o_type is h_type else _new_rows(t, n, o_type, device)  # (1.3 us of the host's time for 2.5)
     else:
-        h_out_stride = _rows(h_out, shape, device, h_type)
+        h_out_stride = _rows(h_out, shape, device, o_type)
     if x_out is not None:
         x_out_stride = _rows(x_out, shape, device)
     elif rows is None:
         x_out = torch.empty_like(h) if h_type is _BF16 and h_stride == n else torch.empty_like(y) if y_type is _BF16 and y_stride == n else _new_rows(t, n, _BF16, device)
     if x_out is not None:
         x_at = x_out.data_ptr()
-    _lib.check(lib.b200_residual_norm(_norm_shape(n, h_type is _F32, y_type is _F32, bool(gate_sigmoid), float(scale), float(eps)), h.data_ptr(), h_stride, y.data_ptr(), y_stride,
+    _lib.check(lib.b200_residual_norm(_norm_shape(n, h_type is _F32, y_type is _F32, bool(gate_sigmoid), float(scale), float(eps), 2 if o_type is _F32 else 1), h.data_ptr(), h_stride, y.data_ptr(), y_stride,
                                       gate_at, gate_stride, _weight(post_weight, n, device), _weight(norm_weight, n, device), t, h_out.data_ptr(), h_out_stride, x_at,
                                       x_out_stride, None if rows is None else rows._h, _raw_stream(device)))
     if rows is not None:
@@ -644,8 +649,8 @@ def residual_norm(h: torch.Tensor, y: torch.Tensor, norm_weight: Optional[torch.
 
 
 @functools.lru_cache(maxsize=256)
-def _norm_shape(n: int, h_f32: bool, y_f32: bool, gate_sigmoid: bool, scale: float, eps: float):
-    return C.byref(_lib.ResidualNormShape(n, h_f32, y_f32, gate_sigmoid, scale, eps))
+def _norm_shape(n: int, h_f32: bool, y_f32: bool, gate_sigmoid: bool, scale: float, eps: float, h_out: int):
+    return C.byref(_lib.ResidualNormShape(n, h_f32, y_f32, gate_sigmoid, scale, eps, h_out))
 
 
 def set_attn_pages_per_chunk(n: int):

@@ -606,18 +606,23 @@ b200_status b200_i8_mm(const b200_i8_weight* w, b200_i8_rows* r, const void* d_x
 enum { B200_ACT_SILU = 0, B200_ACT_GELU = 1 /* erf */, B200_ACT_GELU_TANH = 2 };
 b200_status b200_i8_ffn(const b200_i8_weight* gate_up, const b200_i8_weight* down, b200_i8_rows* r, const void* d_x, int64_t x_stride, int32_t rows,
                         int32_t activation, void* d_y, int64_t y_stride, void* stream);
+/* The same into f32. */
+b200_status b200_i8_ffn_f32(const b200_i8_weight* gate_up, const b200_i8_weight* down, b200_i8_rows* r, const void* d_x, int64_t x_stride, int32_t rows,
+                            int32_t activation, float* d_y, int64_t y_stride, void* stream);
 /* The norms behind and before a block with its gate and its factor on the residual:
  *   p = y, or y / sqrt(mean(y^2) + eps) * post_weight; p = p * gate, or p * sigmoid(gate); h_out = h + scale * p;
  *   x = h_out, or h_out / sqrt(mean(h_out^2) + eps) * norm_weight (h_out before its rounding).
  * f32 in between, one rounding each; the same bits for a row whatever shares its batch where n is a multiple of eight and the rows of all operands start on 16 bytes
- * (elsewhere the order of a row's sums of squares, and with it their last bit, goes by where the row lies and by how many there are).  y and h are rows of n numbers (bf16, or f32 with y_f32, h_f32; h_out is like h and may be h), weights bf16 [n], null =
+ * (elsewhere the order of a row's sums of squares, and with it their last bit, goes by where the row lies and by how many there are).  y and h are rows of n numbers (bf16, or f32 with y_f32, h_f32; h_out is like h, and may be h then, or of a type of its own), weights bf16 [n], null =
  * no norm; gate bf16, null = none, gate_stride 0: one for all rows.  x goes to x_out (bf16) and, in 8 bits, into q_out, either null.  Nothing but h_out and
  * h overlaps (refused).  n up to 32768; strides in elements, any. */
+enum { B200_H_OUT_AS_H = 0, B200_H_OUT_BF16 = 1, B200_H_OUT_F32 = 2 };
 typedef struct b200_residual_norm_shape {
   int32_t n;
   int32_t h_f32, y_f32;
   int32_t gate_sigmoid;
   float scale, eps;
+  int32_t h_out; /* B200_H_OUT_* */
 } b200_residual_norm_shape;
 b200_status b200_residual_norm(const b200_residual_norm_shape* shape, const void* d_h, int64_t h_stride, const void* d_y, int64_t y_stride,
                                const void* d_gate, int64_t gate_stride, const void* d_post_weight, const void* d_norm_weight, int32_t rows, void* d_h_out,

@@ -241,6 +241,30 @@ def test_feed_forward(act, rows, k, f, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,f", [(1, 512, 700), (3, 77, 130), (4, 4096, 1024), (30, 1000, 300), (200, 256, 640), (700, 333, 515)])
+def test_feed_forward_into_f32(rows, k, f):
+    """Rounded, it is the block's result in bf16."""
+    from dmlx_b200 import device as dev
+
+    def scaled(n, k, seed):
+        q, s = _weight(n, k, seed)
+        return q, s * 0.7 * k ** -0.5
+
+    gate, up, down = scaled(f, k, 4), scaled(f, k, 5), scaled(k, f, 6)
+    gate_up, down_w, held, x = dev.I8Weight.gated(*gate, *up), dev.I8Weight(*down), dev.I8Rows(rows, k, f), _x(rows, k, 7).cuda()
+    got = dev.i8_ffn(gate_up, down_w, held, x, f32=True)
+    assert got.dtype == torch.float32 and torch.equal(got.bfloat16(), dev.i8_ffn(gate_up, down_w, held, x))
+    _check_ffn(got, x.cpu(), gate, up, down, "silu")
+    wide = torch.full((rows + 1, k + 5), 7.0, device="cuda")  # on no 16-byte boundary
+    dev.i8_ffn(gate_up, down_w, held, out=wide[:rows, 3:3 + k], f32=True)
+    assert torch.equal(wide[:rows, 3:3 + k], got) and bool((wide[rows:] == 7).all()) and bool((wide[:, :3] == 7).all()) and bool((wide[:, 3 + k:] == 7).all())
+    with pytest.raises(ValueError):
+        dev.i8_ffn(gate_up, down_w, held, x, out=torch.empty((rows, k), dtype=torch.bfloat16, device="cuda"), f32=True)
+    from dmlx_b200 import _lib
+    assert _lib.lib.b200_i8_ffn_f32(gate_up._h, down_w._h, held._h, None, 0, rows, 0, wide.data_ptr() + 2, k + 5, None) == _lib.ERR_INVALID_ARGUMENT
+
+
+@pytest.mark.gpu
 def test_a_row_s_bits_do_not_depend_on_its_batch():
     from dmlx_b200 import device as dev
 

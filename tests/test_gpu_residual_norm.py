@@ -274,6 +274,62 @@ def test_a_gate_s_sigmoid_in_f32():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,n", [(1, 4096), (700, 1000), (3, 16384), (300, 504), (64, 8192), (320, 5003), (5, 131), (2, 32761)])
+@pytest.mark.parametrize("h_f32,y_f32", [(False, False), (False, True), (True, False), (True, True)])
+def test_an_h_that_leaves_as_another_type(rows, n, h_f32, y_f32):
+    from dmlx_b200 import device as dev
+
+    c = _make(rows, n, rows + n, h_f32, y_f32)
+    to = torch.bfloat16 if h_f32 else torch.float32
+    args = dict(post_weight=c["post"].cuda(), gate=c["gate"].cuda(), scale=0.22)
+    h, y, norm = c["h"].cuda(), c["y"].cuda(), c["norm"].cuda()
+    got = dev.residual_norm(h, y, norm, h_dtype=to, **args)
+    assert got[0].dtype == to and got[1].dtype == torch.bfloat16
+    want = _want(c["h"], c["y"], c["post"], c["norm"], c["gate"], False, 0.22, 1e-5)
+    _check(got[0], want[0], want[1])
+    _check(got[1], want[2], want[3])
+    if n % 8 == 0:  # (a row's sums are the same then) what f32 rows give, rounded where it is bf16
+        wide = dev.residual_norm(h.float(), y, norm, **args)
+        assert torch.equal(got[0], wide[0].to(to)) and torch.equal(got[1], wide[1])
+    out = torch.full((rows + 1, n + 5), 7.0, dtype=to, device="cuda")
+    dev.residual_norm(h, y, norm, h_dtype=to, h_out=out[:rows, 3:3 + n], x_out=got[1], **args)
+    _check(out[:rows, 3:3 + n], want[0], want[1])
+    assert bool((out[rows:] == 7).all()) and bool((out[:, :3] == 7).all()) and bool((out[:, 3 + n:] == 7).all())
+
+
+@pytest.mark.gpu
+def test_refusals_of_an_h_of_another_type():
+    from dmlx_b200 import _lib
+    from dmlx_b200 import device as dev
+
+    c = {k: v.cuda() for k, v in _make(4, 64, 14).items()}
+    h, y, norm = c["h"], c["y"], c["norm"]
+    for call in (lambda: dev.residual_norm(h, y, norm, h_dtype=torch.float16), lambda: dev.residual_norm(h, y, norm, h_dtype=torch.float32, h_out=torch.empty_like(h)),
+                 lambda: dev.residual_norm(h.float(), y, norm, h_dtype=torch.bfloat16, h_out=h.float())):
+        with pytest.raises(ValueError):
+            call()
+    both = torch.zeros((8, 64), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(_lib.B200Error) as e:  # over itself, in other strides
+        dev.residual_norm(both[:4], y, norm, h_dtype=torch.float32, h_out=both.view(-1).view(torch.float32).view(4, 64))
+    assert e.value.status == _lib.ERR_INVALID_ARGUMENT
+
+
+def test_a_type_of_h_that_there_is_none_of_is_refused_without_a_device():
+    import ctypes as C
+
+    from dmlx_b200 import _lib
+
+    run = lambda h_f32, h_out, out: _lib.lib.b200_residual_norm(C.byref(_lib.ResidualNormShape(8, h_f32, 0, 0, 1.0, 1e-5, h_out)), 0x1000, 8, 0x2000, 8, None, 0, None, None, 1, out, 8,  # noqa: E731
+                                                               None, 0, None, None)
+    bad = _lib.ERR_INVALID_ARGUMENT
+    assert run(0, 3, 0x3000) == bad and run(0, -1, 0x3000) == bad
+    assert run(0, 2, 0x3002) == bad and run(0, 2, 0x1000) == bad and run(1, 1, 0x1000) == bad  # on no number's boundary, over h of another type
+    if not torch.cuda.is_available():  # these are not run: the addresses are made up
+        for h_f32, h_out, out in ((0, 1, 0x1000), (1, 2, 0x1000), (1, 0, 0x1000), (1, 1, 0x3002), (0, 2, 0x3004)):
+            assert run(h_f32, h_out, out) not in (_lib.OK, bad), (h_f32, h_out)
+
+
+@pytest.mark.gpu
 def test_8_bit_rows_that_are_closed_are_refused():
     from dmlx_b200 import device as dev
 
