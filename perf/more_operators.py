@@ -139,9 +139,9 @@ def run(s):
         if case["op"] == "norm":
             return device.residual_norm(s["h"], s["y"], s["norm_weight"], post_weight=s["post_weight"], gate=s["gate"], gate_sigmoid=case["gate"] == "sigmoid",
                                         scale=s["scale"], eps=EPS)
-        h, _ = device.residual_norm(s["h"], s["y"], s["norm_weight"], post_weight=s["post_weight"], scale=s["scale"], eps=EPS, rows=s["rows"])
-        y = device.i8_ffn(s["gate_up"], s["down_weight"], s["rows"], activation=case["act"])
-        return device.residual_norm(h, y, s["next_weight"], post_weight=s["end_weight"], scale=s["scale"], eps=EPS)
+        h, _ = device.residual_norm(s["h"], s["y"], s["norm_weight"], post_weight=s["post_weight"], scale=s["scale"], eps=EPS, rows=s["rows"], h_dtype=torch.float32)
+        y = device.i8_ffn(s["gate_up"], s["down_weight"], s["rows"], activation=case["act"], f32=True)
+        return device.residual_norm(h, y, s["next_weight"], post_weight=s["end_weight"], scale=s["scale"], eps=EPS, h_dtype=torch.bfloat16)
     if case["op"] == "mm":
         y = _product(s["x"].float(), s["w"], s["w_scale"])
         if s["bias"] is not None:
