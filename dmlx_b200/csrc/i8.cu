@@ -3,9 +3,10 @@
 //
 // The sums are exact (int32 on tcgen05.mma kind::i8), so neither the order of K nor what shares a tile changes a bit of a row.
 //
-// Few rows are bound by the weights: one row of 4096 to 6144 7.3 us in a graph, one through a block of 14336 33 (176 MB, 5.4 TB/s), 96 through it 43.  Many are bound by
-// the tensor cores under the power cap: 8192 rows of 4096 to 6144 127 to 132 us beside 20 to 30 for the rows themselves, 3.2 PFLOP/s, through a block of 14336
-// 1130 to 1200, 600 to 630 of them the first product, 270 to 280 the second, 115 to 140 the inner rows into 8 bits.
+// Few rows are bound by the weights: one row of 4096 to 6144 7.0 us in a graph, one through a block of 14336 32 (176 MB, 5.5 TB/s), 96 through it 42.  Many are bound by
+// the tensor cores under the power cap.  In a run of a second and more (1.49 GHz in the middle, the cap its only reason) 8192 rows of 4096 to 6144 take 185 us; with an event
+// between its kernels, which ends their overlap, 33 for the rows and 157 for the product (2.6 PFLOP/s).  Through a block of 14336 they take 1204 to 1220; apart in the same run
+// 36 the rows, 720 gate and up (2.7 PFLOP/s), 124 the inner rows, 329 down (2.9): 1208.  The first milliseconds are faster, as the clock falls only then: 155 and 1067 in a graph.
 #include <cuda_bf16.h>
 #include <math.h>
 

@@ -5,8 +5,9 @@
 // largest |h' w_norm|, from which the 8-bit form's step follows without a third (r > 0, and rounding keeps the order).  x is made of h' before its rounding.
 // f32 in between, one rounding for each result.  Everything a row needs is asked for before its first sum.
 //
-// Bound by what it reads and writes: 8192 rows of 4096 bf16 with a gate for each take 58 to 61 us, 5.6 TB/s (the gate behind the first sum 64, weights too 75); one row 2.4 us,
-// a launch's latency; 333 rows of 5003, f32 beside bf16, 7.1 (number by number 18).
+// Bound by what it reads and writes: 8192 rows of 4096 bf16 with a gate for each take 55 to 57 us in a graph, 6 TB/s (the gate behind the first sum 64, weights too 75); one row 2.2
+// us, a launch's latency; 333 rows of 5003, f32 beside bf16, 7.1 to 7.7 (number by number 18).  Into 8-bit rows: 8192 of 4096 55.8 (235 MB, 36 at the rate of a copy: the 8 bits
+// take the arithmetic), one 2.5; 333 of 5003 7.6 and 3000 45.6, whose columns are dealt out from the first and whose loads are shifted into place therefore.
 #include <cuda_bf16.h>
 
 #include <algorithm>

@@ -578,7 +578,7 @@ b200_status b200_lora_apply(const b200_lora* l, b200_lora_batch* b, const void* 
  * columns and changes no other row.  The products give a row the same bits whatever shares its batch.
  * A b200_i8_rows holds the rows of a step in 8 bits and is the workspace of the products that read them: steps that may run at the same time (two
  * captured graphs on two streams) have one each.  A captured product without its rows' making works on what the handle holds when it runs.  All calls but
- * those that create are asynchronous on the stream and may be captured.  Rows, strides and widths may be any.  A wait inside the kernels that runs out is
+ * those that create are asynchronous on the stream and may be captured.  Widths may be any, and strides that hold a row (of the gate 0, too).  A wait inside the kernels that runs out is
  * reported through b200_qmm_error_word. */
 typedef struct b200_i8_weight b200_i8_weight;
 typedef struct b200_i8_rows b200_i8_rows;
@@ -615,7 +615,7 @@ b200_status b200_i8_ffn_f32(const b200_i8_weight* gate_up, const b200_i8_weight*
  * f32 in between, one rounding each; the same bits for a row whatever shares its batch where n is a multiple of eight and the rows of all operands start on 16 bytes
  * (elsewhere the order of a row's sums of squares, and with it their last bit, goes by where the row lies and by how many there are).  y and h are rows of n numbers (bf16, or f32 with y_f32, h_f32; h_out is like h, and may be h then, or of a type of its own), weights bf16 [n], null =
  * no norm; gate bf16, null = none, gate_stride 0: one for all rows.  x goes to x_out (bf16) and, in 8 bits, into q_out, either null.  Nothing but h_out and
- * h overlaps (refused).  n up to 32768; strides in elements, any. */
+ * h overlaps (refused).  n up to 32768; strides in elements. */
 enum { B200_H_OUT_AS_H = 0, B200_H_OUT_BF16 = 1, B200_H_OUT_F32 = 2 };
 typedef struct b200_residual_norm_shape {
   int32_t n;
